@@ -39,6 +39,8 @@ enum {
 
 /* ggml tensor type codes (crates/sapient-io/src/gguf.rs:88-129) */
 enum { SP_F32 = 0, SP_F16 = 1, SP_Q4_0 = 2, SP_Q8_0 = 8, SP_Q4_K = 12, SP_Q5_K = 13, SP_Q6_K = 14, SP_BF16 = 30 };
+/* No ggml type: e4m3 values [n, k] with an f32 scale for every 128 x 128 block (sp_cuda_upload_weight_fp8). */
+enum { SP_F8_E4M3 = 128 };
 
 const char* sp_cuda_last_error(void);
 /* number of visible CUDA devices, or 0 */
@@ -136,6 +138,58 @@ int32_t sp_cuda_mul(int32_t device, const float* a, const float* b, int64_t n, f
 int32_t sp_cuda_embed(const SpWeight* table, const uint32_t* ids, int64_t n, float* out_host);
 /* sampler::argmax (crates/sapient-generate/src/sampler.rs:161-168): last maximum wins. */
 int32_t sp_cuda_argmax(int32_t device, const float* logits, int64_t rows, int64_t n, uint32_t* out);
+
+/* ── 8-bit floating-point rows and weights, and token distributions (no counterpart in the reference) ──
+ * An fp8 row of k columns is k e4m3 values and ceil(k / 128) f32 scales; a value stands for e4m3 x the scale of its block of
+ * 128 columns (the last block may be shorter). Rows are quantised by
+ *     scale = max(max |y| of the block / 448, 2^-100),   q = e4m3(y / scale), to nearest even
+ * and a block that holds a NaN or an infinity gets one as its scale. k and dim are multiples of 16.
+ * The _dev calls take device pointers of `device` (the calling thread's current device is what it was when they return) and a
+ * cudaStream_t (NULL: default stream), launch one kernel and do not wait. They keep nothing between calls, so that they may
+ * run at the same time on several streams and be captured into graphs. dtype of a _dev call: SP_F32 or SP_BF16, of x, residual,
+ * sum_out, y or logits; the other float arrays are f32. q, scale and the other outputs must not overlap what is read, except where
+ * the call says so. Rows of x, residual and sum_out start on 16 bytes (strides are multiples of 4 values in f32, 8 in bf16), so do
+ * w, q, xq and wq. rows or m = 0 is a call that does nothing. */
+/* h = x + residual (NULL: h = x), y = h / sqrt(mean(h^2) + eps) * w (NULL: 1); y as fp8 rows to q[rows][dim], scale[rows][blocks],
+ * h to sum_out (NULL: not stored), which may be x or residual with the same stride. y is made from h before h is rounded to
+ * sum_out's type. dim at most 32768. */
+int32_t sp_cuda_rms_norm_fp8_dev(int32_t device, int32_t dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                 void* sum_out, int64_t lds, const float* w, float eps, int64_t rows, int64_t dim, void* q,
+                                 float* scale, void* stream);
+/* y = silu(gu[:, 0 .. ffn)) * gu[:, ffn .. 2 ffn) as fp8 rows. */
+int32_t sp_cuda_swiglu_fp8_dev(int32_t device, int32_t dtype, const void* gu, int64_t ld, int64_t rows, int64_t ffn, void* q,
+                               float* scale, void* stream);
+/* x as fp8 rows. */
+int32_t sp_cuda_quant_fp8_dev(int32_t device, int32_t dtype, const void* x, int64_t ldx, int64_t rows, int64_t dim, void* q,
+                              float* scale, void* stream);
+/* y[m][n] (row stride ldy values of dtype) = X Wᵀ of fp8 rows xq[m][k], xs[m][blocks] and e4m3 weights wq[n][k] with scales
+ * ws[ceil(n / 128)][blocks]. Products are exact, sums f32. */
+int32_t sp_cuda_matmul_fp8_dev(int32_t device, const void* xq, const float* xs, int64_t m, const void* wq, const float* ws, int64_t n,
+                               int64_t k, void* y, int32_t dtype, int64_t ldy, void* stream);
+/* Of each row of logits[rows][vocab] (row stride ld): logprob[rows] of the token ids[row] (NaN for an id outside the vocabulary),
+ * the entropy of the row's distribution (natural logarithms), and the `top` (0 to 32, at most vocab) most likely tokens
+ * top_ids[rows][top], most likely first and the lower id first among equal logits (unlike sp_cuda_argmax, which gives the last),
+ * with their top_logprobs[rows][top]. Each output may be NULL; ids only with logprob. A logit of -inf is a masked token; a row of
+ * nothing else has log probabilities of -inf and entropy 0. A row with a NaN or +inf has NaN everywhere but in top_ids, where a NaN
+ * counts as the largest. */
+#define SP_LOGPROBS_MAX_TOP 32
+int32_t sp_cuda_logprobs_dev(int32_t device, int32_t dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab,
+                             const uint32_t* ids, int32_t top, float* logprob, float* entropy, uint32_t* top_ids,
+                             float* top_logprobs, void* stream);
+/* The same on dense host buffers in f32 (copies inside); an id outside the vocabulary is SP_ERR_VOCAB. */
+int32_t sp_cuda_rms_norm_fp8(int32_t device, const float* x, const float* residual, const float* w, int64_t rows, int64_t dim, float eps,
+                             void* q, float* scale, float* sum_out);
+int32_t sp_cuda_swiglu_fp8(int32_t device, const float* gu, int64_t rows, int64_t ffn, void* q, float* scale);
+int32_t sp_cuda_quant_fp8(int32_t device, const float* x, int64_t rows, int64_t dim, void* q, float* scale);
+int32_t sp_cuda_matmul_fp8(int32_t device, const void* xq, const float* xs, int64_t m, const void* wq, const float* ws, int64_t n,
+                           int64_t k, float* y);
+int32_t sp_cuda_logprobs(int32_t device, const float* logits, int64_t rows, int64_t vocab, const uint32_t* ids, int32_t top,
+                         float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs);
+/* A weight of type SP_F8_E4M3: values[n][k] and scales[ceil(n / 128)][ceil(k / 128)] from host memory. sp_cuda_matmul_nt and
+ * _matmul_nt_dev quantise the rows of x to fp8 first (in a workspace that the weight carries and that grows with m, so that what
+ * sp_cuda_matmul_nt_dev says of streams and of first calls holds for it; y must not overlap x); sp_cuda_dequant, _weight_info and
+ * _free_weight work as for the other types. Not a table for sp_cuda_embed. */
+int32_t sp_cuda_upload_weight_fp8(int32_t device, int64_t n, int64_t k, const void* values, const float* scales, SpWeight** out);
 
 /* ── engine level: replaces ForwardEngine (crates/sapient-models/src/forward/mod.rs:49-65,381-506)
  *    in the shape of the resident WgpuForwardEngine (forward/wgpu_engine.rs:93-110,173-341,362-676) ── */
@@ -313,7 +367,7 @@ int32_t sp_cuda_batcher_forget(SpBatcher* b, uint64_t id);
 #define SP_BATCHER_STATS 9
 int32_t sp_cuda_batcher_stats(const SpBatcher* b, uint64_t* out, int32_t cap);
 /* For tests of what follows a wait that ran out: a kernel reports one of `kind` (0: GEMM on quantised weights, 1: product
- * on bf16 weights, 2: streaming GEMV) as those kernels do, on the engine's stream in the engine's name, or (engine null)
+ * on bf16 weights, 2: streaming GEMV, 3: product on fp8 weights) as those kernels do, on the engine's stream in the engine's name, or (engine null)
  * for `device`'s op-level calls. The owner's next call that waits for the device fails with SP_ERR_CUDA, once. */
 int32_t sp_cuda_report_wait(SpEngine* engine, int32_t device, int32_t kind);
 /* Replay decode steps as CUDA graphs (default on). */

@@ -74,6 +74,17 @@ SIGNATURES = {
     "sp_cuda_mul": (_i32, [_i32, _vp, _vp, _i64, _vp]),
     "sp_cuda_embed": (_i32, [_vp, _vp, _i64, _vp]),
     "sp_cuda_argmax": (_i32, [_i32, _vp, _i64, _i64, _vp]),
+    "sp_cuda_rms_norm_fp8_dev": (_i32, [_i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _f, _i64, _i64, _vp, _vp, _vp]),
+    "sp_cuda_swiglu_fp8_dev": (_i32, [_i32, _i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "sp_cuda_quant_fp8_dev": (_i32, [_i32, _i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "sp_cuda_matmul_fp8_dev": (_i32, [_i32, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp]),
+    "sp_cuda_logprobs_dev": (_i32, [_i32, _i32, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "sp_cuda_rms_norm_fp8": (_i32, [_i32, _vp, _vp, _vp, _i64, _i64, _f, _vp, _vp, _vp]),
+    "sp_cuda_swiglu_fp8": (_i32, [_i32, _vp, _i64, _i64, _vp, _vp]),
+    "sp_cuda_quant_fp8": (_i32, [_i32, _vp, _i64, _i64, _vp, _vp]),
+    "sp_cuda_matmul_fp8": (_i32, [_i32, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "sp_cuda_logprobs": (_i32, [_i32, _vp, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp]),
+    "sp_cuda_upload_weight_fp8": (_i32, [_i32, _i64, _i64, _vp, _vp, C.POINTER(_vp)]),
     "sp_cuda_engine_create": (_i32, [C.POINTER(SpModelDesc), C.POINTER(_vp)]),
     "sp_cuda_engine_set_tensor": (_i32, [_vp, C.c_char_p, _i32, _vp, _i32, _vp, _sz]),
     "sp_cuda_engine_finalize": (_i32, [_vp]),

@@ -10,6 +10,7 @@
 
 #include "batcher.h"
 #include "engine.h"
+#include "fp8.h"
 #include "model_plan.h"
 #include "sp_common.cuh"
 
@@ -25,6 +26,9 @@ struct SpWeight {
     ActWorkspace ws;           // activation digits for up to 16 rows
     RingScratch ring;          // shared-row scratch of the ring GEMV (calls of 1-4 rows)
     RowsScratch rows;          // K-split partials of the one-pass many-row GEMV
+    float* scale = nullptr;    // SP_F8_E4M3: the blocks' scales
+    uint8_t* xq = nullptr;     // and the activations as fp8 rows, their scales behind them
+    int64_t xq_rows = 0;       // rows there is room for
 };
 struct SpEngine {
     Engine* e;
@@ -107,6 +111,58 @@ int binary_op(int device, const float* a, const float* b, int64_t n, float* y,
     SP_CUDA_TRY(cudaMemcpy(db.p, b, (size_t)n * 4, cudaMemcpyHostToDevice));
     SP_CUDA_TRY(fn(da.as<float>(), db.as<float>(), da.as<float>(), n, 0));
     SP_CUDA_TRY(cudaMemcpy(y, da.p, (size_t)n * 4, cudaMemcpyDeviceToHost));
+    return SP_OK;
+}
+
+// The calling thread's current device is `device` while this lives.
+struct OnDevice {
+    int before = -1;
+    cudaError_t enter(int device) {
+        cudaError_t e = cudaGetDevice(&before);
+        if (e != cudaSuccess) before = -1;
+        return e != cudaSuccess || before == device ? e : cudaSetDevice(device);
+    }
+    ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
+};
+
+// The flags of op-level calls on the current device, made on the first one (during another thread's stream capture or this one's, too).
+cudaError_t op_waits(int** waits) {
+    WaitFlags& f = device_wait_flags();
+    if (!f.host.load()) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) return e;
+        e = f.alloc();
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) return e;
+    }
+    *waits = f.dev;
+    return cudaSuccess;
+}
+
+int check_fp8_type(int dtype) {
+    if (dtype != SP_F32 && dtype != SP_BF16) { set_error("fp8: the type of these rows is SP_F32 or SP_BF16"); return SP_ERR_DTYPE; }
+    return SP_OK;
+}
+
+bool unaligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
+
+// Rows whose 16-byte pieces are read or written: address and stride.
+int check_fp8_rows(const char* what, const void* p, int64_t ld, int64_t dim, int dtype) {
+    const int per = dtype == SP_F32 ? 4 : 8;
+    if (unaligned(p, 16)) { set_error(std::string(what) + " must be 16-byte aligned"); return SP_ERR_ARG; }
+    if (ld < dim || ld % per != 0) { set_error(std::string(what) + ": the row stride must hold a row and be a multiple of 16 bytes"); return SP_ERR_SHAPE; }
+    return SP_OK;
+}
+
+int check_fp8_dim(int64_t rows, int64_t dim, const char* name) {
+    if (rows < 0 || dim <= 0 || dim % 16 != 0 || dim > INT32_MAX / 2) { set_error(std::string("fp8: ") + name + " must be a positive multiple of 16"); return SP_ERR_SHAPE; }
+    return SP_OK;
+}
+
+int check_logprobs(int64_t rows, int64_t vocab, int top) {
+    if (rows < 0 || vocab < 1 || vocab > (1 << 30) || rows > (1 << 27)) { set_error("logprobs: bad shape"); return SP_ERR_SHAPE; }
+    if (top < 0 || top > SP_LOGPROBS_MAX_TOP || top > vocab) { set_error("logprobs: top must be 0 to 32 and at most the vocabulary"); return SP_ERR_ARG; }
     return SP_OK;
 }
 
@@ -273,10 +329,35 @@ int32_t sp_cuda_upload_weight(int32_t device, int32_t dtype, int64_t n, int64_t 
     API_END
 }
 
+int32_t sp_cuda_upload_weight_fp8(int32_t device, int64_t n, int64_t k, const void* values, const float* scales, SpWeight** out) {
+    API_BEGIN
+    if (!values || !scales || !out) { set_error("null argument"); return SP_ERR_ARG; }
+    if (n <= 0 || n > INT32_MAX / 2) { set_error("bad shape"); return SP_ERR_SHAPE; }
+    const int st = check_fp8_dim(n, k, "k");
+    if (st != SP_OK) return st;
+    SP_CUDA_TRY(cudaSetDevice(device));
+    const size_t nbytes = (size_t)n * k, scale_bytes = (size_t)(fp8_blocks(n) * fp8_blocks(k)) * 4;
+    SpWeight* w = new SpWeight{device, SP_F8_E4M3, n, k, nullptr, nbytes};
+    cudaError_t ce = cudaMalloc((void**)&w->d, nbytes);
+    if (ce == cudaSuccess) ce = cudaMalloc((void**)&w->scale, scale_bytes);
+    if (ce == cudaSuccess) ce = cudaMemcpy(w->d, values, nbytes, cudaMemcpyHostToDevice);
+    if (ce == cudaSuccess) ce = cudaMemcpy(w->scale, scales, scale_bytes, cudaMemcpyHostToDevice);
+    if (ce != cudaSuccess) {
+        set_error(std::string("upload_weight_fp8: ") + cudaGetErrorString(ce));
+        sp_cuda_free_weight(w);
+        return ce == cudaErrorMemoryAllocation ? SP_ERR_OOM : SP_ERR_CUDA;
+    }
+    *out = w;
+    return SP_OK;
+    API_END
+}
+
 void sp_cuda_free_weight(SpWeight* w) {
     if (!w) return;
     cudaSetDevice(w->device);
     cudaFree(w->d);
+    cudaFree(w->scale);
+    cudaFree(w->xq);
     if (w->tiled) cudaFree(w->tiled);
     w->ws.release();
     w->ring.release();
@@ -299,10 +380,35 @@ int32_t sp_cuda_dequant(const SpWeight* w, float* out_host) {
     SP_CUDA_TRY(cudaSetDevice(w->device));
     DevBuf o;
     SP_CUDA_TRY(o.alloc((size_t)(w->n * w->k) * 4));
-    SP_CUDA_TRY(launch_dequant(w->dtype, w->d, w->n, w->k, o.as<float>(), 0));
+    if (w->dtype == SP_F8_E4M3) SP_CUDA_TRY(launch_fp8_dequant(w->d, w->scale, w->n, w->k, o.as<float>(), 0));
+    else SP_CUDA_TRY(launch_dequant(w->dtype, w->d, w->n, w->k, o.as<float>(), 0));
     SP_CUDA_TRY(cudaMemcpy(out_host, o.p, (size_t)(w->n * w->k) * 4, cudaMemcpyDeviceToHost));
     return SP_OK;
     API_END
+}
+
+// x as fp8 rows in the weight's workspace, then the product.
+static int matmul_nt_fp8(SpWeight* w, const float* x, int64_t m, float* y, cudaStream_t st) {
+    if (m > INT32_MAX / 2) { set_error("bad shape"); return SP_ERR_SHAPE; }
+    if (m == 0) return SP_OK;
+    const size_t row = (size_t)w->k, scales = (size_t)fp8_blocks(w->k);
+    if (m > w->xq_rows) {
+        cudaStreamCaptureStatus capturing;
+        SP_CUDA_TRY(cudaStreamIsCapturing(st, &capturing));
+        if (capturing != cudaStreamCaptureStatusNone) { set_error("matmul: the first call with this many rows allocates and cannot be captured"); return SP_ERR_STATE; }
+        const int64_t rows = (m + 127) / 128 * 128;
+        uint8_t* p = nullptr;
+        SP_CUDA_TRY(cudaMalloc((void**)&p, rows * (row + 4 * scales)));
+        cudaFree(w->xq);  // (waits for the work that uses it)
+        w->xq = p;
+        w->xq_rows = rows;
+    }
+    float* const xs = reinterpret_cast<float*>(w->xq + (size_t)w->xq_rows * row);
+    int* waits = nullptr;
+    SP_CUDA_TRY(op_waits(&waits));
+    SP_CUDA_TRY(launch_fp8_quant(x, w->k, m, w->k, false, false, w->xq, xs, st));
+    SP_CUDA_TRY(launch_fp8_matmul(Fp8MatArgs{w->xq, xs, w->d, w->scale, y, w->n, (int)m, (int)w->n, (int)w->k, false, waits}, st));
+    return SP_OK;
 }
 
 int32_t sp_cuda_matmul_nt_dev(const SpWeight* w, const float* x_dev, int64_t m, float* y_dev, void* stream) {
@@ -310,6 +416,7 @@ int32_t sp_cuda_matmul_nt_dev(const SpWeight* w, const float* x_dev, int64_t m, 
     if (!w || !x_dev || !y_dev || m < 0) { set_error("null argument"); return SP_ERR_ARG; }
     if (((uintptr_t)x_dev & 15) != 0) { set_error("x must be 16-byte aligned"); return SP_ERR_ARG; }
     SP_CUDA_TRY(cudaSetDevice(w->device));
+    if (w->dtype == SP_F8_E4M3) return matmul_nt_fp8(const_cast<SpWeight*>(w), x_dev, m, y_dev, (cudaStream_t)stream);
     if (w->tiled && g_gemv_path.load() == 0 && g_tc5.load() && m >= TC5_MIN_M && tc5_supported(w->dtype, w->k)) {
         SpWeight* wm = const_cast<SpWeight*>(w);
         const bool exact = g_tc5.load() == 2;
@@ -546,6 +653,7 @@ int32_t sp_cuda_mul(int32_t device, const float* a, const float* b, int64_t n, f
 int32_t sp_cuda_embed(const SpWeight* table, const uint32_t* ids, int64_t n, float* out_host) {
     API_BEGIN
     if (!table || !ids || !out_host || n < 0) { set_error("null argument"); return SP_ERR_ARG; }
+    if (table->dtype == SP_F8_E4M3) { set_error("embed: no table of fp8 weights"); return SP_ERR_DTYPE; }
     for (int64_t i = 0; i < n; ++i)
         if ((int64_t)ids[i] >= table->n) { set_error("token id " + std::to_string(ids[i]) + " out of vocab range"); return SP_ERR_VOCAB; }
     SP_CUDA_TRY(cudaSetDevice(table->device));
@@ -569,6 +677,211 @@ int32_t sp_cuda_argmax(int32_t device, const float* logits, int64_t rows, int64_
     SP_CUDA_TRY(cudaMemcpy(dl.p, logits, (size_t)(rows * n) * 4, cudaMemcpyHostToDevice));
     SP_CUDA_TRY(launch_argmax(dl.as<float>(), (int)rows, (int)n, (int)n, dout.as<uint32_t>(), 0));
     SP_CUDA_TRY(cudaMemcpy(out, dout.p, (size_t)rows * 4, cudaMemcpyDeviceToHost));
+    return SP_OK;
+    API_END
+}
+
+// ── 8-bit floating-point rows and weights ──
+int32_t sp_cuda_rms_norm_fp8_dev(int32_t device, int32_t dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, void* sum_out,
+                                 int64_t lds, const float* w, float eps, int64_t rows, int64_t dim, void* q, float* scale, void* stream) {
+    API_BEGIN
+    if (!x || !q || !scale) { set_error("null argument"); return SP_ERR_ARG; }
+    int st = check_fp8_type(dtype);
+    if (st == SP_OK) st = check_fp8_dim(rows, dim, "dim");
+    if (st != SP_OK) return st;
+    if (dim > FP8_NORM_MAX_DIM) { set_error("rms_norm_fp8: dim must be at most 32768"); return SP_ERR_SHAPE; }
+    st = check_fp8_rows("x", x, ldx, dim, dtype);
+    if (st == SP_OK && residual) st = check_fp8_rows("residual", residual, ldr, dim, dtype);
+    if (st == SP_OK && sum_out) st = check_fp8_rows("sum_out", sum_out, lds, dim, dtype);
+    if (st != SP_OK) return st;
+    if ((sum_out == x && sum_out && lds != ldx) || (sum_out == residual && sum_out && lds != ldr)) { set_error("rms_norm_fp8: sum_out in place has another row stride"); return SP_ERR_ARG; }
+    if (unaligned(w, 16) || unaligned(q, 16) || unaligned(scale, 4)) { set_error("w and q must be 16-byte aligned"); return SP_ERR_ARG; }
+    if (rows == 0) return SP_OK;
+    OnDevice on;
+    SP_CUDA_TRY(on.enter(device));
+    SP_CUDA_TRY(launch_fp8_norm(Fp8NormArgs{x, residual, sum_out, w, ldx, ldr, lds, rows, (int)dim, eps, static_cast<uint8_t*>(q), scale}, dtype == SP_BF16,
+                                (cudaStream_t)stream));
+    return SP_OK;
+    API_END
+}
+
+static int quant_fp8_dev(int32_t device, int32_t dtype, const void* x, int64_t ldx, int64_t rows, int64_t dim, bool gated, void* q, float* scale,
+                         void* stream) {
+    if (!x || !q || !scale) { set_error("null argument"); return SP_ERR_ARG; }
+    int st = check_fp8_type(dtype);
+    if (st == SP_OK) st = check_fp8_dim(rows, dim, gated ? "ffn" : "dim");
+    if (st == SP_OK) st = check_fp8_rows(gated ? "gu" : "x", x, ldx, gated ? 2 * dim : dim, dtype);
+    if (st != SP_OK) return st;
+    if (unaligned(q, 16) || unaligned(scale, 4)) { set_error("q must be 16-byte aligned"); return SP_ERR_ARG; }
+    if (rows == 0) return SP_OK;
+    OnDevice on;
+    SP_CUDA_TRY(on.enter(device));
+    SP_CUDA_TRY(launch_fp8_quant(x, ldx, rows, dim, gated, dtype == SP_BF16, static_cast<uint8_t*>(q), scale, (cudaStream_t)stream));
+    return SP_OK;
+}
+
+int32_t sp_cuda_swiglu_fp8_dev(int32_t device, int32_t dtype, const void* gu, int64_t ld, int64_t rows, int64_t ffn, void* q, float* scale,
+                               void* stream) {
+    API_BEGIN
+    return quant_fp8_dev(device, dtype, gu, ld, rows, ffn, true, q, scale, stream);
+    API_END
+}
+
+int32_t sp_cuda_quant_fp8_dev(int32_t device, int32_t dtype, const void* x, int64_t ldx, int64_t rows, int64_t dim, void* q, float* scale, void* stream) {
+    API_BEGIN
+    return quant_fp8_dev(device, dtype, x, ldx, rows, dim, false, q, scale, stream);
+    API_END
+}
+
+int32_t sp_cuda_matmul_fp8_dev(int32_t device, const void* xq, const float* xs, int64_t m, const void* wq, const float* ws, int64_t n, int64_t k, void* y,
+                               int32_t dtype, int64_t ldy, void* stream) {
+    API_BEGIN
+    if (!xq || !xs || !wq || !ws || !y) { set_error("null argument"); return SP_ERR_ARG; }
+    int st = check_fp8_type(dtype);
+    if (st == SP_OK) st = check_fp8_dim(m, k, "k");
+    if (st != SP_OK) return st;
+    if (m > INT32_MAX / 2 || n < 0 || n > INT32_MAX / 2 || ldy < n) { set_error("matmul_fp8: bad shape"); return SP_ERR_SHAPE; }
+    if (unaligned(xq, 16) || unaligned(wq, 16)) { set_error("xq and wq must be 16-byte aligned"); return SP_ERR_ARG; }
+    if (unaligned(xs, 4) || unaligned(ws, 4) || unaligned(y, dtype == SP_F32 ? 4 : 2)) { set_error("misaligned argument"); return SP_ERR_ARG; }
+    if (m == 0 || n == 0) return SP_OK;
+    OnDevice on;
+    SP_CUDA_TRY(on.enter(device));
+    int* waits = nullptr;
+    SP_CUDA_TRY(op_waits(&waits));
+    SP_CUDA_TRY(launch_fp8_matmul(Fp8MatArgs{static_cast<const uint8_t*>(xq), xs, static_cast<const uint8_t*>(wq), ws, y, ldy, (int)m, (int)n, (int)k,
+                                             dtype == SP_BF16, waits}, (cudaStream_t)stream));
+    return SP_OK;
+    API_END
+}
+
+int32_t sp_cuda_logprobs_dev(int32_t device, int32_t dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const uint32_t* ids, int32_t top,
+                             float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs, void* stream) {
+    API_BEGIN
+    if (!logits || (logprob && !ids)) { set_error("null argument"); return SP_ERR_ARG; }
+    if (dtype != SP_F32 && dtype != SP_BF16) { set_error("logprobs: logits are SP_F32 or SP_BF16"); return SP_ERR_DTYPE; }
+    const int st = check_logprobs(rows, vocab, top);
+    if (st != SP_OK) return st;
+    if (ld < vocab) { set_error("logprobs: the row stride must hold a row"); return SP_ERR_SHAPE; }
+    if (unaligned(logits, dtype == SP_F32 ? 4 : 2)) { set_error("misaligned argument"); return SP_ERR_ARG; }
+    if (rows == 0) return SP_OK;
+    OnDevice on;
+    SP_CUDA_TRY(on.enter(device));
+    if (!top_ids && !top_logprobs) top = 0;
+    SP_CUDA_TRY(launch_logprobs(LogprobsArgs{logits, ld, rows, (int)vocab, top, ids, logprob, entropy, top_ids, top_logprobs}, dtype == SP_BF16,
+                                (cudaStream_t)stream));
+    return SP_OK;
+    API_END
+}
+
+// Host buffers: what goes in, the call, what comes out.
+static int to_device(DevBuf& b, const void* p, size_t n) {
+    SP_CUDA_TRY(b.alloc(n));
+    SP_CUDA_TRY(cudaMemcpy(b.p, p, n, cudaMemcpyHostToDevice));
+    return SP_OK;
+}
+static int from_device(void* p, const DevBuf& b, size_t n) {
+    SP_CUDA_TRY(cudaMemcpy(p, b.p, n, cudaMemcpyDeviceToHost));
+    return SP_OK;
+}
+#define SP_STEP(expr)                       \
+    do {                                    \
+        const int step_status = (expr);     \
+        if (step_status != SP_OK) return step_status; \
+    } while (0)
+
+int32_t sp_cuda_rms_norm_fp8(int32_t device, const float* x, const float* residual, const float* w, int64_t rows, int64_t dim, float eps, void* q,
+                             float* scale, float* sum_out) {
+    API_BEGIN
+    if (!x || !q || !scale) { set_error("null argument"); return SP_ERR_ARG; }
+    SP_STEP(check_fp8_dim(rows, dim, "dim"));
+    if (rows == 0) return SP_OK;
+    SP_CUDA_TRY(cudaSetDevice(device));
+    const size_t values = (size_t)(rows * dim), scales = (size_t)(rows * fp8_blocks(dim));
+    DevBuf dx, dr, dw, dq, ds;
+    SP_STEP(to_device(dx, x, values * 4));
+    if (residual) SP_STEP(to_device(dr, residual, values * 4));
+    if (w) SP_STEP(to_device(dw, w, (size_t)dim * 4));
+    SP_CUDA_TRY(dq.alloc(values));
+    SP_CUDA_TRY(ds.alloc(scales * 4));
+    SP_STEP(sp_cuda_rms_norm_fp8_dev(device, SP_F32, dx.p, dim, dr.p, dim, sum_out ? dx.p : nullptr, dim, dw.as<float>(), eps, rows, dim, dq.p, ds.as<float>(),
+                                     nullptr));
+    SP_STEP(from_device(q, dq, values));
+    SP_STEP(from_device(scale, ds, scales * 4));
+    if (sum_out) SP_STEP(from_device(sum_out, dx, values * 4));
+    return SP_OK;
+    API_END
+}
+
+static int quant_fp8_host(int32_t device, const float* x, int64_t rows, int64_t dim, bool gated, void* q, float* scale) {
+    if (!x || !q || !scale) { set_error("null argument"); return SP_ERR_ARG; }
+    SP_STEP(check_fp8_dim(rows, dim, gated ? "ffn" : "dim"));
+    if (rows == 0) return SP_OK;
+    SP_CUDA_TRY(cudaSetDevice(device));
+    const size_t values = (size_t)(rows * dim), scales = (size_t)(rows * fp8_blocks(dim));
+    DevBuf dx, dq, ds;
+    SP_STEP(to_device(dx, x, values * (gated ? 8 : 4)));
+    SP_CUDA_TRY(dq.alloc(values));
+    SP_CUDA_TRY(ds.alloc(scales * 4));
+    SP_STEP(quant_fp8_dev(device, SP_F32, dx.p, gated ? 2 * dim : dim, rows, dim, gated, dq.p, ds.as<float>(), nullptr));
+    SP_STEP(from_device(q, dq, values));
+    return from_device(scale, ds, scales * 4);
+}
+
+int32_t sp_cuda_swiglu_fp8(int32_t device, const float* gu, int64_t rows, int64_t ffn, void* q, float* scale) {
+    API_BEGIN
+    return quant_fp8_host(device, gu, rows, ffn, true, q, scale);
+    API_END
+}
+
+int32_t sp_cuda_quant_fp8(int32_t device, const float* x, int64_t rows, int64_t dim, void* q, float* scale) {
+    API_BEGIN
+    return quant_fp8_host(device, x, rows, dim, false, q, scale);
+    API_END
+}
+
+int32_t sp_cuda_matmul_fp8(int32_t device, const void* xq, const float* xs, int64_t m, const void* wq, const float* ws, int64_t n, int64_t k, float* y) {
+    API_BEGIN
+    if (!xq || !xs || !wq || !ws || !y) { set_error("null argument"); return SP_ERR_ARG; }
+    SP_STEP(check_fp8_dim(m, k, "k"));
+    if (n < 0) { set_error("matmul_fp8: bad shape"); return SP_ERR_SHAPE; }
+    if (m == 0 || n == 0) return SP_OK;
+    SP_CUDA_TRY(cudaSetDevice(device));
+    const int64_t nb = fp8_blocks(k);
+    DevBuf dxq, dxs, dwq, dws, dy;
+    SP_STEP(to_device(dxq, xq, (size_t)(m * k)));
+    SP_STEP(to_device(dxs, xs, (size_t)(m * nb) * 4));
+    SP_STEP(to_device(dwq, wq, (size_t)(n * k)));
+    SP_STEP(to_device(dws, ws, (size_t)(fp8_blocks(n) * nb) * 4));
+    SP_CUDA_TRY(dy.alloc((size_t)(m * n) * 4));
+    SP_STEP(sp_cuda_matmul_fp8_dev(device, dxq.p, dxs.as<float>(), m, dwq.p, dws.as<float>(), n, k, dy.p, SP_F32, n, nullptr));
+    SP_STEP(from_device(y, dy, (size_t)(m * n) * 4));
+    return check_kernel_flags();
+    API_END
+}
+
+int32_t sp_cuda_logprobs(int32_t device, const float* logits, int64_t rows, int64_t vocab, const uint32_t* ids, int32_t top, float* logprob, float* entropy,
+                         uint32_t* top_ids, float* top_logprobs) {
+    API_BEGIN
+    if (!logits || (logprob && !ids)) { set_error("null argument"); return SP_ERR_ARG; }
+    SP_STEP(check_logprobs(rows, vocab, top));
+    for (int64_t i = 0; ids && i < rows; ++i)
+        if ((int64_t)ids[i] >= vocab) { set_error("token id " + std::to_string(ids[i]) + " out of vocab range"); return SP_ERR_VOCAB; }
+    if (rows == 0) return SP_OK;
+    SP_CUDA_TRY(cudaSetDevice(device));
+    const size_t r = (size_t)rows * 4, t = r * top;
+    DevBuf dz, di, dl, de, dti, dtl;
+    SP_STEP(to_device(dz, logits, r * vocab));
+    if (ids) SP_STEP(to_device(di, ids, r));
+    SP_CUDA_TRY(dl.alloc(r));
+    SP_CUDA_TRY(de.alloc(r));
+    SP_CUDA_TRY(dti.alloc(t));
+    SP_CUDA_TRY(dtl.alloc(t));
+    SP_STEP(sp_cuda_logprobs_dev(device, SP_F32, dz.p, vocab, rows, vocab, di.as<uint32_t>(), top, ids ? dl.as<float>() : nullptr, de.as<float>(),
+                                 dti.as<uint32_t>(), dtl.as<float>(), nullptr));
+    if (logprob) SP_STEP(from_device(logprob, dl, r));
+    if (entropy) SP_STEP(from_device(entropy, de, r));
+    if (top_ids) SP_STEP(from_device(top_ids, dti, t));
+    if (top_logprobs) SP_STEP(from_device(top_logprobs, dtl, t));
     return SP_OK;
     API_END
 }

@@ -895,7 +895,8 @@ void WaitFlags::release() {
 const char* WaitFlags::take() {
     static const char* const what[WAIT_KINDS] = {"tcgen05 GEMM: a bounded mbarrier wait expired, the outputs of that launch are not valid",
                                                  "tcgen05 GEMM on bf16 weights: a bounded mbarrier wait expired, the outputs of that launch are not valid",
-                                                 "streaming GEMV: a bounded mbarrier wait expired, the outputs of that launch are not valid"};
+                                                 "streaming GEMV: a bounded mbarrier wait expired, the outputs of that launch are not valid",
+                                                 "product on fp8 weights: a bounded mbarrier wait expired, the outputs of that launch are not valid"};
     const char* said = nullptr;
     int* const h = host;
     for (int i = 0; h && i < WAIT_KINDS; ++i)

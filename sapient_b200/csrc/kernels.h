@@ -66,7 +66,7 @@ int imma_rows_per_pass();
 // A device-side wait that runs out is reported to flags in mapped host memory, a kernel's plain store; whoever owns the launch (an
 // engine; for op-level calls the device) owns the flags, and its launches carry their device address. Looking costs no CUDA call, so
 // it is done after every synchronisation: a mark of what has been launched would miss the replays of a captured step.
-enum WaitKind : int { WAIT_GEMM = 0, WAIT_MAT, WAIT_GEMV, WAIT_KINDS };
+enum WaitKind : int { WAIT_GEMM = 0, WAIT_MAT, WAIT_GEMV, WAIT_FP8, WAIT_KINDS };
 struct WaitFlags {
     std::atomic<int*> host{nullptr};
     int* dev = nullptr;

@@ -13,10 +13,17 @@ from . import _lib
 from ._lib import SapientCudaError, check, lib
 
 F32, F16, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, BF16 = 0, 1, 2, 8, 12, 13, 14, 30
+F8_E4M3 = 128      # Weight.from_fp8
+FP8_BLOCK = 128    # columns of an fp8 row, rows and columns of an fp8 weight, that share a scale
+LOGPROBS_MAX_TOP = 32
 
 
 def _p(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
+
+
+def _blocks(k: int) -> int:
+    return -(-k // FP8_BLOCK)
 
 
 def _f32(a) -> np.ndarray:
@@ -31,6 +38,19 @@ class Weight:
         h = C.c_void_p()
         check(lib().sp_cuda_upload_weight(device, dtype, n, k, _p(raw), raw.size, C.byref(h)))
         self.h, self.dtype, self.n, self.k, self.device, self.nbytes = h, dtype, n, k, device, raw.size
+
+    @classmethod
+    def from_fp8(cls, values, scales, device: int = 0) -> "Weight":
+        """An [n, k] matrix of e4m3 values (uint8: their bits) with an f32 scale for every 128 x 128 block. matmul_nt quantises the
+        rows of x likewise, a scale for every 128 columns."""
+        v, s = np.ascontiguousarray(values, dtype=np.uint8), _f32(scales)
+        if v.ndim != 2 or s.shape != (_blocks(v.shape[0]), _blocks(v.shape[1])):
+            raise SapientCudaError(_lib.SP_ERR_SHAPE, "fp8 weight: values [n, k] and scales [ceil(n / 128), ceil(k / 128)] expected")
+        h = C.c_void_p()
+        check(lib().sp_cuda_upload_weight_fp8(device, *v.shape, _p(v), _p(s), C.byref(h)))
+        w = cls.__new__(cls)
+        w.h, w.dtype, (w.n, w.k), w.device, w.nbytes = h, F8_E4M3, v.shape, device, v.size
+        return w
 
     def dequant(self) -> np.ndarray:
         """Tensor::to_f32_vec — bit-exact f32 values, shape [n, k]."""
@@ -160,6 +180,101 @@ def argmax(logits, device: int = 0) -> np.ndarray:
     out = np.empty(x2.shape[0], np.uint32)
     check(lib().sp_cuda_argmax(device, _p(x2), x2.shape[0], x2.shape[1], _p(out)))
     return out
+
+
+# ── 8-bit floating-point rows and token distributions (no counterpart in the reference; formats in include/sapient_cuda.h) ──
+def _rows2(x, what: str) -> np.ndarray:
+    x = _f32(x)
+    if x.ndim != 2:
+        raise SapientCudaError(_lib.SP_ERR_SHAPE, f"{what} expects 2-D arrays")
+    return x
+
+
+def _fp8_out(rows: int, dim: int):
+    return np.empty((rows, dim), np.uint8), np.empty((rows, _blocks(dim)), np.float32)
+
+
+def rms_norm_fp8(x, w, eps: float, residual=None, device: int = 0):
+    """RMS norm of h = x + residual as fp8 rows: (q [rows, dim] uint8, scale [rows, ceil(dim / 128)], h)."""
+    x = _rows2(x, "rms_norm_fp8")
+    r, wv = None if residual is None else _f32(residual), None if w is None else _f32(w)
+    if (r is not None and r.shape != x.shape) or (wv is not None and wv.shape != x.shape[1:]):
+        raise SapientCudaError(_lib.SP_ERR_SHAPE, "rms_norm_fp8: residual like x and w [dim] expected")
+    (q, s), h = _fp8_out(*x.shape), np.empty_like(x)
+    check(lib().sp_cuda_rms_norm_fp8(device, _p(x), None if r is None else _p(r), None if wv is None else _p(wv), *x.shape, eps, _p(q), _p(s), _p(h)))
+    return q, s, h
+
+
+def swiglu_fp8(gu, device: int = 0):
+    """silu(gate) * up of rows gate | up as fp8 rows: (q, scale)."""
+    gu = _rows2(gu, "swiglu_fp8")
+    if gu.shape[1] % 2:
+        raise SapientCudaError(_lib.SP_ERR_SHAPE, "swiglu_fp8: gate and up side by side expected")
+    q, s = _fp8_out(gu.shape[0], gu.shape[1] // 2)
+    check(lib().sp_cuda_swiglu_fp8(device, _p(gu), *q.shape, _p(q), _p(s)))
+    return q, s
+
+
+def quant_fp8(x, device: int = 0):
+    """x as fp8 rows: (q, scale)."""
+    x = _rows2(x, "quant_fp8")
+    q, s = _fp8_out(*x.shape)
+    check(lib().sp_cuda_quant_fp8(device, _p(x), *x.shape, _p(q), _p(s)))
+    return q, s
+
+
+def matmul_fp8(xq, xs, wq, ws, device: int = 0) -> np.ndarray:
+    """Y[m, n] = X Wᵀ of fp8 rows (xq [m, k] uint8, xs [m, ceil(k / 128)]) and fp8 weights (wq [n, k], ws for 128 x 128 blocks)."""
+    xq, wq = np.ascontiguousarray(xq, dtype=np.uint8), np.ascontiguousarray(wq, dtype=np.uint8)
+    xs, ws = _f32(xs), _f32(ws)
+    if xq.ndim != 2 or wq.ndim != 2 or xq.shape[1] != wq.shape[1]:
+        raise SapientCudaError(_lib.SP_ERR_SHAPE, "matmul_fp8 expects xq [m, k] and wq [n, k]")
+    (m, k), n = xq.shape, wq.shape[0]
+    if xs.shape != (m, _blocks(k)) or ws.shape != (_blocks(n), _blocks(k)):
+        raise SapientCudaError(_lib.SP_ERR_SHAPE, "matmul_fp8: a scale for every 128 columns of a row and 128 x 128 block of the weights expected")
+    y = np.empty((m, n), np.float32)
+    check(lib().sp_cuda_matmul_fp8(device, _p(xq), _p(xs), m, _p(wq), _p(ws), n, k, _p(y)))
+    return y
+
+
+def logprobs(logits, ids, top: int = 0, device: int = 0):
+    """(log probability of ids[row], entropy, top_ids [rows, top], top_logprobs [rows, top]) of rows of logits; among equal logits the
+    lowest id comes first. ids may be None, the first of the four is then, too."""
+    z = _rows2(logits, "logprobs")
+    rows = z.shape[0]
+    i = None if ids is None else np.ascontiguousarray(ids, dtype=np.uint32).reshape(-1)
+    if i is not None and i.size != rows:
+        raise SapientCudaError(_lib.SP_ERR_SHAPE, "logprobs: one id per row expected")
+    if not 0 <= top <= LOGPROBS_MAX_TOP:
+        raise SapientCudaError(_lib.SP_ERR_ARG, "logprobs: top must be 0 to 32 and at most the vocabulary")
+    lp, ent = np.empty(rows, np.float32), np.empty(rows, np.float32)
+    ti, tl = np.empty((rows, top), np.uint32), np.empty((rows, top), np.float32)
+    check(lib().sp_cuda_logprobs(device, _p(z), *z.shape, None if i is None else _p(i), top, None if i is None else _p(lp), _p(ent), _p(ti), _p(tl)))
+    return None if i is None else lp, ent, ti, tl
+
+
+# The same on device pointers (integers; 0: not given), without copies or synchronisation. dtype: F32 or BF16. Row strides in values, 0: dense.
+def rms_norm_fp8_dev(x: int, rows: int, dim: int, w: int, eps: float, q: int, scale: int, dtype: int = F32, residual: int = 0, sum_out: int = 0,
+                     ldx: int = 0, ldr: int = 0, lds: int = 0, device: int = 0, stream: int = 0) -> None:
+    check(lib().sp_cuda_rms_norm_fp8_dev(device, dtype, x, ldx or dim, residual, ldr or dim, sum_out, lds or dim, w, eps, rows, dim, q, scale, stream))
+
+
+def swiglu_fp8_dev(gu: int, rows: int, ffn: int, q: int, scale: int, dtype: int = F32, ld: int = 0, device: int = 0, stream: int = 0) -> None:
+    check(lib().sp_cuda_swiglu_fp8_dev(device, dtype, gu, ld or 2 * ffn, rows, ffn, q, scale, stream))
+
+
+def quant_fp8_dev(x: int, rows: int, dim: int, q: int, scale: int, dtype: int = F32, ldx: int = 0, device: int = 0, stream: int = 0) -> None:
+    check(lib().sp_cuda_quant_fp8_dev(device, dtype, x, ldx or dim, rows, dim, q, scale, stream))
+
+
+def matmul_fp8_dev(xq: int, xs: int, m: int, wq: int, ws: int, n: int, k: int, y: int, dtype: int = F32, ldy: int = 0, device: int = 0,
+                   stream: int = 0) -> None:
+    check(lib().sp_cuda_matmul_fp8_dev(device, xq, xs, m, wq, ws, n, k, y, dtype, ldy or n, stream))
+
+
+def logprobs_dev(logits: int, rows: int, vocab: int, ids: int, logprob: int, entropy: int, top: int = 0, top_ids: int = 0, top_logprobs: int = 0,
+                 dtype: int = F32, ld: int = 0, device: int = 0, stream: int = 0) -> None:
+    check(lib().sp_cuda_logprobs_dev(device, dtype, logits, ld or vocab, rows, vocab, ids, top, logprob, entropy, top_ids, top_logprobs, stream))
 
 
 def set_gemv_path(path: int) -> None:
