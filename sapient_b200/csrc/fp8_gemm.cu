@@ -5,8 +5,11 @@
 #include <algorithm>
 
 #include "fp8.h"
+#include "kernels.h"
 #include "pdl.cuh"
+#include "plan_common.cuh"
 #include "sp_common.cuh"
+#include "tc5_ptx.cuh"
 
 namespace sp {
 
@@ -16,52 +19,231 @@ __device__ __forceinline__ float e4m3_value(uint8_t b) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
 }
 
-constexpr int FG_TILE = 64, FG_K = 32;
+__device__ __forceinline__ void bar_init(uint64_t* bar, uint32_t arrivals) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(tc5_smem_u32(bar)), "r"(arrivals) : "memory");
+}
 
-// A 64 x 64 tile, 4 x 4 values a thread.
-__global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8MatArgs a) {
-    __shared__ float xt[FG_K][FG_TILE + 1], wt[FG_K][FG_TILE + 1];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int m0 = blockIdx.y * FG_TILE, n0 = blockIdx.x * FG_TILE;
-    const int nb = (a.k + FP8_BLOCK - 1) / FP8_BLOCK;
+// e4m3 x e4m3 -> f32, both operands K-major.
+__host__ __device__ constexpr uint32_t fp8_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+__device__ __forceinline__ void fp8_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void store(const Fp8MatArgs& p, int m, int n, float f) {
+    if (p.bf) static_cast<bf16*>(p.y)[(int64_t)m * p.ldy + n] = __float2bfloat16_rn(f);
+    else static_cast<float*>(p.y)[(int64_t)m * p.ldy + n] = f;
+}
+
+// ── Few rows: a stream of weights ──
+constexpr int FS_BM = 128;                     // weight rows of a tile
+constexpr int FS_THREADS = 192;                // MMA warp, TMA warp, four drain warps
+constexpr int FS_W_BYTES = FS_BM * FP8_BLOCK;  // of a stage
+constexpr int FS_SMEM = 108 * 1024;            // per block, two of which share an SM
+constexpr int FS_MAX_STAGES = 6, FS_MAX_PARTS = 8;
+
+struct Fp8StreamArgs {
+    Fp8MatArgs p;
+    int parts, stages;
+};
+
+// BN: activation rows of a tile.
+template <int BN>
+__global__ void __launch_bounds__(FS_THREADS, 2) fp8_stream_kernel(const Fp8StreamArgs a, const __grid_constant__ CUtensorMap map_w,
+                                                               const __grid_constant__ CUtensorMap map_x) {
+    constexpr int BUFS = BN >= 128 ? 2 : 4, COLS = BUFS * BN, STAGE = FS_W_BYTES + BN * FP8_BLOCK;
+    extern __shared__ uint8_t fs_smem_raw[];
+    __shared__ __align__(8) uint64_t full[FS_MAX_STAGES], empty[FS_MAX_STAGES], sum_full[BUFS], sum_empty[BUFS];
+    __shared__ __align__(16) float scales[2][BN];
+    __shared__ uint32_t tmem_slot;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
+    const Fp8MatArgs& p = a.p;
+    const int n0 = blockIdx.x * FS_BM, r0 = blockIdx.y * BN, rows = min(BN, p.m - r0);
+    const int blocks = (p.k + FP8_BLOCK - 1) / FP8_BLOCK, part = blockIdx.z;
+    const int b0 = (int)((int64_t)part * blocks / a.parts), count = (int)((int64_t)(part + 1) * blocks / a.parts) - b0;
+    uint8_t* const smem = fs_smem_raw + ((1024u - (tc5_smem_u32(fs_smem_raw) & 1023u)) & 1023u);
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5_smem_u32(&tmem_slot)), "n"(COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    if (tid == 32) {
+        tc5_prefetch_map(&map_w);
+        tc5_prefetch_map(&map_x);
+        for (int i = 0; i < a.stages; ++i) {
+            bar_init(&full[i], 1);
+            bar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < BUFS; ++i) {
+            bar_init(&sum_full[i], 1);
+            bar_init(&sum_empty[i], 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    const uint32_t tmem = tmem_slot;
     pdl_wait();
     pdl_trigger();
-    float acc[4][4] = {};
-    for (int b = 0; b < nb; ++b) {
-        float part[4][4] = {};
-        for (int k0 = b * FP8_BLOCK; k0 < min(a.k, (b + 1) * FP8_BLOCK); k0 += FG_K) {
-            for (int i = tid; i < FG_TILE * FG_K; i += 256) {
-                const int row = i / FG_K, col = i % FG_K, k = k0 + col;
-                xt[col][row] = m0 + row < a.m && k < a.k ? e4m3_value(a.xq[(int64_t)(m0 + row) * a.k + k]) : 0.f;
-                wt[col][row] = n0 + row < a.n && k < a.k ? e4m3_value(a.wq[(int64_t)(n0 + row) * a.k + k]) : 0.f;
+    bool ok = true;
+    float* const partial = reinterpret_cast<float*>(smem);  // [BN][128], once the ring has drained
+    if (warp == 0) {
+        const bool leader = tc5_elect();
+        const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+        const uint32_t idesc = fp8_idesc(FS_BM, BN);
+        const uint64_t ad0 = tc5_desc(tc5_smem_u32(smem));
+        for (int c = 0, st = 0, u = 0; c < count; ++c) {
+            const int buf = c % BUFS, turn = c / BUFS;
+            if (turn > 0) ok = tc5_wait(&sum_empty[buf], (uint32_t)((turn - 1) & 1));
+            ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&full[st], (uint32_t)(u & 1)));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const uint64_t ad = ad0 + (uint64_t)((uint32_t)(st * STAGE) >> 4), bd = ad + (FS_W_BYTES >> 4);
+            if (leader) {
+#pragma unroll
+                for (int i = 0; i < FP8_BLOCK / 32; ++i) fp8_mma(tm + (uint32_t)(buf * BN), ad + 2u * i, bd + 2u * i, idesc, i > 0);
+                tc5_commit(&empty[st]);
+                tc5_commit(&sum_full[buf]);
             }
-            __syncthreads();
-            for (int k = 0; k < FG_K; ++k)
-                for (int i = 0; i < 4; ++i)
-                    for (int j = 0; j < 4; ++j) part[i][j] = fmaf(xt[k][ty + 16 * i], wt[k][tx + 16 * j], part[i][j]);
-            __syncthreads();
+            __syncwarp();
+            if (++st == a.stages) { st = 0; ++u; }
         }
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-                if (m < a.m && n < a.n) acc[i][j] = fmaf(part[i][j], a.xs[(int64_t)m * nb + b] * a.ws[(int64_t)(n / FP8_BLOCK) * nb + b], acc[i][j]);
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int issued = 0;
+            for (int c = 0, st = 0, u = 0; c < count; ++c, ++st) {
+                if (st == a.stages) { st = 0; ++u; }
+                if (u > 0) ok = tc5_wait(&empty[st], (uint32_t)((u - 1) & 1));
+                if (!ok) break;
+                const uint32_t bar = tc5_smem_u32(&full[st]), dst = tc5_smem_u32(smem + st * STAGE);
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(STAGE) : "memory");
+                tc5_tma_2d(dst, &map_w, (b0 + c) * FP8_BLOCK, n0, bar);
+                tc5_tma_2d(dst + FS_W_BYTES, &map_x, (b0 + c) * FP8_BLOCK, r0, bar);
+                issued = c + 1;
             }
+            if (!ok)  // nothing of this block's is in flight when it leaves
+                for (int c = max(0, issued - a.stages); c < issued; ++c) tc5_wait(&full[c % a.stages], (uint32_t)((c / a.stages) & 1));
+        }
+        __syncwarp();
+    } else {
+        const int q4 = warp & 3, n = n0 + 32 * q4 + lane, t = tid - 64;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * q4) << 16);
+        // the thread whose number is an activation row's brings that row's scale times the weights', a block ahead of its use
+        const bool brings = t < BN && t < rows;
+        const float* const xs = p.xs + (int64_t)(r0 + (brings ? t : 0)) * blocks + b0;
+        const float* const ws = p.ws + (int64_t)(n0 / FP8_BLOCK) * blocks + b0;
+        float acc[BN];
+#pragma unroll
+        for (int j = 0; j < BN; ++j) acc[j] = 0.f;
+        float xv = brings && count > 0 ? xs[0] : 0.f, wv = count > 0 ? ws[0] : 0.f;
+        for (int c = 0; c < count; ++c) {
+            const int buf = c % BUFS;
+            if (t < BN) scales[c & 1][t] = xv * wv;
+            if (c + 1 < count) {
+                if (brings) xv = xs[c + 1];
+                wv = ws[c + 1];
+            }
+            ok = __all_sync(0xFFFFFFFFu, tc5_wait(&sum_full[buf], (uint32_t)((c / BUFS) & 1)));
+            // (the one barrier a block of 128 columns: its scales are there, and those of the one before have been read)
+            int all_ok;
+            asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.and.pred q, 1, 128, p;\nselp.b32 %0, 1, 0, q;\n}\n" : "=r"(all_ok) : "r"((int)ok) : "memory");
+            ok = all_ok != 0;
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+#pragma unroll
+            for (int j0 = 0; j0 < BN; j0 += 16) {
+                uint32_t v[16];
+                tc5_ld16(lanes + (uint32_t)(buf * BN + j0), v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+                if (j0 + 16 == BN) {
+                    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+                    if (lane == 0) tc5_arrive(&sum_empty[buf]);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 s = *reinterpret_cast<const float4*>(&scales[c & 1][j0 + j]);
+                    acc[j0 + j] = fmaf(__uint_as_float(v[j]), s.x, acc[j0 + j]);
+                    acc[j0 + j + 1] = fmaf(__uint_as_float(v[j + 1]), s.y, acc[j0 + j + 1]);
+                    acc[j0 + j + 2] = fmaf(__uint_as_float(v[j + 2]), s.z, acc[j0 + j + 2]);
+                    acc[j0 + j + 3] = fmaf(__uint_as_float(v[j + 3]), s.w, acc[j0 + j + 3]);
+                }
+            }
+        }
+        if (a.parts == 1) {
+            if (ok && n < p.n) {
+#pragma unroll
+                for (int j = 0; j < BN; ++j)
+                    if (j < rows) store(p, r0 + j, n, acc[j]);
+            }
+        } else {
+            if (ok) {
+#pragma unroll
+                for (int j = 0; j < BN; ++j) partial[j * FS_BM + 32 * q4 + lane] = acc[j];
+            }
+            cluster_sync();
+            // the cluster's blocks share out the rows; each adds its rows' parts in order
+            const uint32_t mine = tc5_smem_u32(partial + 32 * q4 + lane);
+            for (int j = part; j < rows && n < p.n; j += a.parts) {
+                float f = 0.f;
+#pragma unroll 8
+                for (int o = 0; o < a.parts; ++o) f += ld_peer(peer_smem(mine, o) + (uint32_t)j * FS_BM * 4);
+                if (ok) store(p, r0 + j, n, f);
+            }
+        }
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-            if (m >= a.m || n >= a.n) continue;
-            if (a.bf) static_cast<__nv_bfloat16*>(a.y)[(int64_t)m * a.ldy + n] = __float2bfloat16_rn(acc[i][j]);
-            else static_cast<float*>(a.y)[(int64_t)m * a.ldy + n] = acc[i][j];
-        }
+    if (a.parts > 1) {
+        if (warp < 2) { __syncwarp(); cluster_sync(); }  // the service warps' share of the first barrier
+        cluster_sync();                                  // nobody leaves while its parts are being read
+    }
+    if (!ok) report_wait(p.waits, WAIT_FP8);
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(COLS) : "memory");
+}
+
+// [rows][k] bytes, boxes of 128 columns x box_rows, zeros past the matrix.
+static bool fp8_map(CUtensorMap* map, const uint8_t* q, int64_t k, int64_t rows, int box_rows) {
+    const PFN_encodeTiled encode = tensor_map_encoder();
+    const cuuint64_t dim[2] = {(cuuint64_t)k, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)k};
+    const cuuint32_t box[2] = {FP8_BLOCK, (cuuint32_t)box_rows}, estr[2] = {1u, 1u};
+    return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(q), dim, stride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN>
+static cudaError_t stream_of(const Fp8MatArgs& a, int parts, cudaStream_t st) {
+    CUtensorMap mw, mx;
+    if (!fp8_map(&mw, a.wq, a.k, a.n, FS_BM) || !fp8_map(&mx, a.xq, a.k, a.m, BN)) return cudaErrorInvalidValue;
+    static PerDeviceOnce once;
+    cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_stream_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, FS_SMEM + 1024); });
+    if (e != cudaSuccess) return e;
+    constexpr int STAGE = FS_W_BYTES + BN * FP8_BLOCK;
+    const Fp8StreamArgs k{a, parts, std::min(FS_MAX_STAGES, FS_SMEM / STAGE)};
+    const dim3 grid((unsigned)((a.n + FS_BM - 1) / FS_BM), (unsigned)((a.m + BN - 1) / BN), (unsigned)parts);
+    e = launch_pdl_cluster(fp8_stream_kernel<BN>, grid, dim3(FS_THREADS), (size_t)(k.stages * STAGE + 1024), st, parts, k, mw, mx);
+    return e != cudaSuccess ? e : count_launch_and_check();
 }
 
 cudaError_t launch_fp8_matmul(const Fp8MatArgs& a, cudaStream_t st) {
     if (a.m == 0 || a.n == 0) return cudaSuccess;
-    const dim3 grid((unsigned)((a.n + FG_TILE - 1) / FG_TILE), (unsigned)((a.m + FG_TILE - 1) / FG_TILE));
-    if (a.m < 0 || a.n < 0 || a.k <= 0 || a.k % 16 != 0 || grid.y > 65535) return cudaErrorInvalidValue;
-    const cudaError_t e = launch_pdl(fp8_tile_kernel, grid, dim3(256), 0, st, a);
-    return e != cudaSuccess ? e : count_launch_and_check();
+    if (a.m < 0 || a.n < 0 || a.k <= 0 || a.k % 16 != 0) return cudaErrorInvalidValue;
+    const int bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
+    const int64_t tiles = (int64_t)((a.n + FS_BM - 1) / FS_BM) * ((a.m + bn - 1) / bn);
+    if ((a.m + bn - 1) / bn > 65535) return cudaErrorInvalidValue;
+    const int blocks = (a.k + FP8_BLOCK - 1) / FP8_BLOCK, sms = device_sm_count();
+    int parts = 1;
+    while (parts < FS_MAX_PARTS && tiles * parts < sms && blocks >= 4 * parts) parts *= 2;
+    switch (bn) {
+        case 16: return stream_of<16>(a, parts, st);
+        case 32: return stream_of<32>(a, parts, st);
+        case 64: return stream_of<64>(a, parts, st);
+        default: return stream_of<128>(a, parts, st);
+    }
 }
 
 // The values of an fp8 weight, as f32.
