@@ -126,8 +126,11 @@ __global__ void __launch_bounds__(FS_THREADS, 2) fp8_stream_kernel(const Fp8Stre
                 tc5_tma_2d(dst + FS_W_BYTES, &map_x, (b0 + c) * FP8_BLOCK, r0, bar);
                 issued = c + 1;
             }
-            if (!ok)  // nothing of this block's is in flight when it leaves
-                for (int c = max(0, issued - a.stages); c < issued; ++c) tc5_wait(&full[c % a.stages], (uint32_t)((c / a.stages) & 1));
+            // nothing is in flight towards this block when it goes on to the end: copies, or the arrivals that follow the last products
+            for (int c = max(0, issued - a.stages); c < issued; ++c) {
+                uint64_t* const bars = ok ? empty : full;
+                ok = tc5_wait(&bars[c % a.stages], (uint32_t)((c / a.stages) & 1)) && ok;
+            }
         }
         __syncwarp();
     } else {
@@ -206,6 +209,257 @@ __global__ void __launch_bounds__(FS_THREADS, 2) fp8_stream_kernel(const Fp8Stre
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(COLS) : "memory");
 }
 
+// Two values a step.
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t v0, uint32_t v1, uint64_t s) {
+    asm("{\n.reg .b64 v;\nmov.b64 v, {%1, %2};\nfma.rn.f32x2 %0, v, %3, %0;\n}\n" : "+l"(acc) : "r"(v0), "r"(v1), "l"(s));
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+
+// A warp's 32 rows x 128 columns (a row a lane) to y through shared memory, 128 bytes of every row at a time, so that whole lines are
+// stored: 16-byte pieces of a row lie at piece ^ (row & 7), which keeps both directions free of bank conflicts.
+template <typename T>
+__device__ __forceinline__ void leave(const Fp8MatArgs& p, const uint64_t (&acc)[64], uint8_t* out, int r0, int n0, int lane) {
+    constexpr int PER = 16 / sizeof(T), PIECE = 8 * PER;  // values of 16 bytes, of 128
+    T* const y = static_cast<T*>(p.y);
+    const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.ldy * (int64_t)sizeof(T))) & 15) == 0;
+#pragma unroll
+    for (int c0 = 0; c0 < 128; c0 += PIECE) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint4 v;
+            uint32_t u[4];
+#pragma unroll
+            for (int j = 0; j < PER / 2; ++j) {
+                const float2 f = both(acc[(c0 + PER * i) / 2 + j]);
+                if constexpr (sizeof(T) == 4) {
+                    u[2 * j] = __float_as_uint(f.x);
+                    u[2 * j + 1] = __float_as_uint(f.y);
+                } else {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+                    u[j] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+            v = make_uint4(u[0], u[1], u[2], u[3]);
+            *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = v;
+        }
+        __syncwarp();
+        const int piece = lane & 7, n = n0 + c0 + piece * PER;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = 4 * i + (lane >> 3), m = r0 + row;
+            const uint4 v = *reinterpret_cast<const uint4*>(out + row * 128 + ((piece ^ (row & 7)) << 4));
+            if (m >= p.m) continue;
+            T* const at = y + (int64_t)m * p.ldy + n;
+            if (wide && n + PER <= p.n) {
+                *reinterpret_cast<uint4*>(at) = v;
+            } else {
+                const T* const e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                for (int j = 0; j < PER; ++j)
+                    if (n + j < p.n) at[j] = e[j];
+            }
+        }
+    }
+}
+
+// ── Many rows: two SMs share a tile ──
+// 256 activation rows (128 a block, the lanes of its tensor memory) x 256 weight rows (each block holds 128 of them in shared memory).
+constexpr int FP_BM = 256, FP_BN = 256;
+constexpr int FP_DRAINS = 8, FP_FIRST_DRAIN = 4;               // warp 0 issues products, warp 1 copies; two idle ones fill their group
+constexpr int FP_THREADS = 32 * (FP_FIRST_DRAIN + FP_DRAINS);
+constexpr int FP_STAGE = 2 * 128 * FP8_BLOCK;                  // a block's share of a stage: 128 rows of either operand
+constexpr int FP_STAGES = 6;
+constexpr int FP_OUT = 32 * 128;                                // a drain warp's piece of the result on its way out
+constexpr int FP_SMEM = FP_STAGES * FP_STAGE + FP_DRAINS * FP_OUT;
+constexpr int FP_COLS = 2 * FP_BN;
+
+__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives on the barrier at this place in both blocks once the products issued so far are done.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(tc5_smem_u32(bar)), "h"((uint16_t)3)
+                 : "memory");
+}
+__device__ __forceinline__ void pair_tma(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst), "l"(map),
+        "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+// 32 consecutive tensor-memory columns of the warp's 32 lanes.
+__device__ __forceinline__ void pair_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+        "%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+struct Fp8PairArgs {
+    Fp8MatArgs p;
+    int row_tiles, tiles;
+};
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
+    fp8_pair_kernel(const Fp8PairArgs a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+    extern __shared__ uint8_t fp_smem_raw[];
+    __shared__ __align__(8) uint64_t full[FP_STAGES], empty[FP_STAGES], sum_full[4], sum_empty[4];
+    __shared__ uint32_t tmem_slot;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
+    const Fp8MatArgs& p = a.p;
+    const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int blocks = (p.k + FP8_BLOCK - 1) / FP8_BLOCK;
+    uint8_t* const smem = fp_smem_raw + ((1024u - (tc5_smem_u32(fp_smem_raw) & 1023u)) & 1023u);
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5_smem_u32(&tmem_slot)), "n"(FP_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    if (tid == 32) {
+        tc5_prefetch_map(&map_w);
+        tc5_prefetch_map(&map_x);
+        for (int i = 0; i < FP_STAGES; ++i) {
+            bar_init(&full[i], 1);
+            bar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            bar_init(&sum_full[i], 1);
+            bar_init(&sum_empty[i], FP_DRAINS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    cluster_sync();  // both blocks' barriers are there
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    pdl_wait();
+    pdl_trigger();
+    bool ok = true;
+    if (warp < FP_FIRST_DRAIN) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");  // 128 x 56 + 256 x 224 = 384 x 168
+        if (warp == 0) {
+            if (rank == 0) {  // one block issues for both
+                const bool leader = tc5_elect();
+                const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+                const uint32_t idesc = fp8_idesc(FP_BM, FP_BN / 2);
+                const uint64_t ad0 = tc5_desc(tc5_smem_u32(smem));
+                int st = 0, u = 0, c = 0;  // stage and its turn; blocks of 128 columns so far, over all tiles
+                for (int tile = pair; ok && tile < a.tiles; tile += pairs)
+                    for (int b = 0; b < blocks; ++b, ++c) {
+                        const int buf = c & 1, turn = c >> 1;
+                        ok = __all_sync(0xFFFFFFFFu, tc5_wait(&full[st], (uint32_t)(u & 1)));
+                        const uint64_t ad = ad0 + (uint64_t)((uint32_t)(st * FP_STAGE) >> 4), bd = ad + ((128 * FP8_BLOCK) >> 4);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (turn > 0) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&sum_empty[2 * buf + h], (uint32_t)((turn - 1) & 1)));
+                            if (!ok) break;
+                            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                            if (leader) {
+#pragma unroll
+                                for (int i = 0; i < FP8_BLOCK / 32; ++i)
+                                    pair_mma(tm + (uint32_t)(buf * FP_BN + 128 * h), ad + 2u * i, bd + (uint32_t)(h * ((64 * FP8_BLOCK) >> 4)) + 2u * i, idesc, i > 0);
+                                if (h) pair_commit(&empty[st]);
+                                pair_commit(&sum_full[2 * buf + h]);
+                            }
+                        }
+                        if (!ok) break;
+                        __syncwarp();
+                        if (++st == FP_STAGES) { st = 0; ++u; }
+                    }
+            }
+        } else if (warp == 1) {
+            if (lane == 0) {
+                int st = 0, u = 0, issued = 0;
+                for (int tile = pair; ok && tile < a.tiles; tile += pairs) {
+                    const int r0 = tile % a.row_tiles * FP_BM + 128 * rank, n0 = tile / a.row_tiles * FP_BN + 64 * rank;
+                    for (int b = 0; b < blocks; ++b) {
+                        if (u > 0) ok = tc5_wait(&empty[st], (uint32_t)((u - 1) & 1));
+                        if (!ok) break;
+                        const uint32_t bar = peer_smem(tc5_smem_u32(&full[st]), 0), dst = tc5_smem_u32(smem + st * FP_STAGE);
+                        // (the other block's bytes may be there before they are expected: the phase waits for this arrival)
+                        if (rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(tc5_smem_u32(&full[st])), "r"(2 * FP_STAGE) : "memory");
+                        pair_tma(dst, &map_x, b * FP8_BLOCK, r0, bar);
+                        pair_tma(dst + 128 * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0, bar);
+                        pair_tma(dst + 192 * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0 + 128, bar);
+                        ++issued;
+                        if (++st == FP_STAGES) { st = 0; ++u; }
+                    }
+                }
+                // nothing is in flight towards this block when it goes on to the end: copies, or the arrivals that follow the last products
+                for (int c = max(0, issued - FP_STAGES); c < issued; ++c)
+                    if (ok) ok = tc5_wait(&empty[c % FP_STAGES], (uint32_t)((c / FP_STAGES) & 1));
+                    else if (rank == 0) tc5_wait(&full[c % FP_STAGES], (uint32_t)((c / FP_STAGES) & 1));
+            }
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
+        const int q4 = warp & 3, half = (warp - FP_FIRST_DRAIN) >> 2;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(128 * half);
+        uint8_t* const out = smem + FP_STAGES * FP_STAGE + (warp - FP_FIRST_DRAIN) * FP_OUT;
+        const uint32_t freed[2] = {peer_smem(tc5_smem_u32(&sum_empty[half]), 0), peer_smem(tc5_smem_u32(&sum_empty[2 + half]), 0)};
+        int c = 0;
+        for (int tile = pair; ok && tile < a.tiles; tile += pairs) {
+            const int r0 = tile % a.row_tiles * FP_BM + 128 * rank + 32 * q4, n0 = tile / a.row_tiles * FP_BN + 128 * half;
+            const float* const xs = p.xs + (int64_t)min(r0 + lane, p.m - 1) * blocks;
+            const float* const ws = p.ws + (int64_t)(min(n0, p.n - 1) / FP8_BLOCK) * blocks;
+            uint64_t acc[64];
+#pragma unroll
+            for (int j = 0; j < 64; ++j) acc[j] = 0;
+            float xv = xs[0], wv = ws[0];
+            for (int b = 0; b < blocks; ++b, ++c) {
+                const int buf = c & 1;
+                const float f = xv * wv;
+                uint64_t scale;
+                asm("mov.b64 %0, {%1, %1};" : "=l"(scale) : "f"(f));
+                if (b + 1 < blocks) { xv = xs[b + 1]; wv = ws[b + 1]; }
+                ok = __all_sync(0xFFFFFFFFu, tc5_wait(&sum_full[2 * buf + half], (uint32_t)((c >> 1) & 1)));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                // (a piece is on its way while the one before is added)
+                uint32_t v[2][32];
+                pair_ld32(lanes + (uint32_t)(buf * FP_BN), v[0]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+                    if (i < 3) {
+                        pair_ld32(lanes + (uint32_t)(buf * FP_BN + 32 * (i + 1)), v[(i + 1) & 1]);
+                    } else {
+                        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+                        if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(freed[buf]) : "memory");
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) fma2(acc[16 * i + j / 2], v[i & 1][j], v[i & 1][j + 1], scale);
+                }
+            }
+            if (!ok) break;
+            if (p.bf) leave<bf16>(p, acc, out, r0, n0, lane);
+            else leave<float>(p, acc, out, r0, n0, lane);
+        }
+    }
+    if (!ok) report_wait(p.waits, WAIT_FP8);
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    cluster_sync();  // neither block leaves before the other's products, copies and arrivals are through
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(FP_COLS) : "memory");
+}
+
 // [rows][k] bytes, boxes of 128 columns x box_rows, zeros past the matrix.
 static bool fp8_map(CUtensorMap* map, const uint8_t* q, int64_t k, int64_t rows, int box_rows) {
     const PFN_encodeTiled encode = tensor_map_encoder();
@@ -229,9 +483,23 @@ static cudaError_t stream_of(const Fp8MatArgs& a, int parts, cudaStream_t st) {
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
+static cudaError_t pair_of(const Fp8MatArgs& a, cudaStream_t st) {
+    CUtensorMap mw, mx;
+    if (!fp8_map(&mw, a.wq, a.k, a.n, 64) || !fp8_map(&mx, a.xq, a.k, a.m, 128)) return cudaErrorInvalidValue;
+    static PerDeviceOnce once;
+    cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FP_SMEM + 1024); });
+    if (e != cudaSuccess) return e;
+    const int64_t row_tiles = (a.m + FP_BM - 1) / FP_BM, tiles = row_tiles * ((a.n + FP_BN - 1) / FP_BN);
+    if (tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
+    const int pairs = (int)std::min<int64_t>(tiles, device_sm_count() / 2);
+    e = launch_pdl(fp8_pair_kernel, dim3((unsigned)(2 * pairs)), dim3(FP_THREADS), (size_t)(FP_SMEM + 1024), st, Fp8PairArgs{a, (int)row_tiles, (int)tiles}, mw, mx);
+    return e != cudaSuccess ? e : count_launch_and_check();
+}
+
 cudaError_t launch_fp8_matmul(const Fp8MatArgs& a, cudaStream_t st) {
     if (a.m == 0 || a.n == 0) return cudaSuccess;
     if (a.m < 0 || a.n < 0 || a.k <= 0 || a.k % 16 != 0) return cudaErrorInvalidValue;
+    if (a.m > 128) return pair_of(a, st);
     const int bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
     const int64_t tiles = (int64_t)((a.n + FS_BM - 1) / FS_BM) * ((a.m + bn - 1) / bn);
     if ((a.m + bn - 1) / bn > 65535) return cudaErrorInvalidValue;
