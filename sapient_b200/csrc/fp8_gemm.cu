@@ -23,6 +23,12 @@ __device__ __forceinline__ void bar_init(uint64_t* bar, uint32_t arrivals) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(tc5_smem_u32(bar)), "r"(arrivals) : "memory");
 }
 
+// Arrives on a barrier of the cluster without waiting for the thread's own loads and stores: what is handed over is tensor memory, which
+// fences of its own order. With the default, a release, an arrival waits for the scales on their way (4096 x 14336 x 4096: 358 us for 217).
+__device__ __forceinline__ void arrive_relaxed(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+
 // e4m3 x e4m3 -> f32, both operands K-major.
 __host__ __device__ constexpr uint32_t fp8_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 __device__ __forceinline__ void fp8_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -165,7 +171,7 @@ __global__ void __launch_bounds__(FS_THREADS, 2) fp8_stream_kernel(const Fp8Stre
                 asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
                 if (j0 + 16 == BN) {
                     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-                    if (lane == 0) tc5_arrive(&sum_empty[buf]);
+                    if (lane == 0) arrive_relaxed(tc5_smem_u32(&sum_empty[buf]));
                 }
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
@@ -219,50 +225,51 @@ __device__ __forceinline__ float2 both(uint64_t v) {
     return f;
 }
 
-// A warp's 32 rows x 128 columns (a row a lane) to y through shared memory, 128 bytes of every row at a time, so that whole lines are
-// stored: 16-byte pieces of a row lie at piece ^ (row & 7), which keeps both directions free of bank conflicts.
+constexpr int FP_OUT = 2 * 32 * 128;  // of a drain warp's part of the result on its way out
+
+// 64 columns of bf16 or 32 of f32, 128 bytes of a lane's row, to shared memory: 16-byte pieces lie at piece ^ (row & 7), as TMA's 128-byte
+// swizzle has them, which keeps both directions free of bank conflicts.
 template <typename T>
-__device__ __forceinline__ void leave(const Fp8MatArgs& p, const uint64_t (&acc)[64], uint8_t* out, int r0, int n0, int lane) {
-    constexpr int PER = 16 / sizeof(T), PIECE = 8 * PER;  // values of 16 bytes, of 128
-    T* const y = static_cast<T*>(p.y);
-    const bool wide = ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.ldy * (int64_t)sizeof(T))) & 15) == 0;
+__device__ __forceinline__ void put_line(uint8_t* out, const uint64_t* acc, int lane) {
 #pragma unroll
-    for (int c0 = 0; c0 < 128; c0 += PIECE) {
-        __syncwarp();
+    for (int i = 0; i < 8; ++i) {
+        uint32_t u[4];
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            uint4 v;
-            uint32_t u[4];
-#pragma unroll
-            for (int j = 0; j < PER / 2; ++j) {
-                const float2 f = both(acc[(c0 + PER * i) / 2 + j]);
-                if constexpr (sizeof(T) == 4) {
-                    u[2 * j] = __float_as_uint(f.x);
-                    u[2 * j + 1] = __float_as_uint(f.y);
-                } else {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
-                    u[j] = *reinterpret_cast<const uint32_t*>(&h);
-                }
+            for (int j = 0; j < 2; ++j) {
+                const float2 f = both(acc[2 * i + j]);
+                u[2 * j] = __float_as_uint(f.x);
+                u[2 * j + 1] = __float_as_uint(f.y);
             }
-            v = make_uint4(u[0], u[1], u[2], u[3]);
-            *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = v;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = both(acc[4 * i + j]);
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+                u[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
         }
-        __syncwarp();
-        const int piece = lane & 7, n = n0 + c0 + piece * PER;
+        *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+// What put_line left of 32 rows, to y: whole lines of 128 bytes where rows start on 16 bytes.
+template <typename T>
+__device__ __forceinline__ void store_lines(const Fp8MatArgs& p, const uint8_t* out, bool wide, int r0, int n0, int lane) {
+    constexpr int PER = 16 / sizeof(T);
+    const int piece = lane & 7, n = n0 + piece * PER;
+    T* at = static_cast<T*>(p.y) + (int64_t)(r0 + (lane >> 3)) * p.ldy + n;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = 4 * i + (lane >> 3), m = r0 + row;
-            const uint4 v = *reinterpret_cast<const uint4*>(out + row * 128 + ((piece ^ (row & 7)) << 4));
-            if (m >= p.m) continue;
-            T* const at = y + (int64_t)m * p.ldy + n;
-            if (wide && n + PER <= p.n) {
-                *reinterpret_cast<uint4*>(at) = v;
-            } else {
-                const T* const e = reinterpret_cast<const T*>(&v);
+    for (int i = 0; i < 8; ++i, at += 4 * p.ldy) {
+        const int row = 4 * i + (lane >> 3);
+        const uint4 v = *reinterpret_cast<const uint4*>(out + row * 128 + ((piece ^ (row & 7)) << 4));
+        if (r0 + row >= p.m) continue;
+        if (wide && n + PER <= p.n) {
+            *reinterpret_cast<uint4*>(at) = v;
+        } else {
+            const T* const e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-                for (int j = 0; j < PER; ++j)
-                    if (n + j < p.n) at[j] = e[j];
-            }
+            for (int j = 0; j < PER; ++j)
+                if (n + j < p.n) at[j] = e[j];
         }
     }
 }
@@ -273,8 +280,7 @@ constexpr int FP_BM = 256, FP_BN = 256;
 constexpr int FP_DRAINS = 8, FP_FIRST_DRAIN = 4;               // warp 0 issues products, warp 1 copies; two idle ones fill their group
 constexpr int FP_THREADS = 32 * (FP_FIRST_DRAIN + FP_DRAINS);
 constexpr int FP_STAGE = 2 * 128 * FP8_BLOCK;                  // a block's share of a stage: 128 rows of either operand
-constexpr int FP_STAGES = 6;
-constexpr int FP_OUT = 32 * 128;                                // a drain warp's piece of the result on its way out
+constexpr int FP_STAGES = 4;
 constexpr int FP_SMEM = FP_STAGES * FP_STAGE + FP_DRAINS * FP_OUT;
 constexpr int FP_COLS = 2 * FP_BN;
 
@@ -312,13 +318,24 @@ __device__ __forceinline__ void pair_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 
 struct Fp8PairArgs {
     Fp8MatArgs p;
-    int row_tiles, tiles;
+    int row_tiles, whole, items;  // items: tiles up to `whole`, halves of the following tiles (128 of their weight rows) after them
+    bool wide;                    // rows of y start on 16 bytes
+};
+struct Fp8Item {
+    int r0, n0, first, last;  // activation and weight rows of the tile, halves
+    __device__ __forceinline__ Fp8Item(const Fp8PairArgs& a, int i) {
+        const int over = i - a.whole, tile = over < 0 ? i : a.whole + (over >> 1);
+        first = over < 0 ? 0 : over & 1;
+        last = over < 0 ? 1 : first;
+        r0 = tile % a.row_tiles * FP_BM;
+        n0 = tile / a.row_tiles * FP_BN;
+    }
 };
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
     fp8_pair_kernel(const Fp8PairArgs a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     extern __shared__ uint8_t fp_smem_raw[];
-    __shared__ __align__(8) uint64_t full[FP_STAGES], empty[FP_STAGES], sum_full[4], sum_empty[4];
+    __shared__ __align__(8) uint64_t full[FP_STAGES], empty[FP_STAGES], sum_full[4], sum_empty[4], out_full[FP_DRAINS], out_empty[FP_DRAINS];
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
     const Fp8MatArgs& p = a.p;
@@ -340,6 +357,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
             bar_init(&sum_full[i], 1);
             bar_init(&sum_empty[i], FP_DRAINS);
         }
+        for (int i = 0; i < FP_DRAINS; ++i) {
+            bar_init(&out_full[i], 32);
+            bar_init(&out_empty[i], 32);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -358,8 +379,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
                 const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
                 const uint32_t idesc = fp8_idesc(FP_BM, FP_BN / 2);
                 const uint64_t ad0 = tc5_desc(tc5_smem_u32(smem));
-                int st = 0, u = 0, c = 0;  // stage and its turn; blocks of 128 columns so far, over all tiles
-                for (int tile = pair; ok && tile < a.tiles; tile += pairs)
+                int st = 0, u = 0, c = 0, item = pair;  // stage and its turn; blocks of 128 columns so far, over all items
+                for (; ok && item < a.whole; item += pairs)
                     for (int b = 0; b < blocks; ++b, ++c) {
                         const int buf = c & 1, turn = c >> 1;
                         ok = __all_sync(0xFFFFFFFFu, tc5_wait(&full[st], (uint32_t)(u & 1)));
@@ -381,21 +402,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
                         __syncwarp();
                         if (++st == FP_STAGES) { st = 0; ++u; }
                     }
+                for (; ok && item < a.items; item += pairs) {
+                    const int h = (item - a.whole) & 1;
+                    for (int b = 0; b < blocks; ++b, ++c) {
+                        const int buf = c & 1, turn = c >> 1;
+                        ok = __all_sync(0xFFFFFFFFu, tc5_wait(&full[st], (uint32_t)(u & 1)));
+                        if (turn > 0) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&sum_empty[2 * buf + h], (uint32_t)((turn - 1) & 1)));
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                        const uint64_t ad = ad0 + (uint64_t)((uint32_t)(st * FP_STAGE) >> 4), bd = ad + (uint32_t)(((128 + 64 * h) * FP8_BLOCK) >> 4);
+                        if (leader) {
+#pragma unroll
+                            for (int i = 0; i < FP8_BLOCK / 32; ++i) pair_mma(tm + (uint32_t)(buf * FP_BN + 128 * h), ad + 2u * i, bd + 2u * i, idesc, i > 0);
+                            pair_commit(&empty[st]);
+                            pair_commit(&sum_full[2 * buf + h]);
+                        }
+                        __syncwarp();
+                        if (++st == FP_STAGES) { st = 0; ++u; }
+                    }
+                }
             }
-        } else if (warp == 1) {
+        } else if (warp != 1) {
+            // stores: warp 2 for the drains of one half, warp 3 for the other's
+            const int half = warp - 2;
+            int turn = 0;
+            for (int item = pair; ok && item + pairs < a.items; item += pairs) {
+                const Fp8Item it(a, item);
+                for (int q = 0; ok && q < 4; ++q) {
+                    const int d = 4 * half + q, q4 = (FP_FIRST_DRAIN + d) & 3, r0 = it.r0 + 128 * rank + 32 * q4, n0 = it.n0 + 128 * half;
+                    const uint8_t* const out = smem + FP_STAGES * FP_STAGE + d * FP_OUT;
+                    ok = __all_sync(0xFFFFFFFFu, tc5_wait(&out_full[d], (uint32_t)(turn & 1)));
+                    if (!ok) break;
+                    for (int i = 0; i < 2; ++i) {
+                        if (p.bf) store_lines<bf16>(p, out + 4096 * i, a.wide, r0, n0 + 64 * i, lane);
+                        else store_lines<float>(p, out + 4096 * i, a.wide, r0, n0 + 64 + 32 * i, lane);
+                    }
+                    tc5_arrive(&out_empty[d]);
+                }
+                ++turn;
+            }
+        } else {
             if (lane == 0) {
                 int st = 0, u = 0, issued = 0;
-                for (int tile = pair; ok && tile < a.tiles; tile += pairs) {
-                    const int r0 = tile % a.row_tiles * FP_BM + 128 * rank, n0 = tile / a.row_tiles * FP_BN + 64 * rank;
+                for (int item = pair; ok && item < a.items; item += pairs) {
+                    const Fp8Item it(a, item);
+                    const int r0 = it.r0 + 128 * rank, n0 = it.n0 + 64 * rank, bytes = 128 * FP8_BLOCK + (it.last - it.first + 1) * 64 * FP8_BLOCK;
                     for (int b = 0; b < blocks; ++b) {
                         if (u > 0) ok = tc5_wait(&empty[st], (uint32_t)((u - 1) & 1));
                         if (!ok) break;
                         const uint32_t bar = peer_smem(tc5_smem_u32(&full[st]), 0), dst = tc5_smem_u32(smem + st * FP_STAGE);
                         // (the other block's bytes may be there before they are expected: the phase waits for this arrival)
-                        if (rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(tc5_smem_u32(&full[st])), "r"(2 * FP_STAGE) : "memory");
+                        if (rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(tc5_smem_u32(&full[st])), "r"(2 * bytes) : "memory");
                         pair_tma(dst, &map_x, b * FP8_BLOCK, r0, bar);
-                        pair_tma(dst + 128 * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0, bar);
-                        pair_tma(dst + 192 * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0 + 128, bar);
+                        if (it.first == 0) pair_tma(dst + 128 * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0, bar);
+                        if (it.last == 1) pair_tma(dst + 192 * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0 + 128, bar);
                         ++issued;
                         if (++st == FP_STAGES) { st = 0; ++u; }
                     }
@@ -413,9 +473,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
         const uint32_t lanes = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(128 * half);
         uint8_t* const out = smem + FP_STAGES * FP_STAGE + (warp - FP_FIRST_DRAIN) * FP_OUT;
         const uint32_t freed[2] = {peer_smem(tc5_smem_u32(&sum_empty[half]), 0), peer_smem(tc5_smem_u32(&sum_empty[2 + half]), 0)};
-        int c = 0;
-        for (int tile = pair; ok && tile < a.tiles; tile += pairs) {
-            const int r0 = tile % a.row_tiles * FP_BM + 128 * rank + 32 * q4, n0 = tile / a.row_tiles * FP_BN + 128 * half;
+        int c = 0, turns = 0;
+        for (int item = pair; ok && item < a.items; item += pairs) {
+            const Fp8Item it(a, item);
+            if (half < it.first || half > it.last) continue;
+            const int r0 = it.r0 + 128 * rank + 32 * q4, n0 = it.n0 + 128 * half;
             const float* const xs = p.xs + (int64_t)min(r0 + lane, p.m - 1) * blocks;
             const float* const ws = p.ws + (int64_t)(min(n0, p.n - 1) / FP8_BLOCK) * blocks;
             uint64_t acc[64];
@@ -441,15 +503,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
                         pair_ld32(lanes + (uint32_t)(buf * FP_BN + 32 * (i + 1)), v[(i + 1) & 1]);
                     } else {
                         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-                        if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(freed[buf]) : "memory");
+                        if (lane == 0) arrive_relaxed(freed[buf]);
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) fma2(acc[16 * i + j / 2], v[i & 1][j], v[i & 1][j + 1], scale);
                 }
             }
             if (!ok) break;
-            if (p.bf) leave<bf16>(p, acc, out, r0, n0, lane);
-            else leave<float>(p, acc, out, r0, n0, lane);
+            // bf16 results leave by the storing warp, of f32 ones, twice the bytes, half; what the pair's last item leaves is stored here
+            if (turns > 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&out_empty[warp - FP_FIRST_DRAIN], (uint32_t)((turns - 1) & 1)));
+            if (!ok) break;
+            ++turns;
+            const bool last = item + pairs >= a.items;
+            auto line = [&](int i) {  // 128 bytes of every row, columns from i x 128 bytes on, to y
+                __syncwarp();
+                if (p.bf) store_lines<bf16>(p, out + 4096 * (i & 1), a.wide, r0, n0 + 64 * i, lane);
+                else store_lines<float>(p, out + 4096 * (i & 1), a.wide, r0, n0 + 32 * i, lane);
+            };
+            if (p.bf) {
+                put_line<bf16>(out, acc, lane);
+                put_line<bf16>(out + 4096, acc + 32, lane);
+            } else {
+                put_line<float>(out, acc, lane);
+                put_line<float>(out + 4096, acc + 16, lane);
+                line(0);
+                line(1);
+                __syncwarp();
+                put_line<float>(out, acc + 32, lane);
+                put_line<float>(out + 4096, acc + 48, lane);
+            }
+            if (last) {
+                line(p.bf ? 0 : 2);
+                line(p.bf ? 1 : 3);
+                break;
+            }
+            tc5_arrive(&out_full[warp - FP_FIRST_DRAIN]);
         }
     }
     if (!ok) report_wait(p.waits, WAIT_FP8);
@@ -490,9 +578,13 @@ static cudaError_t pair_of(const Fp8MatArgs& a, cudaStream_t st) {
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FP_SMEM + 1024); });
     if (e != cudaSuccess) return e;
     const int64_t row_tiles = (a.m + FP_BM - 1) / FP_BM, tiles = row_tiles * ((a.n + FP_BN - 1) / FP_BN);
-    if (tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
-    const int pairs = (int)std::min<int64_t>(tiles, device_sm_count() / 2);
-    e = launch_pdl(fp8_pair_kernel, dim3((unsigned)(2 * pairs)), dim3(FP_THREADS), (size_t)(FP_SMEM + 1024), st, Fp8PairArgs{a, (int)row_tiles, (int)tiles}, mw, mx);
+    if (tiles > INT32_MAX / 4) return cudaErrorInvalidValue;
+    // the last round's tiles are halved where all halves find a pair of SMs
+    const int most = device_sm_count() / 2, left = (int)(tiles % most), halved = 2 * left <= most ? left : 0;
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * (a.bf ? 2 : 4))) & 15) == 0;
+    const Fp8PairArgs k{a, (int)row_tiles, (int)tiles - halved, (int)tiles + halved, wide};
+    const int pairs = std::min(k.items, most);
+    e = launch_pdl(fp8_pair_kernel, dim3((unsigned)(2 * pairs)), dim3(FP_THREADS), (size_t)(FP_SMEM + 1024), st, k, mw, mx);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
