@@ -46,6 +46,100 @@ __device__ __forceinline__ void store(const Fp8MatArgs& p, int m, int n, float f
     else static_cast<float*>(p.y)[(int64_t)m * p.ldy + n] = f;
 }
 
+// ── Up to 16 rows ──
+// A block owns 16 weight rows; its warps take blocks of 128 columns in turn and add up in shared memory. Columns may be multiplied in
+// any order: a lane's 16 bytes of a row are four 4-byte operands of mma.sync, and the activations are read alike, so that nothing is
+// rearranged. No tensor memory, barriers or descriptors to set up, which is most of a small product's time.
+constexpr int FV_ROWS = 16;
+
+__device__ __forceinline__ uint4 fv_stream(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ void fv_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// NT: activation rows / 8. AHEAD: blocks of 128 columns that a warp has on their way.
+template <int NT, int FV_WARPS, int AHEAD>
+__global__ void __launch_bounds__(32 * FV_WARPS, 16 / FV_WARPS) fp8_gemv_kernel(const Fp8MatArgs p) {
+    __shared__ float part[FV_WARPS][8 * NT][FV_ROWS + 1];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * FV_ROWS, blocks = (p.k + FP8_BLOCK - 1) / FP8_BLOCK;
+    const uint8_t* const w0 = p.wq + (int64_t)min(n0 + g, p.n - 1) * p.k + 16 * t;
+    const uint8_t* const w1 = p.wq + (int64_t)min(n0 + 8 + g, p.n - 1) * p.k + 16 * t;
+    const float* const ws = p.ws + (int64_t)(n0 / FP8_BLOCK) * blocks;
+    struct Stage {
+        uint4 w[2][2], x[NT][2];  // [row half][64 columns]
+        float xs[NT][2], ws;
+    } stage[AHEAD];
+    auto load = [&](Stage& s, int b) {
+        const int c = b * FP8_BLOCK;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bool there = c + 64 * h + 16 * t < p.k;
+            s.w[0][h] = there ? fv_stream(w0 + c + 64 * h) : zero;
+            s.w[1][h] = there ? fv_stream(w1 + c + 64 * h) : zero;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                s.x[j][h] = there && 8 * j + g < p.m ? __ldg(reinterpret_cast<const uint4*>(p.xq + (int64_t)(8 * j + g) * p.k + c + 64 * h + 16 * t)) : zero;
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int m = 8 * j + 2 * t + i;
+                s.xs[j][i] = m < p.m ? __ldg(p.xs + (int64_t)m * blocks + b) : 0.f;
+            }
+        s.ws = __ldg(ws + b);
+    };
+    pdl_wait();
+    pdl_trigger();
+    float acc[NT][4] = {};
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d)
+        if (warp + FV_WARPS * d < blocks) load(stage[d], warp + FV_WARPS * d);
+    for (int b0 = warp; b0 < blocks; b0 += FV_WARPS * AHEAD) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) {
+            const int b = b0 + FV_WARPS * d;
+            if (b >= blocks) break;
+            Stage& s = stage[d];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    fv_mma(c, s.w[0][h].x, s.w[1][h].x, s.w[0][h].y, s.w[1][h].y, s.x[j][h].x, s.x[j][h].y);
+                    fv_mma(c, s.w[0][h].z, s.w[1][h].z, s.w[0][h].w, s.w[1][h].w, s.x[j][h].z, s.x[j][h].w);
+                }
+                const float s0 = s.xs[j][0] * s.ws, s1 = s.xs[j][1] * s.ws;
+                acc[j][0] = fmaf(c[0], s0, acc[j][0]);
+                acc[j][1] = fmaf(c[1], s1, acc[j][1]);
+                acc[j][2] = fmaf(c[2], s0, acc[j][2]);
+                acc[j][3] = fmaf(c[3], s1, acc[j][3]);
+            }
+            if (b + FV_WARPS * AHEAD < blocks) load(s, b + FV_WARPS * AHEAD);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[warp][8 * j + 2 * t + (i & 1)][g + 8 * (i >> 1)] = acc[j][i];
+    __syncthreads();
+    const int row = tid & (FV_ROWS - 1), m = tid / FV_ROWS;
+    if (m < p.m && m < 8 * NT && n0 + row < p.n) {
+        float f = 0.f;
+#pragma unroll
+        for (int w = 0; w < FV_WARPS; ++w) f += part[w][m][row];
+        store(p, m, n0 + row, f);
+    }
+}
+
 // ── Few rows: a stream of weights ──
 constexpr int FS_BM = 128;                     // weight rows of a tile
 constexpr int FS_THREADS = 192;                // MMA warp, TMA warp, four drain warps
@@ -588,10 +682,29 @@ static cudaError_t pair_of(const Fp8MatArgs& a, cudaStream_t st) {
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
+// Where the kernel of 16 weight rows a block is the faster one (its blocks / the stream of weights, us, weights past L2): up to 8 rows
+// it starts sooner (1 row: 2048 x 2048 3.0 / 4.8, 4096 x 4096 6.2 / 7.1, 8960 x 1536 6.0 / 6.7), but blocks beyond two an SM come in
+// rounds (6144 x 4096 9.8 / 8.7, 14336 x 4096 16.2 / 13.9) and few long ones leave SMs idle (2560 x 10240 10.4 / 9.0). From 9 rows on
+// each block also reads about as much of the activations as of the weights (12 rows: 2048 x 2048 4.5 / 5.3, 2560 x 2560 6.6 / 6.0).
+static bool gemv_takes(const Fp8MatArgs& a) {
+    const int64_t blocks = (a.n + FV_ROWS - 1) / FV_ROWS, sms = device_sm_count(), values = (int64_t)a.n * a.k;
+    if (a.m > 8) return a.k <= 2048 && values <= 5 << 20;
+    return blocks <= sms || (blocks <= 2 * sms && a.k <= 8192) || (blocks <= 4 * sms && values <= 1 << 24);
+}
+static cudaError_t gemv_of(const Fp8MatArgs& a, cudaStream_t st) {
+    const dim3 grid((unsigned)((a.n + FV_ROWS - 1) / FV_ROWS));
+    const bool wide = (int)grid.x <= device_sm_count();  // 16 warps where a block has its SM for itself (1 row of 2048 x 8192: 7.5 -> 6.3)
+    cudaError_t e;
+    if (a.m <= 8) e = wide ? launch_pdl(fp8_gemv_kernel<1, 16, 4>, grid, dim3(512), 0, st, a) : launch_pdl(fp8_gemv_kernel<1, 8, 4>, grid, dim3(256), 0, st, a);
+    else e = wide ? launch_pdl(fp8_gemv_kernel<2, 16, 2>, grid, dim3(512), 0, st, a) : launch_pdl(fp8_gemv_kernel<2, 8, 2>, grid, dim3(256), 0, st, a);
+    return e != cudaSuccess ? e : count_launch_and_check();
+}
+
 cudaError_t launch_fp8_matmul(const Fp8MatArgs& a, cudaStream_t st) {
     if (a.m == 0 || a.n == 0) return cudaSuccess;
     if (a.m < 0 || a.n < 0 || a.k <= 0 || a.k % 16 != 0) return cudaErrorInvalidValue;
     if (a.m > 128) return pair_of(a, st);
+    if (a.m <= 16 && gemv_takes(a)) return gemv_of(a, st);
     const int bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
     const int64_t tiles = (int64_t)((a.n + FS_BM - 1) / FS_BM) * ((a.m + bn - 1) / bn);
     if ((a.m + bn - 1) / bn > 65535) return cudaErrorInvalidValue;
