@@ -3,6 +3,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "fp8.h"
 #include "kernels.h"
@@ -289,13 +290,22 @@ __global__ void __launch_bounds__(FS_THREADS, 2) fp8_stream_kernel(const Fp8Stre
                 for (int j = 0; j < BN; ++j) partial[j * FS_BM + 32 * q4 + lane] = acc[j];
             }
             cluster_sync();
-            // the cluster's blocks share out the rows; each adds its rows' parts in order
+            // the cluster's blocks share out the rows, eight on their way at a time; each adds its rows' parts in order
             const uint32_t mine = tc5_smem_u32(partial + 32 * q4 + lane);
-            for (int j = part; j < rows && n < p.n; j += a.parts) {
-                float f = 0.f;
-#pragma unroll 8
-                for (int o = 0; o < a.parts; ++o) f += ld_peer(peer_smem(mine, o) + (uint32_t)j * FS_BM * 4);
-                if (ok) store(p, r0 + j, n, f);
+            constexpr int NR = 8;
+            for (int j0 = part; j0 < rows && n < p.n; j0 += NR * a.parts) {
+                float f[NR] = {};
+                for (int o = 0; o < a.parts; ++o) {
+                    const uint32_t peer = peer_smem(mine, o);
+                    float v[NR];
+#pragma unroll
+                    for (int i = 0; i < NR; ++i) v[i] = ld_peer(peer + (uint32_t)(min(j0 + i * a.parts, rows - 1) * FS_BM * 4));
+#pragma unroll
+                    for (int i = 0; i < NR; ++i) f[i] += v[i];
+                }
+#pragma unroll
+                for (int i = 0; i < NR; ++i)
+                    if (ok && j0 + i * a.parts < rows) store(p, r0 + j0 + i * a.parts, n, f[i]);
             }
         }
     }
@@ -313,12 +323,18 @@ __global__ void __launch_bounds__(FS_THREADS, 2) fp8_stream_kernel(const Fp8Stre
 __device__ __forceinline__ void fma2(uint64_t& acc, uint32_t v0, uint32_t v1, uint64_t s) {
     asm("{\n.reg .b64 v;\nmov.b64 v, {%1, %2};\nfma.rn.f32x2 %0, v, %3, %0;\n}\n" : "+l"(acc) : "r"(v0), "r"(v1), "l"(s));
 }
+__device__ __forceinline__ uint64_t pair2(float2 f) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(f.x), "f"(f.y));
+    return v;
+}
 __device__ __forceinline__ float2 both(uint64_t v) {
     float2 f;
     asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
     return f;
 }
 
+constexpr int FP_DRAINS = 8;
 constexpr int FP_OUT = 2 * 32 * 128;  // of a drain warp's part of the result on its way out
 
 // 64 columns of bf16 or 32 of f32, 128 bytes of a lane's row, to shared memory: 16-byte pieces lie at piece ^ (row & 7), as TMA's 128-byte
@@ -368,38 +384,82 @@ __device__ __forceinline__ void store_lines(const Fp8MatArgs& p, const uint8_t* 
     }
 }
 
-// ── Many rows: two SMs share a tile ──
-// 256 activation rows (128 a block, the lanes of its tensor memory) x 256 weight rows (each block holds 128 of them in shared memory).
-constexpr int FP_BM = 256, FP_BN = 256;
-constexpr int FP_DRAINS = 8, FP_FIRST_DRAIN = 4;               // warp 0 issues products, warp 1 copies; two idle ones fill their group
-constexpr int FP_THREADS = 32 * (FP_FIRST_DRAIN + FP_DRAINS);
-constexpr int FP_STAGE = 2 * 128 * FP8_BLOCK;                  // a block's share of a stage: 128 rows of either operand
-constexpr int FP_STAGES = 4;
-constexpr int FP_SMEM = FP_STAGES * FP_STAGE + FP_DRAINS * FP_OUT;
-constexpr int FP_COLS = 2 * FP_BN;
+// 32 columns that put_line left in f32, to y of either type.
+__device__ __forceinline__ void store_f32_lines(const Fp8MatArgs& p, const uint8_t* out, bool wide, int r0, int n0, int lane) {
+    if (!p.bf) {
+        store_lines<float>(p, out, wide, r0, n0, lane);
+        return;
+    }
+    const int piece = lane & 7, n = n0 + 4 * piece;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int row = 4 * i + (lane >> 3);
+        const float4 f = *reinterpret_cast<const float4*>(out + row * 128 + ((piece ^ (row & 7)) << 4));
+        if (r0 + row >= p.m) continue;
+        bf16* const at = static_cast<bf16*>(p.y) + (int64_t)(r0 + row) * p.ldy + n;
+        if (wide && n + 4 <= p.n) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(f.x, f.y), hi = __floats2bfloat162_rn(f.z, f.w);
+            *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        } else {
+            const float e[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < p.n) at[j] = __float2bfloat16_rn(e[j]);
+        }
+    }
+}
 
-__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
+// Whether all drain warps' waits were in time; a barrier between them.
+__device__ __forceinline__ bool drains_agree(bool ok) {
+    int all;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.and.pred q, 1, %2, p;\nselp.b32 %0, 1, 0, q;\n}\n" : "=r"(all) : "r"((int)ok), "n"(32 * FP_DRAINS) : "memory");
+    return all != 0;
 }
-// Arrives on the barrier at this place in both blocks once the products issued so far are done.
-__device__ __forceinline__ void pair_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(tc5_smem_u32(bar)), "h"((uint16_t)3)
-                 : "memory");
+
+// ── Many rows: activation rows are the lanes ──
+// A tile of 128 G activation rows x 256 weight rows, by one block or by a pair (G = 2: each block has 128 activation rows in its tensor
+// memory and half of the weight rows in its shared memory), or by one block 128 x 128 or 128 x 64 of a product that does not fill the SMs.
+constexpr int FP_BN = 256;
+constexpr int FP_FIRST_DRAIN = 4;               // warp 0 issues products, warp 1 copies, warps 2 and 3 store results of drains
+constexpr int FP_THREADS = 32 * (FP_FIRST_DRAIN + FP_DRAINS);
+constexpr int FP_COLS = 2 * FP_BN;
+__host__ __device__ constexpr int fp_stage(int g) { return (128 + FP_BN / g) * FP8_BLOCK; }  // a block's share of a stage
+__host__ __device__ constexpr int fp_stages(int g) { return g == 2 ? 4 : 3; }
+__host__ __device__ constexpr int fp_smem(int g) { return fp_stages(g) * fp_stage(g) + FP_DRAINS * FP_OUT; }
+template <int G>
+__device__ __forceinline__ void wide_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t accumulate) {
+    constexpr uint32_t idesc = fp8_idesc(128 * G, FP_BN / 2);
+    if constexpr (G == 1) {
+        fp8_mma(d_tmem, adesc, bdesc, idesc, accumulate);
+    } else {
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+            "}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
 }
-__device__ __forceinline__ void pair_tma(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst), "l"(map),
-        "r"(x), "r"(y), "r"(bar)
-        : "memory");
+// Arrives on the barrier at this place in the tile's blocks once the products issued so far are done.
+template <int G>
+__device__ __forceinline__ void wide_commit(uint64_t* bar) {
+    if constexpr (G == 1) tc5_commit(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(tc5_smem_u32(bar)), "h"((uint16_t)3)
+                     : "memory");
+}
+template <int G>
+__device__ __forceinline__ void wide_tma(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if constexpr (G == 1) tc5_tma_2d(dst, map, x, y, bar);
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst), "l"(map),
+            "r"(x), "r"(y), "r"(bar)
+            : "memory");
 }
 // 32 consecutive tensor-memory columns of the warp's 32 lanes.
-__device__ __forceinline__ void pair_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void wide_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
         "%29,%30,%31}, [%32];\n"
@@ -410,46 +470,76 @@ __device__ __forceinline__ void pair_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         : "memory");
 }
 
-struct Fp8PairArgs {
+// Adds 32 P columns of a sum, scaled, to the lane's; `freed` hears when they have been read.
+template <int P>
+__device__ __forceinline__ void drain_add(uint32_t taddr, float f, uint64_t (&acc)[16 * P], uint32_t freed, int lane) {
+    const uint64_t scale = pair2(make_float2(f, f));
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    // (a piece is on its way while the one before is added)
+    uint32_t v[2][32];
+    wide_ld32(taddr, v[0]);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+        if (i + 1 < P) {
+            wide_ld32(taddr + (uint32_t)(32 * (i + 1)), v[(i + 1) & 1]);
+        } else {
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            if (lane == 0) arrive_relaxed(freed);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) fma2(acc[16 * i + j / 2], v[i & 1][j], v[i & 1][j + 1], scale);
+    }
+}
+
+struct Fp8WideArgs {
     Fp8MatArgs p;
     int row_tiles, whole, items;  // items: tiles up to `whole`, halves of the following tiles (128 of their weight rows) after them
-    bool wide;                    // rows of y start on 16 bytes
+    bool aligned;                 // rows of y start on 16 bytes
+    bool handed;                  // results leave by warps of their own while the drains go on with the next tile
 };
+template <int G>
 struct Fp8Item {
     int r0, n0, first, last;  // activation and weight rows of the tile, halves
-    __device__ __forceinline__ Fp8Item(const Fp8PairArgs& a, int i) {
+    __device__ __forceinline__ Fp8Item(const Fp8WideArgs& a, int i) {
         const int over = i - a.whole, tile = over < 0 ? i : a.whole + (over >> 1);
         first = over < 0 ? 0 : over & 1;
         last = over < 0 ? 1 : first;
-        r0 = tile % a.row_tiles * FP_BM;
+        r0 = tile % a.row_tiles * (128 * G);
         n0 = tile / a.row_tiles * FP_BN;
     }
 };
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
-    fp8_pair_kernel(const Fp8PairArgs a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+template <int G>
+__global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideArgs a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+    constexpr int STAGES = fp_stages(G), STAGE = fp_stage(G), HALF = FP_BN / 2 / G;  // HALF: weight rows of half a tile in this block
     extern __shared__ uint8_t fp_smem_raw[];
-    __shared__ __align__(8) uint64_t full[FP_STAGES], empty[FP_STAGES], sum_full[4], sum_empty[4], out_full[FP_DRAINS], out_empty[FP_DRAINS];
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], sum_full[4], sum_empty[4], out_full[FP_DRAINS], out_empty[FP_DRAINS];
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
     const Fp8MatArgs& p = a.p;
-    const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int rank = G == 2 ? blockIdx.x & 1 : 0, team = blockIdx.x / G, teams = gridDim.x / G;
     const int blocks = (p.k + FP8_BLOCK - 1) / FP8_BLOCK;
     uint8_t* const smem = fp_smem_raw + ((1024u - (tc5_smem_u32(fp_smem_raw) & 1023u)) & 1023u);
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5_smem_u32(&tmem_slot)), "n"(FP_COLS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+        if constexpr (G == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5_smem_u32(&tmem_slot)), "n"(FP_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5_smem_u32(&tmem_slot)), "n"(FP_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+        }
     }
     if (tid == 32) {
         tc5_prefetch_map(&map_w);
         tc5_prefetch_map(&map_x);
-        for (int i = 0; i < FP_STAGES; ++i) {
+        for (int i = 0; i < STAGES; ++i) {
             bar_init(&full[i], 1);
             bar_init(&empty[i], 1);
         }
         for (int i = 0; i < 4; ++i) {
             bar_init(&sum_full[i], 1);
-            bar_init(&sum_empty[i], FP_DRAINS);
+            bar_init(&sum_empty[i], G * FP_DRAINS / 2);
         }
         for (int i = 0; i < FP_DRAINS; ++i) {
             bar_init(&out_full[i], 32);
@@ -459,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
-    cluster_sync();  // both blocks' barriers are there
+    if (G == 2) cluster_sync();  // both blocks' barriers are there
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     const uint32_t tmem = tmem_slot;
     pdl_wait();
@@ -468,17 +558,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
     if (warp < FP_FIRST_DRAIN) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");  // 128 x 56 + 256 x 224 = 384 x 168
         if (warp == 0) {
-            if (rank == 0) {  // one block issues for both
+            if (rank == 0) {
                 const bool leader = tc5_elect();
                 const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
-                const uint32_t idesc = fp8_idesc(FP_BM, FP_BN / 2);
                 const uint64_t ad0 = tc5_desc(tc5_smem_u32(smem));
-                int st = 0, u = 0, c = 0, item = pair;  // stage and its turn; blocks of 128 columns so far, over all items
-                for (; ok && item < a.whole; item += pairs)
+                int st = 0, u = 0, c = 0, item = team;  // stage and its turn; blocks of 128 columns so far, over all items
+                for (; ok && item < a.whole; item += teams)
                     for (int b = 0; b < blocks; ++b, ++c) {
                         const int buf = c & 1, turn = c >> 1;
                         ok = __all_sync(0xFFFFFFFFu, tc5_wait(&full[st], (uint32_t)(u & 1)));
-                        const uint64_t ad = ad0 + (uint64_t)((uint32_t)(st * FP_STAGE) >> 4), bd = ad + ((128 * FP8_BLOCK) >> 4);
+                        const uint64_t ad = ad0 + (uint64_t)((uint32_t)(st * STAGE) >> 4), bd = ad + ((128 * FP8_BLOCK) >> 4);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             if (turn > 0) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&sum_empty[2 * buf + h], (uint32_t)((turn - 1) & 1)));
@@ -487,16 +576,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
                             if (leader) {
 #pragma unroll
                                 for (int i = 0; i < FP8_BLOCK / 32; ++i)
-                                    pair_mma(tm + (uint32_t)(buf * FP_BN + 128 * h), ad + 2u * i, bd + (uint32_t)(h * ((64 * FP8_BLOCK) >> 4)) + 2u * i, idesc, i > 0);
-                                if (h) pair_commit(&empty[st]);
-                                pair_commit(&sum_full[2 * buf + h]);
+                                    wide_mma<G>(tm + (uint32_t)(buf * FP_BN + 128 * h), ad + 2u * i, bd + (uint32_t)(h * ((HALF * FP8_BLOCK) >> 4)) + 2u * i, i > 0);
+                                if (h) wide_commit<G>(&empty[st]);
+                                wide_commit<G>(&sum_full[2 * buf + h]);
                             }
                         }
                         if (!ok) break;
                         __syncwarp();
-                        if (++st == FP_STAGES) { st = 0; ++u; }
+                        if (++st == STAGES) { st = 0; ++u; }
                     }
-                for (; ok && item < a.items; item += pairs) {
+                for (; ok && item < a.items; item += teams) {
                     const int h = (item - a.whole) & 1;
                     for (int b = 0; b < blocks; ++b, ++c) {
                         const int buf = c & 1, turn = c >> 1;
@@ -504,72 +593,82 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
                         if (turn > 0) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&sum_empty[2 * buf + h], (uint32_t)((turn - 1) & 1)));
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                        const uint64_t ad = ad0 + (uint64_t)((uint32_t)(st * FP_STAGE) >> 4), bd = ad + (uint32_t)(((128 + 64 * h) * FP8_BLOCK) >> 4);
+                        const uint64_t ad = ad0 + (uint64_t)((uint32_t)(st * STAGE) >> 4), bd = ad + (uint32_t)(((128 + HALF * h) * FP8_BLOCK) >> 4);
                         if (leader) {
 #pragma unroll
-                            for (int i = 0; i < FP8_BLOCK / 32; ++i) pair_mma(tm + (uint32_t)(buf * FP_BN + 128 * h), ad + 2u * i, bd + 2u * i, idesc, i > 0);
-                            pair_commit(&empty[st]);
-                            pair_commit(&sum_full[2 * buf + h]);
+                            for (int i = 0; i < FP8_BLOCK / 32; ++i) wide_mma<G>(tm + (uint32_t)(buf * FP_BN + 128 * h), ad + 2u * i, bd + 2u * i, i > 0);
+                            wide_commit<G>(&empty[st]);
+                            wide_commit<G>(&sum_full[2 * buf + h]);
                         }
                         __syncwarp();
-                        if (++st == FP_STAGES) { st = 0; ++u; }
+                        if (++st == STAGES) { st = 0; ++u; }
                     }
                 }
             }
-        } else if (warp != 1) {
-            // stores: warp 2 for the drains of one half, warp 3 for the other's
+        } else if (warp == 1) {
+            if (lane == 0) {
+                int st = 0, u = 0, issued = 0;
+                for (int item = team; ok && item < a.items; item += teams) {
+                    const Fp8Item<G> it(a, item);
+                    const int r0 = it.r0 + 128 * rank, n0 = it.n0 + HALF * rank, bytes = 128 * FP8_BLOCK + (it.last - it.first + 1) * HALF * FP8_BLOCK;
+                    for (int b = 0; b < blocks; ++b) {
+                        if (u > 0) ok = tc5_wait(&empty[st], (uint32_t)((u - 1) & 1));
+                        if (!ok) break;
+                        const uint32_t here = tc5_smem_u32(&full[st]), bar = G == 1 ? here : peer_smem(here, 0), dst = tc5_smem_u32(smem + st * STAGE);
+                        // (the other block's bytes may be there before they are expected: the phase waits for this arrival)
+                        if (rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(here), "r"(G * bytes) : "memory");
+                        wide_tma<G>(dst, &map_x, b * FP8_BLOCK, r0, bar);
+                        if (it.first == 0) wide_tma<G>(dst + 128 * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0, bar);
+                        if (it.last == 1) wide_tma<G>(dst + (128 + HALF) * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0 + 128, bar);
+                        ++issued;
+                        if (++st == STAGES) { st = 0; ++u; }
+                    }
+                }
+                // nothing is in flight towards this block when it goes on to the end: copies, or the arrivals that follow the last products
+                for (int c = max(0, issued - STAGES); c < issued; ++c)
+                    if (ok) ok = tc5_wait(&empty[c % STAGES], (uint32_t)((c / STAGES) & 1));
+                    else if (rank == 0) tc5_wait(&full[c % STAGES], (uint32_t)((c / STAGES) & 1));
+            }
+            __syncwarp();
+        } else {
+            // stores: warp 2 for the drains of one half, warp 3 for the other's; a team's last item is its drains' own
             const int half = warp - 2;
             int turn = 0;
-            for (int item = pair; ok && item + pairs < a.items; item += pairs) {
-                const Fp8Item it(a, item);
+            for (int item = team; ok && a.handed && item + teams < a.items; item += teams) {
+                const Fp8Item<G> it(a, item);
                 for (int q = 0; ok && q < 4; ++q) {
                     const int d = 4 * half + q, q4 = (FP_FIRST_DRAIN + d) & 3, r0 = it.r0 + 128 * rank + 32 * q4, n0 = it.n0 + 128 * half;
-                    const uint8_t* const out = smem + FP_STAGES * FP_STAGE + d * FP_OUT;
+                    const uint8_t* const out = smem + STAGES * STAGE + d * FP_OUT;
                     ok = __all_sync(0xFFFFFFFFu, tc5_wait(&out_full[d], (uint32_t)(turn & 1)));
                     if (!ok) break;
                     for (int i = 0; i < 2; ++i) {
-                        if (p.bf) store_lines<bf16>(p, out + 4096 * i, a.wide, r0, n0 + 64 * i, lane);
-                        else store_lines<float>(p, out + 4096 * i, a.wide, r0, n0 + 64 + 32 * i, lane);
+                        if (p.bf) store_lines<bf16>(p, out + 4096 * i, a.aligned, r0, n0 + 64 * i, lane);
+                        else store_lines<float>(p, out + 4096 * i, a.aligned, r0, n0 + 64 + 32 * i, lane);
                     }
                     tc5_arrive(&out_empty[d]);
                 }
                 ++turn;
             }
-        } else {
-            if (lane == 0) {
-                int st = 0, u = 0, issued = 0;
-                for (int item = pair; ok && item < a.items; item += pairs) {
-                    const Fp8Item it(a, item);
-                    const int r0 = it.r0 + 128 * rank, n0 = it.n0 + 64 * rank, bytes = 128 * FP8_BLOCK + (it.last - it.first + 1) * 64 * FP8_BLOCK;
-                    for (int b = 0; b < blocks; ++b) {
-                        if (u > 0) ok = tc5_wait(&empty[st], (uint32_t)((u - 1) & 1));
-                        if (!ok) break;
-                        const uint32_t bar = peer_smem(tc5_smem_u32(&full[st]), 0), dst = tc5_smem_u32(smem + st * FP_STAGE);
-                        // (the other block's bytes may be there before they are expected: the phase waits for this arrival)
-                        if (rank == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(tc5_smem_u32(&full[st])), "r"(2 * bytes) : "memory");
-                        pair_tma(dst, &map_x, b * FP8_BLOCK, r0, bar);
-                        if (it.first == 0) pair_tma(dst + 128 * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0, bar);
-                        if (it.last == 1) pair_tma(dst + 192 * FP8_BLOCK, &map_w, b * FP8_BLOCK, n0 + 128, bar);
-                        ++issued;
-                        if (++st == FP_STAGES) { st = 0; ++u; }
-                    }
-                }
-                // nothing is in flight towards this block when it goes on to the end: copies, or the arrivals that follow the last products
-                for (int c = max(0, issued - FP_STAGES); c < issued; ++c)
-                    if (ok) ok = tc5_wait(&empty[c % FP_STAGES], (uint32_t)((c / FP_STAGES) & 1));
-                    else if (rank == 0) tc5_wait(&full[c % FP_STAGES], (uint32_t)((c / FP_STAGES) & 1));
-            }
-            __syncwarp();
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
-        const int q4 = warp & 3, half = (warp - FP_FIRST_DRAIN) >> 2;
+        const int q4 = warp & 3, drain = warp - FP_FIRST_DRAIN, half = drain >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(128 * half);
-        uint8_t* const out = smem + FP_STAGES * FP_STAGE + (warp - FP_FIRST_DRAIN) * FP_OUT;
+        uint8_t* const out = smem + STAGES * STAGE + drain * FP_OUT;
         const uint32_t freed[2] = {peer_smem(tc5_smem_u32(&sum_empty[half]), 0), peer_smem(tc5_smem_u32(&sum_empty[2 + half]), 0)};
+        // 64 columns of the warp's rows that are in `out` (f32: in both its lines), to y
+        auto store_out = [&](int r0, int n0) {
+            __syncwarp();
+            if (p.bf) {
+                store_lines<bf16>(p, out, a.aligned, r0, n0, lane);
+            } else {
+                store_lines<float>(p, out, a.aligned, r0, n0, lane);
+                store_lines<float>(p, out + 4096, a.aligned, r0, n0 + 32, lane);
+            }
+        };
         int c = 0, turns = 0;
-        for (int item = pair; ok && item < a.items; item += pairs) {
-            const Fp8Item it(a, item);
+        for (int item = team; ok && item < a.items; item += teams) {
+            const Fp8Item<G> it(a, item);
             if (half < it.first || half > it.last) continue;
             const int r0 = it.r0 + 128 * rank + 32 * q4, n0 = it.n0 + 128 * half;
             const float* const xs = p.xs + (int64_t)min(r0 + lane, p.m - 1) * blocks;
@@ -586,15 +685,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
                 if (b + 1 < blocks) { xv = xs[b + 1]; wv = ws[b + 1]; }
                 ok = __all_sync(0xFFFFFFFFu, tc5_wait(&sum_full[2 * buf + half], (uint32_t)((c >> 1) & 1)));
                 if (!ok) break;
+                // (as drain_add, which costs this loop spills and a tenth of its time)
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                // (a piece is on its way while the one before is added)
                 uint32_t v[2][32];
-                pair_ld32(lanes + (uint32_t)(buf * FP_BN), v[0]);
+                wide_ld32(lanes + (uint32_t)(buf * FP_BN), v[0]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
                     if (i < 3) {
-                        pair_ld32(lanes + (uint32_t)(buf * FP_BN + 32 * (i + 1)), v[(i + 1) & 1]);
+                        wide_ld32(lanes + (uint32_t)(buf * FP_BN + 32 * (i + 1)), v[(i + 1) & 1]);
                     } else {
                         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
                         if (lane == 0) arrive_relaxed(freed[buf]);
@@ -604,42 +703,191 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP_THREADS, 1)
                 }
             }
             if (!ok) break;
-            // bf16 results leave by the storing warp, of f32 ones, twice the bytes, half; what the pair's last item leaves is stored here
-            if (turns > 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&out_empty[warp - FP_FIRST_DRAIN], (uint32_t)((turns - 1) & 1)));
+            // of long products bf16 results leave by the storing warp, of f32 ones, twice the bytes, half
+            const bool handed = a.handed && item + teams < a.items;
+            if (turns > 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&out_empty[drain], (uint32_t)((turns - 1) & 1)));
             if (!ok) break;
-            ++turns;
-            const bool last = item + pairs >= a.items;
-            auto line = [&](int i) {  // 128 bytes of every row, columns from i x 128 bytes on, to y
-                __syncwarp();
-                if (p.bf) store_lines<bf16>(p, out + 4096 * (i & 1), a.wide, r0, n0 + 64 * i, lane);
-                else store_lines<float>(p, out + 4096 * (i & 1), a.wide, r0, n0 + 32 * i, lane);
-            };
+            __syncwarp();
             if (p.bf) {
                 put_line<bf16>(out, acc, lane);
                 put_line<bf16>(out + 4096, acc + 32, lane);
             } else {
                 put_line<float>(out, acc, lane);
                 put_line<float>(out + 4096, acc + 16, lane);
-                line(0);
-                line(1);
+                store_out(r0, n0);
                 __syncwarp();
                 put_line<float>(out, acc + 32, lane);
                 put_line<float>(out + 4096, acc + 48, lane);
             }
-            if (last) {
-                line(p.bf ? 0 : 2);
-                line(p.bf ? 1 : 3);
-                break;
+            if (handed) {
+                tc5_arrive(&out_full[drain]);
+                ++turns;
+            } else if (p.bf) {
+                __syncwarp();
+                store_lines<bf16>(p, out, a.aligned, r0, n0, lane);
+                store_lines<bf16>(p, out + 4096, a.aligned, r0, n0 + 64, lane);
+            } else {
+                store_out(r0, n0 + 64);
             }
-            tc5_arrive(&out_full[warp - FP_FIRST_DRAIN]);
         }
     }
     if (!ok) report_wait(p.waits, WAIT_FP8);
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
-    cluster_sync();  // neither block leaves before the other's products, copies and arrivals are through
+    if (G == 2) cluster_sync();  // neither block leaves before the other's products, copies and arrivals are through
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(FP_COLS) : "memory");
+    if (warp == 0) {
+        if constexpr (G == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(FP_COLS) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(FP_COLS) : "memory");
+    }
+}
+
+// A tile of 128 activation rows x W weight rows a block, no more tiles than SMs: what counts is how many bytes are on their way and how
+// soon the tensor cores go on. All of shared memory is stages; there are four accumulators, and the two groups of drain warps take
+// blocks of 128 columns in turn and add up at the end.
+__host__ __device__ constexpr int lone_stage(int w) { return (128 + w) * FP8_BLOCK; }
+__host__ __device__ constexpr int lone_stages(int w) { return 210 * 1024 / lone_stage(w); }
+
+template <int W>
+__global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArgs p, int aligned, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+    constexpr int STAGES = lone_stages(W), STAGE = lone_stage(W), COLS = 4 * W;
+    extern __shared__ uint8_t fp_smem_raw[];
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], sum_full[4], sum_empty[4];
+    __shared__ uint32_t tmem_slot;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
+    const int n0 = blockIdx.x * W, m0 = blockIdx.y * 128;
+    const int blocks = (p.k + FP8_BLOCK - 1) / FP8_BLOCK;
+    uint8_t* const smem = fp_smem_raw + ((1024u - (tc5_smem_u32(fp_smem_raw) & 1023u)) & 1023u);
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5_smem_u32(&tmem_slot)), "n"(COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    if (tid == 32) {
+        tc5_prefetch_map(&map_w);
+        tc5_prefetch_map(&map_x);
+        for (int i = 0; i < STAGES; ++i) {
+            bar_init(&full[i], 2);
+            bar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            bar_init(&sum_full[i], 1);
+            bar_init(&sum_empty[i], FP_DRAINS / 2);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    pdl_wait();
+    pdl_trigger();
+    bool ok = true;
+    if (warp < FP_FIRST_DRAIN) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");  // 128 x 56 + 256 x 224 = 384 x 168
+        if (warp == 0 || warp == 2) {
+            // blocks of 128 columns in turn: of a warp that issues them all, waits and instructions take 540 cycles a block, its products 192
+            const bool leader = tc5_elect();
+            const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+            const uint64_t ad0 = tc5_desc(tc5_smem_u32(smem));
+            int st = warp >> 1, u = 0;
+            for (int b = warp >> 1; b < blocks; b += 2) {
+                const int q = b & 3, turn = b >> 2;
+                ok = __all_sync(0xFFFFFFFFu, tc5_wait(&full[st], (uint32_t)(u & 1)));
+                if (turn > 0) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&sum_empty[q], (uint32_t)((turn - 1) & 1)));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                const uint64_t ad = ad0 + (uint64_t)((uint32_t)(st * STAGE) >> 4), bd = ad + ((128 * FP8_BLOCK) >> 4);
+                if (leader) {
+#pragma unroll
+                    for (int i = 0; i < FP8_BLOCK / 32; ++i) fp8_mma(tm + (uint32_t)(q * W), ad + 2u * i, bd + 2u * i, fp8_idesc(128, W), i > 0);
+                    tc5_commit(&empty[st]);
+                    tc5_commit(&sum_full[q]);
+                }
+                __syncwarp();
+                if ((st += 2) >= STAGES) { st -= STAGES; ++u; }
+            }
+        } else {
+            // warp 1 copies activations, warp 3 weights
+            if (lane == 0) {
+                const bool x = warp == 1;
+                const CUtensorMap* const map = x ? &map_x : &map_w;
+                const int row = x ? m0 : n0, bytes = (x ? 128 : W) * FP8_BLOCK, place = x ? 0 : 128 * FP8_BLOCK;
+                int issued = 0;
+                for (int st = 0, u = 0; issued < blocks; ++issued) {
+                    if (u > 0) ok = tc5_wait(&empty[st], (uint32_t)((u - 1) & 1));
+                    if (!ok) break;
+                    const uint32_t bar = tc5_smem_u32(&full[st]);
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+                    tc5_tma_2d(tc5_smem_u32(smem + st * STAGE + place), map, issued * FP8_BLOCK, row, bar);
+                    if (++st == STAGES) { st = 0; ++u; }
+                }
+                // nothing is in flight towards this block when it goes on to the end: copies, or the arrivals that follow the last products
+                for (int c = max(0, issued - STAGES); c < issued; ++c) {
+                    uint64_t* const bars = ok ? empty : full;
+                    ok = tc5_wait(&bars[c % STAGES], (uint32_t)((c / STAGES) & 1)) && ok;
+                }
+            }
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
+        const int q4 = warp & 3, group = (warp - FP_FIRST_DRAIN) >> 2, r0 = m0 + 32 * q4;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * q4) << 16);
+        const float* const xs = p.xs + (int64_t)min(r0 + lane, p.m - 1) * blocks;
+        const float* const ws = p.ws + (int64_t)(n0 / FP8_BLOCK) * blocks;
+        uint64_t acc[W / 2];
+#pragma unroll
+        for (int j = 0; j < W / 2; ++j) acc[j] = 0;
+        float xv = group < blocks ? xs[group] : 0.f, wv = group < blocks ? ws[group] : 0.f;
+        for (int b = group; b < blocks; b += 2) {
+            const float f = xv * wv;
+            if (b + 2 < blocks) { xv = xs[b + 2]; wv = ws[b + 2]; }
+            const int q = b & 3;
+            ok = __all_sync(0xFFFFFFFFu, tc5_wait(&sum_full[q], (uint32_t)((b >> 2) & 1)));
+            if (!ok) break;
+            drain_add<W / 32>(lanes + (uint32_t)(q * W), f, acc, peer_smem(tc5_smem_u32(&sum_empty[q]), 0), lane);
+        }
+        // Once all drains are here the products are done and nothing reads the stages any more: in their place the groups exchange half
+        // of their sums, and the results take their way to y. The first group keeps the lower columns.
+        ok = drains_agree(ok);
+        constexpr int LINES = W / 64;  // of 32 f32 columns, that a group keeps
+        uint8_t* const mine = smem + 4096 * LINES * (4 * group + q4);
+        const uint8_t* const others = smem + 4096 * LINES * (4 * (group ^ 1) + q4);
+        auto finish = [&](uint64_t* keep, const uint64_t* give) {
+            if (ok) {
+#pragma unroll
+                for (int i = 0; i < LINES; ++i) put_line<float>(mine + 4096 * i, give + 16 * i, lane);
+            }
+            ok = drains_agree(ok);
+            if (!ok) return;
+#pragma unroll
+            for (int j = 0; j < W / 8; ++j) {
+                const float4 f = *reinterpret_cast<const float4*>(others + 4096 * (j >> 3) + lane * 128 + (((j & 7) ^ (lane & 7)) << 4));
+                const float2 lo = both(keep[2 * j]), hi = both(keep[2 * j + 1]);
+                keep[2 * j] = pair2(make_float2(lo.x + f.x, lo.y + f.y));
+                keep[2 * j + 1] = pair2(make_float2(hi.x + f.z, hi.y + f.w));
+            }
+            // (what this warp gave has its own place: its result goes behind all of those)
+            uint8_t* const out = smem + 4096 * LINES * FP_DRAINS + 4096 * LINES * (4 * group + q4);
+            const int c0 = n0 + W / 2 * group;
+            if (p.bf && LINES == 2) {
+                put_line<bf16>(out, keep, lane);
+                __syncwarp();
+                store_lines<bf16>(p, out, aligned, r0, c0, lane);
+            } else {
+#pragma unroll
+                for (int i = 0; i < LINES; ++i) put_line<float>(out + 4096 * i, keep + 16 * i, lane);
+                __syncwarp();
+                for (int i = 0; i < LINES; ++i) store_f32_lines(p, out + 4096 * i, aligned, r0, c0 + 32 * i, lane);
+            }
+        };
+        if (group == 0) finish(acc, acc + W / 4);
+        else finish(acc + W / 4, acc);
+    }
+    if (!ok) report_wait(p.waits, WAIT_FP8);
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(COLS) : "memory");
 }
 
 // [rows][k] bytes, boxes of 128 columns x box_rows, zeros past the matrix.
@@ -665,20 +913,49 @@ static cudaError_t stream_of(const Fp8MatArgs& a, int parts, cudaStream_t st) {
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
-static cudaError_t pair_of(const Fp8MatArgs& a, cudaStream_t st) {
+template <int G>
+static cudaError_t wide_of(const Fp8MatArgs& a, cudaStream_t st) {
     CUtensorMap mw, mx;
-    if (!fp8_map(&mw, a.wq, a.k, a.n, 64) || !fp8_map(&mx, a.xq, a.k, a.m, 128)) return cudaErrorInvalidValue;
+    if (!fp8_map(&mw, a.wq, a.k, a.n, FP_BN / 2 / G) || !fp8_map(&mx, a.xq, a.k, a.m, 128)) return cudaErrorInvalidValue;
     static PerDeviceOnce once;
-    cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FP_SMEM + 1024); });
+    cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_wide_kernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize, fp_smem(G) + 1024); });
     if (e != cudaSuccess) return e;
-    const int64_t row_tiles = (a.m + FP_BM - 1) / FP_BM, tiles = row_tiles * ((a.n + FP_BN - 1) / FP_BN);
+    const int64_t row_tiles = (a.m + 128 * G - 1) / (128 * G), tiles = row_tiles * ((a.n + FP_BN - 1) / FP_BN);
+    const int most = device_sm_count() / G;
     if (tiles > INT32_MAX / 4) return cudaErrorInvalidValue;
-    // the last round's tiles are halved where all halves find a pair of SMs
-    const int most = device_sm_count() / 2, left = (int)(tiles % most), halved = 2 * left <= most ? left : 0;
-    const bool wide = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * (a.bf ? 2 : 4))) & 15) == 0;
-    const Fp8PairArgs k{a, (int)row_tiles, (int)tiles - halved, (int)tiles + halved, wide};
-    const int pairs = std::min(k.items, most);
-    e = launch_pdl(fp8_pair_kernel, dim3((unsigned)(2 * pairs)), dim3(FP_THREADS), (size_t)(FP_SMEM + 1024), st, k, mw, mx);
+    // the last round's tiles are halved where all halves find a place
+    const int left = (int)(tiles % most), halved = 2 * left <= most ? left : 0;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * (a.bf ? 2 : 4))) & 15) == 0;
+    const Fp8WideArgs k{a, (int)row_tiles, (int)tiles - halved, (int)tiles + halved, aligned, a.k > 1024};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(std::min(k.items, most) * G));
+    cfg.blockDim = dim3(FP_THREADS);
+    cfg.dynamicSmemBytes = (size_t)(fp_smem(G) + 1024);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)G;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = G;
+    e = cudaLaunchKernelEx(&cfg, fp8_wide_kernel<G>, k, mw, mx);
+    return e != cudaSuccess ? e : count_launch_and_check();
+}
+
+template <int W>
+static cudaError_t lone_of(const Fp8MatArgs& a, cudaStream_t st) {
+    CUtensorMap mw, mx;
+    if (!fp8_map(&mw, a.wq, a.k, a.n, W) || !fp8_map(&mx, a.xq, a.k, a.m, 128)) return cudaErrorInvalidValue;
+    constexpr int SMEM = lone_stages(W) * lone_stage(W) + 1024;
+    static_assert(SMEM - 1024 >= 2 * FP_DRAINS * 4096 * (W / 64), "sums and results take the stages' place");
+    static PerDeviceOnce once;
+    cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_lone_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
+    if (e != cudaSuccess) return e;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * (a.bf ? 2 : 4))) & 15) == 0;
+    const dim3 grid((unsigned)((a.n + W - 1) / W), (unsigned)((a.m + 127) / 128));
+    e = launch_pdl(fp8_lone_kernel<W>, grid, dim3(FP_THREADS), (size_t)SMEM, st, a, (int)aligned, mw, mx);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
@@ -700,18 +977,62 @@ static cudaError_t gemv_of(const Fp8MatArgs& a, cudaStream_t st) {
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
+// More than 16 rows, and what the kernel above leaves: the way that takes least time in a model of each, us on 148 SMs, fitted to 1400
+// times of 336 sizes (17 to 2048 rows, 24 matrices of 300 x 512 to 28672 x 4096); what it takes is 1 % over the best way on average.
+// Some of them, bf16 results, us (stream; tiles of 128 x 64 and 128 x 128, one a block; 128 x 256; 256 x 256 by two SMs):
+//    32 x  1024 x  8192    8.6   16.9   19.5   29.0   25.8         256 x  4096 x 4096    -    10.9   12.5   17.2   16.0
+//    64 x  4096 x 14336   17.2   27.4   32.0   48.7   42.8         512 x  4096 x 4096    -      -    13.1   17.4   16.3
+//   128 x  2048 x   512    9.1    4.2    4.9    5.4    5.7         256 x 14336 x 4096    -      -      -    22.6   20.1
+//   128 x 14336 x  4096   24.7     -    15.2   18.9   19.9        2048 x  8192 x 4096    -      -      -    70.1   62.4
+//   128 x 28672 x  4096   37.5     -      -    27.3   36.3
+// Up to 32 rows, tiles of 128 rows pay only where K is short.
+enum Fp8Way { WAY_STREAM, WAY_LONE64, WAY_LONE128, WAY_WIDE1, WAY_WIDE2 };
+static int stream_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
+static int stream_parts(const Fp8MatArgs& a) {
+    const int64_t tiles = (int64_t)((a.n + FS_BM - 1) / FS_BM) * ((a.m + stream_rows(a.m) - 1) / stream_rows(a.m));
+    const int blocks = (int)fp8_blocks(a.k);
+    int parts = 1;
+    while (parts < FS_MAX_PARTS && tiles * parts < device_sm_count() && blocks >= 4 * parts) parts *= 2;
+    return parts;
+}
+static Fp8Way way_of(const Fp8MatArgs& a) {
+    if (a.m <= 16 || (a.m <= 32 && a.k > 1024)) return WAY_STREAM;
+    auto over = [](int64_t v, int by) { return (double)((v + by - 1) / by); };
+    const double sms = device_sm_count(), blocks = (double)fp8_blocks(a.k), weights = (double)a.n * a.k / 6.2e6;
+    Fp8Way best = WAY_WIDE2;
+    double least = 1e30;
+    auto offer = [&](Fp8Way way, double us) {
+        if (us < least) { least = us; best = way; }
+    };
+    for (int g = 1; g <= 2; ++g) {
+        const double teams = floor(sms / g), tiles = over(a.m, 128 * g) * over(a.n, FP_BN), left = fmod(tiles, teams), half = g == 1 ? 0.685 : 0.762;
+        const double rounds = floor(tiles / teams) + (left == 0 ? 0.0 : 2 * left <= teams ? half : 1.0);
+        offer(g == 1 ? WAY_WIDE1 : WAY_WIDE2, g == 1 ? 3.62 + rounds * (0.557 * blocks + 1.47) : 3.77 + rounds * (0.425 * blocks + 1.95));
+    }
+    if (const double tiles = over(a.m, 128) * over(a.n, 64); tiles <= sms) offer(WAY_LONE64, std::max(2.43 + 0.226 * blocks + 2.39 * tiles / sms, 4.7 + weights));
+    if (const double tiles = over(a.m, 128) * over(a.n, 128); tiles <= sms) offer(WAY_LONE128, std::max(2.88 + 0.266 * blocks + 2.48 * tiles / sms, 5.8 + weights));
+    if (a.m <= 128) {
+        const int rows = stream_rows(a.m), parts = stream_parts(a);
+        const double teams = over(a.n, FS_BM) * parts, each = rows == 32 ? 0.442 : rows == 64 ? 0.368 : 0.79;
+        const double load = std::min(std::max(teams / sms, 1.0), 2.0), rounds = over((int64_t)teams, (int)(2 * sms));
+        offer(WAY_STREAM, std::max(3.2 + (parts > 1 ? 0.47 : 0.0) + rounds * (ceil(blocks / parts) * each * (1 + 0.3 * (load - 1)) + 0.038 * a.m), 6.2 + weights));
+    }
+    return best;
+}
+
 cudaError_t launch_fp8_matmul(const Fp8MatArgs& a, cudaStream_t st) {
     if (a.m == 0 || a.n == 0) return cudaSuccess;
     if (a.m < 0 || a.n < 0 || a.k <= 0 || a.k % 16 != 0) return cudaErrorInvalidValue;
-    if (a.m > 128) return pair_of(a, st);
     if (a.m <= 16 && gemv_takes(a)) return gemv_of(a, st);
-    const int bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
-    const int64_t tiles = (int64_t)((a.n + FS_BM - 1) / FS_BM) * ((a.m + bn - 1) / bn);
-    if ((a.m + bn - 1) / bn > 65535) return cudaErrorInvalidValue;
-    const int blocks = (a.k + FP8_BLOCK - 1) / FP8_BLOCK, sms = device_sm_count();
-    int parts = 1;
-    while (parts < FS_MAX_PARTS && tiles * parts < sms && blocks >= 4 * parts) parts *= 2;
-    switch (bn) {
+    switch (way_of(a)) {
+        case WAY_LONE64: return lone_of<64>(a, st);
+        case WAY_LONE128: return lone_of<128>(a, st);
+        case WAY_WIDE1: return wide_of<1>(a, st);
+        case WAY_WIDE2: return wide_of<2>(a, st);
+        case WAY_STREAM: break;
+    }
+    const int parts = stream_parts(a);
+    switch (stream_rows(a.m)) {
         case 16: return stream_of<16>(a, parts, st);
         case 32: return stream_of<32>(a, parts, st);
         case 64: return stream_of<64>(a, parts, st);

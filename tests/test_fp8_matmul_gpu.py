@@ -60,6 +60,19 @@ def test_product(ty, m, n, k):
     assert torch.equal(y, product(*a, ty, 0))  # the stride changes nothing, and twice is the same
 
 
+# a size or two for every way that products take: which kernel, how its columns are shared, whether tiles come in rounds, are halved or
+# leave by warps of their own
+@pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
+@pytest.mark.parametrize("m,n,k", [(8, 9000, 1536), (5, 2000, 8208), (16, 1000, 1040), (12, 4100, 2064), (3, 20000, 1024), (24, 640, 8192), (30, 3000, 512), (48, 1530, 8960),
+                                   (64, 333, 4112), (96, 1536, 8960), (128, 200, 6160), (100, 32000, 896), (128, 28700, 1040), (40, 4000, 640), (128, 9400, 272), (500, 1000, 1040),
+                                   (300, 8200, 1168), (512, 4100, 144), (257, 16500, 528), (2000, 8192, 512), (1500, 8200, 1296), (1300, 5000, 2064), (640, 19000, 1040)])
+def test_every_way(ty, m, n, k):
+    a = inputs(m, n, k, m + n)
+    check(product(*a, ty, 4 * (m % 2)), *a)
+    if m % 4 == 0:
+        check(product(*a, ty, 3), *a)  # rows of y that start anywhere
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 14336, 4096), (24, 28672, 4096), (2048, 4096, 2048), (700, 16400, 1040)])
 def test_large(m, n, k):
     a = inputs(m, n, k, 3)
