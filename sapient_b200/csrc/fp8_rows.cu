@@ -106,18 +106,11 @@ __device__ __forceinline__ float ex2_approx(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v));
     return d;
 }
-// Columns c .. c + 7 of a row; the 16 threads of a block of 128 call together, those past the row with zeros and live false. Multiplied
-// by reciprocals where the definition divides: the scale is off by 2^-23 of itself at most, the quotient by 2^-22, so that of a million
-// values one or two that lie beside a border of the grid fall on its other side; a division takes ten instructions more.
-// y is `factor` times the values given: a norm's one factor for the row need not be multiplied into them.
-__device__ __forceinline__ void quantise8(float (&y)[8], float factor, bool live, int c, uint8_t* q_row, float* scale_row) {
-    float m = max_nan(max_nan(fabsf(y[0]), fabsf(y[1]), fabsf(y[2])), max_nan(fabsf(y[3]), fabsf(y[4]), fabsf(y[5])));
-    m = max_nan(m, fabsf(y[6]), fabsf(y[7]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    const float scale = max_nan(m * factor * (1.f / FP8_MAX), FP8_MIN_SCALE);
-    const float by = factor * rcp_approx(scale);
-    if (!live) return;
+__device__ __forceinline__ float greatest8(const float (&y)[8]) {
+    const float m = max_nan(max_nan(fabsf(y[0]), fabsf(y[1]), fabsf(y[2])), max_nan(fabsf(y[3]), fabsf(y[4]), fabsf(y[5])));
+    return max_nan(m, fabsf(y[6]), fabsf(y[7]));
+}
+__device__ __forceinline__ void store8(float (&y)[8], float by, uint8_t* q) {
     const uint64_t by2 = pack2(by, by);
     uint32_t w[2];
 #pragma unroll
@@ -128,19 +121,55 @@ __device__ __forceinline__ void quantise8(float (&y)[8], float factor, bool live
         const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * i + 2], y[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
         w[i] = lo | hi << 16;
     }
-    *reinterpret_cast<uint2*>(q_row + c) = make_uint2(w[0], w[1]);
-    if ((c & (FP8_BLOCK - 1)) == 0) scale_row[c / FP8_BLOCK] = scale;
+    *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ float scale_of(float greatest, float factor) { return max_nan(greatest * factor * (1.f / FP8_MAX), FP8_MIN_SCALE); }
+
+// Eight columns of a row; the 16 threads of a block of 128 call together, those past the row with zeros and live false. Multiplied by
+// reciprocals where the definition divides: the scale is off by 2^-23 of itself at most, the quotient by 2^-22, so that of a million
+// values one or two that lie beside a border of the grid fall on its other side; a division takes ten instructions more.
+// y is `factor` times the values given: a norm's one factor for the row need not be multiplied into them.
+__device__ __forceinline__ void quantise8(float (&y)[8], float factor, bool live, int lane, uint8_t* q, float* scale_to) {
+    float m = greatest8(y);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const float scale = scale_of(m, factor);
+    if (!live) return;
+    store8(y, factor * rcp_approx(scale), q);
+    if ((lane & 15) == 0) *scale_to = scale;
+}
+// Two times eight columns, of two blocks: half of the 16 threads finish the one's maximum and scale, half the other's. The first thread
+// stores the one's scale, the ninth the other's, where they are given a place.
+__device__ __forceinline__ void quantise8x2(float (&y0)[8], float (&y1)[8], float factor0, float factor1, bool live0, bool live1, int lane, uint8_t* q0, uint8_t* q1,
+                                            float* scale_to0, float* scale_to1) {
+    const float m0 = greatest8(y0), m1 = greatest8(y1);
+    const bool second = lane & 8;
+    float m = max_nan(second ? m1 : m0, __shfl_xor_sync(0xFFFFFFFFu, second ? m0 : m1, 8));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const float factor = second ? factor1 : factor0, scale = scale_of(m, factor), by = factor * rcp_approx(scale), other = __shfl_xor_sync(0xFFFFFFFFu, by, 8);
+    if (live0) store8(y0, second ? other : by, q0);
+    if (live1) store8(y1, second ? by : other, q1);
+    if ((lane & 7) == 0) {
+        float* const to = second ? scale_to1 : scale_to0;
+        if (to) *to = scale;
+    }
 }
 
 // ── RMS norm ──
 __host__ __device__ constexpr int fp8_norm_threads(int nc) { return nc == 1 ? 512 : 1024; }
-// Blocks an SM is to hold: three of bf16 rows of up to 4096 columns (8192 x 4096 with a residual: two 44.8 us, three 40.9).
-__host__ __device__ constexpr int fp8_norm_blocks(int nc, size_t size) { return nc > 1 ? 1 : size == 2 ? 3 : 2; }
+// Blocks an SM is to hold: three of single bf16 rows of up to 4096 columns (8192 x 4096 with a residual: two 44.8 us, three 40.9).
+__host__ __device__ constexpr int fp8_norm_blocks(int nc, int r, size_t size) { return nc > 1 ? 1 : size == 2 && r == 1 ? 3 : 2; }
 
-// blockDim.x / tpr rows at a time, tpr threads (whole warps) a row with NC pieces of eight columns each; a row's values are on their
-// way while the one before is finished.
-template <typename T, int NC>
-__global__ void __launch_bounds__(fp8_norm_threads(NC), fp8_norm_blocks(NC, sizeof(T))) fp8_norm_kernel(const Fp8NormArgs a, int tpr, float inv_dim) {
+// Teams of tpr threads (whole warps) take R rows at a time, NC pieces of eight columns of each a thread; the values of the next rows are
+// on their way while these are finished.
+template <typename T, int NC, int R, bool RES>
+__global__ void __launch_bounds__(fp8_norm_threads(NC), fp8_norm_blocks(NC, R, sizeof(T))) fp8_norm_kernel(const Fp8NormArgs a, int tpr, float inv_dim) {
+    static_assert(R == 1 || NC == 1, "sums of two rows: 16 warps at most");
+    constexpr int P = NC * R;
+    constexpr bool PAIRS = P == 2 && !RES;              // two pieces' scales together: 4096 x 8192 bf16 32.0 us, 26.5; with a residual 43.5 us, 49.5
+    constexpr bool BRANCH = NC == 1 && sizeof(T) == 4;  // a branch around the residual's loads, for what the compiler then keeps in registers:
+                                                        // 600 x 4096 f32 9.0 us, 8.3
     __shared__ float sums[2][32];  // of the warps
     const int tid = threadIdx.x, team = tid / tpr, t = tid - team * tpr, lane = tid & 31;
     const int warps = tpr >> 5, teams = blockDim.x / tpr;
@@ -150,31 +179,31 @@ __global__ void __launch_bounds__(fp8_norm_threads(NC), fp8_norm_blocks(NC, size
     const int nb = (a.dim + FP8_BLOCK - 1) / FP8_BLOCK;
     pdl_wait();
     pdl_trigger();
-    Raw8<T> xv[NC], rv[NC];
+    Raw8<T> xv[P], rv[RES ? P : 1];
     auto fetch = [&](int64_t row) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = (t + i * tpr) * 8;
-            if (row < a.rows && c < a.dim) {
-                xv[i] = ld8(x + row * a.ldx + c);
-                if (res) rv[i] = ld8(res + row * a.ldr + c);
+        for (int i = 0; i < P; ++i) {
+            const int c = (t + i % NC * tpr) * 8;
+            if (row + i / NC < a.rows && c < a.dim) {
+                xv[i] = ld8(x + (row + i / NC) * a.ldx + c);
+                if (RES && (!BRANCH || res)) rv[i] = ld8(res + (row + i / NC) * a.ldr + c);
             }
         }
     };
-    const int64_t step = (int64_t)gridDim.x * teams;
-    if (NC < 4) fetch((int64_t)blockIdx.x * teams + team);
+    const int64_t step = (int64_t)gridDim.x * teams * R;
+    if (NC < 4) fetch(((int64_t)blockIdx.x * teams + team) * R);
     int par = 0;
-    for (int64_t row0 = (int64_t)blockIdx.x * teams; row0 < a.rows; row0 += step, par ^= 1) {
-        const int64_t row = row0 + team;
-        const bool have = row < a.rows;
+    for (int64_t row0 = (int64_t)blockIdx.x * teams * R; row0 < a.rows; row0 += step, par ^= 1) {
+        const int64_t row = row0 + team * R;
         if (NC == 4) fetch(row);  // (no registers for two rows)
-        float h[NC][8];
+        float h[P][8];
+        bool live[P];
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = (t + i * tpr) * 8;
-            if (have && c < a.dim) {
+        for (int i = 0; i < P; ++i) {
+            live[i] = row + i / NC < a.rows && (t + i % NC * tpr) * 8 < a.dim;
+            if (live[i]) {
                 unpack8(xv[i], h[i]);
-                if (res) {
+                if (RES && (!BRANCH || res)) {
                     float r[8];
                     unpack8(rv[i], r);
 #pragma unroll
@@ -186,43 +215,80 @@ __global__ void __launch_bounds__(fp8_norm_threads(NC), fp8_norm_blocks(NC, size
             }
         }
         if (NC < 4) fetch(row + step);
-        uint64_t squares = 0;
+        float ss[R];
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = (t + i * tpr) * 8;
-            if (sum_out && have && c < a.dim) st8(sum_out + row * a.lds + c, h[i]);
+        for (int r = 0; r < R; ++r) {
+            uint64_t squares = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) square2(squares, h[i][j], h[i][j + 1]);
-        }
-        float even, odd;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(even), "=f"(odd) : "l"(squares));
-        float ss = warp_sum(even + odd);
-        if (warps > 1) {
-            if (lane == 0) sums[par][team * warps + (t >> 5)] = ss;
-            __syncthreads();
-            ss = warp_sum(lane < warps ? sums[par][team * warps + lane] : 0.f);
-        }
-        const float rms = rsqrtf(fmaf(ss, inv_dim, a.eps));
-        uint8_t* const q_row = a.q + row * a.dim;
-        float* const scale_row = a.scale + row * nb;
+            for (int i = r * NC; i < (r + 1) * NC; ++i) {
+                if (sum_out && live[i]) st8(sum_out + (row + r) * a.lds + (t + i % NC * tpr) * 8, h[i]);
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = (t + i * tpr) * 8;
-            const bool live = have && c < a.dim;
-            if (live && a.w) {
-                const ulonglong2 w0 = __ldg(reinterpret_cast<const ulonglong2*>(a.w + c)), w1 = __ldg(reinterpret_cast<const ulonglong2*>(a.w + c + 4));
-                mul2(h[i][0], h[i][1], w0.x);
-                mul2(h[i][2], h[i][3], w0.y);
-                mul2(h[i][4], h[i][5], w1.x);
-                mul2(h[i][6], h[i][7], w1.y);
+                for (int j = 0; j < 8; j += 2) square2(squares, h[i][j], h[i][j + 1]);
             }
-            // (past the row zeros, whose norm may be infinite: a factor of 1)
-            quantise8(h[i], live ? rms : 1.f, live, c, q_row, scale_row);
+            float even, odd;
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(even), "=f"(odd) : "l"(squares));
+            ss[r] = even + odd;
+        }
+        float rms[R];
+        if constexpr (R == 1) {
+            float s = warp_sum(ss[0]);
+            if (warps > 1) {
+                if (lane == 0) sums[par][team * warps + (t >> 5)] = s;
+                __syncthreads();
+                s = warp_sum(lane < warps ? sums[par][team * warps + lane] : 0.f);
+            }
+            rms[0] = rsqrtf(fmaf(s, inv_dim, a.eps));
+        } else {  // half of a warp's threads finish the one row's sum, half the other's
+            const bool second = lane & 16;
+            float s = (second ? ss[1] : ss[0]) + __shfl_xor_sync(0xFFFFFFFFu, second ? ss[0] : ss[1], 16);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            if (warps > 1) {
+                const int half = second ? 16 : 0;
+                if ((lane & 15) == 0) sums[par][half + team * warps + (t >> 5)] = s;
+                __syncthreads();
+                s = (lane & 15) < warps ? sums[par][half + team * warps + (lane & 15)] : 0.f;
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            }
+            const float mine = rsqrtf(fmaf(s, inv_dim, a.eps)), other = __shfl_xor_sync(0xFFFFFFFFu, mine, 16);
+            rms[0] = second ? other : mine;
+            rms[1] = second ? mine : other;
+        }
+        uint8_t* q[P];
+        float* scale[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int c = (t + i % NC * tpr) * 8;
+            q[i] = a.q + (row + i / NC) * a.dim + c;
+            scale[i] = a.scale + (row + i / NC) * nb + c / FP8_BLOCK;
+        }
+        if (a.w) {
+            ulonglong2 w0, w1;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const int c = (t + i % NC * tpr) * 8;
+                if (c < a.dim) {
+                    if (i < NC) w0 = __ldg(reinterpret_cast<const ulonglong2*>(a.w + c)), w1 = __ldg(reinterpret_cast<const ulonglong2*>(a.w + c + 4));
+                    mul2(h[i][0], h[i][1], w0.x);
+                    mul2(h[i][2], h[i][3], w0.y);
+                    mul2(h[i][4], h[i][5], w1.x);
+                    mul2(h[i][6], h[i][7], w1.y);
+                }
+            }
+        }
+        if constexpr (PAIRS) {
+            // the first thread of a block decides for the ninth, which stores the second scale
+            const bool there = row + 1 / NC < a.rows && (t - (lane & 15) + 1 % NC * tpr) * 8 < a.dim;
+            quantise8x2(h[0], h[1], rms[0], rms[R - 1], live[0], live[1], lane, q[0], q[1], live[0] ? scale[0] : nullptr, there ? scale[1] : nullptr);
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i) quantise8(h[i], rms[i / NC], live[i], lane, q[i], scale[i]);
         }
     }
 }
 
-template <typename T, int NC>
+template <typename T, int NC, int R, bool RES>
 static cudaError_t norm_with(const Fp8NormArgs& a, cudaStream_t st) {
     const int tpr = ((a.dim + 8 * NC - 1) / (8 * NC) + 31) / 32 * 32;
     const int teams = std::max(1, 256 / tpr), threads = teams * tpr;
@@ -231,24 +297,26 @@ static cudaError_t norm_with(const Fp8NormArgs& a, cudaStream_t st) {
     std::atomic<int>& known = resident[current_device_index()][threads / 32];
     int per_sm = known.load(std::memory_order_relaxed);
     if (per_sm == 0) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fp8_norm_kernel<T, NC>, threads, 0);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fp8_norm_kernel<T, NC, R, RES>, threads, 0);
         if (e != cudaSuccess) return e;
         known.store(per_sm = std::max(1, per_sm), std::memory_order_relaxed);
     }
-    const dim3 grid((unsigned)std::min<int64_t>((a.rows + teams - 1) / teams, (int64_t)device_sm_count() * per_sm));
-    const cudaError_t e = launch_pdl(fp8_norm_kernel<T, NC>, grid, dim3((unsigned)threads), 0, st, a, tpr, 1.f / (float)a.dim);
+    const dim3 grid((unsigned)std::min<int64_t>((a.rows + teams * R - 1) / (teams * R), (int64_t)device_sm_count() * per_sm));
+    const cudaError_t e = launch_pdl(fp8_norm_kernel<T, NC, R, RES>, grid, dim3((unsigned)threads), 0, st, a, tpr, 1.f / (float)a.dim);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
-template <typename T>
+template <typename T, bool RES>
 static cudaError_t norm_of(const Fp8NormArgs& a, cudaStream_t st) {
-    return a.dim <= 4096 ? norm_with<T, 1>(a, st) : a.dim <= 16384 ? norm_with<T, 2>(a, st) : norm_with<T, 4>(a, st);
+    if (a.dim > 4096) return a.dim <= 16384 ? norm_with<T, 2, 1, RES>(a, st) : norm_with<T, 4, 1, RES>(a, st);
+    return norm_with<T, 1, RES ? 1 : 2, RES>(a, st);  // instructions bound rows without a residual, bytes the others: 8192 x 4096 bf16, one row 27.9 us, two 23.1; with it 39.9 and 40.5
 }
 
 cudaError_t launch_fp8_norm(const Fp8NormArgs& a, bool bf, cudaStream_t st) {
     if (a.rows == 0) return cudaSuccess;
     if (a.dim <= 0 || a.dim % 16 != 0 || a.dim > FP8_NORM_MAX_DIM) return cudaErrorInvalidValue;
-    return bf ? norm_of<bf16>(a, st) : norm_of<float>(a, st);
+    if (bf) return a.residual ? norm_of<bf16, true>(a, st) : norm_of<bf16, false>(a, st);
+    return a.residual ? norm_of<float, true>(a, st) : norm_of<float, false>(a, st);
 }
 
 // ── SwiGLU, or rows as they are ──
@@ -284,8 +352,7 @@ __global__ void __launch_bounds__(128) fp8_quant_kernel(const T* x, int64_t ldx,
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] = 0.f;
             }
-            // (the offset within the block decides who stores the scale: 128 columns before c are whole blocks)
-            quantise8(y, 1.f, live, (int)(c & (FP8_BLOCK - 1)), q + (row0 + i) * dim + (c & ~(int64_t)(FP8_BLOCK - 1)), scale + (row0 + i) * nb + c / FP8_BLOCK);
+            quantise8(y, 1.f, live, threadIdx.x & 31, q + (row0 + i) * dim + c, scale + (row0 + i) * nb + c / FP8_BLOCK);
         }
     }
 }
