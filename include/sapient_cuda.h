@@ -186,9 +186,10 @@ int32_t sp_cuda_matmul_fp8(int32_t device, const void* xq, const float* xs, int6
 int32_t sp_cuda_logprobs(int32_t device, const float* logits, int64_t rows, int64_t vocab, const uint32_t* ids, int32_t top,
                          float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs);
 /* A weight of type SP_F8_E4M3: values[n][k] and scales[ceil(n / 128)][ceil(k / 128)] from host memory. sp_cuda_matmul_nt and
- * _matmul_nt_dev quantise the rows of x to fp8 first (in a workspace that the weight carries and that grows with m, so that what
- * sp_cuda_matmul_nt_dev says of streams and of first calls holds for it; y must not overlap x); sp_cuda_dequant, _weight_info and
- * _free_weight work as for the other types. Not a table for sp_cuda_embed. */
+ * _matmul_nt_dev quantise the rows of x to fp8 first, in a workspace that the weight carries: calls on one weight are ordered on one
+ * stream, as sp_cuda_matmul_nt_dev says, and so are replays of graphs that hold some. It grows with m: the first call with more rows
+ * than before allocates and cannot be captured (SP_ERR_STATE); graphs captured earlier keep what they use until _free_weight. y must
+ * not overlap x. sp_cuda_dequant, _weight_info and _free_weight work as for the other types. Not a table for sp_cuda_embed. */
 int32_t sp_cuda_upload_weight_fp8(int32_t device, int64_t n, int64_t k, const void* values, const float* scales, SpWeight** out);
 
 /* ── engine level: replaces ForwardEngine (crates/sapient-models/src/forward/mod.rs:49-65,381-506)

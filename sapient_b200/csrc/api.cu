@@ -29,6 +29,7 @@ struct SpWeight {
     float* scale = nullptr;    // SP_F8_E4M3: the blocks' scales
     uint8_t* xq = nullptr;     // and the activations as fp8 rows, their scales behind them
     int64_t xq_rows = 0;       // rows there is room for
+    std::vector<uint8_t*> xq_before;  // smaller ones, which captured graphs may use
 };
 struct SpEngine {
     Engine* e;
@@ -120,7 +121,9 @@ struct OnDevice {
     cudaError_t enter(int device) {
         cudaError_t e = cudaGetDevice(&before);
         if (e != cudaSuccess) before = -1;
-        return e != cudaSuccess || before == device ? e : cudaSetDevice(device);
+        if (e == cudaSuccess && before != device) e = cudaSetDevice(device);
+        if (e != cudaSuccess) cudaGetLastError();  // (the next launch would find it)
+        return e;
     }
     ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
 };
@@ -358,6 +361,7 @@ void sp_cuda_free_weight(SpWeight* w) {
     cudaFree(w->d);
     cudaFree(w->scale);
     cudaFree(w->xq);
+    for (uint8_t* p : w->xq_before) cudaFree(p);
     if (w->tiled) cudaFree(w->tiled);
     w->ws.release();
     w->ring.release();
@@ -396,10 +400,14 @@ static int matmul_nt_fp8(SpWeight* w, const float* x, int64_t m, float* y, cudaS
         cudaStreamCaptureStatus capturing;
         SP_CUDA_TRY(cudaStreamIsCapturing(st, &capturing));
         if (capturing != cudaStreamCaptureStatusNone) { set_error("matmul: the first call with this many rows allocates and cannot be captured"); return SP_ERR_STATE; }
-        const int64_t rows = (m + 127) / 128 * 128;
+        const int64_t rows = std::max((m + 127) / 128 * 128, 2 * w->xq_rows);  // (doubled: the smaller ones take no more than the last)
+        if (w->xq) w->xq_before.reserve(w->xq_before.size() + 1);
         uint8_t* p = nullptr;
-        SP_CUDA_TRY(cudaMalloc((void**)&p, rows * (row + 4 * scales)));
-        cudaFree(w->xq);  // (waits for the work that uses it)
+        if (const cudaError_t e = cudaMalloc((void**)&p, rows * (row + 4 * scales)); e != cudaSuccess) {
+            cudaGetLastError();
+            SP_CUDA_TRY(e);
+        }
+        if (w->xq) w->xq_before.push_back(w->xq);
         w->xq = p;
         w->xq_rows = rows;
     }
