@@ -6,11 +6,17 @@
 // The maximum's own 1 is kept out of R: where one token has nearly all of the mass, R and T are small numbers of full precision, and
 // so are the two results. Sums are f32 per thread (a few hundred terms) and joined in a fixed order.
 //
-// A row is read by one block, or by a cluster of up to 16 where rows are few; bytes bound it from some hundred rows on, latency below.
-// The largest ones are found on the way: a value that does not exceed the block's threshold, a lower bound of the `top`-th largest
-// that rises as the row goes by, costs one comparison of a thread's 16 values' maximum; the others go to a buffer in shared memory,
-// which is cut to the `top` largest when it fills. Keys (value, then lower index) are distinct, so that the order in which threads push
-// changes nothing. The first threshold is the least of the maxima of 8 or 32 groups of threads: at least that many values reach it.
+// A row is read by one block, or shared by a cluster of up to 16 where rows are few; its values pass through a ring of asynchronous
+// copies in shared memory, 16 a thread at a time. The maximum is a warp's: of a row of random values a thread would find a new one of
+// its own in most of its steps, and all of the warp would rescale. The `top` largest cost the reading pass a comparison a value: a
+// thread keeps the maxima of a quarter each of what it reads (cells); afterwards the `top`-th largest of the maxima of groups of threads
+// is a bound which that many values reach, the few cells that reach it are read again, from L2, and the values above it are ranked.
+// Keys (value, then lower index) are distinct, so that no order of threads changes the result.
+//
+// Bytes bound it from some hundred rows on, with the exponentials close behind (16 a cycle and SM); below that the chain of steps does,
+// a good part of it instructions that are fetched for the first time, so that what runs once is kept short. us (floor at 6.54 TB/s):
+//   1024 x 128256 f32 top 1      91.0 (80.3)     32 x 128256 bf16 top 20   10.8 (1.3)      1 x 151936 f32 top 5    7.2 (0.1)
+//   1024 x 128256 bf16 top 20    68.9 (40.2)     64 x 128256 bf16 top 1    11.2 (2.5)      1 x 151936 f32 top 0    4.6 (0.1)
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -32,7 +38,7 @@ constexpr int LP_STAGES = 3;          // chunks of a block on their way or in us
 constexpr int LP_BUF = 256;           // candidates for the largest
 constexpr int LP_CELLS = 4;           // maxima a thread keeps
 constexpr int LP_QUEUE = 512;         // of them that can be read again
-constexpr int LP_MAX_PARTS = 8;       // blocks of a row
+constexpr int LP_MAX_PARTS = 16;      // blocks of a row
 constexpr float LP_LOW = -200.f;      // lp_exp is zero from here down; keeps 0 x infinity out of T
 constexpr unsigned LP_ALL = 0xFFFFFFFFu;
 
@@ -83,27 +89,16 @@ __device__ __forceinline__ LpSums lp_shfl(const LpSums& a, int o) {
     return LpSums{__shfl_xor_sync(LP_ALL, a.m, o), __shfl_xor_sync(LP_ALL, a.r, o), __shfl_xor_sync(LP_ALL, a.t, o), __shfl_xor_sync(LP_ALL, a.bad, o)};
 }
 
-// The nth largest (from 0) of a warp's values.
-__device__ __forceinline__ uint32_t lp_nth(uint32_t v, int nth, int lane) {
-    int rank = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const uint32_t o = __shfl_sync(LP_ALL, v, i);
-        rank += o > v || (o == v && i < lane);
-    }
-    return __shfl_sync(LP_ALL, v, __ffs(__ballot_sync(LP_ALL, rank == nth)) - 1);
-}
-
-struct LpShared {
-    float cells[LP_CELLS][LP_THREADS];
-    uint64_t inbox[LP_MAX_PARTS * LOGPROBS_MAX_TOP];  // of a cluster's first block: every part's largest
-    LpSums parts[LP_MAX_PARTS];                       // and sums
+struct __align__(16) LpShared {
+    LpSums parts[LP_MAX_PARTS];  // of a cluster's first block
     LpSums sums[LP_WARPS];
+    float cells[LP_CELLS][LP_THREADS];
+    uint32_t low;
     int count, queued;
 };
 // In the ring's place once the row has been read.
-struct LpTail {
-    uint64_t buf[LP_BUF];
+struct __align__(16) LpTail {
+    uint64_t buf[LP_BUF + 4];
     uint64_t list[LOGPROBS_MAX_TOP];  // the result
     union {
         uint32_t first[LP_THREADS];
@@ -111,18 +106,23 @@ struct LpTail {
     };
 };
 
-// The largest of n keys (0: none), sorted, to list: a key's place is the number of greater ones. Every thread calls.
-__device__ __forceinline__ void lp_largest(const uint64_t* keys, int n, uint64_t* list, int tid) {
+// The largest of n keys, sorted, to list: a key's place is the number of greater ones. Every thread calls; room for four more keys.
+__device__ __forceinline__ void lp_largest(uint64_t* keys, int n, uint64_t* list, int tid) {
     const uint64_t mine = tid < n ? keys[tid] : 0;
     if (tid < LOGPROBS_MAX_TOP) list[tid] = 0;
+    if (tid < 4) keys[n + tid] = 0;
     __syncthreads();
-    int rank = 0;
-    if (tid / 32 * 32 < n)
-        for (int i = 0; i < n; ++i) rank += keys[i] > mine;
-    if (mine && rank < LOGPROBS_MAX_TOP) list[rank] = mine;
+    if (tid / 32 * 32 < n) {
+        int rank = 0;
+        const ulonglong2* const pairs = reinterpret_cast<const ulonglong2*>(keys);
+        for (int i = 0; i < n; i += 4) {
+            const ulonglong2 u = pairs[i / 2], v = pairs[i / 2 + 1];
+            rank += (u.x > mine) + (u.y > mine) + (v.x > mine) + (v.y > mine);
+        }
+        if (mine && rank < LOGPROBS_MAX_TOP) list[rank] = mine;
+    }
     __syncthreads();
 }
-
 __device__ __forceinline__ void lp_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void lp_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 // The same place in the cluster's first block.
@@ -135,24 +135,6 @@ __device__ __forceinline__ uint32_t lp_first(const void* p) {
 // Copies a whole 16-byte piece of a row to shared memory, without waiting.
 __device__ __forceinline__ void lp_copy(uint4* to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-// A 16-byte piece of a row whose first value has index e0: nothing outside the row's n values is read.
-template <typename T>
-__device__ __forceinline__ uint4 lp_piece(const T* row, int64_t e0, int n) {
-    constexpr int VEC = 16 / sizeof(T);
-    if (e0 >= 0 && e0 + VEC <= n) return *reinterpret_cast<const uint4*>(row + e0);
-    union {
-        uint4 all;
-        uint16_t half[8];
-        uint32_t word[4];
-    } v;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        const T x = e0 + i >= 0 && e0 + i < n ? row[e0 + i] : (T)-INFINITY;
-        if constexpr (sizeof(T) == 2) v.half[i] = *reinterpret_cast<const uint16_t*>(&x);
-        else v.word[i] = *reinterpret_cast<const uint32_t*>(&x);
-    }
-    return v.all;
 }
 __device__ __forceinline__ void lp_unpack(const uint4& f, float* v, float) {
     v[0] = __uint_as_float(f.x); v[1] = __uint_as_float(f.y); v[2] = __uint_as_float(f.z); v[3] = __uint_as_float(f.w);
@@ -180,6 +162,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     const int pieces = (int)(((int64_t)skew + a.n + VEC - 1) / VEC), per = (pieces + parts - 1) / parts;
     const int begin = min(part * per, pieces), end = min(begin + per, pieces);
     LpTail& tail = *reinterpret_cast<LpTail*>(lp_ring);
+    uint64_t* const inbox = reinterpret_cast<uint64_t*>(lp_ring + LP_STAGES * PIECES * LP_THREADS);  // of a cluster's first block: every part's largest
     if (TOP && tid == 0) sh.count = sh.queued = 0;
     if (parts > 1) lp_cluster_arrive();  // (waited for before a peer's memory is written: all blocks run by then)
     pdl_wait();
@@ -206,7 +189,13 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
                 if (p < end && e0 >= 0 && e0 + VEC <= a.n) {
                     lp_copy(to, row + e0);
                 } else {  // past the part, or a piece that hangs over an end of the row: masked values in the others' places
-                    *to = lp_piece(row, e0, p < end ? a.n : 0);
+                    constexpr uint32_t MASKED = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+                    *to = make_uint4(MASKED, MASKED, MASKED, MASKED);
+                    if (p < end) {
+#pragma unroll 1
+                        for (int i = 0; i < VEC; ++i)
+                            if (e0 + i >= 0 && e0 + i < a.n) reinterpret_cast<T*>(to)[i] = row[e0 + i];
+                    }
                 }
             }
         }
@@ -282,16 +271,38 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     if (lane == 0) sh.sums[warp] = s;
     __syncthreads();
     if (TOP) {
-        // a first threshold: the `top`-th largest of the maxima of 32 groups of eight threads, which that many values reach
+        // a first threshold: the `top`-th largest of the maxima of 32 groups of eight threads, which that many values reach; of 64
+        // where that would be about the least of them (64 rows of 128256 bf16, top 32: 41.8 us, 13.6; they cost others 0.4 us)
+        float cells[LP_CELLS];
         peak = -INFINITY;
-        for (int j = 0; j < n_cells; ++j) peak = lp_max(peak, sh.cells[j][tid]);
+#pragma unroll
+        for (int j = 0; j < LP_CELLS; ++j) {
+            cells[j] = j < n_cells ? sh.cells[j][tid] : -INFINITY;
+            peak = lp_max(peak, cells[j]);
+        }
         tail.first[tid] = lp_mono(peak);
         __syncthreads();
-        uint32_t m = tail.first[lane];
+        auto rank_groups = [&](uint32_t m0, uint32_t m1, int groups) {  // (each warp looks at its share of the groups)
+#pragma unroll 4
+            for (int i = 0; i < groups / LP_WARPS; ++i) {
+                const int c = warp * (groups / LP_WARPS) + i;
+                const uint32_t v = __shfl_sync(LP_ALL, c < 32 ? m0 : m1, c & 31);
+                int greater = __popc(__ballot_sync(LP_ALL, m0 > v || (m0 == v && lane < c)));
+                if (groups > 32) greater += __popc(__ballot_sync(LP_ALL, m1 > v || (m1 == v && lane + 32 < c)));
+                if (greater == a.top - 1 && lane == 0) sh.low = v;
+            }
+        };
+        uint32_t m[2];
 #pragma unroll
-        for (int w = 1; w < LP_WARPS; ++w) m = max(m, tail.first[w * 32 + lane]);
+        for (int h = 0; h < 2; ++h) {
+            m[h] = tail.first[h * (LP_THREADS / 2) + lane];
+#pragma unroll
+            for (int w = 1; w < LP_WARPS / 2; ++w) m[h] = max(m[h], tail.first[h * (LP_THREADS / 2) + w * 32 + lane]);
+        }
+        if (a.top <= 24) rank_groups(max(m[0], m[1]), 0, 32);
+        else rank_groups(m[0], m[1], 64);
         __syncthreads();  // (the maxima's place is the queue's)
-        uint64_t threshold = (uint64_t)lp_nth(m, a.top - 1, lane) << 32;
+        uint64_t threshold = (uint64_t)sh.low << 32;
         float low = lp_value((uint32_t)(threshold >> 32));
         // A value to the buffer, if it is a candidate: 0, there was room; 1, the buffer fills; 2, it is full.
         auto push = [&](float v, int id) {
@@ -302,39 +313,49 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
             if (at < LP_BUF) tail.buf[at] = key;
             return at < LP_BUF / 2 ? 0 : at < LP_BUF ? 1 : 2;
         };
-        // the cells whose maximum is not below the threshold are read again, each by a warp, a piece a lane
-        for (int j = 0; j < n_cells; ++j)
-            if (!(sh.cells[j][tid] < low)) {
+        // the cells whose maximum is not below the threshold are read again, a piece a thread
+#pragma unroll
+        for (int j = 0; j < LP_CELLS; ++j)
+            if (j < n_cells && !(cells[j] < low)) {
                 const int at = atomicAdd(&sh.queued, 1);
                 if (at < LP_QUEUE) tail.queue[at] = (uint16_t)(j * LP_THREADS + tid);
             }
         __syncthreads();
-        const int queued = sh.queued, cell_pieces = cell * PIECES;
+        const int queued = sh.queued, cell_pieces = cell * PIECES, items = min(queued, LP_QUEUE) * cell_pieces;
         bool over = queued > LP_QUEUE;
-        constexpr int AHEAD = 4;  // cells of a warp on their way
-        for (int q0 = warp; !over && q0 < queued; q0 += AHEAD * LP_WARPS)
-            for (int u = lane; u < cell_pieces; u += 32) {
-                uint4 got[AHEAD];
-                int piece[AHEAD];
+        constexpr int AHEAD = 4;  // pieces of a thread on their way
+        for (int i0 = tid; !over && i0 < items; i0 += AHEAD * LP_THREADS) {
+            // (one copy of what follows a candidate, not one for each value: it runs once, and its instructions have to be fetched)
+            auto piece_of = [&](int e) {
+                const int i = i0 + e * LP_THREADS, q = i / cell_pieces, u = i - q * cell_pieces;
+                if (i >= items) return end;
+                const int from = tail.queue[q], k = from / LP_THREADS * cell + u / PIECES;
+                return k < chunks ? begin + k * STEP + u % PIECES * LP_THREADS + from % LP_THREADS : end;
+            };
+            uint4 got[AHEAD];
+            uint32_t edge = 0, reach = 0;
 #pragma unroll
-                for (int e = 0; e < AHEAD; ++e) {
-                    const int q = q0 + e * LP_WARPS;
-                    piece[e] = end;
-                    if (q >= queued) continue;
-                    const int from = tail.queue[q], k = from / LP_THREADS * cell + u / PIECES;
-                    piece[e] = k < chunks ? begin + k * STEP + u % PIECES * LP_THREADS + from % LP_THREADS : end;
-                    got[e] = lp_piece(row, (int64_t)piece[e] * VEC - skew, piece[e] < end ? a.n : 0);
-                }
-#pragma unroll
-                for (int e = 0; e < AHEAD; ++e) {
-                    if (piece[e] >= end) continue;
-                    float v[VEC];
-                    lp_unpack(got[e], v, T());
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i)
-                        if (!(v[i] < low)) over |= push(v[i], piece[e] * VEC - skew + i) == 2;
-                }
+            for (int e = 0; e < AHEAD; ++e) {
+                const int p = piece_of(e), e0 = p * VEC - skew;
+                if (p < end && e0 >= 0 && e0 + VEC <= a.n) got[e] = *reinterpret_cast<const uint4*>(row + e0);
+                else edge |= (p < end) << e;
             }
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e) {
+                float v[VEC];
+                lp_unpack(got[e], v, T());
+                uint32_t mask = 0;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) mask |= !(v[i] < low) << i;
+                if (i0 + e * LP_THREADS >= items) mask = 0;
+                if (edge >> e & 1) mask = (1u << VEC) - 1;
+                reach |= mask << e * VEC;
+            }
+            for (; reach; reach &= reach - 1) {
+                const int at = __ffs(reach) - 1, p = piece_of(at / VEC), id = p * VEC - skew + at % VEC;
+                if (p < end && id >= 0 && id < a.n) over |= push((float)row[id], id) == 2;
+            }
+        }
         if (__syncthreads_or(over)) {
             // More candidates than places (many equal logits at the top): once more, a chunk at a time, cut back to the largest between.
             if (tid == 0) sh.count = 0;
@@ -365,7 +386,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     }
     if (warp == 0) {
         s = sh.sums[lane & (LP_WARPS - 1)];
-#pragma unroll
+#pragma unroll 1
         for (int o = LP_WARPS / 2; o > 0; o >>= 1) s = lp_join(s, lp_shfl(s, o));
     }
     if (parts > 1) {
@@ -376,7 +397,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
                 const uint32_t to = lp_first(&sh.parts[part]);
                 asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(__float_as_uint(s.m)), "r"(__float_as_uint(s.r)), "r"(__float_as_uint(s.t)), "r"(s.bad) : "memory");
             }
-            if (TOP && lane < a.top) asm volatile("st.shared::cluster.u64 [%0], %1;\n" ::"r"(lp_first(&sh.inbox[part * a.top + lane])), "l"(tail.list[lane]) : "memory");
+            if (TOP && lane < a.top) asm volatile("st.shared::cluster.u64 [%0], %1;\n" ::"r"(lp_first(&inbox[part * a.top + lane])), "l"(tail.list[lane]) : "memory");
         }
         __syncwarp();
         lp_cluster_arrive();
@@ -384,10 +405,10 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
         if (part != 0) return;
         if (warp == 0) {
             s = (lane & (LP_MAX_PARTS - 1)) < parts ? sh.parts[lane & (LP_MAX_PARTS - 1)] : LpSums{-INFINITY, 0.f, 0.f, 0};
-#pragma unroll
+#pragma unroll 1
             for (int o = LP_MAX_PARTS / 2; o > 0; o >>= 1) s = lp_join(s, lp_shfl(s, o));
         }
-        if (TOP) lp_largest(sh.inbox, parts * a.top, tail.list, tid);
+        if (TOP) lp_largest(inbox, parts * a.top, tail.list, tid);
     }
     const uint64_t best = TOP && warp == 0 ? tail.list[lane] : 0;
     if (warp != 0) return;
@@ -407,13 +428,17 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
 template <typename T>
 static cudaError_t logprobs_of(const LogprobsArgs& a, cudaStream_t st) {
     const int sms = device_sm_count();
+    // up to two blocks an SM; 16 where rows are few and there are few keys to rank (8 x 128256 f32, 8 parts and 16: top 5 7.9 us, 7.7;
+    // top 16 8.6 us, 10.3; 1 x 151936 top 0 5.9 us, 4.6)
     int parts = 1;
-    while (parts < LP_MAX_PARTS && a.rows * parts * 2 <= 2 * sms && a.n / (parts * 2) >= LP_CHUNK) parts *= 2;
+    while (parts < 8 && a.rows * parts * 2 <= 2 * sms && a.n / (parts * 2) >= LP_CHUNK) parts *= 2;
+    if (parts == 8 && a.rows * 16 <= sms && a.n / 16 >= LP_CHUNK && a.top <= 8) parts = 16;
     if (a.rows * parts > INT32_MAX) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * parts));
     cfg.blockDim = dim3(LP_THREADS);
-    cfg.dynamicSmemBytes = LP_STAGES * LP_CHUNK * sizeof(T);
+    constexpr size_t ring = LP_STAGES * LP_CHUNK * sizeof(T), most = ring + (LP_THREADS + 4) * sizeof(uint64_t);
+    cfg.dynamicSmemBytes = parts > 1 ? ring + (parts * a.top + 4) * sizeof(uint64_t) : ring;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -425,8 +450,12 @@ static cudaError_t logprobs_of(const LogprobsArgs& a, cudaStream_t st) {
     cfg.numAttrs = parts > 1 ? 2 : 1;
     static PerDeviceOnce once;
     cudaError_t e = once.run([] {
-        const cudaError_t f = cudaFuncSetAttribute(logprobs_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_STAGES * LP_CHUNK * sizeof(T));
-        return f != cudaSuccess ? f : cudaFuncSetAttribute(logprobs_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_STAGES * LP_CHUNK * sizeof(T));
+        for (const auto kernel : {logprobs_kernel<T, true>, logprobs_kernel<T, false>}) {
+            cudaError_t f = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+            if (f == cudaSuccess) f = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);  // (more than eight blocks)
+            if (f != cudaSuccess) return f;
+        }
+        return cudaSuccess;
     });
     if (e != cudaSuccess) return e;
     e = a.top > 0 ? cudaLaunchKernelEx(&cfg, logprobs_kernel<T, true>, a, parts) : cudaLaunchKernelEx(&cfg, logprobs_kernel<T, false>, a, parts);

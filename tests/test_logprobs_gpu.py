@@ -69,6 +69,17 @@ def test_rows_that_start_anywhere(ty, ld, off):
 
 
 @pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
+@pytest.mark.parametrize("rows,n,top", [(1, 65536, 8), (1, 65537, 0), (2, 70001, 1), (9, 131072, 5), (10, 131073, 8), (1, 262147, 9), (1, 400000, 24), (3, 90000, 25), (1, 66000, 32), (16, 50257, 31)])
+@pytest.mark.parametrize("off", [0, 1, 6])
+def test_few_long_rows(ty, rows, n, top, off):
+    z, ids = logits(rows, n, ty, rows + n, n + 3, off)
+    check(z, ids, top)
+    z[:, :: n // 40] = 9.0  # as many equal maxima as are asked for, in all parts
+    z[0, n - 1] = 9.5
+    check(z, ids, top)
+
+
+@pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
 @pytest.mark.parametrize("n", [5000, 70000])
 def test_orders_and_ties(ty, n):
     """Ascending rows push every value, constant ones tie everywhere, steps tie in long runs; the lowest id comes first."""
