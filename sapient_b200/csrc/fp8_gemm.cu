@@ -1,4 +1,13 @@
 // Products of fp8 rows with fp8 weights: y[m][n] = sum over blocks b of 128 columns  xs[m][b] ws[n / 128][b] sum_k xq[m][k] wq[n][k].
+//
+// The tensor cores add up a block's 128 columns (products of e4m3 values are exact in f32); what they have is scaled and added in f32
+// registers, since no two blocks of a row need have the same scale. That is 1 multiplication of a thread for 128 of the tensor cores,
+// and each block's sums pass through registers: the accumulators in tensor memory are a ring, not a result.
+//   up to 16 rows, small matrices    fp8_gemv_kernel    mma.sync, 16 weight rows a block
+//   up to 128 rows                   fp8_stream_kernel  tcgen05, 128 weight rows are the lanes, K shared by a cluster
+//   few tiles                        fp8_lone_kernel    tcgen05, 128 activation rows are the lanes, one tile a block
+//   many                             fp8_wide_kernel    the same, tiles of 256 weight rows in rounds, by one SM or a pair
+// Every sum has one order, which depends on the sizes alone. gemv_takes and way_of choose, with the times of both sides.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -50,7 +59,8 @@ __device__ __forceinline__ void store(const Fp8MatArgs& p, int m, int n, float f
 // ── Up to 16 rows ──
 // A block owns 16 weight rows; its warps take blocks of 128 columns in turn and add up in shared memory. Columns may be multiplied in
 // any order: a lane's 16 bytes of a row are four 4-byte operands of mma.sync, and the activations are read alike, so that nothing is
-// rearranged. No tensor memory, barriers or descriptors to set up, which is most of a small product's time.
+// rearranged. No tensor memory, barriers or descriptors to set up, which is most of a small product's time: 1 x 4096 x 4096 takes 6.2 us
+// from cold weights, of which their bytes are 2.6; the rest is the launch, the first loads' latency and the warps' sum.
 constexpr int FV_ROWS = 16;
 
 __device__ __forceinline__ uint4 fv_stream(const uint8_t* p) {
@@ -142,6 +152,9 @@ __global__ void __launch_bounds__(32 * FV_WARPS, 16 / FV_WARPS) fp8_gemv_kernel(
 }
 
 // ── Few rows: a stream of weights ──
+// The weights' bytes bound it (13 x 28672 x 4096: 22.7 us, 5.2 TB/s): they fill the tile's 128 lanes whatever the number of activation
+// rows, which are the products' N of 16 to 128. Two blocks an SM keep 200 KB on their way. Where tiles are fewer than SMs, the blocks of a
+// cluster take parts of K and add them up through distributed shared memory in the parts' order (32 x 1024 x 8192: 8 parts 8.6 us).
 constexpr int FS_BM = 128;                     // weight rows of a tile
 constexpr int FS_THREADS = 192;                // MMA warp, TMA warp, four drain warps
 constexpr int FS_W_BYTES = FS_BM * FP8_BLOCK;  // of a stage
@@ -419,6 +432,12 @@ __device__ __forceinline__ bool drains_agree(bool ok) {
 // ── Many rows: activation rows are the lanes ──
 // A tile of 128 G activation rows x 256 weight rows, by one block or by a pair (G = 2: each block has 128 activation rows in its tensor
 // memory and half of the weight rows in its shared memory), or by one block 128 x 128 or 128 x 64 of a product that does not fill the SMs.
+//
+// The wide kernel's two halves of 128 weight rows have sums and drain warps of their own, two of each: while one is drained three are
+// with the tensor cores. 4096 x 14336 x 4096: 205 to 209 us, 2.3 PFLOP/s, at the 1.5 GHz to which the power limit takes the clock;
+// 168 without drains. The tensor cores are never idle: a half takes 417 cycles for 256 of products (335 without drains), since
+// drains read the tensor memory that products add into. Slower: products of 256 columns with two sums (220 us), 16 drain warps (238),
+// results by TMA (232), columns of tiles first (221). No effect: more stages, a second warp that issues products.
 constexpr int FP_BN = 256;
 constexpr int FP_FIRST_DRAIN = 4;               // warp 0 issues products, warp 1 copies, warps 2 and 3 store results of drains
 constexpr int FP_THREADS = 32 * (FP_FIRST_DRAIN + FP_DRAINS);
@@ -744,7 +763,8 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideAr
 
 // A tile of 128 activation rows x W weight rows a block, no more tiles than SMs: what counts is how many bytes are on their way and how
 // soon the tensor cores go on. All of shared memory is stages; there are four accumulators, and the two groups of drain warps take
-// blocks of 128 columns in turn and add up at the end.
+// blocks of 128 columns in turn and add up at the end. An SM takes in about 60 bytes a cycle, which bounds it: 128 x 4096 x 4096 10.6 us
+// with tiles of 64 weight rows (13.2 with one warp that issues products and one that copies, 12.1 with two and one, two and two here).
 __host__ __device__ constexpr int lone_stage(int w) { return (128 + w) * FP8_BLOCK; }
 __host__ __device__ constexpr int lone_stages(int w) { return 210 * 1024 / lone_stage(w); }
 

