@@ -4,7 +4,7 @@
 // registers, since no two blocks of a row need have the same scale. That is 1 multiplication of a thread for 128 of the tensor cores,
 // and each block's sums pass through registers: the accumulators in tensor memory are a ring, not a result.
 //   up to 16 rows, small matrices    fp8_gemv_kernel    mma.sync, 16 weight rows a block
-//   up to 128 rows                   fp8_stream_kernel  tcgen05, 128 weight rows are the lanes, K shared by a cluster
+//   up to 128 rows, or long K        fp8_stream_kernel  tcgen05, 128 weight rows are the lanes, K shared by a cluster
 //   few tiles                        fp8_lone_kernel    tcgen05, 128 activation rows are the lanes, one tile a block
 //   many                             fp8_wide_kernel    the same, tiles of 256 weight rows in rounds, by one SM or a pair
 // Every sum has one order, which depends on the sizes alone. gemv_takes and way_of choose, with the times of both sides.
@@ -1031,11 +1031,13 @@ static Fp8Way way_of(const Fp8MatArgs& a) {
     }
     if (const double tiles = over(a.m, 128) * over(a.n, 64); tiles <= sms) offer(WAY_LONE64, std::max(2.43 + 0.226 * blocks + 2.39 * tiles / sms, 4.7 + weights));
     if (const double tiles = over(a.m, 128) * over(a.n, 128); tiles <= sms) offer(WAY_LONE128, std::max(2.88 + 0.266 * blocks + 2.48 * tiles / sms, 5.8 + weights));
-    if (a.m <= 128) {
-        const int rows = stream_rows(a.m), parts = stream_parts(a);
-        const double teams = over(a.n, FS_BM) * parts, each = rows == 32 ? 0.442 : rows == 64 ? 0.368 : 0.79;
+    // (several tiles of 128 rows only where K is long and they still fit side by side: 384 x 512 x 14336 16.4 us, tiles of 128 x 64 26.7)
+    const int rows = stream_rows(a.m), parts = stream_parts(a);
+    const double teams = over(a.n, FS_BM) * over(a.m, rows) * parts;
+    if (a.m <= 128 || teams <= sms) {
+        const double each = rows == 32 ? 0.442 : rows == 64 ? 0.368 : 0.79;
         const double load = std::min(std::max(teams / sms, 1.0), 2.0), rounds = over((int64_t)teams, (int)(2 * sms));
-        offer(WAY_STREAM, std::max(3.2 + (parts > 1 ? 0.47 : 0.0) + rounds * (ceil(blocks / parts) * each * (1 + 0.3 * (load - 1)) + 0.038 * a.m), 6.2 + weights));
+        offer(WAY_STREAM, std::max(3.2 + (parts > 1 ? 0.47 : 0.0) + rounds * (ceil(blocks / parts) * each * (1 + 0.3 * (load - 1)) + 0.038 * std::min(a.m, rows)), 6.2 + weights));
     }
     return best;
 }
