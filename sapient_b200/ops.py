@@ -26,6 +26,14 @@ def _blocks(k: int) -> int:
     return -(-k // FP8_BLOCK)
 
 
+def _bits8(a, what: str) -> np.ndarray:
+    """Values of one byte as they are: a number of another type would not be converted but taken for bits."""
+    a = np.asarray(a)
+    if a.dtype.itemsize != 1 or a.dtype.kind == "b":
+        raise SapientCudaError(_lib.SP_ERR_DTYPE, f"{what}: e4m3 values are given as bytes (uint8), not {a.dtype}")
+    return np.ascontiguousarray(a).view(np.uint8)
+
+
 def _f32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.float32)
 
@@ -43,7 +51,7 @@ class Weight:
     def from_fp8(cls, values, scales, device: int = 0) -> "Weight":
         """An [n, k] matrix of e4m3 values (uint8: their bits) with an f32 scale for every 128 x 128 block. matmul_nt quantises the
         rows of x likewise, a scale for every 128 columns."""
-        v, s = np.ascontiguousarray(values, dtype=np.uint8), _f32(scales)
+        v, s = _bits8(values, "fp8 weight"), _f32(scales)
         if v.ndim != 2 or s.shape != (_blocks(v.shape[0]), _blocks(v.shape[1])):
             raise SapientCudaError(_lib.SP_ERR_SHAPE, "fp8 weight: values [n, k] and scales [ceil(n / 128), ceil(k / 128)] expected")
         h = C.c_void_p()
@@ -225,7 +233,7 @@ def quant_fp8(x, device: int = 0):
 
 def matmul_fp8(xq, xs, wq, ws, device: int = 0) -> np.ndarray:
     """Y[m, n] = X Wᵀ of fp8 rows (xq [m, k] uint8, xs [m, ceil(k / 128)]) and fp8 weights (wq [n, k], ws for 128 x 128 blocks)."""
-    xq, wq = np.ascontiguousarray(xq, dtype=np.uint8), np.ascontiguousarray(wq, dtype=np.uint8)
+    xq, wq = _bits8(xq, "matmul_fp8"), _bits8(wq, "matmul_fp8")
     xs, ws = _f32(xs), _f32(ws)
     if xq.ndim != 2 or wq.ndim != 2 or xq.shape[1] != wq.shape[1]:
         raise SapientCudaError(_lib.SP_ERR_SHAPE, "matmul_fp8 expects xq [m, k] and wq [n, k]")

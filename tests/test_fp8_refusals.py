@@ -79,5 +79,15 @@ def test_nothing_to_do_needs_no_device():
     q, s, h = ops.rms_norm_fp8(np.zeros((0, 64), np.float32), None, 1e-5)
     assert q.shape == (0, 64) and s.shape == (0, 1) and h.shape == (0, 64)
     assert ops.swiglu_fp8(np.zeros((0, 64), np.float32))[0].shape == (0, 32)
-    assert ops.matmul_fp8(np.zeros((0, 64)), np.zeros((0, 1)), np.zeros((5, 64)), np.zeros((1, 1))).shape == (0, 5)
+    assert ops.matmul_fp8(np.zeros((0, 64), np.uint8), np.zeros((0, 1)), np.zeros((5, 64), np.uint8), np.zeros((1, 1))).shape == (0, 5)
     assert [a.shape for a in ops.logprobs(np.zeros((0, 9)), [], top=2)] == [(0,), (0,), (0, 2), (0, 2)]
+
+
+def test_values_that_are_not_bytes():
+    """A float8 array of any package has items of one byte; floats and integers are not silently taken for bits."""
+    x, xs, ws = np.zeros((2, 64), np.uint8), np.ones((2, 1), np.float32), np.ones((1, 1), np.float32)
+    for bad in (np.float32, np.int32, np.float16, bool):
+        for call in (lambda: ops.matmul_fp8(x.astype(bad), xs, x, ws), lambda: ops.matmul_fp8(x, xs, x.astype(bad), ws), lambda: ops.Weight.from_fp8(x.astype(bad), ws)):
+            with pytest.raises(_lib.SapientCudaError) as e:
+                call()
+            assert e.value.status == DTYPE
