@@ -155,6 +155,28 @@ def lib():
     return _lib
 
 
+_calls = None
+_CALLS = ("rms_norm_fp8", "swiglu_fp8", "quant_fp8", "matmul_fp8", "logprobs")
+
+
+def calls():
+    """The calls on device pointers under their names without sp_cuda_ and _dev: the module that csrc/calls.cpp becomes, which converts
+    arguments faster than ctypes, or, where it has not been built, lib()'s own."""
+    global _calls
+    if _calls is None:
+        fns = [getattr(lib(), f"sp_cuda_{name}_dev") for name in _CALLS]
+        try:
+            from . import _calls as module
+
+            module.bind(*(C.cast(f, C.c_void_p).value for f in fns))
+            _calls = module
+        except ImportError:
+            import types
+
+            _calls = types.SimpleNamespace(**dict(zip(_CALLS, fns)))
+    return _calls
+
+
 def check(status: int) -> None:
     if status != SP_OK:
         raise SapientCudaError(status, lib().sp_cuda_last_error().decode(errors="replace"))

@@ -4,6 +4,8 @@
 
 nvcc cross-compiles without a GPU. The library links the CUDA runtime statically
 and has no other dependency, so the built file can be copied to a GPU machine.
+Beside it stands a small Python module (csrc/calls.cpp) where Python's headers are
+installed; without it the same calls go through ctypes.
 """
 from __future__ import annotations
 
@@ -20,6 +22,7 @@ SOURCES = ["kernels.cu", "attention.cu", "engine.cu", "engine_forward.cu", "engi
            "engine_plan_latent.cu", "engine_plan_grouped.cu", "mat_f32.cu", "mat_tc5.cu",
            "plan_stream.cu", "latent_attention.cu", "grouped_attention.cu", "mixed_attention.cu", "grouped_conv.cu", "state_mixer.cu", "state_chunk.cu",
            "fp8_rows.cu", "fp8_gemm.cu", "logprobs.cu"]
+CALLS_SRC, CALLS_OUT = os.path.join(CSRC, "calls.cpp"), os.path.join(HERE, "_calls.abi3.so")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--shared",
@@ -30,11 +33,23 @@ def _stale() -> bool:
     if not os.path.exists(OUT):
         return True
     t = os.path.getmtime(OUT)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "sapient_cuda.h")]
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f != "calls.cpp"] + [os.path.join(HERE, "..", "include", "sapient_cuda.h")]
     return any(os.path.getmtime(p) > t for p in deps)
 
 
+def build_calls(force: bool = False) -> None:
+    import sysconfig
+
+    include = sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(include, "Python.h")):
+        return
+    newest = max(os.path.getmtime(p) for p in (CALLS_SRC, os.path.join(HERE, "..", "include", "sapient_cuda.h")))
+    if force or not os.path.exists(CALLS_OUT) or os.path.getmtime(CALLS_OUT) < newest:
+        subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-I", include, CALLS_SRC, "-o", CALLS_OUT], check=True)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    build_calls(force)
     if not force and not _stale():
         return OUT
     from concurrent.futures import ThreadPoolExecutor

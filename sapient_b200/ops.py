@@ -264,25 +264,35 @@ def logprobs(logits, ids, top: int = 0, device: int = 0):
 # The same on device pointers (integers; 0: not given), without copies or synchronisation. dtype: F32 or BF16. Row strides in values, 0: dense.
 def rms_norm_fp8_dev(x: int, rows: int, dim: int, w: int, eps: float, q: int, scale: int, dtype: int = F32, residual: int = 0, sum_out: int = 0,
                      ldx: int = 0, ldr: int = 0, lds: int = 0, device: int = 0, stream: int = 0) -> None:
-    check(lib().sp_cuda_rms_norm_fp8_dev(device, dtype, x, ldx or dim, residual, ldr or dim, sum_out, lds or dim, w, eps, rows, dim, q, scale, stream))
+    status = (_lib._calls or _lib.calls()).rms_norm_fp8(device, dtype, x, ldx or dim, residual, ldr or dim, sum_out, lds or dim, w, eps, rows, dim, q, scale, stream)
+    if status:
+        check(status)
 
 
 def swiglu_fp8_dev(gu: int, rows: int, ffn: int, q: int, scale: int, dtype: int = F32, ld: int = 0, device: int = 0, stream: int = 0) -> None:
-    check(lib().sp_cuda_swiglu_fp8_dev(device, dtype, gu, ld or 2 * ffn, rows, ffn, q, scale, stream))
+    status = (_lib._calls or _lib.calls()).swiglu_fp8(device, dtype, gu, ld or 2 * ffn, rows, ffn, q, scale, stream)
+    if status:
+        check(status)
 
 
 def quant_fp8_dev(x: int, rows: int, dim: int, q: int, scale: int, dtype: int = F32, ldx: int = 0, device: int = 0, stream: int = 0) -> None:
-    check(lib().sp_cuda_quant_fp8_dev(device, dtype, x, ldx or dim, rows, dim, q, scale, stream))
+    status = (_lib._calls or _lib.calls()).quant_fp8(device, dtype, x, ldx or dim, rows, dim, q, scale, stream)
+    if status:
+        check(status)
 
 
 def matmul_fp8_dev(xq: int, xs: int, m: int, wq: int, ws: int, n: int, k: int, y: int, dtype: int = F32, ldy: int = 0, device: int = 0,
                    stream: int = 0) -> None:
-    check(lib().sp_cuda_matmul_fp8_dev(device, xq, xs, m, wq, ws, n, k, y, dtype, ldy or n, stream))
+    status = (_lib._calls or _lib.calls()).matmul_fp8(device, xq, xs, m, wq, ws, n, k, y, dtype, ldy or n, stream)
+    if status:
+        check(status)
 
 
 def logprobs_dev(logits: int, rows: int, vocab: int, ids: int, logprob: int, entropy: int, top: int = 0, top_ids: int = 0, top_logprobs: int = 0,
                  dtype: int = F32, ld: int = 0, device: int = 0, stream: int = 0) -> None:
-    check(lib().sp_cuda_logprobs_dev(device, dtype, logits, ld or vocab, rows, vocab, ids, top, logprob, entropy, top_ids, top_logprobs, stream))
+    status = (_lib._calls or _lib.calls()).logprobs(device, dtype, logits, ld or vocab, rows, vocab, ids, top, logprob, entropy, top_ids, top_logprobs, stream)
+    if status:
+        check(status)
 
 
 def set_gemv_path(path: int) -> None:

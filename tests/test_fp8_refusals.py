@@ -91,3 +91,25 @@ def test_values_that_are_not_bytes():
             with pytest.raises(_lib.SapientCudaError) as e:
                 call()
             assert e.value.status == DTYPE
+
+
+def test_arguments_reach_the_library_as_ctypes_would_pass_them():
+    """The module between Python and the library: the same statuses as ctypes, integers of any package, None for no address; what is no
+    number, does not fit or is one too few raises."""
+    c, L = _lib.calls(), _lib.lib()
+    norm = [0, F32, P, 256, 0, 256, 0, 256, P, 1e-5, 2, 256, P, P, 0]
+    for at, value in [(1, 99), (2, 0), (2, P + 8), (3, 240), (6, P), (10, -1), (11, 24), (11, 1 << 40), (12, None), (10, 0), (10, np.int64(0)), (3, np.int32(255))]:
+        a = list(norm)
+        a[at] = value
+        if a[10] == 2 and at == 6:
+            a[7] = 512
+        assert c.rms_norm_fp8(*a) == L.sp_cuda_rms_norm_fp8_dev(*[None if v is None else v if isinstance(v, float) else int(v) for v in a])
+        assert a[10] == 0 or c.rms_norm_fp8(*a) != OK
+    assert c.matmul_fp8(0, P, P, 0, P, P, 8, 32, P, F32, 8, None) == OK and c.matmul_fp8(0, P, P, 4, P, P, 8, 32, P, F32, 7, 0) == SHAPE
+    assert c.swiglu_fp8(0, F32, P, 128, 0, 64, P, P, 0) == OK and c.quant_fp8(0, F32, P, 64, 0, 64, P, P, 0) == OK
+    assert c.logprobs(0, F32, P, 100, 2, 100, 0, 33, 0, P, P, P, 0) == ARG
+    if hasattr(c, "bind"):  # (ctypes takes a number modulo 2^32)
+        for bad, error in [((0, 1 << 40, P, 64, 0, 64, P, P, 0), OverflowError), ((0, F32, "x", 64, 0, 64, P, P, 0), TypeError), ((0, F32, P, 64.0, 0, 64, P, P, 0), TypeError),
+                           ((0, F32, P, 64, 0, 64, P, P), TypeError), ((0, F32, P, 1 << 80, 0, 64, P, P, 0), OverflowError)]:
+            with pytest.raises(error):
+                c.quant_fp8(*bad)
