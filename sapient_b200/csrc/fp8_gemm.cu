@@ -3,7 +3,7 @@
 // The tensor cores add up a block's 128 columns (products of e4m3 values are exact in f32); what they have is scaled and added in f32
 // registers, since no two blocks of a row need have the same scale. That is 1 multiplication of a thread for 128 of the tensor cores,
 // and each block's sums pass through registers: the accumulators in tensor memory are a ring, not a result.
-//   up to 16 rows, small matrices    fp8_gemv_kernel    mma.sync, 16 weight rows a block
+//   up to 16 rows, but for large     fp8_gemv_kernel    mma.sync, 16 weight rows a block
 //   up to 128 rows, or long K        fp8_stream_kernel  tcgen05, 128 weight rows are the lanes, K shared by a cluster
 //   few tiles                        fp8_lone_kernel    tcgen05, 128 activation rows are the lanes, one tile a block
 //   many                             fp8_wide_kernel    the same, tiles of 256 weight rows in rounds, by one SM or a pair
@@ -58,15 +58,32 @@ __device__ __forceinline__ void store(const Fp8MatArgs& p, int m, int n, float f
 
 // ── Up to 16 rows ──
 // A block owns 16 weight rows; its warps take blocks of 128 columns in turn and add up in shared memory. Columns may be multiplied in
-// any order: a lane's 16 bytes of a row are four 4-byte operands of mma.sync, and the activations are read alike, so that nothing is
-// rearranged. No tensor memory, barriers or descriptors to set up, which is most of a small product's time: 1 x 4096 x 4096 takes 6.2 us
-// from cold weights, of which their bytes are 2.6; the rest is the launch, the first loads' latency and the warps' sum.
+// any order: a lane's 32 bytes of a row are eight 4-byte operands of mma.sync, and the activations are read alike, so that nothing is
+// rearranged. No tensor memory, barriers or descriptors to set up, which is most of a small product's time: 1 x 4096 x 4096 takes 5.3 us
+// from cold weights, of which their bytes are 2.6 (3.7 from L2); the rest is the launch, the first loads' latency and the warps' sum.
+// Four lanes load 128 bytes of a row at once: with 64 the L1's tags bound it (6.2 us, from L2 too). Few registers, so that blocks of the
+// next product start beside the last ones of this: four blocks of columns ahead instead of two took 6.5 us.
 constexpr int FV_ROWS = 16;
 
-__device__ __forceinline__ uint4 fv_stream(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-    return v;
+// 32 bytes, in one load where they start on 32; weights are not kept in L1.
+template <bool ALIGNED>
+__device__ __forceinline__ void fv_weights(const uint8_t* p, uint4 (&v)[2]) {
+    if constexpr (ALIGNED)
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                     : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z), "=r"(v[1].w) : "l"(p) : "memory");
+    else
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w) : "l"(p + 16 * i) : "memory");
+}
+template <bool ALIGNED>
+__device__ __forceinline__ void fv_rows(const uint8_t* p, uint4 (&v)[2]) {
+    if constexpr (ALIGNED)
+        asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                     : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z), "=r"(v[1].w) : "l"(p) : "memory");
+    else
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = *reinterpret_cast<const uint4*>(p + 16 * i);
 }
 __device__ __forceinline__ void fv_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -74,30 +91,40 @@ __device__ __forceinline__ void fv_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// NT: activation rows / 8. AHEAD: blocks of 128 columns that a warp has on their way.
-template <int NT, int FV_WARPS, int AHEAD>
+// NT: activation rows / 8. AHEAD: blocks of 128 columns that a warp has on their way. ALIGNED: rows start on 32 bytes.
+template <int NT, int FV_WARPS, int AHEAD, bool ALIGNED>
 __global__ void __launch_bounds__(32 * FV_WARPS, 16 / FV_WARPS) fp8_gemv_kernel(const Fp8MatArgs p) {
     __shared__ float part[FV_WARPS][8 * NT][FV_ROWS + 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * FV_ROWS, blocks = (p.k + FP8_BLOCK - 1) / FP8_BLOCK;
-    const uint8_t* const w0 = p.wq + (int64_t)min(n0 + g, p.n - 1) * p.k + 16 * t;
-    const uint8_t* const w1 = p.wq + (int64_t)min(n0 + 8 + g, p.n - 1) * p.k + 16 * t;
+    const uint8_t* const w0 = p.wq + (int64_t)min(n0 + g, p.n - 1) * p.k + 32 * t;
+    const uint8_t* const w1 = p.wq + (int64_t)min(n0 + 8 + g, p.n - 1) * p.k + 32 * t;
     const float* const ws = p.ws + (int64_t)(n0 / FP8_BLOCK) * blocks;
     struct Stage {
-        uint4 w[2][2], x[NT][2];  // [row half][64 columns]
+        uint4 w[2][2], x[NT][2];  // [rows 0 to 7, 8 to 15][16 columns]
         float xs[NT][2], ws;
     } stage[AHEAD];
     auto load = [&](Stage& s, int b) {
         const int c = b * FP8_BLOCK;
         const uint4 zero = make_uint4(0, 0, 0, 0);
+        const int left = p.k - c - 32 * t;  // columns from the lane's first on: 32, or of the last block 16 or fewer
+        if (left >= 32) {
+            fv_weights<ALIGNED>(w0 + c, s.w[0]);
+            fv_weights<ALIGNED>(w1 + c, s.w[1]);
+        } else {
+            const bool half = !ALIGNED && left > 0;
+            s.w[0][0] = half ? *reinterpret_cast<const uint4*>(w0 + c) : zero;
+            s.w[1][0] = half ? *reinterpret_cast<const uint4*>(w1 + c) : zero;
+            s.w[0][1] = s.w[1][1] = zero;
+        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const bool there = c + 64 * h + 16 * t < p.k;
-            s.w[0][h] = there ? fv_stream(w0 + c + 64 * h) : zero;
-            s.w[1][h] = there ? fv_stream(w1 + c + 64 * h) : zero;
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                s.x[j][h] = there && 8 * j + g < p.m ? __ldg(reinterpret_cast<const uint4*>(p.xq + (int64_t)(8 * j + g) * p.k + c + 64 * h + 16 * t)) : zero;
+        for (int j = 0; j < NT; ++j) {
+            const uint8_t* const x = p.xq + (int64_t)(8 * j + g) * p.k + c + 32 * t;
+            s.x[j][0] = s.x[j][1] = zero;
+            if (8 * j + g < p.m) {
+                if (left >= 32) fv_rows<ALIGNED>(x, s.x[j]);
+                else if (!ALIGNED && left > 0) s.x[j][0] = *reinterpret_cast<const uint4*>(x);
+            }
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -142,13 +169,14 @@ __global__ void __launch_bounds__(32 * FV_WARPS, 16 / FV_WARPS) fp8_gemv_kernel(
 #pragma unroll
         for (int i = 0; i < 4; ++i) part[warp][8 * j + 2 * t + (i & 1)][g + 8 * (i >> 1)] = acc[j][i];
     __syncthreads();
-    const int row = tid & (FV_ROWS - 1), m = tid / FV_ROWS;
-    if (m < p.m && m < 8 * NT && n0 + row < p.n) {
-        float f = 0.f;
+    const int row = tid & (FV_ROWS - 1);
+    for (int m = tid / FV_ROWS; m < p.m; m += 32 * FV_WARPS / FV_ROWS)
+        if (n0 + row < p.n) {
+            float f = 0.f;
 #pragma unroll
-        for (int w = 0; w < FV_WARPS; ++w) f += part[w][m][row];
-        store(p, m, n0 + row, f);
-    }
+            for (int w = 0; w < FV_WARPS; ++w) f += part[w][m][row];
+            store(p, m, n0 + row, f);
+        }
 }
 
 // ── Few rows: a stream of weights ──
@@ -979,22 +1007,32 @@ static cudaError_t lone_of(const Fp8MatArgs& a, cudaStream_t st) {
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
-// Where the kernel of 16 weight rows a block is the faster one (its blocks / the stream of weights, us, weights past L2): up to 8 rows
-// it starts sooner (1 row: 2048 x 2048 3.0 / 4.8, 4096 x 4096 6.2 / 7.1, 8960 x 1536 6.0 / 6.7), but blocks beyond two an SM come in
-// rounds (6144 x 4096 9.8 / 8.7, 14336 x 4096 16.2 / 13.9) and few long ones leave SMs idle (2560 x 10240 10.4 / 9.0). From 9 rows on
-// each block also reads about as much of the activations as of the weights (12 rows: 2048 x 2048 4.5 / 5.3, 2560 x 2560 6.6 / 6.0).
+// Where the kernel of 16 weight rows a block is the faster one (it / the stream of weights, us, weights from memory). Up to 8 rows until
+// the bytes of 100 MB and more count for all (1 row: 2048 x 2048 2.8 / 5.7, 4096 x 4096 5.3 / 8.2, 14336 x 4096 13.6 / 14.2, 28672 x 4096
+// 22.6 / 22.5); from 9 rows on each block also reads as much of the activations as of the weights (12 rows: 2048 x 2048 3.3 / 7.4,
+// 4096 x 4096 7.2 / 10.6, 6144 x 4096 10.7 / 9.7). Where rows do not start on 32 bytes it loads 16 at a time (4096 x 4096 5.8, 14336 x 4096 14.6).
+static bool gemv_aligned(const Fp8MatArgs& a) { return ((reinterpret_cast<uintptr_t>(a.wq) | reinterpret_cast<uintptr_t>(a.xq) | (uintptr_t)a.k) & 31) == 0; }
 static bool gemv_takes(const Fp8MatArgs& a) {
-    const int64_t blocks = (a.n + FV_ROWS - 1) / FV_ROWS, sms = device_sm_count(), values = (int64_t)a.n * a.k;
-    if (a.m > 8) return a.k <= 2048 && values <= 5 << 20;
-    return blocks <= sms || (blocks <= 2 * sms && a.k <= 8192) || (blocks <= 4 * sms && values <= 1 << 24);
+    return a.m <= 16 && (int64_t)a.n * a.k <= (a.m > 8 ? 1 << 24 : gemv_aligned(a) ? 96 << 20 : 32 << 20);
 }
 static cudaError_t gemv_of(const Fp8MatArgs& a, cudaStream_t st) {
+    const int sms = device_sm_count(), blocks = (int)fp8_blocks(a.k);
     const dim3 grid((unsigned)((a.n + FV_ROWS - 1) / FV_ROWS));
-    const bool wide = (int)grid.x <= device_sm_count();  // 16 warps where a block has its SM for itself (1 row of 2048 x 8192: 7.5 -> 6.3)
-    cudaError_t e;
-    if (a.m <= 8) e = wide ? launch_pdl(fp8_gemv_kernel<1, 16, 4>, grid, dim3(512), 0, st, a) : launch_pdl(fp8_gemv_kernel<1, 8, 4>, grid, dim3(256), 0, st, a);
-    else e = wide ? launch_pdl(fp8_gemv_kernel<2, 16, 2>, grid, dim3(512), 0, st, a) : launch_pdl(fp8_gemv_kernel<2, 8, 2>, grid, dim3(256), 0, st, a);
-    return e != cudaSuccess ? e : count_launch_and_check();
+    auto with = [&](void (*kernel)(Fp8MatArgs), int warps) {
+        const cudaError_t e = launch_pdl(kernel, grid, dim3(32 * warps), 0, st, a);
+        return e != cudaSuccess ? e : count_launch_and_check();
+    };
+    if (!gemv_aligned(a)) return a.m <= 8 ? with(fp8_gemv_kernel<1, 8, 2, false>, 8) : with(fp8_gemv_kernel<2, 8, 1, false>, 8);
+    // 16 warps where a block has its SM for itself, 4 where there are more than two an SM (1 row: 2048 x 8192 5.7, 8 warps 6.8, 4 10.1;
+    // 4096 x 4096 6.7, 5.3, 6.7; 9400 x 1024 7.2, 4.6, 3.7); a third block of columns on its way where a warp has more than six
+    // (4096 x 14336 12.7 for 13.4; 9400 x 1024 4.7 for 4.6). Of 16 rows one block of columns is ahead (4096 x 4096 7.2, two 8.2).
+    if ((int)grid.x <= sms) return a.m <= 8 ? with(fp8_gemv_kernel<1, 16, 3, true>, 16) : with(fp8_gemv_kernel<2, 16, 1, true>, 16);
+    if ((int)grid.x <= 2 * sms) {
+        if (a.m > 8) return with(fp8_gemv_kernel<2, 8, 1, true>, 8);
+        return blocks > 6 * 8 ? with(fp8_gemv_kernel<1, 8, 3, true>, 8) : with(fp8_gemv_kernel<1, 8, 2, true>, 8);
+    }
+    if (a.m > 8) return with(fp8_gemv_kernel<2, 4, 1, true>, 4);
+    return blocks > 6 * 4 ? with(fp8_gemv_kernel<1, 4, 3, true>, 4) : with(fp8_gemv_kernel<1, 4, 2, true>, 4);
 }
 
 // More than 16 rows, and what the kernel above leaves: the way that takes least time in a model of each, us on 148 SMs, fitted to 1400
@@ -1045,7 +1083,7 @@ static Fp8Way way_of(const Fp8MatArgs& a) {
 cudaError_t launch_fp8_matmul(const Fp8MatArgs& a, cudaStream_t st) {
     if (a.m == 0 || a.n == 0) return cudaSuccess;
     if (a.m < 0 || a.n < 0 || a.k <= 0 || a.k % 16 != 0) return cudaErrorInvalidValue;
-    if (a.m <= 16 && gemv_takes(a)) return gemv_of(a, st);
+    if (gemv_takes(a)) return gemv_of(a, st);
     switch (way_of(a)) {
         case WAY_LONE64: return lone_of<64>(a, st);
         case WAY_LONE128: return lone_of<128>(a, st);

@@ -73,7 +73,19 @@ def test_every_way(ty, m, n, k):
         check(product(*a, ty, 3), *a)  # rows of y that start anywhere
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 14336, 4096), (24, 28672, 4096), (2048, 4096, 2048), (700, 16400, 1040)])
+@pytest.mark.parametrize("m", [1, 7, 8, 9, 16])
+@pytest.mark.parametrize("n,k", [(1, 32), (700, 16), (2000, 48), (2300, 992), (2400, 12320), (4700, 6176), (4800, 1056), (9600, 160), (4752, 4096), (17, 5008), (12800, 2096), (30000, 48), (100, 33024)])
+def test_up_to_sixteen_rows(m, n, k):
+    """Every number of warps and of blocks of columns ahead, rows that start on 32 bytes and on 16, a matrix that starts on 16."""
+    a = inputs(m, n, k, m + n)
+    check(product(*a, ops.F32, 1), *a)
+    xq, xs, wq, ws = a
+    off = torch.empty(n * k + 16, device="cuda", dtype=torch.uint8)[16:]
+    off.copy_(wq.view(torch.uint8).reshape(-1))
+    check(product(xq, xs, off.view(n, k).view(torch.float8_e4m3fn), ws, ops.BF16), *a)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 14336, 4096), (5, 26000, 4096), (8, 8200, 4112), (24, 28672, 4096), (2048, 4096, 2048), (700, 16400, 1040)])
 def test_large(m, n, k):
     a = inputs(m, n, k, 3)
     check(product(*a), *a)
