@@ -403,51 +403,79 @@ __device__ __forceinline__ void put_line(uint8_t* out, const uint64_t* acc, int 
         *reinterpret_cast<uint4*>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
-// What put_line left of 32 rows, to y: whole lines of 128 bytes where rows start on 16 bytes.
-template <typename T>
-__device__ __forceinline__ void store_lines(const Fp8MatArgs& p, const uint8_t* out, bool wide, int r0, int n0, int lane) {
+// What put_line left of 32 rows, to rows of y that start anywhere: a row an instruction, so that what it writes lies together, in words of
+// the alignment that the row has. Out: T's columns of y, or 32 of f32 that become bf16.
+template <typename T, typename Out>
+__device__ __forceinline__ void store_rows(void* y, int64_t ldy, int rows, int columns, const uint8_t* out, int lane) {
+    auto word = [&](int row) { return *reinterpret_cast<const uint32_t*>(out + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4); };
+    Out* at = static_cast<Out*>(y);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll 8
+        for (int row = 0; row < 32; ++row, at += ldy) {
+            const float f = __uint_as_float(word(row));
+            if (row < rows && lane < columns) at[lane] = (Out)f;
+        }
+    } else {
+        const int last = min(columns, 64);
+        const bool odd0 = (reinterpret_cast<uintptr_t>(y) & 2) != 0, odd1 = odd0 != ((ldy & 1) != 0);  // whether rows 0, 2, ... and 1, 3, ... start between words
+        uint16_t* to = static_cast<uint16_t*>(y) + 2 * lane;
+        if (!odd0 && !odd1) {
+#pragma unroll 8
+            for (int row = 0; row < 32; ++row, to += ldy) {
+                const uint32_t v = word(row);
+                if (row < rows && 2 * lane + 1 < last) *reinterpret_cast<uint32_t*>(to) = v;
+            }
+        } else {
+#pragma unroll 8
+            for (int row = 0; row < 32; ++row, to += ldy) {
+                const int odd = (row & 1) ? odd1 : odd0;
+                const uint32_t v = word(row), next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
+                if (row < rows && 2 * lane + odd + 1 < last) *reinterpret_cast<uint32_t*>(to + odd) = __funnelshift_r(v, next, 16 * odd);
+            }
+        }
+        // a row a lane: the first column of rows that start between words, the last one that is half a word
+        const int odd = (lane & 1) ? odd1 : odd0;
+        auto one = [&](int c) { static_cast<uint16_t*>(y)[lane * ldy + c] = *reinterpret_cast<const uint16_t*>(out + lane * 128 + (((c >> 3) ^ (lane & 7)) << 4) + (c & 7) * 2); };
+        if (lane < rows && odd && last > 0) one(0);
+        if (lane < rows && last > odd && ((last - odd) & 1)) one(last - 1);
+    }
+}
+// The same where rows start on 16 bytes (ALIGNED): four rows an instruction. Kernels have either as a parameter: the two together cost
+// the aligned way 2 %. (755 x 30158 x 1728 bf16 with the aligned way's pieces stored an element at a time: 87 us for 45.)
+template <typename T, bool ALIGNED, typename Out = T>
+__device__ __forceinline__ void store_lines(const Fp8MatArgs& p, const uint8_t* out, int r0, int n0, int lane) {
     constexpr int PER = 16 / sizeof(T);
+    if constexpr (!ALIGNED) {
+        store_rows<T, Out>(static_cast<Out*>(p.y) + (int64_t)r0 * p.ldy + n0, p.ldy, p.m - r0, p.n - n0, out, lane);
+        return;
+    }
     const int piece = lane & 7, n = n0 + piece * PER;
-    T* at = static_cast<T*>(p.y) + (int64_t)(r0 + (lane >> 3)) * p.ldy + n;
+    Out* at = static_cast<Out*>(p.y) + (int64_t)(r0 + (lane >> 3)) * p.ldy + n;
 #pragma unroll
     for (int i = 0; i < 8; ++i, at += 4 * p.ldy) {
         const int row = 4 * i + (lane >> 3);
         const uint4 v = *reinterpret_cast<const uint4*>(out + row * 128 + ((piece ^ (row & 7)) << 4));
         if (r0 + row >= p.m) continue;
-        if (wide && n + PER <= p.n) {
-            *reinterpret_cast<uint4*>(at) = v;
+        const T* const e = reinterpret_cast<const T*>(&v);
+        if (n + PER <= p.n) {
+            if constexpr (sizeof(Out) < sizeof(T)) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(e[0], e[1]), hi = __floats2bfloat162_rn(e[2], e[3]);
+                *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            } else {
+                *reinterpret_cast<uint4*>(at) = v;
+            }
         } else {
-            const T* const e = reinterpret_cast<const T*>(&v);
 #pragma unroll
             for (int j = 0; j < PER; ++j)
-                if (n + j < p.n) at[j] = e[j];
+                if (n + j < p.n) at[j] = (Out)e[j];
         }
     }
 }
-
 // 32 columns that put_line left in f32, to y of either type.
-__device__ __forceinline__ void store_f32_lines(const Fp8MatArgs& p, const uint8_t* out, bool wide, int r0, int n0, int lane) {
-    if (!p.bf) {
-        store_lines<float>(p, out, wide, r0, n0, lane);
-        return;
-    }
-    const int piece = lane & 7, n = n0 + 4 * piece;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int row = 4 * i + (lane >> 3);
-        const float4 f = *reinterpret_cast<const float4*>(out + row * 128 + ((piece ^ (row & 7)) << 4));
-        if (r0 + row >= p.m) continue;
-        bf16* const at = static_cast<bf16*>(p.y) + (int64_t)(r0 + row) * p.ldy + n;
-        if (wide && n + 4 <= p.n) {
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(f.x, f.y), hi = __floats2bfloat162_rn(f.z, f.w);
-            *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-        } else {
-            const float e[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n + j < p.n) at[j] = __float2bfloat16_rn(e[j]);
-        }
-    }
+template <bool ALIGNED>
+__device__ __forceinline__ void store_f32_lines(const Fp8MatArgs& p, const uint8_t* out, int r0, int n0, int lane) {
+    if (p.bf) store_lines<float, ALIGNED, bf16>(p, out, r0, n0, lane);
+    else store_lines<float, ALIGNED>(p, out, r0, n0, lane);
 }
 
 // Whether all drain warps' waits were in time; a barrier between them.
@@ -542,7 +570,6 @@ __device__ __forceinline__ void drain_add(uint32_t taddr, float f, uint64_t (&ac
 struct Fp8WideArgs {
     Fp8MatArgs p;
     int row_tiles, whole, items;  // items: tiles up to `whole`, halves of the following tiles (128 of their weight rows) after them
-    bool aligned;                 // rows of y start on 16 bytes
     bool handed;                  // results leave by warps of their own while the drains go on with the next tile
 };
 template <int G>
@@ -557,7 +584,8 @@ struct Fp8Item {
     }
 };
 
-template <int G>
+// ALIGNED: rows of y start on 16 bytes.
+template <int G, bool ALIGNED>
 __global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideArgs a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     constexpr int STAGES = fp_stages(G), STAGE = fp_stage(G), HALF = FP_BN / 2 / G;  // HALF: weight rows of half a tile in this block
     extern __shared__ uint8_t fp_smem_raw[];
@@ -689,8 +717,8 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideAr
                     ok = __all_sync(0xFFFFFFFFu, tc5_wait(&out_full[d], (uint32_t)(turn & 1)));
                     if (!ok) break;
                     for (int i = 0; i < 2; ++i) {
-                        if (p.bf) store_lines<bf16>(p, out + 4096 * i, a.aligned, r0, n0 + 64 * i, lane);
-                        else store_lines<float>(p, out + 4096 * i, a.aligned, r0, n0 + 64 + 32 * i, lane);
+                        if (p.bf) store_lines<bf16, ALIGNED>(p, out + 4096 * i, r0, n0 + 64 * i, lane);
+                        else store_lines<float, ALIGNED>(p, out + 4096 * i, r0, n0 + 64 + 32 * i, lane);
                     }
                     tc5_arrive(&out_empty[d]);
                 }
@@ -707,10 +735,10 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideAr
         auto store_out = [&](int r0, int n0) {
             __syncwarp();
             if (p.bf) {
-                store_lines<bf16>(p, out, a.aligned, r0, n0, lane);
+                store_lines<bf16, ALIGNED>(p, out, r0, n0, lane);
             } else {
-                store_lines<float>(p, out, a.aligned, r0, n0, lane);
-                store_lines<float>(p, out + 4096, a.aligned, r0, n0 + 32, lane);
+                store_lines<float, ALIGNED>(p, out, r0, n0, lane);
+                store_lines<float, ALIGNED>(p, out + 4096, r0, n0 + 32, lane);
             }
         };
         int c = 0, turns = 0;
@@ -771,8 +799,8 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideAr
                 ++turns;
             } else if (p.bf) {
                 __syncwarp();
-                store_lines<bf16>(p, out, a.aligned, r0, n0, lane);
-                store_lines<bf16>(p, out + 4096, a.aligned, r0, n0 + 64, lane);
+                store_lines<bf16, ALIGNED>(p, out, r0, n0, lane);
+                store_lines<bf16, ALIGNED>(p, out + 4096, r0, n0 + 64, lane);
             } else {
                 store_out(r0, n0 + 64);
             }
@@ -796,8 +824,8 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideAr
 __host__ __device__ constexpr int lone_stage(int w) { return (128 + w) * FP8_BLOCK; }
 __host__ __device__ constexpr int lone_stages(int w) { return 210 * 1024 / lone_stage(w); }
 
-template <int W>
-__global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArgs p, int aligned, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+template <int W, bool ALIGNED>
+__global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArgs p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     constexpr int STAGES = lone_stages(W), STAGE = lone_stage(W), COLS = 4 * W;
     extern __shared__ uint8_t fp_smem_raw[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], sum_full[4], sum_empty[4];
@@ -921,12 +949,12 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArg
             if (p.bf && LINES == 2) {
                 put_line<bf16>(out, keep, lane);
                 __syncwarp();
-                store_lines<bf16>(p, out, aligned, r0, c0, lane);
+                store_lines<bf16, ALIGNED>(p, out, r0, c0, lane);
             } else {
 #pragma unroll
                 for (int i = 0; i < LINES; ++i) put_line<float>(out + 4096 * i, keep + 16 * i, lane);
                 __syncwarp();
-                for (int i = 0; i < LINES; ++i) store_f32_lines(p, out + 4096 * i, aligned, r0, c0 + 32 * i, lane);
+                for (int i = 0; i < LINES; ++i) store_f32_lines<ALIGNED>(p, out + 4096 * i, r0, c0 + 32 * i, lane);
             }
         };
         if (group == 0) finish(acc, acc + W / 4);
@@ -961,20 +989,19 @@ static cudaError_t stream_of(const Fp8MatArgs& a, int parts, cudaStream_t st) {
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
-template <int G>
-static cudaError_t wide_of(const Fp8MatArgs& a, cudaStream_t st) {
+template <int G, bool ALIGNED>
+static cudaError_t wide_with(const Fp8MatArgs& a, cudaStream_t st) {
     CUtensorMap mw, mx;
     if (!fp8_map(&mw, a.wq, a.k, a.n, FP_BN / 2 / G) || !fp8_map(&mx, a.xq, a.k, a.m, 128)) return cudaErrorInvalidValue;
     static PerDeviceOnce once;
-    cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_wide_kernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize, fp_smem(G) + 1024); });
+    cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_wide_kernel<G, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, fp_smem(G) + 1024); });
     if (e != cudaSuccess) return e;
     const int64_t row_tiles = (a.m + 128 * G - 1) / (128 * G), tiles = row_tiles * ((a.n + FP_BN - 1) / FP_BN);
     const int most = device_sm_count() / G;
     if (tiles > INT32_MAX / 4) return cudaErrorInvalidValue;
     // the last round's tiles are halved where all halves find a place
     const int left = (int)(tiles % most), halved = 2 * left <= most ? left : 0;
-    const bool aligned = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * (a.bf ? 2 : 4))) & 15) == 0;
-    const Fp8WideArgs k{a, (int)row_tiles, (int)tiles - halved, (int)tiles + halved, aligned, a.k > 1024};
+    const Fp8WideArgs k{a, (int)row_tiles, (int)tiles - halved, (int)tiles + halved, a.k > 1024};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(std::min(k.items, most) * G));
     cfg.blockDim = dim3(FP_THREADS);
@@ -988,24 +1015,30 @@ static cudaError_t wide_of(const Fp8MatArgs& a, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = G;
-    e = cudaLaunchKernelEx(&cfg, fp8_wide_kernel<G>, k, mw, mx);
+    e = cudaLaunchKernelEx(&cfg, fp8_wide_kernel<G, ALIGNED>, k, mw, mx);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
-template <int W>
-static cudaError_t lone_of(const Fp8MatArgs& a, cudaStream_t st) {
+static bool y_aligned(const Fp8MatArgs& a) { return ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * (a.bf ? 2 : 4))) & 15) == 0; }
+template <int G>
+static cudaError_t wide_of(const Fp8MatArgs& a, cudaStream_t st) { return y_aligned(a) ? wide_with<G, true>(a, st) : wide_with<G, false>(a, st); }
+
+template <int W, bool ALIGNED>
+static cudaError_t lone_with(const Fp8MatArgs& a, cudaStream_t st) {
     CUtensorMap mw, mx;
     if (!fp8_map(&mw, a.wq, a.k, a.n, W) || !fp8_map(&mx, a.xq, a.k, a.m, 128)) return cudaErrorInvalidValue;
     constexpr int SMEM = lone_stages(W) * lone_stage(W) + 1024;
     static_assert(SMEM - 1024 >= 2 * FP_DRAINS * 4096 * (W / 64), "sums and results take the stages' place");
     static PerDeviceOnce once;
-    cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_lone_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
+    cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_lone_kernel<W, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
     if (e != cudaSuccess) return e;
-    const bool aligned = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * (a.bf ? 2 : 4))) & 15) == 0;
     const dim3 grid((unsigned)((a.n + W - 1) / W), (unsigned)((a.m + 127) / 128));
-    e = launch_pdl(fp8_lone_kernel<W>, grid, dim3(FP_THREADS), (size_t)SMEM, st, a, (int)aligned, mw, mx);
+    e = launch_pdl(fp8_lone_kernel<W, ALIGNED>, grid, dim3(FP_THREADS), (size_t)SMEM, st, a, mw, mx);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
+
+template <int W>
+static cudaError_t lone_of(const Fp8MatArgs& a, cudaStream_t st) { return y_aligned(a) ? lone_with<W, true>(a, st) : lone_with<W, false>(a, st); }
 
 // Where the kernel of 16 weight rows a block is the faster one (it / the stream of weights, us, weights from memory). Up to 8 rows until
 // the bytes of 100 MB and more count for all (1 row: 2048 x 2048 2.8 / 5.7, 4096 x 4096 5.3 / 8.2, 14336 x 4096 13.6 / 14.2, 28672 x 4096
