@@ -10,13 +10,15 @@
 // copies in shared memory, 16 a thread at a time. The maximum is a warp's: of a row of random values a thread would find a new one of
 // its own in most of its steps, and all of the warp would rescale. The `top` largest cost the reading pass a comparison a value: a
 // thread keeps the maxima of a quarter each of what it reads (cells); afterwards the `top`-th largest of the maxima of groups of threads
-// is a bound which that many values reach, the few cells that reach it are read again, from L2, and the values above it are ranked.
+// is a bound which that many values reach, the few cells that reach it are read again, from L2 or, of short rows, from the ring, and the
+// values above it are ranked.
 // Keys (value, then lower index) are distinct, so that no order of threads changes the result.
 //
 // Bytes bound it from some hundred rows on, with the exponentials close behind (16 a cycle and SM); below that the chain of steps does,
 // a good part of it instructions that are fetched for the first time, so that what runs once is kept short. us (floor at 6.54 TB/s):
 //   1024 x 128256 f32 top 1      91.7 (80.3)     32 x 128256 bf16 top 20   10.8 (1.3)      1 x 151936 f32 top 5    7.1 (0.1)
 //   1024 x 128256 bf16 top 1     59.9 (40.2)     64 x 128256 bf16 top 1    10.9 (2.5)      1 x 151936 f32 top 0    4.5 (0.1)
+//   53 x 1913 bf16 top 12         4.7 (0.0; 7.0 with cells from L2)
 // Two values an instruction wherever there is one (1024 x 128256 bf16 top 1: 64.5 us without).
 #include <cuda_bf16.h>
 
@@ -177,6 +179,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     __shared__ LpShared sh;
     extern __shared__ uint4 lp_ring[];  // [stage][piece][thread]: a thread reads what it has copied, so that no barrier stands between
     constexpr int VEC = 16 / sizeof(T), PIECES = LP_VALUES / VEC, STEP = LP_THREADS * PIECES;
+    static_assert(sizeof(LpTail) <= STEP * sizeof(uint4) && LP_STAGES - 1 <= LP_CELLS, "the tail fits one stage, a cell a chunk of those that stay");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t r = blockIdx.x / parts;
     const int part = blockIdx.x - (int)r * parts;
@@ -185,7 +188,6 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     const int pieces = (int)(((int64_t)skew + a.n + VEC - 1) / VEC), per = (pieces + parts - 1) / parts;
     const int begin = min(part * per, pieces), end = min(begin + per, pieces);
-    LpTail& tail = *reinterpret_cast<LpTail*>(lp_ring);
     uint64_t* const inbox = reinterpret_cast<uint64_t*>(lp_ring + LP_STAGES * PIECES * LP_THREADS);  // of a cluster's first block: every part's largest
     if (TOP && tid == 0) sh.count = sh.queued = 0;
     if (parts > 1) lp_cluster_arrive();  // (waited for before a peer's memory is written: all blocks run by then)
@@ -200,6 +202,9 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     LpSums s{-INFINITY, 0.f, 0.f, 0};  // m and bad: of the warp
     bool holds = false;
     const int chunks = (end - begin + STEP - 1) / STEP;
+    // few chunks stay in the ring, whose last stage they do not use: there the largest are looked for where they are
+    const bool stays = chunks < LP_STAGES;
+    LpTail& tail = *reinterpret_cast<LpTail*>(lp_ring + (stays ? (LP_STAGES - 1) * STEP : 0));
     // A thread's maxima over runs of `cell` chunks stay in shared memory: where the largest values are looked for afterwards.
     const int cell = (chunks + LP_CELLS - 1) / LP_CELLS;
     int n_cells = 0, in_cell = 0;
@@ -344,6 +349,26 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
             return at < LP_BUF / 2 ? 0 : at < LP_BUF ? 1 : 2;
         };
         // the cells whose maximum is not below the threshold are read again, a piece a thread
+        bool over = false;
+        if (stays) {  // (a cell is a chunk)
+            for (int k = 0; k < chunks; ++k) {
+                if (sh.cells[k][tid] < low) continue;
+                const uint4* const mine = lp_ring + k * STEP + tid;
+                uint32_t reach = 0;
+#pragma unroll
+                for (int j = 0; j < PIECES; ++j) {
+                    float v[VEC];
+                    lp_unpack(mine[j * LP_THREADS], v, T());
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) reach |= (uint32_t)!(v[i] < low) << (j * VEC + i);
+                }
+                for (; reach; reach &= reach - 1) {
+                    const int at = __ffs(reach) - 1, j = at / VEC, p = begin + k * STEP + j * LP_THREADS + tid, id = p * VEC - skew + at % VEC;
+                    if (p < end) over |= push((float)reinterpret_cast<const T*>(mine + j * LP_THREADS)[at % VEC], id) == 2;
+                }
+            }
+            __syncthreads();
+        } else {
 #pragma unroll
         for (int j = 0; j < LP_CELLS; ++j)
             if (j < n_cells && !(cells[j] < low)) {
@@ -352,7 +377,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
             }
         __syncthreads();
         const int queued = sh.queued, cell_pieces = cell * PIECES, items = min(queued, LP_QUEUE) * cell_pieces;
-        bool over = queued > LP_QUEUE;
+        over = queued > LP_QUEUE;
         constexpr int AHEAD = 4;  // pieces of a thread on their way
         for (int i0 = tid; !over && i0 < items; i0 += AHEAD * LP_THREADS) {
             // (one copy of what follows a candidate, not one for each value: it runs once, and its instructions have to be fetched)
@@ -385,6 +410,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
                 const int at = __ffs(reach) - 1, p = piece_of(at / VEC), id = p * VEC - skew + at % VEC;
                 if (p < end && id >= 0 && id < a.n) over |= push((float)row[id], id) == 2;
             }
+        }
         }
         if (__syncthreads_or(over)) {
             // More candidates than places (many equal logits at the top): once more, a chunk at a time, cut back to the largest between.
