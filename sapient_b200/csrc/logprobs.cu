@@ -34,13 +34,10 @@ cudaError_t count_launch_and_check();  // kernels.cu
 
 using bf16 = __nv_bfloat16;
 
-constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_VALUES = 16;         // a thread's share of a chunk
-constexpr int LP_CHUNK = LP_THREADS * LP_VALUES;
 constexpr int LP_STAGES = 3;          // chunks of a block on their way or in use
-constexpr int LP_BUF = 256;           // candidates for the largest
 constexpr int LP_CELLS = 4;           // maxima a thread keeps
-constexpr int LP_QUEUE = 512;         // of them that can be read again
+constexpr int LP_QUEUE = 512;         // of the cells that can be read again
 constexpr int LP_MAX_PARTS = 16;      // blocks of a row
 constexpr float LP_LOW = -200.f;      // lp_exp is zero from here down; keeps 0 x infinity out of T
 constexpr unsigned LP_ALL = 0xFFFFFFFFu;
@@ -115,19 +112,21 @@ __device__ __forceinline__ LpSums lp_shfl(const LpSums& a, int o) {
     return LpSums{__shfl_xor_sync(LP_ALL, a.m, o), __shfl_xor_sync(LP_ALL, a.r, o), __shfl_xor_sync(LP_ALL, a.t, o), __shfl_xor_sync(LP_ALL, a.bad, o)};
 }
 
+template <int THREADS>
 struct __align__(16) LpShared {
     LpSums parts[LP_MAX_PARTS];  // of a cluster's first block
-    LpSums sums[LP_WARPS];
-    float cells[LP_CELLS][LP_THREADS];
+    LpSums sums[THREADS / 32];
+    float cells[LP_CELLS][THREADS];
     uint32_t low;
     int count, queued;
 };
 // In the ring's place once the row has been read.
+template <int THREADS>
 struct __align__(16) LpTail {
-    uint64_t buf[LP_BUF + 4];
+    uint64_t buf[THREADS + 4];  // candidates for the largest
     uint64_t list[LOGPROBS_MAX_TOP];  // the result
     union {
-        uint32_t first[LP_THREADS];
+        uint32_t first[THREADS];
         uint16_t queue[LP_QUEUE];
     };
 };
@@ -174,12 +173,12 @@ __device__ __forceinline__ void lp_unpack(const uint4& f, float* v, bf16) {
     }
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsArgs a, int parts) {
-    __shared__ LpShared sh;
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const LogprobsArgs a, int parts) {
+    __shared__ LpShared<THREADS> sh;
     extern __shared__ uint4 lp_ring[];  // [stage][piece][thread]: a thread reads what it has copied, so that no barrier stands between
-    constexpr int VEC = 16 / sizeof(T), PIECES = LP_VALUES / VEC, STEP = LP_THREADS * PIECES;
-    static_assert(sizeof(LpTail) <= STEP * sizeof(uint4) && LP_STAGES - 1 <= LP_CELLS, "the tail fits one stage, a cell a chunk of those that stay");
+    constexpr int VEC = 16 / sizeof(T), PIECES = LP_VALUES / VEC, STEP = THREADS * PIECES;
+    static_assert(sizeof(LpTail<THREADS>) <= STEP * sizeof(uint4) && LP_STAGES - 1 <= LP_CELLS, "the tail fits one stage, a cell a chunk of those that stay");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t r = blockIdx.x / parts;
     const int part = blockIdx.x - (int)r * parts;
@@ -188,7 +187,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     const int pieces = (int)(((int64_t)skew + a.n + VEC - 1) / VEC), per = (pieces + parts - 1) / parts;
     const int begin = min(part * per, pieces), end = min(begin + per, pieces);
-    uint64_t* const inbox = reinterpret_cast<uint64_t*>(lp_ring + LP_STAGES * PIECES * LP_THREADS);  // of a cluster's first block: every part's largest
+    uint64_t* const inbox = reinterpret_cast<uint64_t*>(lp_ring + LP_STAGES * PIECES * THREADS);  // of a cluster's first block: every part's largest
     if (TOP && tid == 0) sh.count = sh.queued = 0;
     if (parts > 1) lp_cluster_arrive();  // (waited for before a peer's memory is written: all blocks run by then)
     pdl_wait();
@@ -204,7 +203,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     const int chunks = (end - begin + STEP - 1) / STEP;
     // few chunks stay in the ring, whose last stage they do not use: there the largest are looked for where they are
     const bool stays = chunks < LP_STAGES;
-    LpTail& tail = *reinterpret_cast<LpTail*>(lp_ring + (stays ? (LP_STAGES - 1) * STEP : 0));
+    LpTail<THREADS>& tail = *reinterpret_cast<LpTail<THREADS>*>(lp_ring + (stays ? (LP_STAGES - 1) * STEP : 0));
     // A thread's maxima over runs of `cell` chunks stay in shared memory: where the largest values are looked for afterwards.
     const int cell = (chunks + LP_CELLS - 1) / LP_CELLS;
     int n_cells = 0, in_cell = 0;
@@ -213,8 +212,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
         if (k < chunks) {
 #pragma unroll
             for (int j = 0; j < PIECES; ++j) {
-                uint4* const to = lp_ring + (k % LP_STAGES * PIECES + j) * LP_THREADS + tid;
-                const int p = begin + k * STEP + j * LP_THREADS + tid, e0 = p * VEC - skew;
+                uint4* const to = lp_ring + (k % LP_STAGES * PIECES + j) * THREADS + tid;
+                const int p = begin + k * STEP + j * THREADS + tid, e0 = p * VEC - skew;
                 if (p < end && e0 >= 0 && e0 + VEC <= a.n) {
                     lp_copy(to, row + e0);
                 } else {  // past the part, or a piece that hangs over an end of the row: masked values in the others' places
@@ -235,10 +234,10 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     for (int k = 0; k < chunks; ++k) {
         fetch(k + LP_STAGES - 1);
         asm volatile("cp.async.wait_group %0;\n" ::"n"(LP_STAGES - 1) : "memory");
-        const uint4* const mine = lp_ring + k % LP_STAGES * PIECES * LP_THREADS + tid;
+        const uint4* const mine = lp_ring + k % LP_STAGES * PIECES * THREADS + tid;
         float x[LP_VALUES];
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) lp_unpack(mine[j * LP_THREADS], x + j * VEC, T());
+        for (int j = 0; j < PIECES; ++j) lp_unpack(mine[j * THREADS], x + j * VEC, T());
         float c = lp_max(x[0], x[1]);
 #pragma unroll
         for (int i = 2; i < LP_VALUES; i += 2) c = lp_max(c, x[i], x[i + 1]);
@@ -319,8 +318,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
         __syncthreads();
         auto rank_groups = [&](uint32_t m0, uint32_t m1, int groups) {  // (each warp looks at its share of the groups)
 #pragma unroll 4
-            for (int i = 0; i < groups / LP_WARPS; ++i) {
-                const int c = warp * (groups / LP_WARPS) + i;
+            for (int i = 0; i < groups / (THREADS / 32); ++i) {
+                const int c = warp * (groups / (THREADS / 32)) + i;
                 const uint32_t v = __shfl_sync(LP_ALL, c < 32 ? m0 : m1, c & 31);
                 int greater = __popc(__ballot_sync(LP_ALL, m0 > v || (m0 == v && lane < c)));
                 if (groups > 32) greater += __popc(__ballot_sync(LP_ALL, m1 > v || (m1 == v && lane + 32 < c)));
@@ -330,9 +329,9 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
         uint32_t m[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            m[h] = tail.first[h * (LP_THREADS / 2) + lane];
+            m[h] = tail.first[h * (THREADS / 2) + lane];
 #pragma unroll
-            for (int w = 1; w < LP_WARPS / 2; ++w) m[h] = max(m[h], tail.first[h * (LP_THREADS / 2) + w * 32 + lane]);
+            for (int w = 1; w < THREADS / 64; ++w) m[h] = max(m[h], tail.first[h * (THREADS / 2) + w * 32 + lane]);
         }
         if (a.top <= 24) rank_groups(max(m[0], m[1]), 0, 32);
         else rank_groups(m[0], m[1], 64);
@@ -345,8 +344,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
             const uint64_t key = lp_key(v, id);
             if (key <= threshold) return 0;
             const int at = atomicAdd(&sh.count, 1);
-            if (at < LP_BUF) tail.buf[at] = key;
-            return at < LP_BUF / 2 ? 0 : at < LP_BUF ? 1 : 2;
+            if (at < THREADS) tail.buf[at] = key;
+            return at < THREADS / 2 ? 0 : at < THREADS ? 1 : 2;
         };
         // the cells whose maximum is not below the threshold are read again, a piece a thread
         bool over = false;
@@ -358,13 +357,13 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
 #pragma unroll
                 for (int j = 0; j < PIECES; ++j) {
                     float v[VEC];
-                    lp_unpack(mine[j * LP_THREADS], v, T());
+                    lp_unpack(mine[j * THREADS], v, T());
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) reach |= (uint32_t)!(v[i] < low) << (j * VEC + i);
                 }
                 for (; reach; reach &= reach - 1) {
-                    const int at = __ffs(reach) - 1, j = at / VEC, p = begin + k * STEP + j * LP_THREADS + tid, id = p * VEC - skew + at % VEC;
-                    if (p < end) over |= push((float)reinterpret_cast<const T*>(mine + j * LP_THREADS)[at % VEC], id) == 2;
+                    const int at = __ffs(reach) - 1, j = at / VEC, p = begin + k * STEP + j * THREADS + tid, id = p * VEC - skew + at % VEC;
+                    if (p < end) over |= push((float)reinterpret_cast<const T*>(mine + j * THREADS)[at % VEC], id) == 2;
                 }
             }
             __syncthreads();
@@ -373,19 +372,19 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
         for (int j = 0; j < LP_CELLS; ++j)
             if (j < n_cells && !(cells[j] < low)) {
                 const int at = atomicAdd(&sh.queued, 1);
-                if (at < LP_QUEUE) tail.queue[at] = (uint16_t)(j * LP_THREADS + tid);
+                if (at < LP_QUEUE) tail.queue[at] = (uint16_t)(j * THREADS + tid);
             }
         __syncthreads();
         const int queued = sh.queued, cell_pieces = cell * PIECES, items = min(queued, LP_QUEUE) * cell_pieces;
         over = queued > LP_QUEUE;
         constexpr int AHEAD = 4;  // pieces of a thread on their way
-        for (int i0 = tid; !over && i0 < items; i0 += AHEAD * LP_THREADS) {
+        for (int i0 = tid; !over && i0 < items; i0 += AHEAD * THREADS) {
             // (one copy of what follows a candidate, not one for each value: it runs once, and its instructions have to be fetched)
             auto piece_of = [&](int e) {
-                const int i = i0 + e * LP_THREADS, q = i / cell_pieces, u = i - q * cell_pieces;
+                const int i = i0 + e * THREADS, q = i / cell_pieces, u = i - q * cell_pieces;
                 if (i >= items) return end;
-                const int from = tail.queue[q], k = from / LP_THREADS * cell + u / PIECES;
-                return k < chunks ? begin + k * STEP + u % PIECES * LP_THREADS + from % LP_THREADS : end;
+                const int from = tail.queue[q], k = from / THREADS * cell + u / PIECES;
+                return k < chunks ? begin + k * STEP + u % PIECES * THREADS + from % THREADS : end;
             };
             uint4 got[AHEAD];
             uint32_t edge = 0, reach = 0;
@@ -402,7 +401,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
                 uint32_t mask = 0;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) mask |= !(v[i] < low) << i;
-                if (i0 + e * LP_THREADS >= items) mask = 0;
+                if (i0 + e * THREADS >= items) mask = 0;
                 if (edge >> e & 1) mask = (1u << VEC) - 1;
                 reach |= mask << e * VEC;
             }
@@ -421,13 +420,13 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
                 for (;;) {
                     int said = 0;
                     for (uint32_t left = pending; left; left &= left - 1) {
-                        const int i = __ffs(left) - 1, p = begin + k * STEP + i / VEC * LP_THREADS + tid, id = p * VEC - skew + i % VEC;
+                        const int i = __ffs(left) - 1, p = begin + k * STEP + i / VEC * THREADS + tid, id = p * VEC - skew + i % VEC;
                         const int got = p < end && id >= 0 && id < a.n ? push((float)row[id], id) : 0;
                         if (got < 2) pending &= ~(1u << i);
                         said = max(said, got);
                     }
                     if (!__syncthreads_or(said)) break;
-                    lp_largest(tail.buf, min(sh.count, LP_BUF), tail.list, tid);
+                    lp_largest(tail.buf, min(sh.count, THREADS), tail.list, tid);
                     const uint64_t key = tail.list[lane];
                     const int kept = __popc(__ballot_sync(LP_ALL, key != 0));
                     if (warp == 0) tail.buf[lane] = key;
@@ -441,9 +440,9 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
         lp_largest(tail.buf, sh.count, tail.list, tid);
     }
     if (warp == 0) {
-        s = sh.sums[lane & (LP_WARPS - 1)];
+        s = sh.sums[lane & (THREADS / 32 - 1)];
 #pragma unroll 1
-        for (int o = LP_WARPS / 2; o > 0; o >>= 1) s = lp_join(s, lp_shfl(s, o));
+        for (int o = THREADS / 64; o > 0; o >>= 1) s = lp_join(s, lp_shfl(s, o));
     }
     if (parts > 1) {
         // every block writes its part into the first one's memory, which goes on alone
@@ -481,19 +480,13 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobsA
     }
 }
 
-template <typename T>
-static cudaError_t logprobs_of(const LogprobsArgs& a, cudaStream_t st) {
-    const int sms = device_sm_count();
-    // up to two blocks an SM; 16 where rows are few and there are few keys to rank (8 x 128256 f32, 8 parts and 16: top 5 7.9 us, 7.7;
-    // top 16 8.6 us, 10.3; 1 x 151936 top 0 5.9 us, 4.6)
-    int parts = 1;
-    while (parts < 8 && a.rows * parts * 2 <= 2 * sms && a.n / (parts * 2) >= LP_CHUNK) parts *= 2;
-    if (parts == 8 && a.rows * 16 <= sms && a.n / 16 >= LP_CHUNK && a.top <= 8) parts = 16;
+template <typename T, int THREADS>
+static cudaError_t logprobs_with(const LogprobsArgs& a, int parts, cudaStream_t st) {
     if (a.rows * parts > INT32_MAX) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * parts));
-    cfg.blockDim = dim3(LP_THREADS);
-    constexpr size_t ring = LP_STAGES * LP_CHUNK * sizeof(T), most = ring + (LP_THREADS + 4) * sizeof(uint64_t);
+    cfg.blockDim = dim3(THREADS);
+    constexpr size_t ring = LP_STAGES * (THREADS * LP_VALUES) * sizeof(T), most = ring + (THREADS + 4) * sizeof(uint64_t);
     cfg.dynamicSmemBytes = parts > 1 ? ring + (parts * a.top + 4) * sizeof(uint64_t) : ring;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -506,7 +499,7 @@ static cudaError_t logprobs_of(const LogprobsArgs& a, cudaStream_t st) {
     cfg.numAttrs = parts > 1 ? 2 : 1;
     static PerDeviceOnce once;
     cudaError_t e = once.run([] {
-        for (const auto kernel : {logprobs_kernel<T, true>, logprobs_kernel<T, false>}) {
+        for (const auto kernel : {logprobs_kernel<T, true, THREADS>, logprobs_kernel<T, false, THREADS>}) {
             cudaError_t f = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
             if (f == cudaSuccess) f = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);  // (more than eight blocks)
             if (f != cudaSuccess) return f;
@@ -514,8 +507,22 @@ static cudaError_t logprobs_of(const LogprobsArgs& a, cudaStream_t st) {
         return cudaSuccess;
     });
     if (e != cudaSuccess) return e;
-    e = a.top > 0 ? cudaLaunchKernelEx(&cfg, logprobs_kernel<T, true>, a, parts) : cudaLaunchKernelEx(&cfg, logprobs_kernel<T, false>, a, parts);
+    e = a.top > 0 ? cudaLaunchKernelEx(&cfg, logprobs_kernel<T, true, THREADS>, a, parts) : cudaLaunchKernelEx(&cfg, logprobs_kernel<T, false, THREADS>, a, parts);
     return e != cudaSuccess ? e : count_launch_and_check();
+}
+
+template <typename T>
+static cudaError_t logprobs_of(const LogprobsArgs& a, cudaStream_t st) {
+    const int sms = device_sm_count();
+    // up to two blocks an SM; 16 where rows are few and there are few keys to rank (8 x 128256 f32, 8 parts and 16: top 5 7.9 us, 7.7;
+    // top 16 8.6 us, 10.3; 1 x 151936 top 0 5.9 us, 4.6)
+    int parts = 1;
+    while (parts < 8 && a.rows * parts * 2 <= 2 * sms && a.n / (parts * 2) >= 256 * LP_VALUES) parts *= 2;
+    if (parts == 8 && a.rows * 16 <= sms && a.n / 16 >= 256 * LP_VALUES && a.top <= 8) parts = 16;
+    // Many short rows: twice as many of half as many threads, for more of the chains that follow the reading (4000 x 1500 f32 top 5 30.3 us,
+    // 18.0; 2561 x 10581 bf16 top 20 40.0, 32.8; not 894 x 28496 f32 27.2, 28.9, and a few rows 1 x 5000 4.2, 5.1).
+    if (a.rows > 2 * sms && (int64_t)a.n * sizeof(T) <= 65536) return logprobs_with<T, 128>(a, 1, st);
+    return logprobs_with<T, 256>(a, parts, st);
 }
 
 cudaError_t launch_logprobs(const LogprobsArgs& a, bool bf, cudaStream_t st) {

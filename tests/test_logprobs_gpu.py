@@ -80,6 +80,19 @@ def test_few_long_rows(ty, rows, n, top, off):
 
 
 @pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
+@pytest.mark.parametrize("rows,n,top", [(300, 100, 32), (301, 1500, 7), (400, 16384, 25), (310, 9001, 1), (2500, 33, 3), (330, 4097, 0), (299, 32768, 32), (700, 1, 1), (320, 6145, 24)])
+def test_many_short_rows(ty, rows, n, top):
+    z, ids = logits(rows, n, ty, rows + n, n + 1, 1)
+    check(z, ids, top)
+    if top:
+        z[::3] = 1.5                                  # rows of nothing but ties
+        z[1::3, : n // 2] = torch.finfo(z.dtype).min  # and half masked ones
+        z[2::3] = (torch.arange(n, device="cuda") * 30 // n).to(z.dtype)
+        ids[:] = n - 1
+        check(z, ids, top)
+
+
+@pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
 @pytest.mark.parametrize("n", [5000, 70000])
 def test_orders_and_ties(ty, n):
     """Ascending rows push every value, constant ones tie everywhere, steps tie in long runs; the lowest id comes first."""
