@@ -821,18 +821,47 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideAr
 // soon the tensor cores go on. All of shared memory is stages; there are four accumulators, and the two groups of drain warps take
 // blocks of 128 columns in turn and add up at the end. An SM takes in about 60 bytes a cycle, which bounds it: 128 x 4096 x 4096 10.6 us
 // with tiles of 64 weight rows (13.2 with one warp that issues products and one that copies, 12.1 with two and one, two and two here).
+// Of tiles of 64 two or four blocks of a cluster may share K; they add up through distributed shared memory, each its share of the rows.
 __host__ __device__ constexpr int lone_stage(int w) { return (128 + w) * FP8_BLOCK; }
 __host__ __device__ constexpr int lone_stages(int w) { return 210 * 1024 / lone_stage(w); }
 
+// A cluster's blocks share out the rows that put_line left in each, in f32: of a warp's 32 each block adds up its own, the parts in order,
+// eight values of a lane on their way at a time, and stores them.
+template <int LINES>
+__device__ __forceinline__ void add_parts(const Fp8MatArgs& p, const uint8_t* out, int parts, int part, int r0, int c0, int lane) {
+    const uint32_t at = tc5_smem_u32(out);
+    const int rows = 32 / parts;
+    for (int i0 = 0; i0 < rows * LINES; i0 += 8) {
+        float f[8] = {};
+        for (int o = 0; o < parts; ++o) {
+            const uint32_t peer = peer_smem(at, o);
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int u = min(i0 + i, rows * LINES - 1), line = u / rows, row = part * rows + u - line * rows;
+                v[i] = ld_peer(peer + (uint32_t)(4096 * line + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] += v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int u = i0 + i, line = u / rows, row = r0 + part * rows + u - line * rows, n = c0 + 32 * line + lane;
+            if (u < rows * LINES && row < p.m && n < p.n) store(p, row, n, f[i]);
+        }
+    }
+}
+
 template <int W, bool ALIGNED>
-__global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArgs p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+__global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArgs p, int k_parts, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     constexpr int STAGES = lone_stages(W), STAGE = lone_stage(W), COLS = 4 * W;
     extern __shared__ uint8_t fp_smem_raw[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], sum_full[4], sum_empty[4];
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
     const int n0 = blockIdx.x * W, m0 = blockIdx.y * 128;
-    const int blocks = (p.k + FP8_BLOCK - 1) / FP8_BLOCK;
+    const int all = (p.k + FP8_BLOCK - 1) / FP8_BLOCK, parts = W == 64 ? k_parts : 1, part = W == 64 ? blockIdx.z : 0;
+    const int first = (int)((int64_t)part * all / parts), blocks = (int)((int64_t)(part + 1) * all / parts) - first;
     uint8_t* const smem = fp_smem_raw + ((1024u - (tc5_smem_u32(fp_smem_raw) & 1023u)) & 1023u);
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5_smem_u32(&tmem_slot)), "n"(COLS) : "memory");
@@ -894,7 +923,7 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArg
                     if (!ok) break;
                     const uint32_t bar = tc5_smem_u32(&full[st]);
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
-                    tc5_tma_2d(tc5_smem_u32(smem + st * STAGE + place), map, issued * FP8_BLOCK, row, bar);
+                    tc5_tma_2d(tc5_smem_u32(smem + st * STAGE + place), map, (first + issued) * FP8_BLOCK, row, bar);
                     if (++st == STAGES) { st = 0; ++u; }
                 }
                 // nothing is in flight towards this block when it goes on to the end: copies, or the arrivals that follow the last products
@@ -909,8 +938,8 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArg
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
         const int q4 = warp & 3, group = (warp - FP_FIRST_DRAIN) >> 2, r0 = m0 + 32 * q4;
         const uint32_t lanes = tmem + ((uint32_t)(32 * q4) << 16);
-        const float* const xs = p.xs + (int64_t)min(r0 + lane, p.m - 1) * blocks;
-        const float* const ws = p.ws + (int64_t)(n0 / FP8_BLOCK) * blocks;
+        const float* const xs = p.xs + (int64_t)min(r0 + lane, p.m - 1) * all + first;
+        const float* const ws = p.ws + (int64_t)(n0 / FP8_BLOCK) * all + first;
         uint64_t acc[W / 2];
 #pragma unroll
         for (int j = 0; j < W / 2; ++j) acc[j] = 0;
@@ -921,7 +950,7 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArg
             const int q = b & 3;
             ok = __all_sync(0xFFFFFFFFu, tc5_wait(&sum_full[q], (uint32_t)((b >> 2) & 1)));
             if (!ok) break;
-            drain_add<W / 32>(lanes + (uint32_t)(q * W), f, acc, peer_smem(tc5_smem_u32(&sum_empty[q]), 0), lane);
+            drain_add<W / 32>(lanes + (uint32_t)(q * W), f, acc, tc5_smem_u32(&sum_empty[q]), lane);
         }
         // Once all drains are here the products are done and nothing reads the stages any more: in their place the groups exchange half
         // of their sums, and the results take their way to y. The first group keeps the lower columns.
@@ -929,6 +958,9 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArg
         constexpr int LINES = W / 64;  // of 32 f32 columns, that a group keeps
         uint8_t* const mine = smem + 4096 * LINES * (4 * group + q4);
         const uint8_t* const others = smem + 4096 * LINES * (4 * (group ^ 1) + q4);
+        // (what a warp gave has its own place: its result goes behind all of those)
+        uint8_t* const out = smem + 4096 * LINES * FP_DRAINS + 4096 * LINES * (4 * group + q4);
+        const int c0 = n0 + W / 2 * group;
         auto finish = [&](uint64_t* keep, const uint64_t* give) {
             if (ok) {
 #pragma unroll
@@ -943,10 +975,7 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArg
                 keep[2 * j] = pair2(make_float2(lo.x + f.x, lo.y + f.y));
                 keep[2 * j + 1] = pair2(make_float2(hi.x + f.z, hi.y + f.w));
             }
-            // (what this warp gave has its own place: its result goes behind all of those)
-            uint8_t* const out = smem + 4096 * LINES * FP_DRAINS + 4096 * LINES * (4 * group + q4);
-            const int c0 = n0 + W / 2 * group;
-            if (p.bf && LINES == 2) {
+            if (p.bf && LINES == 2 && parts == 1) {
                 put_line<bf16>(out, keep, lane);
                 __syncwarp();
                 store_lines<bf16, ALIGNED>(p, out, r0, c0, lane);
@@ -954,11 +983,20 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArg
 #pragma unroll
                 for (int i = 0; i < LINES; ++i) put_line<float>(out + 4096 * i, keep + 16 * i, lane);
                 __syncwarp();
-                for (int i = 0; i < LINES; ++i) store_f32_lines<ALIGNED>(p, out + 4096 * i, r0, c0 + 32 * i, lane);
+                if (parts == 1)
+                    for (int i = 0; i < LINES; ++i) store_f32_lines<ALIGNED>(p, out + 4096 * i, r0, c0 + 32 * i, lane);
             }
         };
         if (group == 0) finish(acc, acc + W / 4);
         else finish(acc + W / 4, acc);
+        if (parts > 1) {
+            cluster_sync();
+            if (ok) add_parts<LINES>(p, out, parts, part, r0, c0, lane);
+        }
+    }
+    if (parts > 1) {
+        if (warp < FP_FIRST_DRAIN) { __syncwarp(); cluster_sync(); }  // the service warps' share of the first barrier
+        cluster_sync();                                               // nobody leaves while its parts are being read
     }
     if (!ok) report_wait(p.waits, WAIT_FP8);
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -1024,7 +1062,7 @@ template <int G>
 static cudaError_t wide_of(const Fp8MatArgs& a, cudaStream_t st) { return y_aligned(a) ? wide_with<G, true>(a, st) : wide_with<G, false>(a, st); }
 
 template <int W, bool ALIGNED>
-static cudaError_t lone_with(const Fp8MatArgs& a, cudaStream_t st) {
+static cudaError_t lone_with(const Fp8MatArgs& a, int parts, cudaStream_t st) {
     CUtensorMap mw, mx;
     if (!fp8_map(&mw, a.wq, a.k, a.n, W) || !fp8_map(&mx, a.xq, a.k, a.m, 128)) return cudaErrorInvalidValue;
     constexpr int SMEM = lone_stages(W) * lone_stage(W) + 1024;
@@ -1032,13 +1070,15 @@ static cudaError_t lone_with(const Fp8MatArgs& a, cudaStream_t st) {
     static PerDeviceOnce once;
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_lone_kernel<W, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)((a.n + W - 1) / W), (unsigned)((a.m + 127) / 128));
-    e = launch_pdl(fp8_lone_kernel<W, ALIGNED>, grid, dim3(FP_THREADS), (size_t)SMEM, st, a, mw, mx);
+    const dim3 grid((unsigned)((a.n + W - 1) / W), (unsigned)((a.m + 127) / 128), (unsigned)parts), block(FP_THREADS);
+    static_assert(W == 64 || W == 128, "clusters share K of the lower tiles only");
+    e = parts == 1 ? launch_pdl(fp8_lone_kernel<W, ALIGNED>, grid, block, (size_t)SMEM, st, a, parts, mw, mx)
+                   : launch_pdl_cluster(fp8_lone_kernel<W, ALIGNED>, grid, block, (size_t)SMEM, st, parts, a, parts, mw, mx);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
 template <int W>
-static cudaError_t lone_of(const Fp8MatArgs& a, cudaStream_t st) { return y_aligned(a) ? lone_with<W, true>(a, st) : lone_with<W, false>(a, st); }
+static cudaError_t lone_of(const Fp8MatArgs& a, int parts, cudaStream_t st) { return y_aligned(a) ? lone_with<W, true>(a, parts, st) : lone_with<W, false>(a, parts, st); }
 
 // Where the kernel of 16 weight rows a block is the faster one (it / the stream of weights, us, weights from memory). Up to 8 rows until
 // the bytes of 100 MB and more count for all (1 row: 2048 x 2048 2.8 / 5.7, 4096 x 4096 5.3 / 8.2, 14336 x 4096 13.6 / 14.2, 28672 x 4096
@@ -1068,16 +1108,18 @@ static cudaError_t gemv_of(const Fp8MatArgs& a, cudaStream_t st) {
     return blocks > 6 * 4 ? with(fp8_gemv_kernel<1, 4, 3, true>, 4) : with(fp8_gemv_kernel<1, 4, 2, true>, 4);
 }
 
-// More than 16 rows, and what the kernel above leaves: the way that takes least time in a model of each, us on 148 SMs, fitted to 1400
-// times of 336 sizes (17 to 2048 rows, 24 matrices of 300 x 512 to 28672 x 4096); what it takes is 1 % over the best way on average.
-// Some of them, bf16 results, us (stream; tiles of 128 x 64 and 128 x 128, one a block; 128 x 256; 256 x 256 by two SMs):
-//    32 x  1024 x  8192    8.6   16.9   19.5   29.0   25.8         256 x  4096 x 4096    -    10.9   12.5   17.2   16.0
-//    64 x  4096 x 14336   17.2   27.4   32.0   48.7   42.8         512 x  4096 x 4096    -      -    13.1   17.4   16.3
-//   128 x  2048 x   512    9.1    4.2    4.9    5.4    5.7         256 x 14336 x 4096    -      -      -    22.6   20.1
-//   128 x 14336 x  4096   24.7     -    15.2   18.9   19.9        2048 x  8192 x 4096    -      -      -    70.1   62.4
-//   128 x 28672 x  4096   37.5     -      -    27.3   36.3
-// Up to 32 rows, tiles of 128 rows pay only where K is short.
-enum Fp8Way { WAY_STREAM, WAY_LONE64, WAY_LONE128, WAY_WIDE1, WAY_WIDE2 };
+// More than 16 rows, and what the kernel above leaves: the way that takes least time in a model of each, us on 148 SMs, fitted to 2500
+// times of 580 sizes (17 to 2048 rows, 40 matrices of 300 x 512 to 28672 x 4096); what it takes is 1 % over the best way on average.
+// Some of them, bf16 results, us (stream; tiles of 128 x 64, one a block, K whole or shared by 2 or 4; 128 x 128; 128 x 256; 256 x 256 by
+// two SMs):
+//    32 x  1024 x  8192    8.5   10.1 (4)   19.5   29.0   25.8         256 x  4096 x 4096    -    10.9   12.5   17.2   16.0
+//    64 x  4096 x 14336   17.2   19.4 (2)   32.0   48.7   42.8         512 x  4096 x 4096    -      -    13.1   17.4   16.3
+//   128 x  2048 x   512    9.1    3.9        4.9    5.4    5.7         256 x 14336 x 4096    -      -      -    22.6   20.1
+//   128 x  4096 x  8192   18.2   14.6 (2)   20.3   29.5   26.4         384 x  1536 x 8960    -  14.6 (2) 20.9   31.4   27.9
+//   128 x 14336 x  4096   24.7     -        15.2   18.9   19.9        2048 x  8192 x 4096    -      -      -    70.1   62.4
+//   128 x 28672 x  4096   37.5     -          -    27.3   36.3
+// A cluster of the tiles' blocks starts 3 us later than as many blocks. Up to 32 rows, tiles of 128 rows pay only where K is short.
+enum Fp8Way { WAY_STREAM, WAY_LONE64, WAY_LONE64_2, WAY_LONE64_4, WAY_LONE128, WAY_WIDE1, WAY_WIDE2 };
 static int stream_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
 static int stream_parts(const Fp8MatArgs& a) {
     const int64_t tiles = (int64_t)((a.n + FS_BM - 1) / FS_BM) * ((a.m + stream_rows(a.m) - 1) / stream_rows(a.m));
@@ -1100,8 +1142,11 @@ static Fp8Way way_of(const Fp8MatArgs& a) {
         const double rounds = floor(tiles / teams) + (left == 0 ? 0.0 : 2 * left <= teams ? half : 1.0);
         offer(g == 1 ? WAY_WIDE1 : WAY_WIDE2, g == 1 ? 3.62 + rounds * (0.557 * blocks + 1.47) : 3.77 + rounds * (0.425 * blocks + 1.95));
     }
-    if (const double tiles = over(a.m, 128) * over(a.n, 64); tiles <= sms) offer(WAY_LONE64, std::max(2.43 + 0.226 * blocks + 2.39 * tiles / sms, 4.7 + weights));
-    if (const double tiles = over(a.m, 128) * over(a.n, 128); tiles <= sms) offer(WAY_LONE128, std::max(2.88 + 0.266 * blocks + 2.48 * tiles / sms, 5.8 + weights));
+    const double low = over(a.m, 128) * over(a.n, 64), high = over(a.m, 128) * over(a.n, 128);
+    if (low <= sms) offer(WAY_LONE64, std::max(2.68 + 0.216 * blocks + 2.2 * low / sms, 3.9 + weights));
+    if (2 * low <= sms && blocks >= 16) offer(WAY_LONE64_2, std::max(6.1 + 0.22 * ceil(blocks / 2) + 1.7 * 2 * low / sms, 6.9 + weights));
+    if (4 * low <= 0.87 * sms && blocks >= 32) offer(WAY_LONE64_4, std::max(6.1 + 0.225 * ceil(blocks / 4) + 0.7 * 4 * low / sms, 6.5 + weights));
+    if (high <= sms) offer(WAY_LONE128, std::max(3.3 + 0.25 * blocks + 3.2 * high / sms, 4.9 + weights));
     // (several tiles of 128 rows only where K is long and they still fit side by side: 384 x 512 x 14336 16.4 us, tiles of 128 x 64 26.7)
     const int rows = stream_rows(a.m), parts = stream_parts(a);
     const double teams = over(a.n, FS_BM) * over(a.m, rows) * parts;
@@ -1118,8 +1163,10 @@ cudaError_t launch_fp8_matmul(const Fp8MatArgs& a, cudaStream_t st) {
     if (a.m < 0 || a.n < 0 || a.k <= 0 || a.k % 16 != 0) return cudaErrorInvalidValue;
     if (gemv_takes(a)) return gemv_of(a, st);
     switch (way_of(a)) {
-        case WAY_LONE64: return lone_of<64>(a, st);
-        case WAY_LONE128: return lone_of<128>(a, st);
+        case WAY_LONE64: return lone_of<64>(a, 1, st);
+        case WAY_LONE64_2: return lone_of<64>(a, 2, st);
+        case WAY_LONE64_4: return lone_of<64>(a, 4, st);
+        case WAY_LONE128: return lone_of<128>(a, 1, st);
         case WAY_WIDE1: return wide_of<1>(a, st);
         case WAY_WIDE2: return wide_of<2>(a, st);
         case WAY_STREAM: break;
