@@ -191,7 +191,7 @@ constexpr int FS_MAX_STAGES = 6, FS_MAX_PARTS = 8;
 
 struct Fp8StreamArgs {
     Fp8MatArgs p;
-    int parts, stages;
+    int parts, stages, x_rows;  // x_rows: of activations that a copy brings
 };
 
 // BN: activation rows of a tile.
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(FS_THREADS, 2) fp8_stream_kernel(const Fp8Stre
                 if (u > 0) ok = tc5_wait(&empty[st], (uint32_t)((u - 1) & 1));
                 if (!ok) break;
                 const uint32_t bar = tc5_smem_u32(&full[st]), dst = tc5_smem_u32(smem + st * STAGE);
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(STAGE) : "memory");
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(FS_W_BYTES + a.x_rows * FP8_BLOCK) : "memory");
                 tc5_tma_2d(dst, &map_w, (b0 + c) * FP8_BLOCK, n0, bar);
                 tc5_tma_2d(dst + FS_W_BYTES, &map_x, (b0 + c) * FP8_BLOCK, r0, bar);
                 issued = c + 1;
@@ -853,7 +853,7 @@ __device__ __forceinline__ void add_parts(const Fp8MatArgs& p, const uint8_t* ou
 }
 
 template <int W, bool ALIGNED>
-__global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArgs p, int k_parts, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+__global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArgs p, int k_parts, int x_rows, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     constexpr int STAGES = lone_stages(W), STAGE = lone_stage(W), COLS = 4 * W;
     extern __shared__ uint8_t fp_smem_raw[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], sum_full[4], sum_empty[4];
@@ -916,7 +916,7 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_lone_kernel(const Fp8MatArg
             if (lane == 0) {
                 const bool x = warp == 1;
                 const CUtensorMap* const map = x ? &map_x : &map_w;
-                const int row = x ? m0 : n0, bytes = (x ? 128 : W) * FP8_BLOCK, place = x ? 0 : 128 * FP8_BLOCK;
+                const int row = x ? m0 : n0, bytes = (x ? x_rows : W) * FP8_BLOCK, place = x ? 0 : 128 * FP8_BLOCK;
                 int issued = 0;
                 for (int st = 0, u = 0; issued < blocks; ++issued) {
                     if (u > 0) ok = tc5_wait(&empty[st], (uint32_t)((u - 1) & 1));
@@ -1013,15 +1013,20 @@ static bool fp8_map(CUtensorMap* map, const uint8_t* q, int64_t k, int64_t rows,
                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Rows past the last that a copy would fill with zeros cost more than those that are there (17 x 14336 x 4096 with boxes of 128 rows:
+// 24.5 us, of 24 rows 15.0), so where there is one tile of rows it copies those, in eights; sums of what lies behind them are not stored.
+static int copied_rows(int m, int tile) { return std::min(tile, (m + 7) / 8 * 8); }
+
 template <int BN>
 static cudaError_t stream_of(const Fp8MatArgs& a, int parts, cudaStream_t st) {
+    const int x_rows = copied_rows(a.m, BN);
     CUtensorMap mw, mx;
-    if (!fp8_map(&mw, a.wq, a.k, a.n, FS_BM) || !fp8_map(&mx, a.xq, a.k, a.m, BN)) return cudaErrorInvalidValue;
+    if (!fp8_map(&mw, a.wq, a.k, a.n, FS_BM) || !fp8_map(&mx, a.xq, a.k, a.m, x_rows)) return cudaErrorInvalidValue;
     static PerDeviceOnce once;
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_stream_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, FS_SMEM + 1024); });
     if (e != cudaSuccess) return e;
     constexpr int STAGE = FS_W_BYTES + BN * FP8_BLOCK;
-    const Fp8StreamArgs k{a, parts, std::min(FS_MAX_STAGES, FS_SMEM / STAGE)};
+    const Fp8StreamArgs k{a, parts, std::min(FS_MAX_STAGES, FS_SMEM / STAGE), x_rows};
     const dim3 grid((unsigned)((a.n + FS_BM - 1) / FS_BM), (unsigned)((a.m + BN - 1) / BN), (unsigned)parts);
     e = launch_pdl_cluster(fp8_stream_kernel<BN>, grid, dim3(FS_THREADS), (size_t)(k.stages * STAGE + 1024), st, parts, k, mw, mx);
     return e != cudaSuccess ? e : count_launch_and_check();
@@ -1063,8 +1068,9 @@ static cudaError_t wide_of(const Fp8MatArgs& a, cudaStream_t st) { return y_alig
 
 template <int W, bool ALIGNED>
 static cudaError_t lone_with(const Fp8MatArgs& a, int parts, cudaStream_t st) {
+    const int x_rows = copied_rows(a.m, 128);
     CUtensorMap mw, mx;
-    if (!fp8_map(&mw, a.wq, a.k, a.n, W) || !fp8_map(&mx, a.xq, a.k, a.m, 128)) return cudaErrorInvalidValue;
+    if (!fp8_map(&mw, a.wq, a.k, a.n, W) || !fp8_map(&mx, a.xq, a.k, a.m, x_rows)) return cudaErrorInvalidValue;
     constexpr int SMEM = lone_stages(W) * lone_stage(W) + 1024;
     static_assert(SMEM - 1024 >= 2 * FP_DRAINS * 4096 * (W / 64), "sums and results take the stages' place");
     static PerDeviceOnce once;
@@ -1072,8 +1078,8 @@ static cudaError_t lone_with(const Fp8MatArgs& a, int parts, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)((a.n + W - 1) / W), (unsigned)((a.m + 127) / 128), (unsigned)parts), block(FP_THREADS);
     static_assert(W == 64 || W == 128, "clusters share K of the lower tiles only");
-    e = parts == 1 ? launch_pdl(fp8_lone_kernel<W, ALIGNED>, grid, block, (size_t)SMEM, st, a, parts, mw, mx)
-                   : launch_pdl_cluster(fp8_lone_kernel<W, ALIGNED>, grid, block, (size_t)SMEM, st, parts, a, parts, mw, mx);
+    e = parts == 1 ? launch_pdl(fp8_lone_kernel<W, ALIGNED>, grid, block, (size_t)SMEM, st, a, parts, x_rows, mw, mx)
+                   : launch_pdl_cluster(fp8_lone_kernel<W, ALIGNED>, grid, block, (size_t)SMEM, st, parts, a, parts, x_rows, mw, mx);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
@@ -1118,7 +1124,7 @@ static cudaError_t gemv_of(const Fp8MatArgs& a, cudaStream_t st) {
 //   128 x  4096 x  8192   18.2   14.6 (2)   20.3   29.5   26.4         384 x  1536 x 8960    -  14.6 (2) 20.9   31.4   27.9
 //   128 x 14336 x  4096   24.7     -        15.2   18.9   19.9        2048 x  8192 x 4096    -      -      -    70.1   62.4
 //   128 x 28672 x  4096   37.5     -          -    27.3   36.3
-// A cluster of the tiles' blocks starts 3 us later than as many blocks. Up to 32 rows, tiles of 128 rows pay only where K is short.
+// A cluster of the tiles' blocks starts 3 us later than as many blocks.
 enum Fp8Way { WAY_STREAM, WAY_LONE64, WAY_LONE64_2, WAY_LONE64_4, WAY_LONE128, WAY_WIDE1, WAY_WIDE2 };
 static int stream_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
 static int stream_parts(const Fp8MatArgs& a) {
@@ -1129,7 +1135,7 @@ static int stream_parts(const Fp8MatArgs& a) {
     return parts;
 }
 static Fp8Way way_of(const Fp8MatArgs& a) {
-    if (a.m <= 16 || (a.m <= 32 && a.k > 1024)) return WAY_STREAM;
+    if (a.m <= 16) return WAY_STREAM;
     auto over = [](int64_t v, int by) { return (double)((v + by - 1) / by); };
     const double sms = device_sm_count(), blocks = (double)fp8_blocks(a.k), weights = (double)a.n * a.k / 6.2e6;
     Fp8Way best = WAY_WIDE2;
@@ -1153,7 +1159,7 @@ static Fp8Way way_of(const Fp8MatArgs& a) {
     if (a.m <= 128 || teams <= sms) {
         const double each = rows == 32 ? 0.442 : rows == 64 ? 0.368 : 0.79;
         const double load = std::min(std::max(teams / sms, 1.0), 2.0), rounds = over((int64_t)teams, (int)(2 * sms));
-        offer(WAY_STREAM, std::max(3.2 + (parts > 1 ? 0.47 : 0.0) + rounds * (ceil(blocks / parts) * each * (1 + 0.3 * (load - 1)) + 0.038 * std::min(a.m, rows)), 6.2 + weights));
+        offer(WAY_STREAM, std::max(3.2 + (parts > 1 ? 0.47 : 0.0) + rounds * (ceil(blocks / parts) * each * (1 + 0.3 * (load - 1)) + 0.038 * rows), 6.4 + weights));
     }
     return best;
 }
