@@ -569,7 +569,8 @@ __device__ __forceinline__ void drain_add(uint32_t taddr, float f, uint64_t (&ac
 
 struct Fp8WideArgs {
     Fp8MatArgs p;
-    int row_tiles, whole, items;  // items: tiles up to `whole`, halves of the following tiles (128 of their weight rows) after them
+    int row_tiles, x_rows;        // x_rows: of activations that a copy brings
+    int whole, items;             // items: tiles up to `whole`, halves of the following tiles (128 of their weight rows) after them
     bool handed;                  // results leave by warps of their own while the drains go on with the next tile
 };
 template <int G>
@@ -685,7 +686,7 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideAr
                 int st = 0, u = 0, issued = 0;
                 for (int item = team; ok && item < a.items; item += teams) {
                     const Fp8Item<G> it(a, item);
-                    const int r0 = it.r0 + 128 * rank, n0 = it.n0 + HALF * rank, bytes = 128 * FP8_BLOCK + (it.last - it.first + 1) * HALF * FP8_BLOCK;
+                    const int r0 = it.r0 + 128 * rank, n0 = it.n0 + HALF * rank, bytes = a.x_rows * FP8_BLOCK + (it.last - it.first + 1) * HALF * FP8_BLOCK;
                     for (int b = 0; b < blocks; ++b) {
                         if (u > 0) ok = tc5_wait(&empty[st], (uint32_t)((u - 1) & 1));
                         if (!ok) break;
@@ -1034,8 +1035,9 @@ static cudaError_t stream_of(const Fp8MatArgs& a, int parts, cudaStream_t st) {
 
 template <int G, bool ALIGNED>
 static cudaError_t wide_with(const Fp8MatArgs& a, cudaStream_t st) {
+    const int x_rows = G == 1 ? copied_rows(a.m, 128) : 128;
     CUtensorMap mw, mx;
-    if (!fp8_map(&mw, a.wq, a.k, a.n, FP_BN / 2 / G) || !fp8_map(&mx, a.xq, a.k, a.m, 128)) return cudaErrorInvalidValue;
+    if (!fp8_map(&mw, a.wq, a.k, a.n, FP_BN / 2 / G) || !fp8_map(&mx, a.xq, a.k, a.m, x_rows)) return cudaErrorInvalidValue;
     static PerDeviceOnce once;
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(fp8_wide_kernel<G, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, fp_smem(G) + 1024); });
     if (e != cudaSuccess) return e;
@@ -1044,7 +1046,7 @@ static cudaError_t wide_with(const Fp8MatArgs& a, cudaStream_t st) {
     if (tiles > INT32_MAX / 4) return cudaErrorInvalidValue;
     // the last round's tiles are halved where all halves find a place
     const int left = (int)(tiles % most), halved = 2 * left <= most ? left : 0;
-    const Fp8WideArgs k{a, (int)row_tiles, (int)tiles - halved, (int)tiles + halved, a.k > 1024};
+    const Fp8WideArgs k{a, (int)row_tiles, x_rows, (int)tiles - halved, (int)tiles + halved, a.k > 1024};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(std::min(k.items, most) * G));
     cfg.blockDim = dim3(FP_THREADS);

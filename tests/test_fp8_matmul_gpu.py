@@ -66,7 +66,7 @@ def test_product(ty, m, n, k):
 @pytest.mark.parametrize("m,n,k", [(8, 9000, 1536), (5, 2000, 8208), (16, 1000, 1040), (12, 4100, 2064), (3, 20000, 1024), (24, 640, 8192), (30, 3000, 512), (48, 1530, 8960),
                                    (64, 333, 4112), (96, 1536, 8960), (128, 200, 6160), (100, 32000, 896), (128, 28700, 1040), (40, 4000, 640), (128, 9400, 272), (500, 1000, 1040),
                                    (300, 8200, 1168), (512, 4100, 144), (257, 16500, 528), (2000, 8192, 512), (1500, 8200, 1296), (1300, 5000, 2064), (640, 19000, 1040), (300, 500, 12304), (513, 129, 8208), (128, 4096, 4112), (100, 2500, 8208), (60, 4090, 8192), (384, 1500, 8976), (130, 1001, 6160), (70, 2600, 14352),
-                                   (40, 600, 14336), (256, 1024, 6400)])
+                                   (40, 600, 14336), (256, 1024, 6400), (17, 28800, 1040), (41, 20000, 2064), (19, 9300, 2576)])
 def test_every_way(ty, m, n, k):
     a = inputs(m, n, k, m + n)
     check(product(*a, ty, 4 * (m % 2)), *a)
