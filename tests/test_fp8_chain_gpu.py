@@ -114,7 +114,7 @@ def test_captured_replayed_and_side_by_side(m):
         assert all(torch.equal(t, u) for t, u in zip(c.results(), w))
 
 
-@pytest.mark.parametrize("m,n,k", [(3, 9000, 4096), (64, 4000, 8192), (200, 2000, 2064), (900, 16400, 1168), (2048, 8192, 2064)])
+@pytest.mark.parametrize("m,n,k", [(3, 9000, 4096), (64, 4000, 8192), (128, 4096, 8208), (384, 500, 12304), (200, 2000, 2064), (900, 16400, 1168), (2048, 8192, 2064)])
 def test_products_on_two_streams_at_once(m, n, k):
     a = [mat.inputs(m, n, k, s) for s in (1, 2)]
     want = [mat.product(*x, ops.BF16) for x in a]
