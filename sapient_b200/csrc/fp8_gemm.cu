@@ -1140,6 +1140,9 @@ static Fp8Way way_of(const Fp8MatArgs& a) {
     if (a.m <= 16) return WAY_STREAM;
     auto over = [](int64_t v, int by) { return (double)((v + by - 1) / by); };
     const double sms = device_sm_count(), blocks = (double)fp8_blocks(a.k), weights = (double)a.n * a.k / 6.2e6;
+    // Rows that do not start on 128 bytes, or not on the 32 of a sector: an SM takes in more lines for the same columns (325 x 4266, tiles of
+    // 128 x 128: K of 7040 21.0 us, 7008 26.1, 7024 32.6; 256 x 256 by two SMs 24.9, 25.3, 25.9).
+    const double skew = a.k % 128 == 0 ? 0.0 : a.k % 32 == 0 ? 0.4 : 1.0;
     Fp8Way best = WAY_WIDE2;
     double least = 1e30;
     auto offer = [&](Fp8Way way, double us) {
@@ -1148,13 +1151,13 @@ static Fp8Way way_of(const Fp8MatArgs& a) {
     for (int g = 1; g <= 2; ++g) {
         const double teams = floor(sms / g), tiles = over(a.m, 128 * g) * over(a.n, FP_BN), left = fmod(tiles, teams), half = g == 1 ? 0.685 : 0.762;
         const double rounds = floor(tiles / teams) + (left == 0 ? 0.0 : 2 * left <= teams ? half : 1.0);
-        offer(g == 1 ? WAY_WIDE1 : WAY_WIDE2, g == 1 ? 3.62 + rounds * (0.557 * blocks + 1.47) : 3.77 + rounds * (0.425 * blocks + 1.95));
+        offer(g == 1 ? WAY_WIDE1 : WAY_WIDE2, g == 1 ? 3.62 + rounds * ((0.557 + 0.06 * skew) * blocks + 1.47) : 3.77 + rounds * (0.425 * blocks + 1.95));
     }
     const double low = over(a.m, 128) * over(a.n, 64), high = over(a.m, 128) * over(a.n, 128);
-    if (low <= sms) offer(WAY_LONE64, std::max(2.68 + 0.216 * blocks + 2.2 * low / sms, 3.9 + weights));
-    if (2 * low <= sms && blocks >= 16) offer(WAY_LONE64_2, std::max(6.1 + 0.22 * ceil(blocks / 2) + 1.7 * 2 * low / sms, 6.9 + weights));
-    if (4 * low <= 0.87 * sms && blocks >= 32) offer(WAY_LONE64_4, std::max(6.1 + 0.225 * ceil(blocks / 4) + 0.7 * 4 * low / sms, 6.5 + weights));
-    if (high <= sms) offer(WAY_LONE128, std::max(3.3 + 0.25 * blocks + 3.2 * high / sms, 4.9 + weights));
+    if (low <= sms) offer(WAY_LONE64, std::max(2.68 + (0.216 + 0.03 * skew) * blocks + 2.2 * low / sms, 3.9 + weights));
+    if (2 * low <= sms && blocks >= 16) offer(WAY_LONE64_2, std::max(6.1 + (0.22 + 0.03 * skew) * ceil(blocks / 2) + 1.7 * 2 * low / sms, 6.9 + weights));
+    if (4 * low <= 0.87 * sms && blocks >= 32) offer(WAY_LONE64_4, std::max(6.1 + (0.225 + 0.03 * skew) * ceil(blocks / 4) + 0.7 * 4 * low / sms, 6.5 + weights));
+    if (high <= sms) offer(WAY_LONE128, std::max(3.3 + (0.25 + 0.17 * skew) * blocks + 3.2 * high / sms, 4.9 + weights));
     // (several tiles of 128 rows only where K is long and they still fit side by side: 384 x 512 x 14336 16.4 us, tiles of 128 x 64 26.7)
     const int rows = stream_rows(a.m), parts = stream_parts(a);
     const double teams = over(a.n, FS_BM) * over(a.m, rows) * parts;
