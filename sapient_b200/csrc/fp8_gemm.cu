@@ -491,7 +491,7 @@ __device__ __forceinline__ bool drains_agree(bool ok) {
 //
 // The wide kernel's two halves of 128 weight rows have sums and drain warps of their own, two of each: while one is drained three are
 // with the tensor cores. 4096 x 14336 x 4096: 205 to 209 us, 2.3 PFLOP/s, at the 1.5 GHz to which the power limit takes the clock;
-// 168 without drains. The tensor cores are never idle: a half takes 417 cycles for 256 of products (335 without drains), since
+// 168 without drains. The tensor cores always have products to do, but a half takes 417 cycles for 256 of products (335 without drains):
 // drains read the tensor memory that products add into. Slower: products of 256 columns with two sums (220 us), 16 drain warps (238),
 // results by TMA (232), columns of tiles first (221). No effect: more stages, a second warp that issues products.
 constexpr int FP_BN = 256;
