@@ -92,6 +92,12 @@ def test_large(m, n, k):
     check(product(*a), *a)
 
 
+@pytest.mark.parametrize("m,n,k", [(70000, 16, 16), (17, 200000, 16), (16, 100003, 16), (33, 65537, 128), (200001, 7, 32), (1000, 3, 16400), (2, 5, 60000), (129, 1, 16), (40000, 130, 48)])
+def test_long_in_one_direction(m, n, k):
+    a = inputs(m, n, k, 11)
+    check(product(*a, ops.BF16, 1), *a)
+
+
 def test_each_row_is_its_own_whatever_the_others():
     """Rows of a batch, of a prompt and alone: within the tolerance of each other, since all are of the formula; a NaN or an infinite
     scale in one row leaves the others."""

@@ -90,6 +90,25 @@ def test_the_sum_may_take_the_place_of_either_input(ty):
     assert torch.equal(y, (x.float() * 2).to(TYPES[ty]))
 
 
+@pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
+@pytest.mark.parametrize("n,dim", [(1, 16), (2, 208), (3, 4096), (901, 1040), (5, 8208), (2001, 144), (3, 20000)])
+def test_norm_without_a_residual(ty, n, dim):
+    """Rows in twos, odd numbers of them; the sum is a copy, elsewhere or in place."""
+    g = torch.Generator(device="cuda").manual_seed(n + dim)
+    x, w = rows(g, n, dim, dim + 8, ty), 0.5 + torch.rand(dim, generator=g, device="cuda")
+    want = norm64(x, None, w)[1]
+    total = torch.zeros(n + 1, dim, device="cuda", dtype=TYPES[ty])
+    q, s = norm(x, None, w, total=total[:n])
+    check(q, s, want)
+    assert torch.equal(total[:n], x) and (total[n] == 0).all()
+    y = x.clone(memory_format=torch.preserve_format)
+    assert torch.equal(norm(y, None, w, total=y)[0], q) and torch.equal(x, y)
+    x[n // 2] = 0  # a row of zeros beside others
+    q, s = norm(x, None, w)
+    assert (q[n // 2] & 0x7F == 0).all() and torch.isfinite(s).all()
+    check(q, s, norm64(x, None, w)[1])
+
+
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
 @pytest.mark.parametrize("n,dim,pad", [(1, 16, 0), (3, 112, 8), (2, 1040, 0), (7, 4864, 0), (64, 2560, 16), (3, 14336, 0), (70000, 16, 0)])
