@@ -152,7 +152,8 @@ int32_t sp_cuda_argmax(int32_t device, const float* logits, int64_t rows, int64_
  * w, q, xq and wq. rows or m = 0 is a call that does nothing. */
 /* h = x + residual (NULL: h = x), y = h / sqrt(mean(h^2) + eps) * w (NULL: 1); y as fp8 rows to q[rows][dim], scale[rows][blocks],
  * h to sum_out (NULL: not stored), which may be x or residual with the same stride. y is made from h before h is rounded to
- * sum_out's type. dim at most 32768. h^2 is added up in f32, so that |h| above 2^63 / sqrt(dim) is outside of its range. */
+ * sum_out's type. dim at most 32768. h^2 is added up in f32, so that |h| above 2^63 / sqrt(dim) is outside of its range, and so is
+ * mean(h^2) + eps below 2^-126; a row of zeros at eps = 0 is 0 / 0, NaN. */
 int32_t sp_cuda_rms_norm_fp8_dev(int32_t device, int32_t dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
                                  void* sum_out, int64_t lds, const float* w, float eps, int64_t rows, int64_t dim, void* q,
                                  float* scale, void* stream);

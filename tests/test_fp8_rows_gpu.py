@@ -171,3 +171,25 @@ def test_host_forms_and_another_stream():
         q, s = norm(a, None, ww)
     st.synchronize()
     check(q, s, norm64(a, None, ww)[1])
+
+
+@pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
+@pytest.mark.parametrize("dim", [272, 4096, 8208, 20000])
+@pytest.mark.parametrize("with_sum", [False, True])
+def test_norms_of_zeros_and_of_very_small_rows(ty, dim, with_sum):
+    """1 / sqrt(mean(h^2) + eps) and 1 / scale are both large here, their product past the largest f32: a block of zeros is zeros all the
+    same, and small values keep their digits. Of h and w only values whose sums and products f32 holds without a rounding of their own
+    below 2^-126: eight bits of a sum of two equal rows, w a power of two."""
+    g = torch.Generator(device="cuda").manual_seed(dim + ty)
+    w = torch.full((dim,), 2.0, device="cuda")
+    for size, eps in [(0.0, 1e-18), (0.0, 1e-20), (0.0, 1e-30), (1e-10, 0.0), (1e-17, 0.0), (1e-37, 1e-30), (1e-37, 1e-37), (1e-41, 1e-37)]:
+        x = (torch.randn(5, dim, generator=g, device="cuda").bfloat16().float() * size).to(TYPES[ty])
+        x[:, 128:256] = 0
+        if size:
+            x[:, 0] = size  # bf16 has few of the smallest
+        if with_sum and size == 0:
+            x = rows(g, 5, dim, dim, ty)
+        r = None if not with_sum else -x if size == 0 else x.clone()
+        q, s = norm(x, r, w, eps)
+        check(q, s, norm64(x, r, w, eps)[1])
+        assert (q[:, 128:256] & 0x7F == 0).all() and (s[:, 1] == 2.0**-100).all()
