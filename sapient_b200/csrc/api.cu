@@ -122,7 +122,6 @@ struct OnDevice {
         cudaError_t e = cudaGetDevice(&before);
         if (e != cudaSuccess) before = -1;
         if (e == cudaSuccess && before != device) e = cudaSetDevice(device);
-        if (e != cudaSuccess) cudaGetLastError();  // (the next launch would find it)
         return e;
     }
     ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
@@ -403,10 +402,7 @@ static int matmul_nt_fp8(SpWeight* w, const float* x, int64_t m, float* y, cudaS
         const int64_t rows = std::max((m + 127) / 128 * 128, 2 * w->xq_rows);  // (doubled: the smaller ones take no more than the last)
         if (w->xq) w->xq_before.reserve(w->xq_before.size() + 1);
         uint8_t* p = nullptr;
-        if (const cudaError_t e = cudaMalloc((void**)&p, rows * (row + 4 * scales)); e != cudaSuccess) {
-            cudaGetLastError();
-            SP_CUDA_TRY(e);
-        }
+        SP_CUDA_TRY(cudaMalloc((void**)&p, rows * (row + 4 * scales)));
         if (w->xq) w->xq_before.push_back(w->xq);
         w->xq = p;
         w->xq_rows = rows;

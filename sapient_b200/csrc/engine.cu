@@ -19,7 +19,12 @@ namespace sp {
     } while (0)
 
 static thread_local std::string g_err;
-void set_error(const std::string& msg) { g_err = msg; }
+// A call that fails says so here, and that is the end of its CUDA error: the thread's next launch, which asks the runtime for the last
+// one, does not find it.
+void set_error(const std::string& msg) {
+    g_err = msg;
+    cudaGetLastError();
+}
 const char* get_error() { return g_err.c_str(); }
 
 // IEEE half <-> float on the host (round-to-nearest-even), used only at load time.

@@ -2,6 +2,8 @@
 captured graphs, on several streams at once; rows far apart in memory; a wait that ran out; a device that is not there.
 
 Each step is held against its formula in 64 bits on the inputs that it was given, with the tolerances of its own tests."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -10,7 +12,7 @@ import test_fp8_matmul_gpu as mat
 import test_fp8_rows_gpu as rows
 import test_logprobs_gpu as lp
 from sapient_b200 import ops
-from sapient_b200._lib import SP_ERR_CUDA, SP_ERR_STATE, SapientCudaError, check, lib
+from sapient_b200._lib import SP_ERR_CUDA, SP_ERR_OOM, SP_ERR_STATE, SapientCudaError, check, lib
 
 pytestmark = pytest.mark.gpu
 TYPES = {ops.F32: torch.float32, ops.BF16: torch.bfloat16}
@@ -225,3 +227,32 @@ def test_a_device_that_is_not_there():
     ops.quant_fp8_dev(x.data_ptr(), 2, 256, q.data_ptr(), s.data_ptr())
     torch.cuda.synchronize()
     rows.check(q, s, x.double())
+
+
+def test_a_refused_call_leaves_no_error_for_the_next_one():
+    """Each call that fails says so itself; the launch that follows it on the same thread is not the one to answer for it."""
+    x = torch.ones(2, 256, device="cuda")
+    q, s = torch.empty(2, 256, device="cuda", dtype=torch.uint8), torch.empty(2, 2, device="cuda")
+    host, bytes_, ones = np.ones((2, 256), np.float32), np.ones((2, 256), np.uint8), np.ones((1, 2), np.float32)
+    h, some = C.c_void_p(), host.ctypes.data_as(C.c_void_p)
+
+    def more_than_there_is():  # (2^56 bytes: refused before anything is read)
+        check(lib().sp_cuda_upload_weight_fp8(0, 1 << 28, 1 << 28, some, some, C.byref(h)))
+
+    fails = [(SP_ERR_CUDA, lambda: ops.quant_fp8(host, device=63)), (SP_ERR_CUDA, lambda: ops.swiglu_fp8(host, device=63)),
+             (SP_ERR_CUDA, lambda: ops.rms_norm_fp8(host, None, EPS, device=63)), (SP_ERR_CUDA, lambda: ops.logprobs(host, [0, 1], device=63)),
+             (SP_ERR_CUDA, lambda: ops.matmul_fp8(bytes_, np.ones((2, 2)), bytes_, ones, device=63)), (SP_ERR_CUDA, lambda: ops.Weight.from_fp8(bytes_, ones, device=63)),
+             (SP_ERR_CUDA, lambda: ops.silu(host, device=63)), (SP_ERR_CUDA, lambda: ops.Weight(ops.F32, 2, 256, host.view(np.uint8), device=63)),
+             (SP_ERR_OOM, more_than_there_is)]
+    wrong = []
+    for i, (status, call) in enumerate(fails):
+        with pytest.raises(SapientCudaError) as e:
+            call()
+        assert e.value.status == status
+        q.zero_()
+        try:
+            ops.quant_fp8_dev(x.data_ptr(), 2, 256, q.data_ptr(), s.data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+            rows.check(q, s, x.double())
+        except SapientCudaError:
+            wrong.append(i)
+    assert not wrong
