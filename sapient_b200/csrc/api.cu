@@ -306,6 +306,7 @@ int32_t sp_cuda_upload_weight(int32_t device, int32_t dtype, int64_t n, int64_t 
     SpWeight* w = new SpWeight{device, dtype, n, k, nullptr, nbytes};
     cudaError_t ce = cudaMalloc((void**)&w->d, nbytes + 16);
     if (ce == cudaSuccess) ce = cudaMemcpy(w->d, host_blocks, nbytes, cudaMemcpyHostToDevice);
+    if (ce == cudaSuccess) ce = cudaStreamSynchronize(0);  // (a copy from pageable memory may return ahead of its end, and the weight's first use be on any stream)
     if (ce == cudaSuccess && imma_supported(dtype, k) && n > 0) {
         ce = cudaMalloc((void**)&w->tiled, imma_tiled_bytes(dtype, n, k) + 16);
         if (ce == cudaSuccess) ce = launch_repack(dtype, w->d, n, k, w->tiled, 0);
@@ -344,6 +345,7 @@ int32_t sp_cuda_upload_weight_fp8(int32_t device, int64_t n, int64_t k, const vo
     if (ce == cudaSuccess) ce = cudaMalloc((void**)&w->scale, scale_bytes);
     if (ce == cudaSuccess) ce = cudaMemcpy(w->d, values, nbytes, cudaMemcpyHostToDevice);
     if (ce == cudaSuccess) ce = cudaMemcpy(w->scale, scales, scale_bytes, cudaMemcpyHostToDevice);
+    if (ce == cudaSuccess) ce = cudaStreamSynchronize(0);  // (as for the other types)
     if (ce != cudaSuccess) {
         set_error(std::string("upload_weight_fp8: ") + cudaGetErrorString(ce));
         sp_cuda_free_weight(w);

@@ -256,3 +256,23 @@ def test_a_refused_call_leaves_no_error_for_the_next_one():
         except SapientCudaError:
             wrong.append(i)
     assert not wrong
+
+
+def test_a_weight_is_there_when_its_upload_returns():
+    """The first product may be on any stream, one that does not wait for the default stream among them."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    st = torch.cuda.Stream()
+    for n, k in [(16, 64), (130, 272), (1000, 1040), (4096, 4096)]:
+        q, s = weight(n, k, g)
+        values, scales = q.view(torch.uint8).cpu().numpy(), s.cpu().numpy()
+        x = torch.randn(3, k, generator=g, device="cuda")
+        y = torch.zeros(20, 3, n, device="cuda")
+        torch.cuda.synchronize()
+        for i in range(20):
+            w = ops.Weight.from_fp8(values, scales)
+            w.matmul_nt_dev(x.data_ptr(), 3, y[i].data_ptr(), st.cuda_stream)
+            st.synchronize()
+            w.free()
+        xq, sx = (torch.from_numpy(t).cuda() for t in ops.quant_fp8(x.cpu().numpy()))
+        mat.check(y[0], xq.view(torch.float8_e4m3fn), sx, q, s)
+        assert (y == y[0]).all()
