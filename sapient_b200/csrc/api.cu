@@ -421,6 +421,7 @@ int32_t sp_cuda_matmul_nt_dev(const SpWeight* w, const float* x_dev, int64_t m, 
     API_BEGIN
     if (!w || !x_dev || !y_dev || m < 0) { set_error("null argument"); return SP_ERR_ARG; }
     if (((uintptr_t)x_dev & 15) != 0) { set_error("x must be 16-byte aligned"); return SP_ERR_ARG; }
+    if (unaligned(y_dev, 4)) { set_error("y must be 4-byte aligned"); return SP_ERR_ARG; }
     SP_CUDA_TRY(cudaSetDevice(w->device));
     if (w->dtype == SP_F8_E4M3) return matmul_nt_fp8(const_cast<SpWeight*>(w), x_dev, m, y_dev, (cudaStream_t)stream);
     if (w->tiled && g_gemv_path.load() == 0 && g_tc5.load() && m >= TC5_MIN_M && tc5_supported(w->dtype, w->k)) {
@@ -768,7 +769,11 @@ int32_t sp_cuda_logprobs_dev(int32_t device, int32_t dtype, const void* logits, 
     const int st = check_logprobs(rows, vocab, top);
     if (st != SP_OK) return st;
     if (ld < vocab) { set_error("logprobs: the row stride must hold a row"); return SP_ERR_SHAPE; }
-    if (unaligned(logits, dtype == SP_F32 ? 4 : 2)) { set_error("misaligned argument"); return SP_ERR_ARG; }
+    if (unaligned(logits, dtype == SP_F32 ? 4 : 2) || unaligned(ids, 4) || unaligned(logprob, 4) || unaligned(entropy, 4) || unaligned(top_ids, 4) ||
+        unaligned(top_logprobs, 4)) {
+        set_error("misaligned argument");
+        return SP_ERR_ARG;
+    }
     if (rows == 0) return SP_OK;
     OnDevice on;
     SP_CUDA_TRY(on.enter(device));

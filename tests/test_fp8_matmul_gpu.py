@@ -149,3 +149,16 @@ def test_weights_on_the_device():
             w.embed([0])
         assert e.value.status == SP_ERR_DTYPE
         w.free()
+
+
+def test_results_that_start_inside_a_value():
+    from sapient_b200._lib import SP_ERR_ARG, SapientCudaError
+
+    w = ops.Weight.from_fp8(np.ones((4, 32), np.uint8), np.ones((1, 1)))
+    x, y = torch.ones(2, 32, device="cuda"), torch.zeros(16, device="cuda")
+    for off in (1, 2, 3):
+        with pytest.raises(SapientCudaError) as e:
+            w.matmul_nt_dev(x.data_ptr(), 2, y.data_ptr() + off, torch.cuda.current_stream().cuda_stream)
+        assert e.value.status == SP_ERR_ARG
+    w.matmul_nt_dev(x.data_ptr(), 2, y.data_ptr() + 4, torch.cuda.current_stream().cuda_stream)
+    assert (y[1:9] != 0).all() and (y[9:] == 0).all() and y[0] == 0

@@ -113,3 +113,11 @@ def test_arguments_reach_the_library_as_ctypes_would_pass_them():
                            ((0, F32, P, 64, 0, 64, P, P), TypeError), ((0, F32, P, 1 << 80, 0, 64, P, P, 0), OverflowError)]:
             with pytest.raises(error):
                 c.quant_fp8(*bad)
+
+
+def test_addresses_of_distributions():
+    """Of each array the call writes or reads: addresses inside a value would fault."""
+    f = _lib.lib().sp_cuda_logprobs_dev
+    call = lambda ids=P, lp=P, ent=P, ti=P, tl=P: f(0, F32, P, 100, 2, 100, ids, 3, lp, ent, ti, tl, None)  # noqa: E731
+    for name in ("ids", "lp", "ent", "ti", "tl"):
+        assert [call(**{name: P + off}) for off in (1, 2, 3)] == [ARG] * 3
