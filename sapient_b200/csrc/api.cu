@@ -159,6 +159,7 @@ int check_fp8_rows(const char* what, const void* p, int64_t ld, int64_t dim, int
 
 int check_fp8_dim(int64_t rows, int64_t dim, const char* name) {
     if (rows < 0 || dim <= 0 || dim % 16 != 0 || dim > INT32_MAX / 2) { set_error(std::string("fp8: ") + name + " must be a positive multiple of 16"); return SP_ERR_SHAPE; }
+    if (rows > INT64_MAX / 16 / dim) { set_error("fp8: more rows than bytes can be counted"); return SP_ERR_SHAPE; }
     return SP_OK;
 }
 
@@ -854,7 +855,7 @@ int32_t sp_cuda_matmul_fp8(int32_t device, const void* xq, const float* xs, int6
     API_BEGIN
     if (!xq || !xs || !wq || !ws || !y) { set_error("null argument"); return SP_ERR_ARG; }
     SP_STEP(check_fp8_dim(m, k, "k"));
-    if (n < 0) { set_error("matmul_fp8: bad shape"); return SP_ERR_SHAPE; }
+    if (m > INT32_MAX / 2 || n < 0 || n > INT32_MAX / 2) { set_error("matmul_fp8: bad shape"); return SP_ERR_SHAPE; }
     if (m == 0 || n == 0) return SP_OK;
     SP_CUDA_TRY(cudaSetDevice(device));
     const int64_t nb = fp8_blocks(k);

@@ -121,3 +121,14 @@ def test_addresses_of_distributions():
     call = lambda ids=P, lp=P, ent=P, ti=P, tl=P: f(0, F32, P, 100, 2, 100, ids, 3, lp, ent, ti, tl, None)  # noqa: E731
     for name in ("ids", "lp", "ent", "ti", "tl"):
         assert [call(**{name: P + off}) for off in (1, 2, 3)] == [ARG] * 3
+
+
+def test_more_rows_than_bytes_can_be_counted():
+    """Host forms multiply sizes before they allocate: products past 64 bits are refused, not taken modulo them."""
+    x = np.zeros((2, 64), np.float32)
+    p, L = x.ctypes.data_as(C.c_void_p), _lib.lib()
+    for rows, dim in [(1 << 60, 16), ((1 << 62) + 1, 64), ((1 << 63) - 1, 32768)]:
+        assert L.sp_cuda_rms_norm_fp8(0, p, None, None, rows, dim, 1e-5, p, p, p) == SHAPE
+        assert L.sp_cuda_quant_fp8(0, p, rows, dim, p, p) == SHAPE and L.sp_cuda_swiglu_fp8(0, p, rows, dim, p, p) == SHAPE
+    for m, n, k in [(1 << 60, 2, 16), (2, 1 << 60, 16), (1 << 31, 2, 16), (2, 1 << 31, 16), ((1 << 62) + 1, (1 << 62) + 1, 64)]:
+        assert L.sp_cuda_matmul_fp8(0, p, p, m, p, p, n, k, p) == SHAPE
