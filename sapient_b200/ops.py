@@ -34,6 +34,16 @@ def _bits8(a, what: str) -> np.ndarray:
     return np.ascontiguousarray(a).view(np.uint8)
 
 
+def _ids32(a, what: str) -> np.ndarray:
+    """Token ids as they are: a number that is none is not cut down to one."""
+    a = np.asarray(a).reshape(-1)
+    if a.size and a.dtype.kind not in "iu":
+        raise SapientCudaError(_lib.SP_ERR_DTYPE, f"{what}: ids are whole numbers, not {a.dtype}")
+    if a.size and (a.min() < 0 or a.max() > 0xFFFFFFFF):
+        raise SapientCudaError(_lib.SP_ERR_VOCAB, f"{what}: token id out of vocab range")
+    return np.ascontiguousarray(a, dtype=np.uint32)
+
+
 def _f32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.float32)
 
@@ -250,7 +260,7 @@ def logprobs(logits, ids, top: int = 0, device: int = 0):
     lowest id comes first. ids may be None, the first of the four is then, too."""
     z = _rows2(logits, "logprobs")
     rows = z.shape[0]
-    i = None if ids is None else np.ascontiguousarray(ids, dtype=np.uint32).reshape(-1)
+    i = None if ids is None else _ids32(ids, "logprobs")
     if i is not None and i.size != rows:
         raise SapientCudaError(_lib.SP_ERR_SHAPE, "logprobs: one id per row expected")
     if not 0 <= top <= LOGPROBS_MAX_TOP:

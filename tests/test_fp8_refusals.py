@@ -132,3 +132,13 @@ def test_more_rows_than_bytes_can_be_counted():
         assert L.sp_cuda_quant_fp8(0, p, rows, dim, p, p) == SHAPE and L.sp_cuda_swiglu_fp8(0, p, rows, dim, p, p) == SHAPE
     for m, n, k in [(1 << 60, 2, 16), (2, 1 << 60, 16), (1 << 31, 2, 16), (2, 1 << 31, 16), ((1 << 62) + 1, (1 << 62) + 1, 64)]:
         assert L.sp_cuda_matmul_fp8(0, p, p, m, p, p, n, k, p) == SHAPE
+
+
+def test_ids_that_are_none():
+    """A token id is a whole number of 32 bits: others are not cut down to one."""
+    x = np.zeros((2, 64), np.float32)
+    for status, ids in [(VOCAB, [-1, 0]), (VOCAB, np.array([0, (1 << 32) + 5])), (VOCAB, np.array([0, -(1 << 32)])), (VOCAB, np.array([1 << 63, 0], np.uint64)),
+                        (DTYPE, [0.0, 1.5]), (DTYPE, np.array([True, False])), (DTYPE, ["1", "2"]), (DTYPE, [1 << 70, 0])]:
+        with pytest.raises(_lib.SapientCudaError) as e:
+            ops.logprobs(x, ids)
+        assert e.value.status == status
