@@ -143,7 +143,9 @@ int32_t sp_cuda_argmax(int32_t device, const float* logits, int64_t rows, int64_
  * An fp8 row of k columns is k e4m3 values and ceil(k / 128) f32 scales; a value stands for e4m3 x the scale of its block of
  * 128 columns (the last block may be shorter). Rows are quantised by
  *     scale = max(max |y| of the block / 448, 2^-100),   q = e4m3(y / scale), to nearest even
- * and a block that holds a NaN or an infinity gets one as its scale. k and dim are multiples of 16.
+ * in f32, y / scale by a reciprocal: off by up to 2^-22 of itself before the rounding to e4m3, so that a value beside a border of
+ * e4m3's grid (one or two of a million) may fall on its other side. A block that holds a NaN or an infinity (a y past f32's range
+ * is one) gets one as its scale. k and dim are multiples of 16.
  * The _dev calls take device pointers of `device` (the calling thread's current device is what it was when they return) and a
  * cudaStream_t (NULL: default stream), launch one kernel and do not wait. They keep nothing between calls, so that they may
  * run at the same time on several streams and be captured into graphs. dtype of a _dev call: SP_F32 or SP_BF16, of x, residual,
@@ -157,14 +159,15 @@ int32_t sp_cuda_argmax(int32_t device, const float* logits, int64_t rows, int64_
 int32_t sp_cuda_rms_norm_fp8_dev(int32_t device, int32_t dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
                                  void* sum_out, int64_t lds, const float* w, float eps, int64_t rows, int64_t dim, void* q,
                                  float* scale, void* stream);
-/* y = silu(gu[:, 0 .. ffn)) * gu[:, ffn .. 2 ffn) as fp8 rows. */
+/* y = silu(gu[:, 0 .. ffn)) * gu[:, ffn .. 2 ffn) as fp8 rows; a sigmoid below 2^-126 (gates below -87.3) counts as 0. */
 int32_t sp_cuda_swiglu_fp8_dev(int32_t device, int32_t dtype, const void* gu, int64_t ld, int64_t rows, int64_t ffn, void* q,
                                float* scale, void* stream);
 /* x as fp8 rows. */
 int32_t sp_cuda_quant_fp8_dev(int32_t device, int32_t dtype, const void* x, int64_t ldx, int64_t rows, int64_t dim, void* q,
                               float* scale, void* stream);
 /* y[m][n] (row stride ldy values of dtype) = X Wᵀ of fp8 rows xq[m][k], xs[m][blocks] and e4m3 weights wq[n][k] with scales
- * ws[ceil(n / 128)][blocks]. Products are exact, sums f32. */
+ * ws[ceil(n / 128)][blocks]. Products are exact, sums f32; xs x ws is formed in f32 first, with full digits from 2^-126 to 2^128. The
+ * order of a sum, and with it its last bits, depends on the sizes, on whether xq and wq start on 32 bytes, and on the device's SMs. */
 int32_t sp_cuda_matmul_fp8_dev(int32_t device, const void* xq, const float* xs, int64_t m, const void* wq, const float* ws, int64_t n,
                                int64_t k, void* y, int32_t dtype, int64_t ldy, void* stream);
 /* Of each row of logits[rows][vocab] (row stride ld): logprob[rows] of the token ids[row] (NaN for an id outside the vocabulary),
@@ -172,7 +175,8 @@ int32_t sp_cuda_matmul_fp8_dev(int32_t device, const void* xq, const float* xs, 
  * top_ids[rows][top], most likely first and the lower id first among equal logits (unlike sp_cuda_argmax, which gives the last),
  * with their top_logprobs[rows][top]. Each output may be NULL; ids only with logprob. A logit of -inf is a masked token; a row of
  * nothing else has log probabilities of -inf and entropy 0. A row with a NaN or +inf has NaN everywhere but in top_ids, where a NaN
- * counts as the largest. */
+ * counts as the largest. Sums are f32, in an order that depends on rows, vocab, top, dtype, where a row starts within 16 bytes, and the
+ * device's SMs. */
 #define SP_LOGPROBS_MAX_TOP 32
 int32_t sp_cuda_logprobs_dev(int32_t device, int32_t dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab,
                              const uint32_t* ids, int32_t top, float* logprob, float* entropy, uint32_t* top_ids,

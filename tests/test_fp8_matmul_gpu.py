@@ -162,3 +162,12 @@ def test_results_that_start_inside_a_value():
         assert e.value.status == SP_ERR_ARG
     w.matmul_nt_dev(x.data_ptr(), 2, y.data_ptr() + 4, torch.cuda.current_stream().cuda_stream)
     assert (y[1:9] != 0).all() and (y[9:] == 0).all() and y[0] == 0
+
+
+@pytest.mark.parametrize("n,k", [(384, 528), (4100, 2064), (2000, 8208)])
+def test_rows_alone_and_among_others(n, k):
+    """Which kernel a row goes through depends on how many there are, and so do its bits; the bounds of the formula do not."""
+    xq, xs, wq, ws = inputs(600, n, k, 12)
+    for at, m in [(0, 1), (599, 1), (5, 7), (64, 16), (10, 40), (100, 128), (0, 300), (0, 600)]:
+        a = (xq[at : at + m], xs[at : at + m], wq, ws)
+        check(product(*a), *a)

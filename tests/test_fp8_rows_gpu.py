@@ -193,3 +193,40 @@ def test_norms_of_zeros_and_of_very_small_rows(ty, dim, with_sum):
         q, s = norm(x, r, w, eps)
         check(q, s, norm64(x, r, w, eps)[1])
         assert (q[:, 128:256] & 0x7F == 0).all() and (s[:, 1] == 2.0**-100).all()
+
+
+@pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
+@pytest.mark.parametrize("u_size", [1.0, 1e4, 1e30])
+def test_gates_far_from_zero(ty, u_size):
+    """The sigmoid is taken for zero below 2^-126, and off by 2^-21 + |g| 2^-23 of itself above (|g| 2^-24 and half as much again from the
+    exponent's product, exp and reciprocal 2^-22 each); products, the scale and its reciprocal add less than 2^-21."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    gates = torch.tensor([-1e30, -200.0, -89.0, -88.5, -87.5, -87.25, -87.0, -80.0, -40.0, -0.0, 0.0, 40.0, 80.0, 87.5, 89.0, 200.0, 1e4], device="cuda").repeat_interleave(128)
+    dim = gates.numel()
+    x = torch.empty(3, 2 * dim, device="cuda")
+    x[:, :dim], x[:, dim:] = gates, u_size * torch.randn(3, dim, generator=g, device="cuda")
+    x = x.to(TYPES[ty])
+    q, s = torch.empty(3, dim, device="cuda", dtype=torch.uint8), torch.empty(3, dim // 128, device="cuda")
+    ops.swiglu_fp8_dev(x.data_ptr(), 3, dim, q.data_ptr(), s.data_ptr(), ty, stream=torch.cuda.current_stream().cuda_stream)
+    gd, u = x.double().chunk(2, 1)
+    y = gd / (1 + torch.exp(-gd)) * u
+    off = (2.0**-20 + gd.abs().clamp_max(200) * 2.0**-23) * y.abs() + torch.where(gd < -87, gd.abs().clamp_max(200) * u.abs() * 2.0**-126, 0.0)
+    off[:, :128] = 0  # (at -1e30 nothing is left of it, in 64 bits either)
+    most = torch.nn.functional.max_pool1d((y.abs() + off)[:, None], 128)[:, 0] / 448
+    least = torch.nn.functional.max_pool1d((y.abs() - off).clamp_min(0)[:, None], 128)[:, 0] / 448
+    assert (s <= most.clamp_min(2.0**-100) * (1 + 2.0**-21)).all() and (s >= least.clamp_min(2.0**-100) * (1 - 2.0**-21)).all()
+    step = torch.maximum(2.0**-4 * (y.abs() + off), 2.0**-10 * s.double().repeat_interleave(128, 1)) * (1 + 2.0**-20)
+    assert ((held(q, s) - y).abs() <= step + off).all()
+
+
+@pytest.mark.parametrize("gate,up", [("inf", 1.0), ("-inf", 1.0), ("nan", 1.0), ("inf", 0.0), (0.0, "inf"), (-200.0, "inf"), (3.0, "-inf"), (3.0, "nan"), (100.0, 3e38)])
+def test_swiglu_of_what_is_not_finite_reaches_its_block(gate, up):
+    x = torch.ones(3, 800, device="cuda")
+    x[1, 130], x[1, 530] = float(gate), float(up)
+    q, s = torch.empty(3, 400, device="cuda", dtype=torch.uint8), torch.empty(3, 4, device="cuda")
+    ops.swiglu_fp8_dev(x.data_ptr(), 3, 400, q.data_ptr(), s.data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+    assert not torch.isfinite(s[1, 1]) and torch.isnan(held(q, s)[1, 128:256]).all()
+    s[1, 1] = 1.0
+    v = held(q, s)
+    v[1, 128:256] = 1 / (1 + np.exp(-1.0))
+    assert ((v - 1 / (1 + np.exp(-1.0))).abs() <= 2.0**-4).all()

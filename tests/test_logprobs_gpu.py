@@ -177,3 +177,12 @@ def test_host_form():
     near(torch.from_numpy(lp).cuda(), e[0]), near(torch.from_numpy(ent).cuda(), e[1]), near(torch.from_numpy(tl).cuda(), e[3])
     assert np.array_equal(ti.astype(np.int32), e[2].cpu().numpy())
     assert ops.logprobs(z.cpu().numpy(), None)[0] is None
+
+
+@pytest.mark.parametrize("n", [700, 40000, 128256])
+@pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
+def test_rows_alone_and_among_others(ty, n):
+    """Blocks and threads of a row go by how many rows there are: its bits may differ, its tokens not, nor the bounds of its numbers."""
+    z, ids = logits(320, n, ty, 8)
+    for at, count in [(0, 1), (199, 1), (0, 3), (40, 30), (7, 75), (0, 160), (0, 320)]:
+        check(z[at : at + count], ids[at : at + count].clone(), 20)
