@@ -11,7 +11,7 @@ namespace sp {
 
 constexpr int FP8_BLOCK = 128;
 constexpr float FP8_MAX = 448.f;              // largest e4m3 value
-constexpr float FP8_MIN_SCALE = 0x1p-100f;    // what a block of zeros keeps: products of two scales stay normal only down to here
+constexpr float FP8_MIN_SCALE = 0x1p-100f;    // what a block of zeros keeps; its reciprocal is finite. (Products of two scales are formed in f32: normal from 2^-126 up.)
 constexpr int FP8_NORM_MAX_DIM = 32768;
 inline int64_t fp8_blocks(int64_t k) { return (k + FP8_BLOCK - 1) / FP8_BLOCK; }
 

@@ -7,7 +7,8 @@
 //   up to 128 rows, or long K        fp8_stream_kernel  tcgen05, 128 weight rows are the lanes, K shared by a cluster
 //   few tiles                        fp8_lone_kernel    tcgen05, 128 activation rows are the lanes, one tile a block
 //   many                             fp8_wide_kernel    the same, tiles of 256 weight rows in rounds, by one SM or a pair
-// Every sum has one order, which depends on the sizes alone. gemv_takes and way_of choose, with the times of both sides.
+// Every sum has one order, which depends on the sizes, on whether the operands start on 32 bytes (up to 16 rows) and on the number of SMs.
+// gemv_takes and way_of choose, with the times of both sides. Times are of kernels launched back to back, where nothing else is said.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -490,8 +491,8 @@ __device__ __forceinline__ bool drains_agree(bool ok) {
 // memory and half of the weight rows in its shared memory), or by one block 128 x 128 or 128 x 64 of a product that does not fill the SMs.
 //
 // The wide kernel's two halves of 128 weight rows have sums and drain warps of their own, two of each: while one is drained three are
-// with the tensor cores. 4096 x 14336 x 4096: 205 to 209 us, 2.3 PFLOP/s, at the 1.5 GHz to which the power limit takes the clock;
-// 168 without drains. The tensor cores always have products to do, but a half takes 417 cycles for 256 of products (335 without drains):
+// with the tensor cores. 4096 x 14336 x 4096: 205 to 209 us in a burst, 2.3 PFLOP/s, at the 1.5 GHz to which the power limit takes the
+// clock (168 without drains); calls without a pause on inputs that change 237 to 244, 2.0 PFLOP/s. The tensor cores always have products to do, but a half takes 417 cycles for 256 of products (335 without drains):
 // drains read the tensor memory that products add into. Slower: products of 256 columns with two sums (220 us), 16 drain warps (238),
 // results by TMA (232), columns of tiles first (221). No effect: more stages, a second warp that issues products.
 constexpr int FP_BN = 256;
@@ -820,7 +821,7 @@ __global__ void __launch_bounds__(FP_THREADS, 1) fp8_wide_kernel(const Fp8WideAr
 
 // A tile of 128 activation rows x W weight rows a block, no more tiles than SMs: what counts is how many bytes are on their way and how
 // soon the tensor cores go on. All of shared memory is stages; there are four accumulators, and the two groups of drain warps take
-// blocks of 128 columns in turn and add up at the end. An SM takes in about 60 bytes a cycle, which bounds it: 128 x 4096 x 4096 10.6 us
+// blocks of 128 columns in turn and add up at the end (W = 128 spills 80 bytes a thread). An SM takes in about 60 bytes a cycle, which bounds it: 128 x 4096 x 4096 10.6 us
 // with tiles of 64 weight rows (13.2 with one warp that issues products and one that copies, 12.1 with two and one, two and two here).
 // Of tiles of 64 two or four blocks of a cluster may share K; they add up through distributed shared memory, each its share of the rows.
 __host__ __device__ constexpr int lone_stage(int w) { return (128 + w) * FP8_BLOCK; }

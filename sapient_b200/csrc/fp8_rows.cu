@@ -5,8 +5,13 @@
 //
 // A thread holds eight columns, so a block of 128 is half a warp and its maximum four shuffles. A NaN or an infinity in a block makes
 // its scale one too (the maximum lets NaN through), so that whatever reads the block sees it. Each value is read once and kept in
-// registers until its row's norm is known. Bytes bound SwiGLU (4096 x 14336 bf16: 46.9 us, 45.2 at 6.54 TB/s) and norms with a residual
-// (8192 x 4096 bf16: 39.9 us, 36.1), instructions norms without (23.1 us, 15.6); a few rows take a launch and two latencies, 2.5 to 3.3 us.
+// registers until its row's norm is known. Times here are of one kernel launched back to back by a small program; calls from Python on
+// inputs that change, with their outputs not in L2, take what stands behind the semicolon. Bytes bound SwiGLU (4096 x 14336 bf16: 46.9 us, 45.2 at
+// 6.54 TB/s; 50.8 to 53.7) and norms with a residual (8192 x 4096 bf16: 39.9 us, 36.1; 40.7 to 43.0). Norms without one (23.1 us, 15.6; 23.5)
+// fill nothing: 2.5 of 4 instructions a cycle, 31 % of DRAM, 46 % of the warps, since registers leave room for two blocks an SM. A few rows
+// take a launch and two latencies, 2.5 to 3.3 us.
+// Rows of more than 4096 columns spill: in f32 with a residual 88 bytes a thread (4096 x 8192: 90.8 us for 66.9 of bytes, calls), of more
+// than 16384 columns 404 (2048 x 16400: 143.2 us for 66.9; bf16 172 bytes, 98.6 us for 36.1).
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -83,7 +88,7 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     return d;
 }
 
-// Two values an instruction: these kernels have more instructions than bytes.
+// Two values an instruction.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t d;
     asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
@@ -127,8 +132,9 @@ __device__ __forceinline__ void store8(float (&y)[8], float by, uint8_t* q) {
 __device__ __forceinline__ float scale_of(float greatest, float factor) { return max_nan(greatest * factor * (1.f / FP8_MAX), FP8_MIN_SCALE); }
 
 // Eight columns of a row; the 16 threads of a block of 128 call together, those past the row with zeros and live false. Multiplied by
-// reciprocals where the definition divides: the scale is off by 2^-23 of itself at most, the quotient by 2^-22, so that of a million
-// values one or two that lie beside a border of the grid fall on its other side; a division takes ten instructions more.
+// reciprocals where the definition divides: the quotient is off by 2^-22 of itself at most, so that of a million values one or two that
+// lie beside a border of the grid fall on its other side; a division takes ten instructions more. The scale has the roundings of two
+// products and of 1 / 448, 3 x 2^-24 together (rows as they are: 2^-23), a norm's the error of its rsqrtf as well.
 // y is `factor` (up to FACTOR_MAX) times the values given: a norm's one factor for the row need not be multiplied into them.
 constexpr float FACTOR_MAX = 0x1p27f;  // times the reciprocal of the smallest scale, 2^100, it is finite
 __device__ __forceinline__ void quantise8(float (&y)[8], float factor, bool live, int lane, uint8_t* q, float* scale_to) {
@@ -328,7 +334,7 @@ static cudaError_t norm_with(const Fp8NormArgs& a, cudaStream_t st) {
 template <typename T, bool RES>
 static cudaError_t norm_of(const Fp8NormArgs& a, cudaStream_t st) {
     if (a.dim > 4096) return a.dim <= 16384 ? norm_with<T, 2, 1, RES>(a, st) : norm_with<T, 4, 1, RES>(a, st);
-    return norm_with<T, 1, RES ? 1 : 2, RES>(a, st);  // instructions bound rows without a residual, bytes the others: 8192 x 4096 bf16, one row 27.9 us, two 23.1; with it 39.9 and 40.5
+    return norm_with<T, 1, RES ? 1 : 2, RES>(a, st);  // two rows share their reductions where bytes leave time for those: 8192 x 4096 bf16, one row 27.9 us, two 23.1; with a residual 39.9 and 40.5
 }
 
 cudaError_t launch_fp8_norm(const Fp8NormArgs& a, bool bf, cudaStream_t st) {
@@ -366,7 +372,7 @@ __global__ void __launch_bounds__(128) fp8_quant_kernel(const T* x, int64_t ldx,
                     float v[8];
                     unpack8(u[i], v);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] = y[j] * rcp_approx(1.f + ex2_approx(y[j] * -1.4426950408889634f)) * v[j];  // errors of a few 2^-22, ahead of a rounding of 2^-4
+                    for (int j = 0; j < 8; ++j) y[j] = y[j] * rcp_approx(1.f + ex2_approx(y[j] * -1.4426950408889634f)) * v[j];  // off by |g| 2^-23 and a few 2^-22 of itself, ahead of a rounding of 2^-4; zero where it is below 2^-126
                 }
             } else {
 #pragma unroll

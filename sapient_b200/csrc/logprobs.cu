@@ -15,7 +15,8 @@
 // Keys (value, then lower index) are distinct, so that no order of threads changes the result.
 //
 // Bytes bound it from some hundred rows on, with the exponentials close behind (16 a cycle and SM); below that the chain of steps does,
-// a good part of it instructions that are fetched for the first time, so that what runs once is kept short. us (floor at 6.54 TB/s):
+// a good part of it instructions that are fetched for the first time, so that what runs once is kept short. us, launched back
+// to back by a small program (floor at 6.54 TB/s); calls on logits that change take 94.8 to 101.8 us for the first, 65 for the second:
 //   1024 x 128256 f32 top 1      91.7 (80.3)     32 x 128256 bf16 top 20   10.8 (1.3)      1 x 151936 f32 top 5    7.1 (0.1)
 //   1024 x 128256 bf16 top 1     59.9 (40.2)     64 x 128256 bf16 top 1    10.9 (2.5)      1 x 151936 f32 top 0    4.5 (0.1)
 //   53 x 1913 bf16 top 12         4.7 (0.0; 7.0 with cells from L2)
