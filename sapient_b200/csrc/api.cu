@@ -127,15 +127,20 @@ struct OnDevice {
     ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
 };
 
-// The flags of op-level calls on the current device, made on the first one (during another thread's stream capture or this one's, too).
+// While this lives the calling thread may allocate beside stream captures, another thread's or its own: they neither fail nor end them.
+struct BesideCaptures {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const cudaError_t status = cudaThreadExchangeStreamCaptureMode(&mode);
+    ~BesideCaptures() { if (status == cudaSuccess) cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// The flags of op-level calls on the current device, made on the first one.
 cudaError_t op_waits(int** waits) {
     WaitFlags& f = device_wait_flags();
     if (!f.host.load()) {
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
-        if (e != cudaSuccess) return e;
-        e = f.alloc();
-        cudaThreadExchangeStreamCaptureMode(&mode);
+        BesideCaptures beside;
+        cudaError_t e = beside.status;
+        if (e == cudaSuccess) e = f.alloc();
         if (e != cudaSuccess) return e;
     }
     *waits = f.dev;
@@ -405,7 +410,11 @@ static int matmul_nt_fp8(SpWeight* w, const float* x, int64_t m, float* y, cudaS
         const int64_t rows = std::max((m + 127) / 128 * 128, 2 * w->xq_rows);  // (doubled: the smaller ones take no more than the last)
         if (w->xq) w->xq_before.reserve(w->xq_before.size() + 1);
         uint8_t* p = nullptr;
-        SP_CUDA_TRY(cudaMalloc((void**)&p, rows * (row + 4 * scales)));
+        {
+            BesideCaptures beside;
+            SP_CUDA_TRY(beside.status);
+            SP_CUDA_TRY(cudaMalloc((void**)&p, rows * (row + 4 * scales)));
+        }
         if (w->xq) w->xq_before.push_back(w->xq);
         w->xq = p;
         w->xq_rows = rows;

@@ -276,3 +276,36 @@ def test_a_weight_is_there_when_its_upload_returns():
         xq, sx = (torch.from_numpy(t).cuda() for t in ops.quant_fp8(x.cpu().numpy()))
         mat.check(y[0], xq.view(torch.float8_e4m3fn), sx, q, s)
         assert (y == y[0]).all()
+
+
+def test_a_weight_grows_beside_a_capture_of_another_thread():
+    """The workspace's allocation is none of a capture that goes on elsewhere, and does not end it."""
+    import threading
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, s = weight(300, HIDDEN, g)
+    w = ops.Weight.from_fp8(q.view(torch.uint8).cpu().numpy(), s.cpu().numpy())
+    x, y = torch.randn(40, HIDDEN, generator=g, device="cuda"), torch.zeros(40, 300, device="cuda")
+    a, b = torch.ones(1000, device="cuda"), torch.zeros(1000, device="cuda")
+    ops.quant_fp8(np.ones((1, 16), np.float32))  # (the library is there)
+    st, graph, said = torch.cuda.Stream(), torch.cuda.CUDAGraph(), []
+
+    def grow():
+        try:
+            w.matmul_nt_dev(x.data_ptr(), 40, y.data_ptr(), st.cuda_stream)
+        except SapientCudaError as e:
+            said.append(e)
+
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        b.copy_(a)
+        t = threading.Thread(target=grow)
+        t.start()
+        t.join()
+        b.mul_(2)
+    assert not said
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (b == 2).all()
+    xq, sx = (torch.from_numpy(t).cuda() for t in ops.quant_fp8(x.cpu().numpy()))
+    mat.check(y, xq.view(torch.float8_e4m3fn), sx, q, s)
