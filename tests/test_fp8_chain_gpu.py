@@ -309,3 +309,29 @@ def test_a_weight_grows_beside_a_capture_of_another_thread():
     assert (b == 2).all()
     xq, sx = (torch.from_numpy(t).cuda() for t in ops.quant_fp8(x.cpu().numpy()))
     mat.check(y, xq.view(torch.float8_e4m3fn), sx, q, s)
+
+
+@pytest.mark.parametrize("m", [3, 160, 700])
+def test_the_first_calls_of_a_process_may_be_captured(m):
+    """What a first call sets up (attributes, flags, addresses of the driver) needs no call before."""
+    import os
+    import subprocess
+    import sys
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = f"""import torch
+import test_fp8_chain_gpu as c
+b = c.Block({m}, c.ops.BF16, 1)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    b.run()
+for t in b.results():
+    t.zero_()
+g.replay()
+torch.cuda.synchronize()
+b.check()
+print("held")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=here, env=os.environ | {"PYTHONPATH": os.pathsep.join([os.path.dirname(here), here])}, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "held" in r.stdout, r.stderr[-2000:]
