@@ -335,3 +335,65 @@ print("held")
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=here, env=os.environ | {"PYTHONPATH": os.pathsep.join([os.path.dirname(here), here])}, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "held" in r.stdout, r.stderr[-2000:]
+
+
+class Hopping(Block):
+    """The steps by turns on two streams, each after the one before by an event; what `run` asks for is the stream of a step."""
+
+    def __init__(self, *a):
+        super().__init__(*a)
+        self.streams, self.steps = [torch.cuda.Stream(), torch.cuda.Stream()], 0
+
+    def hop(self):
+        last, new = self.streams[self.steps % 2], self.streams[(self.steps + 1) % 2]
+        new.wait_stream(last)
+        self.steps += 1
+        return new
+
+    def run(self):
+        p = lambda t: t.data_ptr()  # noqa: E731
+        at = lambda: self.hop().cuda_stream  # noqa: E731
+        ops.rms_norm_fp8_dev(p(self.x), self.m, HIDDEN, p(self.norms[0]), EPS, p(self.q[0]), p(self.s[0]), self.ty, stream=at())
+        self.product(0, self.gu, at())
+        ops.swiglu_fp8_dev(p(self.gu), self.m, FFN, p(self.q[1]), p(self.s[1]), self.ty, stream=at())
+        self.product(1, self.down, at())
+        ops.rms_norm_fp8_dev(p(self.down), self.m, HIDDEN, p(self.norms[1]), EPS, p(self.q[2]), p(self.s[2]), self.ty, residual=p(self.x), sum_out=p(self.total), stream=at())
+        self.product(2, self.z, at())
+        o = self.out
+        ops.logprobs_dev(p(self.z), self.m, VOCAB, p(self.ids), p(o[0]), p(o[1]), TOP, p(o[2]), p(o[3]), self.ty, stream=at())
+
+
+@pytest.mark.parametrize("m", [1, 24, 160, 700])
+def test_steps_on_two_streams_by_turns(m):
+    """In streams, then in one graph with a second chain beside it: an event keeps a step back as the stream itself does."""
+    a, b = Hopping(m, ops.BF16, 1), Hopping(m, ops.BF16, 2)
+    here = torch.cuda.current_stream()
+    xs = [torch.randn(m, HIDDEN, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)).to(TYPES[a.ty]) for i in range(10)]
+    for x in xs:
+        a.x.copy_(x)
+        for st in a.streams:
+            st.wait_stream(here)
+        a.run()
+        for st in a.streams:
+            here.wait_stream(st)
+    a.check()
+    b.streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = torch.cuda.current_stream()
+        for c in (a, b):
+            for st in c.streams:
+                st.wait_stream(inside)
+        for c in (a, b):
+            c.run()
+        for c in (a, b):
+            for st in c.streams:
+                inside.wait_stream(st)
+    for t in a.results() + b.results():
+        t.zero_()
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    a.check()
+    b.check()
