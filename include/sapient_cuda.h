@@ -197,6 +197,51 @@ int32_t sp_cuda_logprobs(int32_t device, const float* logits, int64_t rows, int6
  * not overlap x. sp_cuda_dequant, _weight_info and _free_weight work as for the other types. Not a table for sp_cuda_embed. */
 int32_t sp_cuda_upload_weight_fp8(int32_t device, int64_t n, int64_t k, const void* values, const float* scales, SpWeight** out);
 
+/* ── A paged cache of 8-bit rows: writing keys and values with the norms and the rotation that precede it, attention over it, reading it
+ * back (no counterpart in the reference, whose cache holds Q8_0 rows of one sequence: crates/sapient-models/src/forward/common.rs:336-348) ──
+ * values[page][keys | values][n_kv_heads][16 tokens][head_dim] in e4m3, scales[page][keys | values][n_kv_heads][16] in f32: a token's head is
+ * an fp8 row as above with one scale. page_table[slot][i] is the page of tokens 16 i .. 16 i + 15 of a slot; an entry that is not a page's
+ * number is not followed. All of it is the caller's device memory, of one layer; values, scales and page_table start on 16, 16 and 4
+ * bytes. head_dim is a multiple of 16, at most 128. `cache` of a call is an SpCacheFp8's address, which is read during the call only; device, n_pages, n_slots, max_pages and
+ * n_kv_heads are positive but for device.
+ * The calls take device pointers, launch one kernel on `stream` and do not wait; they keep nothing between calls, so that they may run at
+ * the same time on several streams and be captured into graphs. dtype (SP_F32 or SP_BF16) is the type of q, k, v, q_out and out; rows of
+ * those start on 16 bytes (strides are multiples of 4 values in f32, 8 in bf16) and hold their heads side by side, head_dim apart.
+ * Outputs must not overlap what is read, except where the call says so. Positions, slots and lengths are not looked at on the host. */
+typedef struct SpCacheFp8 {
+    void* values;
+    float* scales;
+    const int32_t* page_table; /* [n_slots][max_pages] */
+    int32_t device, n_pages, n_slots, max_pages, n_kv_heads, head_dim;
+} SpCacheFp8;
+/* For each token i: its n_heads queries (q may be NULL, with n_heads 0) and the keys are divided by sqrt(mean(x^2) + eps) and multiplied by
+ * q_w, k_w [head_dim] where those are given, and their first rotary_dim coordinates (a multiple of 16, 0: none) are rotated by the angles of
+ * positions[i]: angles[n_angles][rotary_dim / 2][cosine, sine], starting on 16 bytes (any base and any scaling for long contexts: ops.rope_table).
+ * pairs 0: coordinates c and c + rotary_dim / 2 are a pair, 1: coordinates 2 c and 2 c + 1. Queries go to q_out, which may be q with the
+ * same stride; keys and values (those as they are) go to the cache as fp8 rows, at positions[i] of slot slots[i]. A token whose slot is not
+ * one of the cache's, or whose position lies past its page table or past the angles, is skipped with all that belongs to it; where its page is
+ * not one, only its keys and values are. A place of the cache may occur once in a call. h^2 is added up in f32: |x| up to 2^63 / sqrt(head_dim). */
+int32_t sp_cuda_cache_fp8_append_dev(const void* cache, int32_t dtype, int64_t n_tok, const int32_t* slots, const int32_t* positions,
+                                     const void* q, int64_t ldq, int32_t n_heads, void* q_out, int64_t ldqo, const void* k, int64_t ldk,
+                                     const void* v, int64_t ldv, const float* q_w, const float* k_w, float eps, const float* angles,
+                                     int64_t n_angles, int32_t rotary_dim, int32_t pairs, void* stream);
+/* Keys and values (either may be NULL) at positions[i] of slot slots[i] as rows k[i], v[i]: e4m3 value x scale. A row whose slot, position or
+ * page is not there stays as it is. */
+int32_t sp_cuda_cache_fp8_read_dev(const void* cache, int32_t dtype, int64_t n_tok, const int32_t* slots, const int32_t* positions, void* k,
+                                   int64_t ldk, void* v, int64_t ldv, void* stream);
+/* Causal attention of new tokens, whose keys and values are in the cache already. Rows row_start[i] .. row_start[i + 1] - 1 of q and out are the
+ * newest tokens of sequence i, in order; seq_len[i] counts its tokens with them. The last row sees all of them, each one before it one less;
+ * window > 0: no row sees more than its newest `window`. Sequence i lies in slot seq_slot[i] (NULL: i). out = softmax(scale q K^T) V per head,
+ * n_heads / n_kv_heads queries in a row sharing a key head; a row that sees nothing (a length of 0, a slot that is not there) is zeros, and
+ * tokens on pages that are not there are not seen. out may be q with the same stride. max_rows: of any sequence, not less than they
+ * have (rows past it stay as they are); max_len: of any sequence, by which the work is shared out (a wrong one costs time only). Rows in front of
+ * row_start[0] and behind row_start[n_seqs] stay as they are. Products of bf16 rows are exact but for weights rounded to 11 bits, those of f32 rows
+ * take q and the weights with 22; sums are f32, in an order that depends on the sizes, max_rows, max_len and the device's SMs. A key or value row whose scale is
+ * NaN or infinite makes the rows that see it NaN, and no others. n_seqs is at most 65535. */
+int32_t sp_cuda_attention_fp8_dev(const void* cache, int32_t dtype, const void* q, int64_t ldq, int32_t n_heads, void* out, int64_t ldo,
+                                  int32_t n_seqs, const int32_t* seq_slot, const int32_t* row_start, const int32_t* seq_len, int32_t max_rows,
+                                  int32_t max_len, float scale, int32_t window, void* stream);
+
 /* ── engine level: replaces ForwardEngine (crates/sapient-models/src/forward/mod.rs:49-65,381-506)
  *    in the shape of the resident WgpuForwardEngine (forward/wgpu_engine.rs:93-110,173-341,362-676) ── */
 typedef struct SpEngine SpEngine;

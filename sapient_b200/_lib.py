@@ -33,6 +33,13 @@ class SpModelDesc(C.Structure):
     ]
 
 
+class SpCacheFp8(C.Structure):
+    _fields_ = [
+        ("values", C.c_void_p), ("scales", C.c_void_p), ("page_table", C.c_void_p), ("device", C.c_int32), ("n_pages", C.c_int32),
+        ("n_slots", C.c_int32), ("max_pages", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+    ]
+
+
 _vp, _i32, _i64, _sz, _f = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_float
 
 # name -> (restype, argtypes); must list every symbol include/sapient_cuda.h declares
@@ -84,6 +91,9 @@ SIGNATURES = {
     "sp_cuda_quant_fp8": (_i32, [_i32, _vp, _i64, _i64, _vp, _vp]),
     "sp_cuda_matmul_fp8": (_i32, [_i32, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp]),
     "sp_cuda_logprobs": (_i32, [_i32, _vp, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp]),
+    "sp_cuda_cache_fp8_append_dev": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _f, _vp, _i64, _i32, _i32, _vp]),
+    "sp_cuda_cache_fp8_read_dev": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp]),
+    "sp_cuda_attention_fp8_dev": (_i32, [_vp, _i32, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _f, _i32, _vp]),
     "sp_cuda_upload_weight_fp8": (_i32, [_i32, _i64, _i64, _vp, _vp, C.POINTER(_vp)]),
     "sp_cuda_engine_create": (_i32, [C.POINTER(SpModelDesc), C.POINTER(_vp)]),
     "sp_cuda_engine_set_tensor": (_i32, [_vp, C.c_char_p, _i32, _vp, _i32, _vp, _sz]),
@@ -156,7 +166,7 @@ def lib():
 
 
 _calls = None
-_CALLS = ("rms_norm_fp8", "swiglu_fp8", "quant_fp8", "matmul_fp8", "logprobs")
+_CALLS = ("rms_norm_fp8", "swiglu_fp8", "quant_fp8", "matmul_fp8", "logprobs", "cache_fp8_append", "cache_fp8_read", "attention_fp8")
 
 
 def calls():

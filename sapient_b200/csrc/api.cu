@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "batcher.h"
+#include "cache_fp8.h"
 #include "engine.h"
 #include "fp8.h"
 #include "model_plan.h"
@@ -171,6 +172,32 @@ int check_fp8_dim(int64_t rows, int64_t dim, const char* name) {
 int check_logprobs(int64_t rows, int64_t vocab, int top) {
     if (rows < 0 || vocab < 1 || vocab > (1 << 30) || rows > (1 << 27)) { set_error("logprobs: bad shape"); return SP_ERR_SHAPE; }
     if (top < 0 || top > SP_LOGPROBS_MAX_TOP || top > vocab) { set_error("logprobs: top must be 0 to 32 and at most the vocabulary"); return SP_ERR_ARG; }
+    return SP_OK;
+}
+
+// A cache of 8-bit rows as a call is given it.
+int check_cache(const void* cache, int dtype, CacheFp8* out) {
+    const SpCacheFp8* const c = static_cast<const SpCacheFp8*>(cache);
+    if (!c || !c->values || !c->scales || !c->page_table) { set_error("cache_fp8: null argument"); return SP_ERR_ARG; }
+    if (dtype != SP_F32 && dtype != SP_BF16) { set_error("cache_fp8: rows are SP_F32 or SP_BF16"); return SP_ERR_DTYPE; }
+    if (c->head_dim <= 0 || c->head_dim % 16 != 0 || c->head_dim > CACHE_MAX_DIM) { set_error("cache_fp8: head_dim must be a multiple of 16, at most 128"); return SP_ERR_SHAPE; }
+    if (c->n_pages <= 0 || c->n_slots <= 0 || c->max_pages <= 0 || c->max_pages > INT32_MAX / KV_PAGE || c->n_kv_heads <= 0 || c->n_kv_heads > 65535) {
+        set_error("cache_fp8: bad shape");
+        return SP_ERR_SHAPE;
+    }
+    if (unaligned(c->values, 16) || unaligned(c->scales, 16) || unaligned(c->page_table, 4)) { set_error("cache_fp8: values and scales must be 16-byte aligned"); return SP_ERR_ARG; }
+    *out = CacheFp8{static_cast<uint8_t*>(c->values), c->scales, c->page_table, c->n_pages, c->n_slots, c->max_pages, c->n_kv_heads, c->head_dim};
+    return SP_OK;
+}
+
+// Queries, keys or values side by side: how many heads, address and stride.
+int check_heads(const char* what, const void* p, int64_t ld, int64_t heads, int dim, int dtype) {
+    if (!p) { set_error(std::string(what) + ": null argument"); return SP_ERR_ARG; }
+    return check_fp8_rows(what, p, ld, heads * dim, dtype);
+}
+
+int check_queries(int n_heads, int n_kv) {
+    if (n_heads <= 0 || n_heads % n_kv != 0 || n_heads > (1 << 20)) { set_error("cache_fp8: n_heads must be a multiple of n_kv_heads"); return SP_ERR_SHAPE; }
     return SP_OK;
 }
 
@@ -790,6 +817,129 @@ int32_t sp_cuda_logprobs_dev(int32_t device, int32_t dtype, const void* logits, 
     if (!top_ids && !top_logprobs) top = 0;
     SP_CUDA_TRY(launch_logprobs(LogprobsArgs{logits, ld, rows, (int)vocab, top, ids, logprob, entropy, top_ids, top_logprobs}, dtype == SP_BF16,
                                 (cudaStream_t)stream));
+    return SP_OK;
+    API_END
+}
+
+// ── a paged cache of 8-bit rows ──
+static int check_tokens(int64_t n_tok, const int32_t* slots, const int32_t* positions) {
+    if (n_tok < 0 || n_tok > INT32_MAX) { set_error("cache_fp8: bad number of tokens"); return SP_ERR_SHAPE; }
+    if (!slots || !positions) { set_error("cache_fp8: null argument"); return SP_ERR_ARG; }
+    if (unaligned(slots, 4) || unaligned(positions, 4)) { set_error("misaligned argument"); return SP_ERR_ARG; }
+    return SP_OK;
+}
+
+int32_t sp_cuda_cache_fp8_append_dev(const void* cache, int32_t dtype, int64_t n_tok, const int32_t* slots, const int32_t* positions, const void* q,
+                                     int64_t ldq, int32_t n_heads, void* q_out, int64_t ldqo, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                     const float* q_w, const float* k_w, float eps, const float* angles, int64_t n_angles, int32_t rotary_dim, int32_t pairs,
+                                     void* stream) {
+    API_BEGIN
+    CacheAppendArgs a{};
+    int st = check_cache(cache, dtype, &a.c);
+    if (st == SP_OK) st = check_tokens(n_tok, slots, positions);
+    if (st == SP_OK) st = check_heads("k", k, ldk, a.c.n_kv, a.c.dim, dtype);
+    if (st == SP_OK) st = check_heads("v", v, ldv, a.c.n_kv, a.c.dim, dtype);
+    if (st != SP_OK) return st;
+    if (q) {
+        st = check_queries(n_heads, a.c.n_kv);
+        if (st == SP_OK) st = check_heads("q", q, ldq, n_heads, a.c.dim, dtype);
+        if (st == SP_OK) st = check_heads("q_out", q_out, ldqo, n_heads, a.c.dim, dtype);
+        if (st != SP_OK) return st;
+        if (q_out == q && ldqo != ldq) { set_error("cache_fp8_append: q_out in place has another row stride"); return SP_ERR_ARG; }
+    } else if (n_heads != 0 || q_out) {
+        set_error("cache_fp8_append: no q, but heads or q_out");
+        return SP_ERR_ARG;
+    }
+    if (rotary_dim < 0 || rotary_dim > a.c.dim || rotary_dim % 16 != 0) { set_error("cache_fp8_append: rotary_dim must be a multiple of 16, at most head_dim"); return SP_ERR_SHAPE; }
+    if (pairs < 0 || pairs > 1) { set_error("cache_fp8_append: pairs must be 0 or 1"); return SP_ERR_ARG; }
+    if (rotary_dim > 0 && (!angles || n_angles < 1)) { set_error("cache_fp8_append: rotation without angles"); return SP_ERR_ARG; }
+    if (unaligned(angles, 16) || unaligned(q_w, 16) || unaligned(k_w, 16)) { set_error("cache_fp8_append: angles and weights must be 16-byte aligned"); return SP_ERR_ARG; }
+    if (n_tok == 0) return SP_OK;
+    a.slots = slots;
+    a.positions = positions;
+    a.n_tok = n_tok;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_out = q_out;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.ldqo = ldqo;
+    a.n_heads = n_heads;
+    a.q_w = q_w;
+    a.k_w = k_w;
+    a.eps = eps;
+    a.angles = reinterpret_cast<const float2*>(angles);
+    a.n_angles = n_angles;
+    a.rotary = rotary_dim;
+    a.pairs = pairs != 0;
+    OnDevice on;
+    SP_CUDA_TRY(on.enter(static_cast<const SpCacheFp8*>(cache)->device));
+    SP_CUDA_TRY(launch_cache_append(a, dtype == SP_BF16, (cudaStream_t)stream));
+    return SP_OK;
+    API_END
+}
+
+int32_t sp_cuda_cache_fp8_read_dev(const void* cache, int32_t dtype, int64_t n_tok, const int32_t* slots, const int32_t* positions, void* k, int64_t ldk,
+                                   void* v, int64_t ldv, void* stream) {
+    API_BEGIN
+    CacheReadArgs a{};
+    int st = check_cache(cache, dtype, &a.c);
+    if (st == SP_OK) st = check_tokens(n_tok, slots, positions);
+    if (st == SP_OK && k) st = check_heads("k", k, ldk, a.c.n_kv, a.c.dim, dtype);
+    if (st == SP_OK && v) st = check_heads("v", v, ldv, a.c.n_kv, a.c.dim, dtype);
+    if (st != SP_OK) return st;
+    if (n_tok == 0 || (!k && !v)) return SP_OK;
+    a.slots = slots;
+    a.positions = positions;
+    a.n_tok = n_tok;
+    a.k = k;
+    a.v = v;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    OnDevice on;
+    SP_CUDA_TRY(on.enter(static_cast<const SpCacheFp8*>(cache)->device));
+    SP_CUDA_TRY(launch_cache_read(a, dtype == SP_BF16, (cudaStream_t)stream));
+    return SP_OK;
+    API_END
+}
+
+int32_t sp_cuda_attention_fp8_dev(const void* cache, int32_t dtype, const void* q, int64_t ldq, int32_t n_heads, void* out, int64_t ldo, int32_t n_seqs,
+                                  const int32_t* seq_slot, const int32_t* row_start, const int32_t* seq_len, int32_t max_rows, int32_t max_len, float scale,
+                                  int32_t window, void* stream) {
+    API_BEGIN
+    AttentionFp8Args a{};
+    int st = check_cache(cache, dtype, &a.c);
+    if (st == SP_OK) st = check_queries(n_heads, a.c.n_kv);
+    if (st == SP_OK) st = check_heads("q", q, ldq, n_heads, a.c.dim, dtype);
+    if (st == SP_OK) st = check_heads("out", out, ldo, n_heads, a.c.dim, dtype);
+    if (st != SP_OK) return st;
+    if (out == q && ldo != ldq) { set_error("attention_fp8: out in place has another row stride"); return SP_ERR_ARG; }
+    if (!row_start || !seq_len) { set_error("attention_fp8: null argument"); return SP_ERR_ARG; }
+    if (unaligned(row_start, 4) || unaligned(seq_len, 4) || unaligned(seq_slot, 4)) { set_error("misaligned argument"); return SP_ERR_ARG; }
+    if (n_seqs < 0 || n_seqs > 65535) { set_error("attention_fp8: n_seqs must be 0 to 65535"); return SP_ERR_SHAPE; }
+    if (max_rows < 0 || max_len < 0 || (int64_t)max_rows * n_heads > INT32_MAX / 2) { set_error("attention_fp8: bad shape"); return SP_ERR_SHAPE; }
+    if (window < 0) { set_error("attention_fp8: window must not be negative"); return SP_ERR_ARG; }
+    if (!std::isfinite(scale)) { set_error("attention_fp8: scale is not a number"); return SP_ERR_ARG; }
+    if (n_seqs == 0 || max_rows == 0) return SP_OK;
+    a.q = q;
+    a.out = out;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.n_heads = n_heads;
+    a.n_seqs = n_seqs;
+    a.seq_slot = seq_slot;
+    a.row_start = row_start;
+    a.seq_len = seq_len;
+    a.max_rows = max_rows;
+    a.max_len = max_len;
+    a.scale = scale;
+    a.window = window;
+    OnDevice on;
+    SP_CUDA_TRY(on.enter(static_cast<const SpCacheFp8*>(cache)->device));
+    SP_CUDA_TRY(op_waits(&a.waits));
+    SP_CUDA_TRY(launch_attention_fp8(a, dtype == SP_BF16, (cudaStream_t)stream));
     return SP_OK;
     API_END
 }

@@ -65,15 +65,15 @@ PyObject* call(int32_t (*f)(A...), PyObject* const* args, Py_ssize_t n) {
     return call_with(f, args, std::index_sequence_for<A...>());
 }
 
-#define CALLS(X) X(rms_norm_fp8) X(swiglu_fp8) X(quant_fp8) X(matmul_fp8) X(logprobs)
+#define CALLS(X) X(rms_norm_fp8) X(swiglu_fp8) X(quant_fp8) X(matmul_fp8) X(logprobs) X(cache_fp8_append) X(cache_fp8_read) X(attention_fp8)
 #define DEFINE(name)                                        \
     decltype(&sp_cuda_##name##_dev) f_##name = nullptr;     \
     PyObject* py_##name(PyObject*, PyObject* const* args, Py_ssize_t n) { return call(f_##name, args, n); }
 CALLS(DEFINE)
 
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 5) {
-        PyErr_SetString(PyExc_TypeError, "five addresses expected");
+    if (n != 8) {
+        PyErr_SetString(PyExc_TypeError, "eight addresses expected");
         return nullptr;
     }
     Py_ssize_t i = 0;

@@ -305,6 +305,71 @@ def logprobs_dev(logits: int, rows: int, vocab: int, ids: int, logprob: int, ent
         check(status)
 
 
+# ── a paged cache of 8-bit rows (layout in include/sapient_cuda.h) ──
+CACHE_PAGE = 16  # tokens of a page
+
+
+class CacheFp8:
+    """Where a layer's cache lies: device addresses of values [n_pages, 2, n_kv_heads, 16, head_dim] (e4m3; keys, then values), scales
+    [n_pages, 2, n_kv_heads, 16] (f32) and page_table [n_slots, max_pages] (int32), which stay the caller's."""
+
+    def __init__(self, values: int, scales: int, page_table: int, n_pages: int, n_slots: int, max_pages: int, n_kv_heads: int, head_dim: int, device: int = 0):
+        self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
+        self.desc = _lib.SpCacheFp8(values, scales, page_table, device, n_pages, n_slots, max_pages, n_kv_heads, head_dim)
+        self.at = C.addressof(self.desc)
+
+
+def cache_fp8_bytes(n_pages: int, n_kv_heads: int, head_dim: int) -> tuple[int, int]:
+    """Bytes of a layer's values and scales."""
+    rows = n_pages * 2 * n_kv_heads * CACHE_PAGE
+    return rows * head_dim, rows * 4
+
+
+def rope_table(n_positions: int, rotary_dim: int, base: float, factor: float = 1.0, original: int = 0, low: float = 0.25, high: float = 1.0) -> np.ndarray:
+    """Angles for cache_fp8_append_dev: [n_positions, rotary_dim / 2, 2] f32 cosines and sines of position x base^(-2 i / rotary_dim), made in
+    64 bits. For contexts longer than a model was trained on: factor alone divides every frequency; with `original` (the length of
+    training) only those that make at most `low` turns within it are divided, those of `high` turns and more stay, and between the two it goes over."""
+    if n_positions < 0 or rotary_dim < 0 or rotary_dim % 2:
+        raise SapientCudaError(_lib.SP_ERR_SHAPE, "rope_table: rotary_dim must be even")
+    if not (factor > 0 and base > 0) or (original and not 0 <= low < high):
+        raise SapientCudaError(_lib.SP_ERR_ARG, "rope_table: factor and base must be positive, low below high")
+    f = float(base) ** (-np.arange(0, rotary_dim, 2, dtype=np.float64) / max(rotary_dim, 1))
+    keep = np.clip((original * f / (2 * np.pi) - low) / (high - low), 0, 1) if original else np.zeros_like(f)
+    angle = np.arange(n_positions, dtype=np.float64)[:, None] * (f * keep + f / factor * (1 - keep))
+    return np.stack([np.cos(angle), np.sin(angle)], -1).astype(np.float32)
+
+
+def cache_fp8_append_dev(cache: CacheFp8, n_tok: int, slots: int, positions: int, k: int, v: int, q: int = 0, n_heads: int = 0, q_out: int = 0, q_w: int = 0,
+                         k_w: int = 0, eps: float = 0.0, angles: int = 0, n_angles: int = 0, rotary_dim: int = 0, pairs: bool = False, dtype: int = F32, ldq: int = 0,
+                         ldk: int = 0, ldv: int = 0, ldqo: int = 0, stream: int = 0) -> None:
+    """Norms of queries and keys for each head, their rotation, queries to q_out, keys and values into the cache. Device addresses (0: not
+    given), row strides in values (0: dense), on the cache's device."""
+    d, kv = cache.head_dim, cache.n_kv_heads * cache.head_dim
+    status = (_lib._calls or _lib.calls()).cache_fp8_append(cache.at, dtype, n_tok, slots, positions, q, ldq or n_heads * d, n_heads, q_out, ldqo or n_heads * d, k, ldk or kv,
+                                                            v, ldv or kv, q_w, k_w, eps, angles, n_angles, rotary_dim, 1 if pairs else 0, stream)
+    if status:
+        check(status)
+
+
+def cache_fp8_read_dev(cache: CacheFp8, n_tok: int, slots: int, positions: int, k: int = 0, v: int = 0, dtype: int = F32, ldk: int = 0, ldv: int = 0, stream: int = 0) -> None:
+    """Keys and values of tokens of the cache as rows."""
+    kv = cache.n_kv_heads * cache.head_dim
+    status = (_lib._calls or _lib.calls()).cache_fp8_read(cache.at, dtype, n_tok, slots, positions, k, ldk or kv, v, ldv or kv, stream)
+    if status:
+        check(status)
+
+
+def attention_fp8_dev(cache: CacheFp8, q: int, n_heads: int, out: int, n_seqs: int, row_start: int, seq_len: int, max_rows: int, max_len: int, scale: float,
+                      window: int = 0, seq_slot: int = 0, dtype: int = F32, ldq: int = 0, ldo: int = 0, stream: int = 0) -> None:
+    """Causal attention of the newest tokens of n_seqs sequences over the cache, which holds them already."""
+    wide = n_heads * cache.head_dim
+    status = (_lib._calls or _lib.calls()).attention_fp8(cache.at, dtype, q, ldq or wide, n_heads, out, ldo or wide, n_seqs, seq_slot, row_start, seq_len, max_rows, max_len,
+                                                         scale, window, stream)
+    if status:
+        check(status)
+
+
+
 def set_gemv_path(path: int) -> None:
     """0: tensor-core GEMV on tile-repacked weights (default); 1: CUDA-core GEMV on raw blocks; 3: per-warp streaming
     variant; 4: bulk-copy ring GEMV for calls of 1-5 rows."""
