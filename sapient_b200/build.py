@@ -21,7 +21,7 @@ SOURCES = ["kernels.cu", "attention.cu", "engine.cu", "engine_forward.cu", "engi
            "model_plan.cu", "safetensors.cu", "engine_plan.cu", "engine_plan_post_norm.cu", "engine_plan_parallel.cu", "engine_plan_pre_norm.cu", "engine_plan_state.cu",
            "engine_plan_latent.cu", "engine_plan_grouped.cu", "mat_f32.cu", "mat_tc5.cu",
            "plan_stream.cu", "latent_attention.cu", "grouped_attention.cu", "mixed_attention.cu", "grouped_conv.cu", "state_mixer.cu", "state_chunk.cu",
-           "fp8_rows.cu", "fp8_gemm.cu", "logprobs.cu", "cache_fp8.cu", "attention_fp8.cu"]
+           "fp8_rows.cu", "fp8_gemm.cu", "logprobs.cu", "cache_fp8.cu", "attention_fp8.cu", "attention_fp8_tile.cu"]
 CALLS_SRC, CALLS_OUT = os.path.join(CSRC, "calls.cpp"), os.path.join(HERE, "_calls.abi3.so")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -1,0 +1,83 @@
+// What the kernels of attention over a cache of 8-bit rows share (attention_fp8.cu, attention_fp8_tile.cu).
+#pragma once
+#include <cuda_fp16.h>
+
+#include "cache_fp8.h"
+#include "plan_common.cuh"
+
+namespace sp {
+
+constexpr float AF_LOG2E = 1.4426950408889634f;
+// A row's reference m is the largest score when it was last moved; it is moved when a score passes it by more than this (log2).
+constexpr float AF_LAZY = 6.f;
+constexpr float AF_LIFT = 512.f;  // 2^(15 - LAZY)
+
+__device__ __forceinline__ float af_ex2(float v) {
+    float d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v));
+    return d;
+}
+// Four e4m3 values of a word as two pairs of fp16.
+__device__ __forceinline__ void af_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}\n" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// NaN bytes become 448: a key that is masked for a row must not reach it through 0 x NaN. One that is visible has NaN or infinity as its
+// scale, and through that as its weight.
+__device__ __forceinline__ uint32_t af_finite(uint32_t two) {
+    uint32_t d;
+    asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(two), "r"(0x5F005F00u));
+    return d;
+}
+__device__ __forceinline__ uint32_t af_pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// fp16 of two values, and of what that rounding dropped.
+__device__ __forceinline__ void af_split(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = af_pack(a - f.x, b - f.y);
+}
+__device__ __forceinline__ void af_mma(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void af_copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void af_copy8(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
+}
+// A power of two by which a row is multiplied so that its largest value lies in [2^12, 2^13), and its reciprocal. Rows of zeros and
+// those with infinities or NaN: 1.
+__device__ __forceinline__ void af_row_scale(float most, float& by, float& back) {
+    const int e = (int)(__float_as_uint(most) >> 23);  // (most >= 0)
+    const int up = e == 0 || e == 255 ? 0 : min(max(139 - e, -126), 126);
+    by = __uint_as_float((uint32_t)(127 + up) << 23);
+    back = __uint_as_float((uint32_t)(127 - up) << 23);
+}
+// The smallest power of two that is not below a scale (positive and finite), within what has a reciprocal.
+__device__ __forceinline__ float af_power(float s) {
+    const uint32_t u = (__float_as_uint(s) + 0x7FFFFFu) & 0x7F800000u;
+    return __uint_as_float(min(max(u, 1u << 23), 253u << 23));
+}
+
+// What a block works on: rows of one key head of one sequence.
+struct AfTile {
+    int slot, len, rows, first;  // of the sequence; first: its first row in q
+    int row0, n;                 // of the tile, in (token, head) rows of the sequence's key head
+};
+__device__ __forceinline__ AfTile af_tile(const AttentionFp8Args& a, int seq, int tile, int height) {
+    AfTile t;
+    t.first = a.row_start[seq];
+    t.rows = a.row_start[seq + 1] - t.first;
+    t.slot = a.seq_slot ? a.seq_slot[seq] : seq;
+    t.len = t.slot >= 0 && t.slot < a.c.n_slots ? max(a.seq_len[seq], 0) : 0;  // (a slot that is not there holds nothing)
+    t.row0 = tile * height;
+    t.n = min(height, min(t.rows, a.max_rows) * (a.n_heads / a.c.n_kv) - t.row0);
+    return t;
+}
+
+}  // namespace sp
