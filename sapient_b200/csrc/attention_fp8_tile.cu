@@ -2,10 +2,11 @@
 //
 // A block has two groups of four warps, each with 128 rows whose scores S = Q K^T [128 x 128 keys] and sums O [128 x head_dim] lie in
 // tensor memory, a row a lane. While one group turns scores into weights, the tensor cores work for the other:
-//   warps 0-3, 4-7   weights: a thread has a row; S to registers, its maximum, exponentials, weights as fp16 back over S, from where they are
-//                    the first operand of the second product. O is rescaled only when a row's reference moves.
-//   warps 8-11       keys and values: e4m3 rows to fp16 in shared memory (128-byte swizzle; keys K-major, values as they lie: MN-major)
-//   warp 12          issues the products
+//   warps 0-3, 4-7   weights: a thread has a row; S is read twice, for its maximum and for the exponentials, which go back over it as fp16
+//                    and are the first operand of the second product from there. O is rescaled only when a row's reference moves.
+//   warps 8-11       keys: e4m3 rows to fp16 in shared memory (128-byte swizzle, K-major), and the scales of keys and values
+//   warps 12-15      values, as they lie (MN-major)
+//   warp 16          issues the products
 // ROWS: the groups have 128 rows each of 256, and keys in common. KEYS (up to 128 rows): the same rows, key tiles by turns; their sums
 // are added up at the end. Keys may be shared out to the blocks of a cluster as well, which add up through shared memory.
 //
@@ -22,7 +23,7 @@ namespace sp {
 
 cudaError_t count_launch_and_check();  // kernels.cu
 
-constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 512, AT_RING = 4, AT_MAX_PARTS = 8;
+constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 640, AT_RING = 4, AT_MAX_PARTS = 8;
 constexpr float AT_MOST = 15.f, AT_SET = 9.f;  // log2 of the largest weight, and of it when M is set
 
 template <typename T, int DP, bool KEYS>
@@ -33,7 +34,8 @@ struct AtShape {
     static constexpr int TILE = 128 * DP * 2;                             // bytes of 128 rows in fp16
     static constexpr int Q = PLANES * TILES * TILE, SMEM = Q + 2 * STAGES * TILE + 1024;
     static constexpr int LDO = DP + 4, SUMS = 2 * 128 * LDO * 4;          // takes the operands' place
-    static_assert(SUMS <= SMEM - 1024, "sums of both groups");
+    static constexpr int WEIGHTS = KEYS ? 128 * 2 * 4 : 256 * 4;           // of the sums of a block's share of rows, behind them (parts x rows of a share is at most that)
+    static_assert(SUMS + WEIGHTS <= SMEM - 1024, "sums of both groups");
 };
 
 __device__ __forceinline__ void at_init(uint64_t* bar, uint32_t arrivals) {
@@ -70,6 +72,16 @@ __device__ __forceinline__ void at_st16(uint32_t taddr, const uint32_t (&r)[16])
                  "r"(r[15]), "r"(taddr)
                  : "memory");
 }
+// The values that the wait is for go through it, so that nothing looks at them before.
+__device__ __forceinline__ void at_wait_for(float (&f)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3]), "+f"(f[4]), "+f"(f[5]), "+f"(f[6]), "+f"(f[7]), "+f"(f[8]), "+f"(f[9]), "+f"(f[10]), "+f"(f[11]),
+                   "+f"(f[12]), "+f"(f[13]), "+f"(f[14]), "+f"(f[15]), "+f"(f[16]), "+f"(f[17]), "+f"(f[18]), "+f"(f[19]), "+f"(f[20]), "+f"(f[21]), "+f"(f[22]),
+                   "+f"(f[23]), "+f"(f[24]), "+f"(f[25]), "+f"(f[26]), "+f"(f[27]), "+f"(f[28]), "+f"(f[29])
+                 :
+                 : "memory");
+    asm volatile("" : "+f"(f[30]), "+f"(f[31]) : : "memory");
+}
 __device__ __forceinline__ void at_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void at_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void at_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
@@ -87,6 +99,11 @@ __device__ __forceinline__ void at_fma2(float& a, float& b, float u, float v) { 
 __device__ __forceinline__ void at_add2(float& a, float& b, float u, float v) {
     asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n" : "+f"(a), "+f"(b) : "f"(u), "f"(v));
 }
+__device__ __forceinline__ float4 at_peer4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ float at_max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -101,7 +118,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     extern __shared__ uint8_t at_smem_raw[];
     __shared__ __align__(8) uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_full;
     __shared__ __align__(16) float k_scale[AT_RING][AT_KEYS], v_scale[AT_RING][AT_KEYS];
-    __shared__ uint32_t gone_s[AT_RING][4];  // pages of the tile that are not there, of the pages that a producer warp looks after
+    __shared__ uint32_t gone_s[AT_RING];  // pages of the tile that are not there
     __shared__ float row_factor[ROWS];
     __shared__ float part_m[2][128], part_l[2][128];
     __shared__ uint32_t tmem_slot;
@@ -122,7 +139,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     const int t_begin = k_begin / AT_KEYS, t_end = k_end > k_begin ? (k_end + AT_KEYS - 1) / AT_KEYS : t_begin;
     const int per = (t_end - t_begin + parts - 1) / parts;
     const int b_begin = min(t_end, t_begin + part * per), n_kv = min(t_end, b_begin + per) - b_begin;  // key tiles of the block
-    const int jobs = KEYS ? n_kv : 2 * n_kv;  // job j is group j % 2's
+    const int groups = KEYS || tile.n > 128 ? 2 : 1, jobs = KEYS ? n_kv : groups * n_kv;  // job j is group j % groups'
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(tc5_smem_u32(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -142,8 +159,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     // ── queries: fp16 operands, eight values a thread ──
-    {
-        constexpr int PER = DP / 8, AT_ONCE = AT_THREADS / PER;  // threads of a row, rows at once
+    if (warp < 16) {
+        constexpr int PER = DP / 8, AT_ONCE = 512 / PER;  // threads of a row, rows at once
         const int u = tid % PER;
         constexpr int BATCH = 4;
         for (int r0 = tid / PER; r0 < ROWS; r0 += BATCH * AT_ONCE) {
@@ -201,148 +218,147 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     at_after();
     const uint32_t tmem = tmem_slot;  // S of the groups at columns 0 and 128, O at 256 and 256 + DP
     bool ok = true;
-    if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");  // 128 x 48 + 128 x 96 + 256 x 184 = 512 x 128
-        if (warp == 12) {
-            const bool leader = tc5_elect();
-            const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
-            const uint32_t id_s = at_idesc(AT_KEYS, false), id_o = at_idesc(dim, true);
-            const uint64_t qd = tc5_desc(tc5_smem_u32(smem)), kd = tc5_desc(tc5_smem_u32(ks_)), vd = at_desc_values(tc5_smem_u32(vs_));
-            const int steps = dim / 16;
-            auto scores = [&](int j) {
-                const int t = j & 1, kv = KEYS ? j : j >> 1, st = kv % STAGES;
-                if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&k_full[st], (uint32_t)((kv / STAGES) & 1)));
-                if (!ok) return;
-                at_after();
-                if (leader) {
-                    const uint64_t q = qd + (uint64_t)((KEYS ? 0 : t) * (Sh::TILE >> 4)), k = kd + (uint64_t)(st * (Sh::TILE >> 4));
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");  // 128 x 48 + 256 x 80 + 256 x 136 = 640 x 96
+        if (warp == 16) {
+        const bool leader = tc5_elect();
+        const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+        const uint32_t id_s = at_idesc(AT_KEYS, false), id_o = at_idesc(dim, true);
+        const uint64_t qd = tc5_desc(tc5_smem_u32(smem)), kd = tc5_desc(tc5_smem_u32(ks_)), vd = at_desc_values(tc5_smem_u32(vs_));
+        const int steps = dim / 16;
+        auto scores = [&](int j) {
+            const int t = groups == 2 ? j & 1 : 0, kv = KEYS || groups == 1 ? j : j >> 1, st = kv % STAGES;
+            if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&k_full[st], (uint32_t)((kv / STAGES) & 1)));
+            if (!ok) return;
+            at_after();
+            if (leader) {
+                const uint64_t q = qd + (uint64_t)((KEYS ? 0 : t) * (Sh::TILE >> 4)), k = kd + (uint64_t)(st * (Sh::TILE >> 4));
+#pragma unroll
+                for (int p = Sh::PLANES - 1; p >= 0; --p)
+                    for (int s = 0; s < steps; ++s) {
+                        const uint64_t at = (uint64_t)((s >> 2) * (128 * 128 >> 4) + (s & 3) * 2);
+                        tc5_mma(tm + 128u * t, q + at + (uint64_t)(p * Sh::TILES * (Sh::TILE >> 4)), k + at, id_s, p != Sh::PLANES - 1 || s > 0);
+                    }
+                tc5_commit(&s_full[t]);
+                if (KEYS || t == groups - 1) tc5_commit(&k_empty[st]);
+            }
+            __syncwarp();
+        };
+        for (int j = 0; j < groups && j < jobs && ok; ++j) scores(j);
+        for (int j = 0; j < jobs && ok; ++j) {
+            const int t = groups == 2 ? j & 1 : 0, i = groups == 2 ? j >> 1 : j, kv = KEYS ? j : i, st = kv % STAGES;
+            bool here = tc5_wait(&p_full[t], (uint32_t)(i & 1));
+            if (KEYS || t == 0) here = here && tc5_wait(&v_full[st], (uint32_t)((kv / STAGES) & 1));
+            ok = __all_sync(0xFFFFFFFFu, here);
+            if (!ok) break;
+            at_after();
+            if (leader) {
+                const uint64_t v = vd + (uint64_t)(st * (Sh::TILE >> 4));
+#pragma unroll
+                for (int s = 0; s < AT_KEYS / 16; ++s)
 #pragma unroll
                     for (int p = Sh::PLANES - 1; p >= 0; --p)
-                        for (int s = 0; s < steps; ++s) {
-                            const uint64_t at = (uint64_t)((s >> 2) * (128 * 128 >> 4) + (s & 3) * 2);
-                            tc5_mma(tm + 128u * t, q + at + (uint64_t)(p * Sh::TILES * (Sh::TILE >> 4)), k + at, id_s, p != Sh::PLANES - 1 || s > 0);
-                        }
-                    tc5_commit(&s_full[t]);
-                    if (KEYS || t == 1) tc5_commit(&k_empty[st]);
-                }
-                __syncwarp();
-            };
-            for (int j = 0; j < 2 && j < jobs && ok; ++j) scores(j);
-            for (int j = 0; j < jobs && ok; ++j) {
-                const int t = j & 1, i = j >> 1, kv = KEYS ? j : i, st = kv % STAGES;
-                bool here = tc5_wait(&p_full[t], (uint32_t)(i & 1));
-                if (KEYS || t == 0) here = here && tc5_wait(&v_full[st], (uint32_t)((kv / STAGES) & 1));
-                ok = __all_sync(0xFFFFFFFFu, here);
-                if (!ok) break;
-                at_after();
-                if (leader) {
-                    const uint64_t v = vd + (uint64_t)(st * (Sh::TILE >> 4));
-#pragma unroll
-                    for (int s = 0; s < AT_KEYS / 16; ++s)
-#pragma unroll
-                        for (int p = Sh::PLANES - 1; p >= 0; --p)
-                            at_mma_tmem(tm + 256u + (uint32_t)(DP * t), tm + 128u * t + (uint32_t)(64 * p + 8 * s), v + (uint64_t)(s * (2048 >> 4)), id_o,
-                                        i > 0 || s > 0 || p != Sh::PLANES - 1);
-                    if (KEYS || t == 1) tc5_commit(&v_empty[st]);
-                }
-                __syncwarp();
-                if (j + 2 < jobs) scores(j + 2);
+                        at_mma_tmem(tm + 256u + (uint32_t)(DP * t), tm + 128u * t + (uint32_t)(F32 ? 32 * (s / 2) + 16 * p + 8 * (s % 2) : 8 * s), v + (uint64_t)(s * (2048 >> 4)), id_o,
+                                    i > 0 || s > 0 || p != Sh::PLANES - 1);
+                if (KEYS || t == groups - 1) tc5_commit(&v_empty[st]);
             }
-            if (jobs > 0) {
-                if (ok && leader) tc5_commit(&o_full);
-                __syncwarp();
-                // no arrival is on its way to this block when it goes on to the end
-                for (int kv = max(0, n_kv - STAGES); kv < n_kv; ++kv) {
-                    const uint32_t parity = (uint32_t)((kv / STAGES) & 1);
-                    ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&k_empty[kv % STAGES], parity) && tc5_wait(&v_empty[kv % STAGES], parity));
-                }
-                ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&o_full, 0));
+            __syncwarp();
+            if (j + groups < jobs) scores(j + groups);
+        }
+        if (jobs > 0) {
+            if (ok && leader) tc5_commit(&o_full);
+            __syncwarp();
+            // no arrival is on its way to this block when it goes on to the end
+            for (int kv = max(0, n_kv - STAGES); kv < n_kv; ++kv) {
+                const uint32_t parity = (uint32_t)((kv / STAGES) & 1);
+                ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&k_empty[kv % STAGES], parity) && tc5_wait(&v_empty[kv % STAGES], parity));
             }
+            ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&o_full, 0));
+        }
         }
         if (parts > 1) {
             cluster_sync();
             cluster_sync();
         }
     } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
-        // 16 bytes of a row a copy: thread p has the coordinates 16 (p % 8) of tokens p / 8 + 16 i (of 64 coordinates: 16 (p % 4), p / 4 + 32 i)
-        constexpr int CH = DP / 16, N = AT_KEYS * CH / 128, PER = 128 / CH;  // pieces of a row, copies of a thread, tokens between them
-        const int p = tid - 256, ch = p % CH, tok0 = p / CH;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
+        // Sixteen bytes of a row a copy, 64 coordinates of eight tokens a warp at once: stores of eight threads fall on 32 different banks.
+        const bool values = warp >= 12;
+        constexpr int HALVES = DP / 64, N = 4 * HALVES;  // copies of a thread: tokens tok0 + 32 i, coordinates 16 ch and 64 + 16 ch
+        const int p = tid - (values ? 384 : 256), ch = p % 4, tok0 = p / 4;
         const int32_t* const table = a.c.page_table + (int64_t)max(0, min(tile.slot, a.c.n_slots - 1)) * a.c.max_pages;
-        const bool in_row = 16 * ch < dim;
         auto page_of = [&](int kv) {  // lanes 0 to 7: the tile's pages
             const int index = (b_begin + kv) * AT_PAGES + (lane & 7);
             const int page = kv < n_kv && index < a.c.max_pages && index * KV_PAGE < k_end ? table[index] : -1;
             return page < a.c.n_pages ? max(page, -1) : -1;
         };
-        uint4 raw_k[N], raw_v[N];
-        float sk = 0.f, sv = 0.f;
-        auto load = [&](uint4 (&raw)[N], int pages, int which) {
+        const int64_t page_rows = (int64_t)2 * a.c.n_kv * KV_PAGE;
+        const uint8_t* const from = a.c.values + (a.c.row(0, values ? 1 : 0, head) + tok0 % KV_PAGE) * dim + 16 * ch;
+        uint4 raw[N];
+        auto load = [&](int pages) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int tok = tok0 + PER * i, page = __shfl_sync(0xFFFFFFFFu, pages, tok / KV_PAGE);
-                raw[i] = make_uint4(0, 0, 0, 0);
-                if (page >= 0 && in_row) raw[i] = __ldg(reinterpret_cast<const uint4*>(a.c.values + (a.c.row(page, which, head) + tok % KV_PAGE) * dim + 16 * ch));
+            for (int i = 0; i < 4; ++i) {
+                const int page = __shfl_sync(0xFFFFFFFFu, pages, tok0 / KV_PAGE + 2 * i);
+                const uint8_t* const row = from + (int64_t)max(page, 0) * page_rows * dim;
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) {
+                    raw[HALVES * i + h] = make_uint4(0, 0, 0, 0);
+                    if (page >= 0 && 64 * h + 16 * ch < dim) raw[HALVES * i + h] = __ldg(reinterpret_cast<const uint4*>(row + 64 * h));
+                }
             }
         };
-        auto store = [&](const uint4 (&raw)[N], uint8_t* to, bool finite) {
+        uint8_t* const to0 = (values ? vs_ : ks_) + tok0 * 128;
+        const int u0 = ((2 * ch) ^ (tok0 & 7)) * 16, u1 = ((2 * ch + 1) ^ (tok0 & 7)) * 16;
+        uint64_t *const full = values ? v_full : k_full, *const empty = values ? v_empty : k_empty;
+        int pages = page_of(0);
+        load(pages);
+        for (int kv = 0; kv < n_kv; ++kv) {
+            const int st = kv % STAGES, use = kv / STAGES;
+            float sk = 0.f, sv = 0.f;
+            if (!values) {  // of token p
+                const int page = __shfl_sync(0xFFFFFFFFu, pages, p / KV_PAGE);
+                if (page >= 0) {
+                    const int64_t at = a.c.row(page, 0, head) + p % KV_PAGE;
+                    sk = __ldg(a.c.scales + at);
+                    sv = __ldg(a.c.scales + at + (int64_t)a.c.n_kv * KV_PAGE);
+                }
+            }
+            const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
+            pages = page_of(kv + 1);
+            if (use > 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&empty[st], (uint32_t)((use - 1) & 1)));
+            if (!ok) break;
+            uint8_t* const to = to0 + st * Sh::TILE;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int tok = tok0 + PER * i;
-                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                 uint32_t h[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) af_halves(w[j], h[2 * j], h[2 * j + 1]);
-                if (finite) {
+                af_halves(raw[i].x, h[0], h[1]);
+                af_halves(raw[i].y, h[2], h[3]);
+                af_halves(raw[i].z, h[4], h[5]);
+                af_halves(raw[i].w, h[6], h[7]);
+                if (values) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) h[j] = af_finite(h[j]);
                 }
-                uint8_t* const row = to + ch / 4 * (128 * 128) + tok * 128;
-                const int u = 2 * (ch % 4), x = tok & 7, odd = ch / 4;  // (threads of the second half of a row store the other piece first: no bank twice)
-                const uint4 first = make_uint4(h[0], h[1], h[2], h[3]), second = make_uint4(h[4], h[5], h[6], h[7]);
-                *reinterpret_cast<uint4*>(row + ((u + odd) ^ x) * 16) = odd ? second : first;
-                *reinterpret_cast<uint4*>(row + ((u + 1 - odd) ^ x) * 16) = odd ? first : second;
+                uint8_t* const row = to + i / HALVES * (32 * 128) + i % HALVES * (128 * 128);
+                *reinterpret_cast<uint4*>(row + u0) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(row + u1) = make_uint4(h[4], h[5], h[6], h[7]);
             }
-        };
-        auto hand_over = [&](uint64_t* bar) {
+            if (!values) {
+                k_scale[kv % AT_RING][p] = sk;
+                v_scale[kv % AT_RING][p] = sv;
+                if (p == 0) gone_s[kv % AT_RING] = gone;
+            }
             at_fence_smem();
             __syncwarp();
-            if (lane == 0) tc5_arrive(bar);
-        };
-        int pages = page_of(0);
-        load(raw_k, pages, 0);
-        for (int kv = 0; kv < n_kv && ok; ++kv) {
-            const int st = kv % STAGES, use = kv / STAGES;
-            const int mine = __shfl_sync(0xFFFFFFFFu, pages, p / KV_PAGE);  // (of the thread's token p)
-            sk = sv = 0.f;
-            if (mine >= 0) {
-                const int64_t at = a.c.row(mine, 0, head) + p % KV_PAGE;
-                sk = __ldg(a.c.scales + at);
-                sv = __ldg(a.c.scales + at + (int64_t)a.c.n_kv * KV_PAGE);
-            }
-            const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
-            load(raw_v, pages, 1);
-            const int next = page_of(kv + 1);
-            if (use > 0) ok = tc5_wait(&k_empty[st], (uint32_t)((use - 1) & 1));
-            if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
-            store(raw_k, ks_ + st * Sh::TILE, false);
-            k_scale[kv % AT_RING][p] = sk;
-            v_scale[kv % AT_RING][p] = sv;
-            if (lane == 0) gone_s[kv % AT_RING][warp - 8] = gone;
-            hand_over(&k_full[st]);
-            pages = next;
-            load(raw_k, pages, 0);
-            if (use > 0) ok = tc5_wait(&v_empty[st], (uint32_t)((use - 1) & 1));
-            if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
-            store(raw_v, vs_ + st * Sh::TILE, true);
-            hand_over(&v_full[st]);
+            if (lane == 0) tc5_arrive(&full[st]);
+            if (kv + 1 < n_kv) load(pages);
         }
         if (parts > 1) {
             cluster_sync();
             cluster_sync();
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;\n");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;\n");
         const int t = warp >> 2, r = 32 * (warp & 3) + lane, row = (KEYS ? 0 : 128 * t) + r;  // of the block's rows
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), S = lanes + 128u * t, O = lanes + 256u + (uint32_t)(DP * t);
         const int at = tile.row0 + row, pos = tile.len - tile.rows + at / group;
@@ -351,19 +367,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         const int row_a = KEYS ? 0 : 128 * t, row_b = min(row_a + 127, tile.n - 1);
         const int whole_to = min(tile.len - tile.rows + (tile.row0 + row_a) / group, held - 1), whole_from = a.window > 0 ? tile.len - tile.rows + (tile.row0 + row_b) / group - a.window + 1 : 0;
         const float c = row_factor[row];
-        const int mine = jobs > t ? (jobs - t + 1) / 2 : 0;  // jobs of the group
+        const int mine = t >= groups ? 0 : (jobs - t + groups - 1) / groups;  // jobs of the group
         float m = -INFINITY, l0 = 0.f, l1 = 0.f;
         for (int i = 0; i < mine; ++i) {
             const int kv = KEYS ? 2 * i + t : i, key0 = (b_begin + kv) * AT_KEYS, slot = kv % AT_RING;
             ok = __all_sync(0xFFFFFFFFu, tc5_wait(&s_full[t], (uint32_t)(i & 1)));
             if (!ok) break;
             at_after();
-            float s[AT_KEYS];
-#pragma unroll
-            for (int k = 0; k < AT_KEYS; k += 32) at_ld32(S + k, s + k);
-            at_wait_ld();
-            const uint32_t gone = gone_s[slot][0];
+            float s0[32], s1[32];
+            at_ld32(S, s0);
+            const uint32_t gone = gone_s[slot];
             const bool masked = gone != 0 || key0 < whole_from || key0 + AT_KEYS - 1 > whole_to;
+            const int hi = limit - key0, lo = low - key0;
             // the power of two not below the largest finite scale of values that the block may see
             uint32_t big = 0;
             {
@@ -377,27 +392,41 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 big = __reduce_max_sync(0xFFFFFFFFu, big);
             }
             const float up = (float)(min(max((int)((big + 0x7FFFFFu) >> 23), 27), 253) - 127);
+            // keys k0 .. k0 + 31: scores times their scale; what a row does not see is -inf
+            auto scaled = [&](float (&s)[32], int k0) {
 #pragma unroll
-            for (int k = 0; k < AT_KEYS; k += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(&k_scale[slot][k]);
-                at_mul2(s[k], s[k + 1], f.x, f.y);
-                at_mul2(s[k + 2], s[k + 3], f.z, f.w);
-            }
-            if (masked) {
-                const int hi = limit - key0, lo = low - key0;
+                for (int k = 0; k < 32; k += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(&k_scale[slot][k0 + k]);
+                    at_mul2(s[k], s[k + 1], f.x, f.y);
+                    at_mul2(s[k + 2], s[k + 3], f.z, f.w);
+                }
+                if (masked) {
+                    const uint32_t no = gone >> (k0 / KV_PAGE);
 #pragma unroll
-                for (int k = 0; k < AT_KEYS; ++k)
-                    if (k > hi || k < lo || (gone >> (k / KV_PAGE) & 1)) s[k] = -INFINITY;
-            }
-            float b0 = s[0], b1 = s[1], b2 = s[2], b3 = s[3];
+                    for (int k = 0; k < 32; ++k)
+                        if (k > hi - k0 || k < lo - k0 || (no >> (k / KV_PAGE) & 1)) s[k] = -INFINITY;
+                }
+            };
+            float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
+            auto largest = [&](const float (&s)[32]) {
 #pragma unroll
-            for (int k = 4; k < AT_KEYS; k += 8) {
-                b0 = at_max3(b0, s[k], s[k + 1]);
-                b1 = at_max3(b1, s[k + 2], s[k + 3]);
-                if (k + 4 < AT_KEYS) {
+                for (int k = 0; k < 32; k += 8) {
+                    b0 = at_max3(b0, s[k], s[k + 1]);
+                    b1 = at_max3(b1, s[k + 2], s[k + 3]);
                     b2 = at_max3(b2, s[k + 4], s[k + 5]);
                     b3 = at_max3(b3, s[k + 6], s[k + 7]);
                 }
+            };
+#pragma unroll 1
+            for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {  // the next 32 are on their way while these are looked at
+                at_wait_for(s0);
+                at_ld32(S + k0 + 32, s1);
+                scaled(s0, k0);
+                largest(s0);
+                at_wait_for(s1);
+                at_ld32(S + (k0 + 64) % AT_KEYS, s0);  // at the end: the first again
+                scaled(s1, k0 + 32);
+                largest(s1);
             }
             const float best = fmaxf(fmaxf(b0, b1), fmaxf(b2, b3));
             // (nothing seen: best is -inf, which a factor of 0 would turn into NaN)
@@ -409,6 +438,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 l0 *= by;
                 l1 *= by;
                 if (i > 0) {
+#pragma unroll 1
                     for (int d = 0; d < dim; d += 16) {
                         uint32_t o[16];
                         tc5_ld16(O + d, o);
@@ -420,38 +450,50 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 }
             }
             const float base = m == -INFINITY ? 0.f : -m;
+            auto weights = [&](float (&s)[32], int k0) {
+                uint32_t w_hi[16], w_lo[16];
+                scaled(s, k0);
 #pragma unroll
-            for (int k0 = 0; k0 < AT_KEYS; k0 += 32) {
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int k = k0; k < k0 + 32; k += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(&v_scale[slot][k]);
+                for (int k = 0; k < 32; k += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(&v_scale[slot][k0 + k]);
                     const float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
                     for (int j = 0; j < 4; j += 2) {
                         float p0 = s[k + j], p1 = s[k + j + 1];
-                        if (masked) {
-                            const bool no0 = p0 == -INFINITY, no1 = p1 == -INFINITY;
-                            at_fma2(p0, p1, c, base);
-                            p0 = no0 ? 0.f : af_ex2(p0);
-                            p1 = no1 ? 0.f : af_ex2(p1);
-                            at_add2(l0, l1, p0, p1);
-                            p0 = no0 ? 0.f : p0 * v[j];  // (what is masked may have any scale)
-                            p1 = no1 ? 0.f : p1 * v[j + 1];
-                        } else {
-                            at_fma2(p0, p1, c, base);
-                            p0 = af_ex2(p0);
-                            p1 = af_ex2(p1);
-                            at_add2(l0, l1, p0, p1);
-                            at_mul2(p0, p1, v[j], v[j + 1]);
+                        const bool no0 = masked && p0 == -INFINITY, no1 = masked && p1 == -INFINITY;
+                        at_fma2(p0, p1, c, base);
+                        p0 = af_ex2(p0);
+                        p1 = af_ex2(p1);
+                        if (masked) {  // (-inf times a factor of 0 is NaN)
+                            if (no0) p0 = 0.f;
+                            if (no1) p1 = 0.f;
                         }
-                        const int w = (k - k0 + j) / 2;
-                        if constexpr (F32) af_split(p0, p1, hi[w], lo[w]);
-                        else hi[w] = af_pack(p0, p1);
+                        at_add2(l0, l1, p0, p1);
+                        at_mul2(p0, p1, v[j], v[j + 1]);
+                        if (masked) {  // (what is masked may have any scale)
+                            if (no0) p0 = 0.f;
+                            if (no1) p1 = 0.f;
+                        }
+                        const int w = (k + j) / 2;
+                        if constexpr (F32) af_split(p0, p1, w_hi[w], w_lo[w]);
+                        else w_hi[w] = af_pack(p0, p1);
                     }
                 }
-                at_st16(S + k0 / 2, hi);
-                if constexpr (F32) at_st16(S + 64 + k0 / 2, lo);
+                if constexpr (F32) {  // over the scores that they come from
+                    at_st16(S + k0, w_hi);
+                    at_st16(S + k0 + 16, w_lo);
+                } else {
+                    at_st16(S + k0 / 2, w_hi);
+                }
+            };
+#pragma unroll 1
+            for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {
+                at_wait_for(s0);
+                at_ld32(S + k0 + 32, s1);
+                weights(s0, k0);
+                at_wait_for(s1);
+                if (k0 + 64 < AT_KEYS) at_ld32(S + k0 + 64, s0);
+                weights(s1, k0 + 32);
             }
             at_wait_st();
             at_before();
@@ -463,70 +505,95 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         at_after();
         T* const out = static_cast<T*>(a.out) + (int64_t)head * group * dim;
         if (!KEYS && parts == 1) {
-            const float by = l == 0.f ? 0.f : 1.f / l;
+            const float by = l == 0.f || mine == 0 ? 0.f : 1.f / l;
             T* const to = out + (int64_t)(tile.first + at / group) * a.ldo + (int64_t)(at % group) * dim;
-            for (int d = 0; ok && d < dim; d += 16) {
-                uint32_t o[16];
-                if (mine > 0) {
-                    tc5_ld16(O + d, o);
-                    at_wait_ld();
-                }
+#pragma unroll 1
+            for (int d = 0; ok && d < dim; d += 32) {
+                float o[32];
+                at_ld32(O + d, o);
+                at_wait_for(o);
                 if (row < tile.n) {
+                    constexpr int PER = 16 / (int)sizeof(T);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 16 / (int)sizeof(T)) {
+                    for (int j = 0; j < 32; j += PER) {
                         uint4 w;
                         uint32_t* const u = &w.x;
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            if constexpr (F32) u[q] = __float_as_uint(mine > 0 ? __uint_as_float(o[j + q]) * by : 0.f);
-                            else u[q] = mine > 0 ? pack_bf16(__uint_as_float(o[j + 2 * q]) * by, __uint_as_float(o[j + 2 * q + 1]) * by) : 0u;
+                            if constexpr (F32) u[q] = mine > 0 ? __float_as_uint(o[j + q] * by) : 0u;
+                            else u[q] = mine > 0 ? pack_bf16(o[j + 2 * q] * by, o[j + 2 * q + 1] * by) : 0u;
                         }
-                        *reinterpret_cast<uint4*>(to + d + j) = w;
+                        if (d + j < dim) *reinterpret_cast<uint4*>(to + d + j) = w;
                     }
                 }
             }
         } else {
             float* const sums = reinterpret_cast<float*>(smem);  // [group][row][LDO], over the operands, which have been read
-            for (int d = 0; d < dim; d += 16) {
-                uint32_t o[16];
+            float* const weights = sums + Sh::SUMS / 4;          // [row of the block's share][sum]
+#pragma unroll 1
+            for (int d = 0; d < dim; d += 32) {
+                float o[32];
                 if (mine > 0 && ok) {
-                    tc5_ld16(O + d, o);
-                    at_wait_ld();
+                    at_ld32(O + d, o);
+                    at_wait_for(o);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[j] = 0;
+                    for (int j = 0; j < 32; ++j) o[j] = 0.f;
                 }
 #pragma unroll
-                for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(&sums[(128 * t + r) * Sh::LDO + d + j]) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                for (int j = 0; j < 32; j += 4)
+                    if (d + j < dim) *reinterpret_cast<float4*>(&sums[(128 * t + r) * Sh::LDO + d + j]) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
             }
             part_m[t][r] = m;
             part_l[t][r] = l;
             asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
             if (parts > 1) cluster_sync();
-            // the cluster's warps share the rows out; lane i looks at sum i: of part i / SETS, group i % SETS (KEYS) or the row's
+            // The blocks share the rows out: row q of the block's is part + parts q of the tile. Sum s of a row is part s / SETS's, group s % SETS's
+            // (KEYS) or its own group's.
             constexpr int SETS = KEYS ? 2 : 1;
-            for (int q = part + parts * warp; q < tile.n; q += parts * 8) {
-                const int g = KEYS ? lane % SETS : q / 128, from = KEYS ? lane / SETS : lane;
-                const bool there = lane < parts * SETS;
-                const uint32_t at_m = smem_addr(&part_m[g][q % 128]), at_l = smem_addr(&part_l[g][q % 128]);
-                const float pm = !there ? -INFINITY : parts > 1 ? ld_peer(peer_smem(at_m, from)) : part_m[g][q % 128];
-                const float pl = !there ? 0.f : parts > 1 ? ld_peer(peer_smem(at_l, from)) : part_l[g][q % 128];
-                const float top = warp_max(pm), w = pm == -INFINITY ? 0.f : af_ex2(pm - top), total = warp_sum(pl * w);
-                float y[DP / 32] = {};
-                for (int s = 0; s < parts * SETS; ++s) {
-                    const float ws = __shfl_sync(0xFFFFFFFFu, w, s);
-                    const float* const src = sums + ((KEYS ? s % SETS : q / 128) * 128 + q % 128) * Sh::LDO + lane;
-                    const uint32_t peer = parts > 1 ? peer_smem(smem_addr(src), s / SETS) : 0;
-#pragma unroll
-                    for (int e = 0; e < DP / 32; ++e)
-                        if (32 * e + lane < dim) y[e] = fmaf(parts > 1 ? ld_peer(peer + 128u * e) : src[32 * e], ws, y[e]);
+            const int sets = parts * SETS, rows_here = (tile.n - part + parts - 1) / parts;
+            for (int e = tid; e < rows_here * sets; e += 256) {
+                const int q = e / sets, s = e - q * sets, of = part + parts * q;
+                float pm = 0.f, top = -INFINITY, total = 0.f;
+                for (int x = 0; x < sets; ++x) {
+                    const int g = KEYS ? x % SETS : of / 128;
+                    const uint32_t at_m = smem_addr(&part_m[g][of % 128]), at_l = smem_addr(&part_l[g][of % 128]);
+                    const float xm = parts > 1 ? ld_peer(peer_smem(at_m, x / SETS)) : part_m[g][of % 128], xl = parts > 1 ? ld_peer(peer_smem(at_l, x / SETS)) : part_l[g][of % 128];
+                    const float to = fmaxf(top, xm);
+                    total = total * (top == to ? 1.f : af_ex2(top - to)) + (xm == to ? xl : xl * af_ex2(xm - to));
+                    top = to;
+                    if (x == s) pm = xm;
                 }
-                const float by = total == 0.f ? 0.f : 1.f / total;
-                const int where = tile.row0 + q;
-                T* const to = out + (int64_t)(tile.first + where / group) * a.ldo + (int64_t)(where % group) * dim;
+                weights[e] = total == 0.f || pm == -INFINITY ? 0.f : af_ex2(pm - top) / total;
+            }
+            asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
+            const int quads = dim / 4;
+            for (int e = tid; e < rows_here * quads; e += 256) {
+                const int q = e / quads, d = 4 * (e - q * quads), of = part + parts * q;
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int x0 = 0; x0 < sets; x0 += 4) {
+                    float4 v[4];
 #pragma unroll
-                for (int e = 0; e < DP / 32; ++e)
-                    if (ok && 32 * e + lane < dim) to[32 * e + lane] = from_f32<T>(y[e] * by);
+                    for (int x = 0; x < 4; ++x) {
+                        if (x0 + x >= sets) break;
+                        const float* const src = sums + ((KEYS ? (x0 + x) % SETS : of / 128) * 128 + of % 128) * Sh::LDO + d;
+                        v[x] = parts > 1 ? at_peer4(peer_smem(smem_addr(src), (x0 + x) / SETS)) : *reinterpret_cast<const float4*>(src);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        if (x0 + x >= sets) break;
+                        const float w = weights[q * sets + x0 + x];
+                        y.x = fmaf(v[x].x, w, y.x);
+                        y.y = fmaf(v[x].y, w, y.y);
+                        y.z = fmaf(v[x].z, w, y.z);
+                        y.w = fmaf(v[x].w, w, y.w);
+                    }
+                }
+                const int where = tile.row0 + of;
+                T* const to = out + (int64_t)(tile.first + where / group) * a.ldo + (int64_t)(where % group) * dim + d;
+                if (!ok) continue;
+                if constexpr (F32) *reinterpret_cast<float4*>(to) = y;
+                else *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
             }
             if (parts > 1) cluster_sync();  // nobody leaves while its sums are being read
         }
