@@ -13,6 +13,7 @@
 // A row's weights are e^(z - M) s' with one M for the lift of the header and the scales' size: with u the power of two not below the tile's largest
 // finite scale, M is moved when z + u passes M + 15 (log2), to z + u - 9; sum of e^(z - M) and O move along.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_fp8.cuh"
 #include "kernels.h"
@@ -392,109 +393,122 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 big = __reduce_max_sync(0xFFFFFFFFu, big);
             }
             const float up = (float)(min(max((int)((big + 0x7FFFFFu) >> 23), 27), 253) - 127);
-            // keys k0 .. k0 + 31: scores times their scale; what a row does not see is -inf
-            auto scaled = [&](float (&s)[32], int k0) {
-#pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(&k_scale[slot][k0 + k]);
-                    at_mul2(s[k], s[k + 1], f.x, f.y);
-                    at_mul2(s[k + 2], s[k + 3], f.z, f.w);
-                }
-                if (masked) {
+            // One job, with and without keys that a row does not see: both as code of its own, since decided at each value it is 6 instructions more.
+            auto job = [&](auto with_mask) {
+                constexpr bool MASK = decltype(with_mask)::value;
+                // bits of the keys k0 .. k0 + 31 that the row sees
+                auto seen = [&](int k0) {
+                    const int from = lo - k0, to = hi - k0;
+                    uint32_t bits = to >= 31 ? 0xFFFFFFFFu : to < 0 ? 0u : (2u << to) - 1u;
+                    bits = from <= 0 ? bits : from > 31 ? 0u : bits & (0xFFFFFFFFu << from);
                     const uint32_t no = gone >> (k0 / KV_PAGE);
+                    return bits & ~((no & 1 ? 0xFFFFu : 0u) | (no & 2 ? 0xFFFF0000u : 0u));
+                };
+                // keys k0 .. k0 + 31: scores times their scale; what a row does not see is -inf
+                auto scaled = [&](float (&s)[32], int k0, uint32_t bits) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (k > hi - k0 || k < lo - k0 || (no >> (k / KV_PAGE) & 1)) s[k] = -INFINITY;
-                }
-            };
-            float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
-            auto largest = [&](const float (&s)[32]) {
+                    for (int k = 0; k < 32; k += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&k_scale[slot][k0 + k]);
+                        at_mul2(s[k], s[k + 1], f.x, f.y);
+                        at_mul2(s[k + 2], s[k + 3], f.z, f.w);
+                    }
+                    if constexpr (MASK) {
 #pragma unroll
-                for (int k = 0; k < 32; k += 8) {
-                    b0 = at_max3(b0, s[k], s[k + 1]);
-                    b1 = at_max3(b1, s[k + 2], s[k + 3]);
-                    b2 = at_max3(b2, s[k + 4], s[k + 5]);
-                    b3 = at_max3(b3, s[k + 6], s[k + 7]);
-                }
-            };
+                        for (int k = 0; k < 32; ++k)
+                            if (!(bits >> k & 1)) s[k] = -INFINITY;
+                    }
+                };
+                float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
+                auto largest = [&](const float (&s)[32]) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        b0 = at_max3(b0, s[k], s[k + 1]);
+                        b1 = at_max3(b1, s[k + 2], s[k + 3]);
+                        b2 = at_max3(b2, s[k + 4], s[k + 5]);
+                        b3 = at_max3(b3, s[k + 6], s[k + 7]);
+                    }
+                };
 #pragma unroll 1
-            for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {  // the next 32 are on their way while these are looked at
-                at_wait_for(s0);
-                at_ld32(S + k0 + 32, s1);
-                scaled(s0, k0);
-                largest(s0);
-                at_wait_for(s1);
-                at_ld32(S + (k0 + 64) % AT_KEYS, s0);  // at the end: the first again
-                scaled(s1, k0 + 32);
-                largest(s1);
-            }
-            const float best = fmaxf(fmaxf(b0, b1), fmaxf(b2, b3));
-            // (nothing seen: best is -inf, which a factor of 0 would turn into NaN)
-            const float x = best == -INFINITY ? -INFINITY : fmaf(best, c, up);
-            const bool moves = x > m + AT_MOST;
-            if (__any_sync(0xFFFFFFFFu, moves)) {
-                const float to = moves ? x - AT_SET : m, by = moves ? af_ex2(m - to) : 1.f;  // (m = -inf: 0)
-                m = to;
-                l0 *= by;
-                l1 *= by;
-                if (i > 0) {
+                for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {  // the next 32 are on their way while these are looked at
+                    at_wait_for(s0);
+                    at_ld32(S + k0 + 32, s1);
+                    scaled(s0, k0, MASK ? seen(k0) : 0u);
+                    largest(s0);
+                    at_wait_for(s1);
+                    at_ld32(S + (k0 + 64) % AT_KEYS, s0);  // at the end: the first again
+                    scaled(s1, k0 + 32, MASK ? seen(k0 + 32) : 0u);
+                    largest(s1);
+                }
+                const float best = fmaxf(fmaxf(b0, b1), fmaxf(b2, b3));
+                // (nothing seen: best is -inf, which a factor of 0 would turn into NaN)
+                const float x = best == -INFINITY ? -INFINITY : fmaf(best, c, up);
+                const bool moves = x > m + AT_MOST;
+                if (__any_sync(0xFFFFFFFFu, moves)) {
+                    const float to = moves ? x - AT_SET : m, by = moves ? af_ex2(m - to) : 1.f;  // (m = -inf: 0)
+                    m = to;
+                    l0 *= by;
+                    l1 *= by;
+                    if (i > 0) {
 #pragma unroll 1
-                    for (int d = 0; d < dim; d += 16) {
-                        uint32_t o[16];
-                        tc5_ld16(O + d, o);
-                        at_wait_ld();
+                        for (int d = 0; d < dim; d += 16) {
+                            uint32_t o[16];
+                            tc5_ld16(O + d, o);
+                            at_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
-                        at_st16(O + d, o);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+                            at_st16(O + d, o);
+                        }
                     }
                 }
-            }
-            const float base = m == -INFINITY ? 0.f : -m;
-            auto weights = [&](float (&s)[32], int k0) {
-                uint32_t w_hi[16], w_lo[16];
-                scaled(s, k0);
+                const float base = m == -INFINITY ? 0.f : -m;
+                auto weights = [&](float (&s)[32], int k0) {
+                    uint32_t w_hi[16], w_lo[16];
+                    const uint32_t bits = MASK ? seen(k0) : 0u;
+                    scaled(s, k0, bits);
 #pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(&v_scale[slot][k0 + k]);
-                    const float v[4] = {f.x, f.y, f.z, f.w};
+                    for (int k = 0; k < 32; k += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&v_scale[slot][k0 + k]);
+                        const float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-                    for (int j = 0; j < 4; j += 2) {
-                        float p0 = s[k + j], p1 = s[k + j + 1];
-                        const bool no0 = masked && p0 == -INFINITY, no1 = masked && p1 == -INFINITY;
-                        at_fma2(p0, p1, c, base);
-                        p0 = af_ex2(p0);
-                        p1 = af_ex2(p1);
-                        if (masked) {  // (-inf times a factor of 0 is NaN)
-                            if (no0) p0 = 0.f;
-                            if (no1) p1 = 0.f;
+                        for (int j = 0; j < 4; j += 2) {
+                            float p0 = s[k + j], p1 = s[k + j + 1];
+                            at_fma2(p0, p1, c, base);
+                            p0 = af_ex2(p0);
+                            p1 = af_ex2(p1);
+                            if constexpr (MASK) {  // (-inf times a factor of 0 is NaN)
+                                if (!(bits >> (k + j) & 1)) p0 = 0.f;
+                                if (!(bits >> (k + j + 1) & 1)) p1 = 0.f;
+                            }
+                            at_add2(l0, l1, p0, p1);
+                            at_mul2(p0, p1, v[j], v[j + 1]);
+                            if constexpr (MASK) {  // (what is masked may have any scale)
+                                if (!(bits >> (k + j) & 1)) p0 = 0.f;
+                                if (!(bits >> (k + j + 1) & 1)) p1 = 0.f;
+                            }
+                            const int w = (k + j) / 2;
+                            if constexpr (F32) af_split(p0, p1, w_hi[w], w_lo[w]);
+                            else w_hi[w] = af_pack(p0, p1);
                         }
-                        at_add2(l0, l1, p0, p1);
-                        at_mul2(p0, p1, v[j], v[j + 1]);
-                        if (masked) {  // (what is masked may have any scale)
-                            if (no0) p0 = 0.f;
-                            if (no1) p1 = 0.f;
-                        }
-                        const int w = (k + j) / 2;
-                        if constexpr (F32) af_split(p0, p1, w_hi[w], w_lo[w]);
-                        else w_hi[w] = af_pack(p0, p1);
                     }
-                }
-                if constexpr (F32) {  // over the scores that they come from
-                    at_st16(S + k0, w_hi);
-                    at_st16(S + k0 + 16, w_lo);
-                } else {
-                    at_st16(S + k0 / 2, w_hi);
+                    if constexpr (F32) {  // over the scores that they come from
+                        at_st16(S + k0, w_hi);
+                        at_st16(S + k0 + 16, w_lo);
+                    } else {
+                        at_st16(S + k0 / 2, w_hi);
+                    }
+                };
+#pragma unroll 1
+                for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {
+                    at_wait_for(s0);
+                    at_ld32(S + k0 + 32, s1);
+                    weights(s0, k0);
+                    at_wait_for(s1);
+                    if (k0 + 64 < AT_KEYS) at_ld32(S + k0 + 64, s0);
+                    weights(s1, k0 + 32);
                 }
             };
-#pragma unroll 1
-            for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {
-                at_wait_for(s0);
-                at_ld32(S + k0 + 32, s1);
-                weights(s0, k0);
-                at_wait_for(s1);
-                if (k0 + 64 < AT_KEYS) at_ld32(S + k0 + 64, s0);
-                weights(s1, k0 + 32);
-            }
+            if (masked) job(std::true_type{});
+            else job(std::false_type{});
             at_wait_st();
             at_before();
             __syncwarp();
