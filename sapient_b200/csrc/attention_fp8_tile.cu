@@ -10,8 +10,10 @@
 // ROWS: the groups have 128 rows each of 256, and keys in common. KEYS (up to 128 rows): the same rows, key tiles by turns; their sums
 // are added up at the end. Keys may be shared out to the blocks of a cluster as well, which add up through shared memory.
 //
-// A row's weights are e^(z - M) s' with one M for the lift of the header and the scales' size: with u the power of two not below the tile's largest
-// finite scale, M is moved when z + u passes M + 15 (log2), to z + u - 9; sum of e^(z - M) and O move along.
+// A tile's values have a power of two 2^u, not below the largest of their scales. For bf16 rows they are multiplied by s' 2^(7 - u) as they become
+// fp16 (off by 2^-11 of themselves), so that a weight is one exponential, 2^(z - M + u - 7); for f32 rows values stay exact and weights
+// are 2^(z - M) s', as fp16 plus the fp16 of the remainder. Either way they must stay below 2^16: the row's reference M is moved when
+// z + u - 7 (f32: z + u) passes M + 15, to 9 below it, and the sums move along. A scale that is NaN or infinite counts as 0 and makes the token's scores NaN.
 #include <algorithm>
 #include <type_traits>
 
@@ -26,6 +28,7 @@ cudaError_t count_launch_and_check();  // kernels.cu
 
 constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 640, AT_RING = 4, AT_MAX_PARTS = 8;
 constexpr float AT_MOST = 15.f, AT_SET = 9.f;  // log2 of the largest weight, and of it when M is set
+constexpr int AT_UP = 7, AT_LEAST = -80;       // values times 2^7 are below 2^16; smaller u would let a sum of 2^(z - M) pass 2^127
 
 template <typename T, int DP, bool KEYS>
 struct AtShape {
@@ -38,6 +41,9 @@ struct AtShape {
     static constexpr int WEIGHTS = KEYS ? 128 * 2 * 4 : 256 * 4;           // of the sums of a block's share of rows, behind them (parts x rows of a share is at most that)
     static_assert(SUMS + WEIGHTS <= SMEM - 1024, "sums of both groups");
 };
+
+// log2 of the power of two not below a scale, given by its bits (positive and finite, or 0).
+__device__ __forceinline__ int at_power(uint32_t bits) { return max((int)((bits + 0x7FFFFFu) >> 23) - 127, AT_LEAST); }
 
 __device__ __forceinline__ void at_init(uint64_t* bar, uint32_t arrivals) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(tc5_smem_u32(bar)), "r"(arrivals) : "memory");
@@ -56,15 +62,53 @@ __device__ __forceinline__ void at_mma_tmem(uint32_t d, uint32_t a, uint64_t b, 
         "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void at_ld32(uint32_t taddr, float* f) {
-    uint32_t* const r = reinterpret_cast<uint32_t*>(f);
+// 32 columns of the warp's lanes, two in a register pair.
+__device__ __forceinline__ void at_ld32(uint32_t taddr, uint64_t (&v)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
-        "%29,%30,%31}, [%32];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "{\n.reg .b32 r<32>;\n"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15, r16, r17, r18, r19, r20, r21, r22, r23, r24, r25, r26, r27, r28, r29, r30, r31}, [%16];\n"
+        "mov.b64 %0, {r0, r1};\n"
+        "mov.b64 %1, {r2, r3};\n"
+        "mov.b64 %2, {r4, r5};\n"
+        "mov.b64 %3, {r6, r7};\n"
+        "mov.b64 %4, {r8, r9};\n"
+        "mov.b64 %5, {r10, r11};\n"
+        "mov.b64 %6, {r12, r13};\n"
+        "mov.b64 %7, {r14, r15};\n"
+        "mov.b64 %8, {r16, r17};\n"
+        "mov.b64 %9, {r18, r19};\n"
+        "mov.b64 %10, {r20, r21};\n"
+        "mov.b64 %11, {r22, r23};\n"
+        "mov.b64 %12, {r24, r25};\n"
+        "mov.b64 %13, {r26, r27};\n"
+        "mov.b64 %14, {r28, r29};\n"
+        "mov.b64 %15, {r30, r31};\n"
+        "}\n"
+        : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3]), "=l"(v[4]), "=l"(v[5]), "=l"(v[6]), "=l"(v[7]), "=l"(v[8]), "=l"(v[9]), "=l"(v[10]), "=l"(v[11]), "=l"(v[12]), "=l"(v[13]), "=l"(v[14]), "=l"(v[15])
         : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void at_st32(uint32_t taddr, const uint64_t (&v)[16]) {
+    asm volatile(
+        "{\n.reg .b32 r<32>;\n"
+        "mov.b64 {r0, r1}, %0;\n"
+        "mov.b64 {r2, r3}, %1;\n"
+        "mov.b64 {r4, r5}, %2;\n"
+        "mov.b64 {r6, r7}, %3;\n"
+        "mov.b64 {r8, r9}, %4;\n"
+        "mov.b64 {r10, r11}, %5;\n"
+        "mov.b64 {r12, r13}, %6;\n"
+        "mov.b64 {r14, r15}, %7;\n"
+        "mov.b64 {r16, r17}, %8;\n"
+        "mov.b64 {r18, r19}, %9;\n"
+        "mov.b64 {r20, r21}, %10;\n"
+        "mov.b64 {r22, r23}, %11;\n"
+        "mov.b64 {r24, r25}, %12;\n"
+        "mov.b64 {r26, r27}, %13;\n"
+        "mov.b64 {r28, r29}, %14;\n"
+        "mov.b64 {r30, r31}, %15;\n"
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%16], {r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15, r16, r17, r18, r19, r20, r21, r22, r23, r24, r25, r26, r27, r28, r29, r30, r31};\n"
+        "}\n" ::"l"(v[0]), "l"(v[1]), "l"(v[2]), "l"(v[3]), "l"(v[4]), "l"(v[5]), "l"(v[6]), "l"(v[7]), "l"(v[8]), "l"(v[9]), "l"(v[10]), "l"(v[11]), "l"(v[12]), "l"(v[13]), "l"(v[14]), "l"(v[15]), "r"(taddr)
         : "memory");
 }
 __device__ __forceinline__ void at_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -74,14 +118,11 @@ __device__ __forceinline__ void at_st16(uint32_t taddr, const uint32_t (&r)[16])
                  : "memory");
 }
 // The values that the wait is for go through it, so that nothing looks at them before.
-__device__ __forceinline__ void at_wait_for(float (&f)[32]) {
+__device__ __forceinline__ void at_wait_for(uint64_t (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;\n"
-                 : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3]), "+f"(f[4]), "+f"(f[5]), "+f"(f[6]), "+f"(f[7]), "+f"(f[8]), "+f"(f[9]), "+f"(f[10]), "+f"(f[11]),
-                   "+f"(f[12]), "+f"(f[13]), "+f"(f[14]), "+f"(f[15]), "+f"(f[16]), "+f"(f[17]), "+f"(f[18]), "+f"(f[19]), "+f"(f[20]), "+f"(f[21]), "+f"(f[22]),
-                   "+f"(f[23]), "+f"(f[24]), "+f"(f[25]), "+f"(f[26]), "+f"(f[27]), "+f"(f[28]), "+f"(f[29])
+                 : "+l"(v[0]), "+l"(v[1]), "+l"(v[2]), "+l"(v[3]), "+l"(v[4]), "+l"(v[5]), "+l"(v[6]), "+l"(v[7]), "+l"(v[8]), "+l"(v[9]), "+l"(v[10]), "+l"(v[11]), "+l"(v[12]), "+l"(v[13]), "+l"(v[14]), "+l"(v[15])
                  :
                  : "memory");
-    asm volatile("" : "+f"(f[30]), "+f"(f[31]) : : "memory");
 }
 __device__ __forceinline__ void at_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void at_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
@@ -89,25 +130,41 @@ __device__ __forceinline__ void at_after() { asm volatile("tcgen05.fence::after_
 __device__ __forceinline__ void at_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void at_fence_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-// Two values an instruction.
-__device__ __forceinline__ void at_mul2(float& a, float& b, float u, float v) {
-    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nmul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n" : "+f"(a), "+f"(b) : "f"(u), "f"(v));
+// Two values an instruction, kept in register pairs.
+__device__ __forceinline__ uint64_t at_pair(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
 }
-__device__ __forceinline__ void at_fma2(float& a, float& b, float u, float v) {  // a u + v, b u + v
-    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %2};\nmov.b64 z, {%3, %3};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}\n"
-        : "+f"(a), "+f"(b) : "f"(u), "f"(v));
+__device__ __forceinline__ float2 at_two(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
 }
-__device__ __forceinline__ void at_add2(float& a, float& b, float u, float v) {
-    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n" : "+f"(a), "+f"(b) : "f"(u), "f"(v));
+__device__ __forceinline__ uint64_t at_mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t at_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t at_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 __device__ __forceinline__ float4 at_peer4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ float at_max3(float a, float b, float c) {
+__device__ __forceinline__ float at_max3(float a, uint64_t two) {
+    const float2 f = at_two(two);
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(f.x), "f"(f.y));
     return d;
 }
 
@@ -117,9 +174,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     constexpr bool F32 = Sh::F32;
     constexpr int STAGES = Sh::STAGES, ROWS = 128 * Sh::TILES;
     extern __shared__ uint8_t at_smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_full;
-    __shared__ __align__(16) float k_scale[AT_RING][AT_KEYS], v_scale[AT_RING][AT_KEYS];
+    __shared__ __align__(8) uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_full, q_full;
+    __shared__ __align__(16) float k_scale[AT_RING][AT_KEYS], v_scale[AT_RING][F32 ? AT_KEYS : 4];
     __shared__ uint32_t gone_s[AT_RING];  // pages of the tile that are not there
+    __shared__ __align__(16) uint32_t largest_s[AT_RING][4];  // scales of values, of 32 tokens each
     __shared__ float row_factor[ROWS];
     __shared__ float part_m[2][128], part_l[2][128];
     __shared__ uint32_t tmem_slot;
@@ -141,7 +199,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     const int per = (t_end - t_begin + parts - 1) / parts;
     const int b_begin = min(t_end, t_begin + part * per), n_kv = min(t_end, b_begin + per) - b_begin;  // key tiles of the block
     const int groups = KEYS || tile.n > 128 ? 2 : 1, jobs = KEYS ? n_kv : groups * n_kv;  // job j is group j % groups'
-    if (warp == 0) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(tc5_smem_u32(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
@@ -157,63 +215,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             at_init(&p_full[i], 4);
         }
         at_init(&o_full, 1);
+        at_init(&q_full, 8);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    // ── queries: fp16 operands, eight values a thread ──
-    if (warp < 16) {
-        constexpr int PER = DP / 8, AT_ONCE = 512 / PER;  // threads of a row, rows at once
-        const int u = tid % PER;
-        constexpr int BATCH = 4;
-        for (int r0 = tid / PER; r0 < ROWS; r0 += BATCH * AT_ONCE) {
-            float x[BATCH][8];
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const int r = r0 + i * AT_ONCE, row = tile.row0 + min(r, tile.n - 1);
-                const T* const src = static_cast<const T*>(a.q) + (int64_t)(tile.first + row / group) * a.ldq + (int64_t)(head * group + row % group) * dim + 8 * u;
-                if (r < tile.n && 8 * u < dim) {
-                    if constexpr (F32) {
-                        const float4 v = reinterpret_cast<const float4*>(src)[0], w = reinterpret_cast<const float4*>(src)[1];
-                        x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
-                        x[i][4] = w.x; x[i][5] = w.y; x[i][6] = w.z; x[i][7] = w.w;
-                    } else {
-                        const uint4 v = *reinterpret_cast<const uint4*>(src);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            x[i][2 * j] = __uint_as_float(w[j] << 16);
-                            x[i][2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const int r = r0 + i * AT_ONCE;
-                float most = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[i][j]));
-#pragma unroll
-                for (int o = PER / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-                float by, back;
-                af_row_scale(most, by, back);
-                if (a.scale < 0.f) by = -by;
-                if (r < ROWS) {
-                    if (u == 0) row_factor[r] = back * fabsf(a.scale) * AF_LOG2E;
-                    uint4 hi, lo;
-                    uint32_t *const h = &hi.x, *const l = &lo.x;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) af_split(x[i][2 * j] * by, x[i][2 * j + 1] * by, h[j], l[j]);
-                    uint8_t* const to = smem + r / 128 * Sh::TILE + u / 8 * (128 * 128) + r % 128 * 128 + ((u % 8) ^ (r & 7)) * 16;
-                    *reinterpret_cast<uint4*>(to) = hi;
-                    if constexpr (F32) *reinterpret_cast<uint4*>(to + Sh::TILES * Sh::TILE) = lo;
-                }
-            }
-        }
-    }
-    at_fence_smem();
     at_before();
     __syncthreads();
     at_after();
@@ -227,6 +231,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         const uint32_t id_s = at_idesc(AT_KEYS, false), id_o = at_idesc(dim, true);
         const uint64_t qd = tc5_desc(tc5_smem_u32(smem)), kd = tc5_desc(tc5_smem_u32(ks_)), vd = at_desc_values(tc5_smem_u32(vs_));
         const int steps = dim / 16;
+        if (jobs > 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&q_full, 0));
         auto scores = [&](int j) {
             const int t = groups == 2 ? j & 1 : 0, kv = KEYS || groups == 1 ? j : j >> 1, st = kv % STAGES;
             if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&k_full[st], (uint32_t)((kv / STAGES) & 1)));
@@ -295,16 +300,34 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         };
         const int64_t page_rows = (int64_t)2 * a.c.n_kv * KV_PAGE;
         const uint8_t* const from = a.c.values + (a.c.row(0, values ? 1 : 0, head) + tok0 % KV_PAGE) * dim + 16 * ch;
+        const float* const v_scales = a.c.scales + a.c.row(0, 1, head);
         uint4 raw[N];
-        auto load = [&](int pages) {
+        float own[4];       // scales of the thread's tokens (values)
+        float4 four;        // of tokens 4 lane .. 4 lane + 3 (values); of token p: key's, value's (keys)
+        // A value's scale as it counts: none of what no row of the block sees, nor of what is NaN or infinite
+        auto counts = [&](float s, int token) { return s > 0.f && s < INFINITY && token >= k_begin && token < k_end; };
+        auto load = [&](int kv, int pages) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int page = __shfl_sync(0xFFFFFFFFu, pages, tok0 / KV_PAGE + 2 * i);
-                const uint8_t* const row = from + (int64_t)max(page, 0) * page_rows * dim;
+                const int64_t rows = (int64_t)max(page, 0) * page_rows;
+                const uint8_t* const row = from + rows * dim;
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h) {
                     raw[HALVES * i + h] = make_uint4(0, 0, 0, 0);
                     if (page >= 0 && 64 * h + 16 * ch < dim) raw[HALVES * i + h] = __ldg(reinterpret_cast<const uint4*>(row + 64 * h));
+                }
+                if (!F32 && values) own[i] = page >= 0 ? __ldg(v_scales + rows + tok0 % KV_PAGE) : 0.f;
+            }
+            four = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int page = __shfl_sync(0xFFFFFFFFu, pages, values ? lane / 4 : p / KV_PAGE);
+            if (page >= 0) {
+                const float* const at = v_scales + (int64_t)page * page_rows;
+                if (!values) {
+                    four.x = __ldg(at + p % KV_PAGE - (int64_t)a.c.n_kv * KV_PAGE);
+                    four.y = __ldg(at + p % KV_PAGE);
+                } else if (!F32) {
+                    four = __ldg(reinterpret_cast<const float4*>(at + 4 * lane % KV_PAGE));
                 }
             }
         };
@@ -312,20 +335,31 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         const int u0 = ((2 * ch) ^ (tok0 & 7)) * 16, u1 = ((2 * ch + 1) ^ (tok0 & 7)) * 16;
         uint64_t *const full = values ? v_full : k_full, *const empty = values ? v_empty : k_empty;
         int pages = page_of(0);
-        load(pages);
+        load(0, pages);
         for (int kv = 0; kv < n_kv; ++kv) {
-            const int st = kv % STAGES, use = kv / STAGES;
-            float sk = 0.f, sv = 0.f;
-            if (!values) {  // of token p
-                const int page = __shfl_sync(0xFFFFFFFFu, pages, p / KV_PAGE);
-                if (page >= 0) {
-                    const int64_t at = a.c.row(page, 0, head) + p % KV_PAGE;
-                    sk = __ldg(a.c.scales + at);
-                    sv = __ldg(a.c.scales + at + (int64_t)a.c.n_kv * KV_PAGE);
-                }
-            }
+            const int st = kv % STAGES, use = kv / STAGES, slot = kv % AT_RING, key0 = (b_begin + kv) * AT_KEYS;
             const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
-            pages = page_of(kv + 1);
+            const int next = page_of(kv + 1);
+            uint32_t by[4] = {};  // what values are multiplied by, as pairs of fp16
+            float sk = 0.f, sv = 0.f;
+            uint32_t big;
+            if (values) {
+                if constexpr (!F32) {
+                    const int k = key0 + 4 * lane;
+                    big = max(max(counts(four.x, k) ? __float_as_uint(four.x) : 0u, counts(four.y, k + 1) ? __float_as_uint(four.y) : 0u),
+                              max(counts(four.z, k + 2) ? __float_as_uint(four.z) : 0u, counts(four.w, k + 3) ? __float_as_uint(four.w) : 0u));
+                    const float lift = __uint_as_float((uint32_t)(127 + AT_UP - at_power(__reduce_max_sync(0xFFFFFFFFu, big))) << 23);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float f = counts(own[i], key0 + tok0 + 32 * i) ? own[i] * lift : 0.f;
+                        by[i] = af_pack(f, f);
+                    }
+                }
+            } else {
+                sv = counts(four.y, key0 + p) ? four.y : 0.f;
+                sk = four.y < INFINITY && four.y > -INFINITY ? four.x : __uint_as_float(0x7FC00000u);
+                big = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(sv));
+            }
             if (use > 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&empty[st], (uint32_t)((use - 1) & 1)));
             if (!ok) break;
             uint8_t* const to = to0 + st * Sh::TILE;
@@ -338,21 +372,26 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 af_halves(raw[i].w, h[6], h[7]);
                 if (values) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) h[j] = af_finite(h[j]);
+                    for (int j = 0; j < 8; ++j) {
+                        h[j] = af_finite(h[j]);
+                        if constexpr (!F32) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(by[i / HALVES]));
+                    }
                 }
                 uint8_t* const row = to + i / HALVES * (32 * 128) + i % HALVES * (128 * 128);
                 *reinterpret_cast<uint4*>(row + u0) = make_uint4(h[0], h[1], h[2], h[3]);
                 *reinterpret_cast<uint4*>(row + u1) = make_uint4(h[4], h[5], h[6], h[7]);
             }
             if (!values) {
-                k_scale[kv % AT_RING][p] = sk;
-                v_scale[kv % AT_RING][p] = sv;
-                if (p == 0) gone_s[kv % AT_RING] = gone;
+                k_scale[slot][p] = sk;
+                if constexpr (F32) v_scale[slot][p] = sv;
+                if (lane == 0) largest_s[slot][warp - 8] = big;
+                if (p == 0) gone_s[slot] = gone;
             }
             at_fence_smem();
             __syncwarp();
             if (lane == 0) tc5_arrive(&full[st]);
-            if (kv + 1 < n_kv) load(pages);
+            pages = next;
+            if (kv + 1 < n_kv) load(kv + 1, pages);
         }
         if (parts > 1) {
             cluster_sync();
@@ -367,196 +406,255 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         // keys that all rows of the group see
         const int row_a = KEYS ? 0 : 128 * t, row_b = min(row_a + 127, tile.n - 1);
         const int whole_to = min(tile.len - tile.rows + (tile.row0 + row_a) / group, held - 1), whole_from = a.window > 0 ? tile.len - tile.rows + (tile.row0 + row_b) / group - a.window + 1 : 0;
-        const float c = row_factor[row];
         const int mine = t >= groups ? 0 : (jobs - t + groups - 1) / groups;  // jobs of the group
-        float m = -INFINITY, l0 = 0.f, l1 = 0.f;
+        // ── queries: fp16 operands, eight values a thread and row ──
+        float c;  // scale log2(e) / what the row is multiplied by; never 0, since scores of -inf are multiplied by it
+        {
+            constexpr int PER = DP / 8, AT_ONCE = 32 / PER, N = 32 / AT_ONCE;  // threads of a row, rows at once, rows of a thread
+            // KEYS: the groups share the rows out, 16 a warp
+            constexpr int COUNT = KEYS ? N / 2 : N;
+            const int u = lane % PER, first = KEYS ? 16 * warp + lane / PER : 128 * t + 32 * (warp & 3) + lane / PER;
+            uint4 raw[COUNT][F32 ? 2 : 1];
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) {
+                const int q = first + i * AT_ONCE, where = tile.row0 + q;
+#pragma unroll
+                for (int e = 0; e < (F32 ? 2 : 1); ++e) {
+                    raw[i][e] = make_uint4(0, 0, 0, 0);
+                    if (q < tile.n && 8 * u < dim)
+                        raw[i][e] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(tile.first + where / group) * a.ldq + (int64_t)(head * group + where % group) * dim + 8 * u)[e];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) {
+                const int q = first + i * AT_ONCE;
+                float x[8];
+                if constexpr (F32) {
+                    const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w, raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
+                } else {
+                    const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[2 * j] = __uint_as_float(w[j] << 16);
+                        x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+                    }
+                }
+                float most = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+#pragma unroll
+                for (int o = PER / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+                float by, back;
+                af_row_scale(most, by, back);
+                if (a.scale < 0.f) by = -by;
+                if (u == 0) row_factor[q] = fmaxf(back * fabsf(a.scale) * AF_LOG2E, 0x1p-149f);
+                uint4 hi, lo;
+                uint32_t *const h = &hi.x, *const l = &lo.x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) af_split(x[2 * j] * by, x[2 * j + 1] * by, h[j], l[j]);
+                uint8_t* const to = smem + q / 128 * Sh::TILE + u / 8 * (128 * 128) + q % 128 * 128 + ((u % 8) ^ (q & 7)) * 16;
+                *reinterpret_cast<uint4*>(to) = hi;
+                if constexpr (F32) *reinterpret_cast<uint4*>(to + Sh::TILES * Sh::TILE) = lo;
+            }
+            at_fence_smem();
+            if constexpr (KEYS) asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");  // (the factors of rows that other warps have done)
+            else __syncwarp();
+            if (lane == 0) tc5_arrive(&q_full);
+            c = row_factor[row];
+        }
+        float m = -INFINITY, l = 0.f;
         for (int i = 0; i < mine; ++i) {
             const int kv = KEYS ? 2 * i + t : i, key0 = (b_begin + kv) * AT_KEYS, slot = kv % AT_RING;
             ok = __all_sync(0xFFFFFFFFu, tc5_wait(&s_full[t], (uint32_t)(i & 1)));
             if (!ok) break;
             at_after();
-            float s0[32], s1[32];
+            uint64_t s0[16], s1[16];  // 32 scores each, two a register pair
             at_ld32(S, s0);
+            const uint4 big = *reinterpret_cast<const uint4*>(largest_s[slot]);
+            const int power = at_power(max(max(big.x, big.y), max(big.z, big.w))) - (F32 ? 0 : AT_UP);
             const uint32_t gone = gone_s[slot];
-            const bool masked = gone != 0 || key0 < whole_from || key0 + AT_KEYS - 1 > whole_to;
-            const int hi = limit - key0, lo = low - key0;
-            // the power of two not below the largest finite scale of values that the block may see
-            uint32_t big = 0;
-            {
-                const float4 v = *reinterpret_cast<const float4*>(&v_scale[slot][4 * lane]);
-                const float f[4] = {v.x, v.y, v.z, v.w};
+            // scores times their scale go back to tensor memory; the largest
+            float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
+            auto scaled = [&](uint64_t (&s)[16], int k0) {
+                const ulonglong2* const f = reinterpret_cast<const ulonglong2*>(&k_scale[slot][k0]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int k = key0 + 4 * lane + j;
-                    if (f[j] > 0.f && f[j] < INFINITY && (!masked || (k >= k_begin && k < k_end))) big = max(big, __float_as_uint(f[j]));
+                for (int k = 0; k < 16; k += 2) {
+                    const ulonglong2 w = f[k / 2];
+                    s[k] = at_mul2(s[k], w.x);
+                    s[k + 1] = at_mul2(s[k + 1], w.y);
                 }
-                big = __reduce_max_sync(0xFFFFFFFFu, big);
-            }
-            const float up = (float)(min(max((int)((big + 0x7FFFFFu) >> 23), 27), 253) - 127);
-            // One job, with and without keys that a row does not see: both as code of its own, since decided at each value it is 6 instructions more.
-            auto job = [&](auto with_mask) {
-                constexpr bool MASK = decltype(with_mask)::value;
-                // bits of the keys k0 .. k0 + 31 that the row sees
-                auto seen = [&](int k0) {
-                    const int from = lo - k0, to = hi - k0;
-                    uint32_t bits = to >= 31 ? 0xFFFFFFFFu : to < 0 ? 0u : (2u << to) - 1u;
-                    bits = from <= 0 ? bits : from > 31 ? 0u : bits & (0xFFFFFFFFu << from);
-                    const uint32_t no = gone >> (k0 / KV_PAGE);
-                    return bits & ~((no & 1 ? 0xFFFFu : 0u) | (no & 2 ? 0xFFFF0000u : 0u));
-                };
-                // keys k0 .. k0 + 31: scores times their scale; what a row does not see is -inf
-                auto scaled = [&](float (&s)[32], int k0, uint32_t bits) {
+            };
+            auto largest = [&](const uint64_t (&s)[16]) {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(&k_scale[slot][k0 + k]);
-                        at_mul2(s[k], s[k + 1], f.x, f.y);
-                        at_mul2(s[k + 2], s[k + 3], f.z, f.w);
-                    }
-                    if constexpr (MASK) {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (!(bits >> k & 1)) s[k] = -INFINITY;
-                    }
-                };
-                float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
-                auto largest = [&](const float (&s)[32]) {
-#pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        b0 = at_max3(b0, s[k], s[k + 1]);
-                        b1 = at_max3(b1, s[k + 2], s[k + 3]);
-                        b2 = at_max3(b2, s[k + 4], s[k + 5]);
-                        b3 = at_max3(b3, s[k + 6], s[k + 7]);
-                    }
-                };
+                for (int k = 0; k < 16; k += 4) {
+                    b0 = at_max3(b0, s[k]);
+                    b1 = at_max3(b1, s[k + 1]);
+                    b2 = at_max3(b2, s[k + 2]);
+                    b3 = at_max3(b3, s[k + 3]);
+                }
+            };
+            if (gone == 0 && key0 >= whole_from && key0 + AT_KEYS - 1 <= whole_to) {
 #pragma unroll 1
                 for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {  // the next 32 are on their way while these are looked at
                     at_wait_for(s0);
                     at_ld32(S + k0 + 32, s1);
-                    scaled(s0, k0, MASK ? seen(k0) : 0u);
+                    scaled(s0, k0);
                     largest(s0);
-                    at_wait_for(s1);
-                    at_ld32(S + (k0 + 64) % AT_KEYS, s0);  // at the end: the first again
-                    scaled(s1, k0 + 32, MASK ? seen(k0 + 32) : 0u);
-                    largest(s1);
-                }
-                const float best = fmaxf(fmaxf(b0, b1), fmaxf(b2, b3));
-                // (nothing seen: best is -inf, which a factor of 0 would turn into NaN)
-                const float x = best == -INFINITY ? -INFINITY : fmaf(best, c, up);
-                const bool moves = x > m + AT_MOST;
-                if (__any_sync(0xFFFFFFFFu, moves)) {
-                    const float to = moves ? x - AT_SET : m, by = moves ? af_ex2(m - to) : 1.f;  // (m = -inf: 0)
-                    m = to;
-                    l0 *= by;
-                    l1 *= by;
-                    if (i > 0) {
-#pragma unroll 1
-                        for (int d = 0; d < dim; d += 16) {
-                            uint32_t o[16];
-                            tc5_ld16(O + d, o);
-                            at_wait_ld();
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
-                            at_st16(O + d, o);
-                        }
-                    }
-                }
-                const float base = m == -INFINITY ? 0.f : -m;
-                auto weights = [&](float (&s)[32], int k0) {
-                    uint32_t w_hi[16], w_lo[16];
-                    const uint32_t bits = MASK ? seen(k0) : 0u;
-                    scaled(s, k0, bits);
-#pragma unroll
-                    for (int k = 0; k < 32; k += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(&v_scale[slot][k0 + k]);
-                        const float v[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                        for (int j = 0; j < 4; j += 2) {
-                            float p0 = s[k + j], p1 = s[k + j + 1];
-                            at_fma2(p0, p1, c, base);
-                            p0 = af_ex2(p0);
-                            p1 = af_ex2(p1);
-                            if constexpr (MASK) {  // (-inf times a factor of 0 is NaN)
-                                if (!(bits >> (k + j) & 1)) p0 = 0.f;
-                                if (!(bits >> (k + j + 1) & 1)) p1 = 0.f;
-                            }
-                            at_add2(l0, l1, p0, p1);
-                            at_mul2(p0, p1, v[j], v[j + 1]);
-                            if constexpr (MASK) {  // (what is masked may have any scale)
-                                if (!(bits >> (k + j) & 1)) p0 = 0.f;
-                                if (!(bits >> (k + j + 1) & 1)) p1 = 0.f;
-                            }
-                            const int w = (k + j) / 2;
-                            if constexpr (F32) af_split(p0, p1, w_hi[w], w_lo[w]);
-                            else w_hi[w] = af_pack(p0, p1);
-                        }
-                    }
-                    if constexpr (F32) {  // over the scores that they come from
-                        at_st16(S + k0, w_hi);
-                        at_st16(S + k0 + 16, w_lo);
-                    } else {
-                        at_st16(S + k0 / 2, w_hi);
-                    }
-                };
-#pragma unroll 1
-                for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {
-                    at_wait_for(s0);
-                    at_ld32(S + k0 + 32, s1);
-                    weights(s0, k0);
+                    at_st32(S + k0, s0);
                     at_wait_for(s1);
                     if (k0 + 64 < AT_KEYS) at_ld32(S + k0 + 64, s0);
-                    weights(s1, k0 + 32);
+                    scaled(s1, k0 + 32);
+                    largest(s1);
+                    at_st32(S + k0 + 32, s1);
+                }
+            } else {
+                const int hi = limit - key0, lo = low - key0;
+#pragma unroll 1
+                for (int k0 = 0; k0 < AT_KEYS; k0 += 32) {
+                    if (k0 > 0) at_ld32(S + k0, s0);
+                    const int from = lo - k0, to = hi - k0;
+                    uint32_t bits = to >= 31 ? 0xFFFFFFFFu : to < 0 ? 0u : (2u << to) - 1u;  // of the keys that the row sees
+                    bits = from <= 0 ? bits : from > 31 ? 0u : bits & (0xFFFFFFFFu << from);
+                    const uint32_t no = gone >> (k0 / KV_PAGE);
+                    bits &= ~((no & 1 ? 0xFFFFu : 0u) | (no & 2 ? 0xFFFF0000u : 0u));
+                    at_wait_for(s0);
+                    scaled(s0, k0);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 f = at_two(s0[k]);
+                        s0[k] = at_pair(bits >> (2 * k) & 1 ? f.x : -INFINITY, bits >> (2 * k + 1) & 1 ? f.y : -INFINITY);
+                    }
+                    largest(s0);
+                    at_st32(S + k0, s0);
+                }
+            }
+            at_wait_st();
+            at_ld32(S, s0);
+            const float x = fmaf(fmaxf(fmaxf(b0, b1), fmaxf(b2, b3)), c, (float)power);
+            const bool moves = x > m + AT_MOST;
+            if (__any_sync(0xFFFFFFFFu, moves)) {
+                const float to = moves ? x - AT_SET : m, by = moves ? af_ex2(m - to) : 1.f;  // (m = -inf: 0)
+                m = to;
+                l *= by;
+                if (i > 0) {
+#pragma unroll 1
+                    for (int d = 0; d < dim; d += 16) {
+                        uint32_t o[16];
+                        tc5_ld16(O + d, o);
+                        at_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+                        at_st16(O + d, o);
+                    }
+                }
+            }
+            const float base = (m == -INFINITY ? 0.f : -m) + (F32 ? 0.f : (float)power);
+            const uint64_t c2 = at_pair(c, c), base2 = at_pair(base, base);
+            uint64_t sum0 = 0, sum1 = 0;
+            auto weights = [&](const uint64_t (&s)[16], int k0) {
+                uint32_t w_hi[16];
+                [[maybe_unused]] uint32_t w_lo[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    float2 p = at_two(at_fma2(s[k], c2, base2));
+                    p.x = af_ex2(p.x);
+                    p.y = af_ex2(p.y);
+                    const uint64_t pair = at_pair(p.x, p.y);
+                    if (k % 2) sum1 = at_add2(sum1, pair);
+                    else sum0 = at_add2(sum0, pair);
+                    if constexpr (F32) {
+                        const float2 w = at_two(at_mul2(pair, *reinterpret_cast<const uint64_t*>(&v_scale[slot][k0 + 2 * k])));
+                        af_split(w.x, w.y, w_hi[k], w_lo[k]);
+                    } else {
+                        w_hi[k] = af_pack(p.x, p.y);
+                    }
+                }
+                if constexpr (F32) {  // over the scores that they come from
+                    at_st16(S + k0, w_hi);
+                    at_st16(S + k0 + 16, w_lo);
+                } else {
+                    at_st16(S + k0 / 2, w_hi);
                 }
             };
-            if (masked) job(std::true_type{});
-            else job(std::false_type{});
+#pragma unroll 1
+            for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {
+                at_wait_for(s0);
+                at_ld32(S + k0 + 32, s1);
+                weights(s0, k0);
+                at_wait_for(s1);
+                if (k0 + 64 < AT_KEYS) at_ld32(S + k0 + 64, s0);
+                weights(s1, k0 + 32);
+            }
             at_wait_st();
             at_before();
             __syncwarp();
             if (lane == 0) tc5_arrive(&p_full[t]);
+            const float2 sum = at_two(at_add2(sum0, sum1));
+            l = fmaf(sum.x + sum.y, F32 ? 1.f : __uint_as_float((uint32_t)(127 - power) << 23), l);
         }
-        const float l = l0 + l1;
+        // what comes now takes the operands' place: the products have been made, or there are none and the queries have been written
         if (jobs > 0) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&o_full, 0));
+        else asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
         at_after();
         T* const out = static_cast<T*>(a.out) + (int64_t)head * group * dim;
         if (!KEYS && parts == 1) {
             const float by = l == 0.f || mine == 0 ? 0.f : 1.f / l;
-            T* const to = out + (int64_t)(tile.first + at / group) * a.ldo + (int64_t)(at % group) * dim;
+            // A warp's 32 rows through its part of shared memory (the operands have been read), so that stores write whole lines
+            constexpr int UNITS = DP * (int)sizeof(T) / 16, AT_ONCE = 32 / UNITS;  // pieces of a row, rows a store
+            uint8_t* const mem = smem + warp * (32 * DP * (int)sizeof(T));
 #pragma unroll 1
-            for (int d = 0; ok && d < dim; d += 32) {
-                float o[32];
-                at_ld32(O + d, o);
-                at_wait_for(o);
-                if (row < tile.n) {
-                    constexpr int PER = 16 / (int)sizeof(T);
-#pragma unroll
-                    for (int j = 0; j < 32; j += PER) {
-                        uint4 w;
-                        uint32_t* const u = &w.x;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            if constexpr (F32) u[q] = mine > 0 ? __float_as_uint(o[j + q] * by) : 0u;
-                            else u[q] = mine > 0 ? pack_bf16(o[j + 2 * q] * by, o[j + 2 * q + 1] * by) : 0u;
-                        }
-                        if (d + j < dim) *reinterpret_cast<uint4*>(to + d + j) = w;
-                    }
+            for (int d = 0; d < DP; d += 32) {
+                uint64_t o[16];
+                if (mine > 0 && ok) {
+                    at_ld32(O + d, o);
+                    at_wait_for(o);
                 }
+                const uint64_t by2 = at_pair(by, by);
+#pragma unroll
+                for (int j = 0; j < 16; j += 8 / (int)sizeof(T)) {
+                    uint4 w;
+                    uint32_t* const u = &w.x;
+#pragma unroll
+                    for (int q = 0; q < 4; q += F32 ? 2 : 1) {
+                        const float2 f = at_two(mine > 0 ? at_mul2(o[j + (F32 ? q / 2 : q)], by2) : 0);
+                        if constexpr (F32) {
+                            u[q] = __float_as_uint(f.x);
+                            u[q + 1] = __float_as_uint(f.y);
+                        } else {
+                            u[q] = pack_bf16(f.x, f.y);
+                        }
+                    }
+                    const int unit = (d + 2 * j) * (int)sizeof(T) / 16;
+                    *reinterpret_cast<uint4*>(mem + lane * (16 * UNITS) + ((unit & ~7) | ((unit ^ lane) & 7)) * 16) = w;
+                }
+            }
+            __syncwarp();
+            const int row_w = (KEYS ? 0 : 128 * t) + 32 * (warp & 3), unit = lane % UNITS;
+#pragma unroll 1
+            for (int q0 = 0; ok && q0 < 32; q0 += AT_ONCE) {
+                const int q = q0 + lane / UNITS, where = tile.row0 + row_w + q;
+                const uint4 w = *reinterpret_cast<const uint4*>(mem + q * (16 * UNITS) + ((unit & ~7) | ((unit ^ q) & 7)) * 16);
+                if (row_w + q < tile.n && unit * 16 < dim * (int)sizeof(T))
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + (int64_t)(tile.first + where / group) * a.ldo + (int64_t)(where % group) * dim) + unit * 16) = w;
             }
         } else {
             float* const sums = reinterpret_cast<float*>(smem);  // [group][row][LDO], over the operands, which have been read
             float* const weights = sums + Sh::SUMS / 4;          // [row of the block's share][sum]
 #pragma unroll 1
             for (int d = 0; d < dim; d += 32) {
-                float o[32];
+                uint64_t o[16];
                 if (mine > 0 && ok) {
                     at_ld32(O + d, o);
                     at_wait_for(o);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = 0.f;
+                    for (int j = 0; j < 16; ++j) o[j] = 0;
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    if (d + j < dim) *reinterpret_cast<float4*>(&sums[(128 * t + r) * Sh::LDO + d + j]) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                for (int j = 0; j < 16; j += 2)
+                    if (d + 2 * j < dim) *reinterpret_cast<ulonglong2*>(&sums[(128 * t + r) * Sh::LDO + d + 2 * j]) = make_ulonglong2(o[j], o[j + 1]);
             }
             part_m[t][r] = m;
             part_l[t][r] = l;
@@ -615,7 +713,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     if (!ok) report_wait(a.waits, WAIT_ATTENTION);
     at_before();
     __syncthreads();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
 }
 
 template <typename T, int DP, bool KEYS>

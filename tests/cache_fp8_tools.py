@@ -76,13 +76,15 @@ def attention64(c, q, seqs, scale, window=0):
                 out[at: at + r, h] = y
                 # Scores: q rounded to 22 bits (bf16: exact), dim / 16 additions of the tensor cores (a plane), which cut off up to 2^-23 of the
                 # terms' sum each, and four roundings in f32 of z, its scale and its distance to m (in units of log 2: 1.45 |z| 2^-24 each).
-                # Weights: that, ex2's 2^-22, two roundings, and their own to 22 bits (f32) or 11. Sums: an addition for 16 keys and a plane,
-                # the accumulators' and the parts' factors (2^-22 each, of which 64 at most). All relative to sums of absolute values.
+                # Weights: that, ex2's 2^-22 and two roundings. Sums: an addition for 16 keys and a plane, the accumulators' and the parts' factors (2^-22
+                # each, of which 64 at most). All of it in numerator and denominator, hence twice; relative to sums of absolute values. In the
+                # numerator alone: f32: weights as fp16 + fp16 of the remainder (2^-22). bf16: fp16 of the weight, of the value's
+                # factor and of their product with the value, which is exact before: half a step of fp16 is 2^-11 of the value, so (1 + 2^-11)^3 - 1.
                 planes = 2 if f32 else 1
                 size = (x.abs() @ k[:, h // group].nan_to_num().abs().T * scale).masked_fill(~seen, 0).amax(-1, keepdim=True)
                 dz = size * (2.0**-22 * f32 + planes * dim / 16 * 2.0**-23 + 6 * 2.0**-23) + 2.0**-21
-                w = dz + (2.0**-22 if f32 else 2.0**-12) + planes * (held / 16 + 2) * 2.0**-23 + 64 * 2.0**-22
-                far[at: at + r, h] = 2 * w * (p @ u.abs()) + (2 * STEP[ops.F32] if f32 else 1.01 * STEP[ops.BF16]) * y.abs() + 2.0**-100
+                w = 2 * (dz + planes * (held / 16 + 2) * 2.0**-23 + 64 * 2.0**-22) + (2.0**-22 if f32 else (1 + 2.0**-11) ** 3 - 1)
+                far[at: at + r, h] = w * (p @ u.abs()) + (2 * STEP[ops.F32] if f32 else 1.01 * STEP[ops.BF16]) * y.abs() + 2.0**-100
         at += r
     return out, far
 
