@@ -2,11 +2,10 @@
 //
 // A block has two groups of four warps, each with 128 rows whose scores S = Q K^T [128 x 128 keys] and sums O [128 x head_dim] lie in
 // tensor memory, a row a lane. While one group turns scores into weights, the tensor cores work for the other:
-//   warps 0-3, 4-7   weights: a thread has a row; S is read twice, for its maximum and for the exponentials, which go back over it as fp16
+//   warps 0-3, 4-7   weights: a thread has a row of S in registers; its maximum, exponentials, which go back over S as fp16, half a tile at a time,
 //                    and are the first operand of the second product from there. O is rescaled only when a row's reference moves.
-//   warps 8-11       keys: e4m3 rows to fp16 in shared memory (128-byte swizzle, K-major), and the scales of keys and values
-//   warps 12-15      values, as they lie (MN-major)
-//   warp 16          issues the products
+//   warps 8-11       keys and values: e4m3 rows to fp16 in shared memory (128-byte swizzle; keys K-major, values as they lie: MN-major)
+//   warp 12          issues the products
 // ROWS: the groups have 128 rows each of 256, and keys in common. KEYS (up to 128 rows): the same rows, key tiles by turns; their sums
 // are added up at the end. Keys may be shared out to the blocks of a cluster as well, which add up through shared memory.
 //
@@ -26,7 +25,7 @@ namespace sp {
 
 cudaError_t count_launch_and_check();  // kernels.cu
 
-constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 640, AT_RING = 4, AT_MAX_PARTS = 8;
+constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 512, AT_RING = 4, AT_MAX_PARTS = 8;
 constexpr float AT_MOST = 15.f, AT_SET = 9.f;  // log2 of the largest weight, and of it when M is set
 constexpr int AT_UP = 7, AT_LEAST = -80;       // values times 2^7 are below 2^16; smaller u would let a sum of 2^(z - M) pass 2^127
 
@@ -44,6 +43,15 @@ struct AtShape {
 
 // log2 of the power of two not below a scale, given by its bits (positive and finite, or 0).
 __device__ __forceinline__ int at_power(uint32_t bits) { return max((int)((bits + 0x7FFFFFu) >> 23) - 127, AT_LEAST); }
+
+// tc5_wait for warps that are ahead of the others: it looks now and then, so that the others have the issue slots.
+__device__ __forceinline__ bool at_wait_idle(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < 64; ++i) {
+        if (tc5_peek(bar, parity)) return true;
+        __nanosleep(100);
+    }
+    return tc5_wait(bar, parity);
+}
 
 __device__ __forceinline__ void at_init(uint64_t* bar, uint32_t arrivals) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(tc5_smem_u32(bar)), "r"(arrivals) : "memory");
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     constexpr bool F32 = Sh::F32;
     constexpr int STAGES = Sh::STAGES, ROWS = 128 * Sh::TILES;
     extern __shared__ uint8_t at_smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], o_full, q_full;
+    __shared__ __align__(8) uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2][2], o_full, q_full;
     __shared__ __align__(16) float k_scale[AT_RING][AT_KEYS], v_scale[AT_RING][F32 ? AT_KEYS : 4];
     __shared__ uint32_t gone_s[AT_RING];  // pages of the tile that are not there
     __shared__ __align__(16) uint32_t largest_s[AT_RING][4];  // scales of values, of 32 tokens each
@@ -192,14 +200,25 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     uint8_t *const ks_ = smem + Sh::Q, *const vs_ = ks_ + STAGES * Sh::TILE;
     // ── the block's keys ──
     const int last_row = tile.row0 + tile.n - 1;
-    const int pos_first = tile.len - tile.rows + tile.row0 / group, pos_last = tile.len - tile.rows + last_row / group;
+    // Token and head of the block's row q: with rem = row0 % group, (rem + q) / group by a reciprocal is exact, since (rem + q + 1/2) / group is at
+    // least 1 / (2 group) from a whole number and rem + q < 2^21
+    const int tok_base = tile.row0 / group, rem = tile.row0 - tok_base * group;
+    const float per_group = 1.f / (float)group;
+    auto token_of = [&](int q) { return (int)(((float)(rem + q) + 0.5f) * per_group); };
+    const int64_t q_first = (int64_t)(tile.first + tok_base);
+    // offset of row q's head in a matrix of row stride ld
+    auto offset_of = [&](int q, int64_t ld) {
+        const int tok = token_of(q);
+        return (q_first + tok) * ld + (int64_t)(head * group + rem + q - tok * group) * dim;
+    };
+    const int pos_first = tile.len - tile.rows + tok_base, pos_last = tile.len - tile.rows + last_row / group;
     const int held = (int)min((int64_t)tile.len, (int64_t)a.c.max_pages * KV_PAGE);
     const int k_end = min(pos_last + 1, held), k_begin = a.window > 0 ? max(0, pos_first - a.window + 1) : 0;
     const int t_begin = k_begin / AT_KEYS, t_end = k_end > k_begin ? (k_end + AT_KEYS - 1) / AT_KEYS : t_begin;
     const int per = (t_end - t_begin + parts - 1) / parts;
     const int b_begin = min(t_end, t_begin + part * per), n_kv = min(t_end, b_begin + per) - b_begin;  // key tiles of the block
     const int groups = KEYS || tile.n > 128 ? 2 : 1, jobs = KEYS ? n_kv : groups * n_kv;  // job j is group j % groups'
-    if (warp == 16) {
+    if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(tc5_smem_u32(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
@@ -212,7 +231,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         }
         for (int i = 0; i < 2; ++i) {
             at_init(&s_full[i], 1);
-            at_init(&p_full[i], 4);
+            at_init(&p_full[i][0], 4);
+            at_init(&p_full[i][1], 4);
         }
         at_init(&o_full, 1);
         at_init(&q_full, 8);
@@ -223,9 +243,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     at_after();
     const uint32_t tmem = tmem_slot;  // S of the groups at columns 0 and 128, O at 256 and 256 + DP
     bool ok = true;
-    if (warp >= 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");  // 128 x 48 + 256 x 80 + 256 x 136 = 640 x 96
-        if (warp == 16) {
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");  // 128 x 56 + 128 x 104 + 256 x 176 = 512 x 128
+        if (warp == 12) {
         const bool leader = tc5_elect();
         const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
         const uint32_t id_s = at_idesc(AT_KEYS, false), id_o = at_idesc(dim, true);
@@ -253,22 +273,26 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         for (int j = 0; j < groups && j < jobs && ok; ++j) scores(j);
         for (int j = 0; j < jobs && ok; ++j) {
             const int t = groups == 2 ? j & 1 : 0, i = groups == 2 ? j >> 1 : j, kv = KEYS ? j : i, st = kv % STAGES;
-            bool here = tc5_wait(&p_full[t], (uint32_t)(i & 1));
-            if (KEYS || t == 0) here = here && tc5_wait(&v_full[st], (uint32_t)((kv / STAGES) & 1));
-            ok = __all_sync(0xFFFFFFFFu, here);
-            if (!ok) break;
-            at_after();
-            if (leader) {
-                const uint64_t v = vd + (uint64_t)(st * (Sh::TILE >> 4));
+            if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&v_full[st], (uint32_t)((kv / STAGES) & 1)));
+#pragma unroll 1
+            for (int half = 0; half < 2 && ok; ++half) {
+                ok = __all_sync(0xFFFFFFFFu, tc5_wait(&p_full[t][half], (uint32_t)(i & 1)));
+                if (!ok) break;
+                at_after();
+                if (leader) {
+                    const uint64_t v = vd + (uint64_t)(st * (Sh::TILE >> 4) + half * (4 * 2048 >> 4));
+                    const uint32_t w = tm + 128u * t + (F32 ? 64u : 32u) * half;
 #pragma unroll
-                for (int s = 0; s < AT_KEYS / 16; ++s)
+                    for (int s = 0; s < 4; ++s)
 #pragma unroll
-                    for (int p = Sh::PLANES - 1; p >= 0; --p)
-                        at_mma_tmem(tm + 256u + (uint32_t)(DP * t), tm + 128u * t + (uint32_t)(F32 ? 32 * (s / 2) + 16 * p + 8 * (s % 2) : 8 * s), v + (uint64_t)(s * (2048 >> 4)), id_o,
-                                    i > 0 || s > 0 || p != Sh::PLANES - 1);
-                if (KEYS || t == groups - 1) tc5_commit(&v_empty[st]);
+                        for (int p = Sh::PLANES - 1; p >= 0; --p)
+                            at_mma_tmem(tm + 256u + (uint32_t)(DP * t), w + (uint32_t)(F32 ? 32 * (s / 2) + 16 * p + 8 * (s % 2) : 8 * s), v + (uint64_t)(s * (2048 >> 4)), id_o,
+                                        i > 0 || half > 0 || s > 0 || p != Sh::PLANES - 1);
+                    if (half == 1 && (KEYS || t == groups - 1)) tc5_commit(&v_empty[st]);
+                }
+                __syncwarp();
             }
-            __syncwarp();
+            if (!ok) break;
             if (j + groups < jobs) scores(j + groups);
         }
         if (jobs > 0) {
@@ -287,82 +311,55 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             cluster_sync();
         }
     } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
         // Sixteen bytes of a row a copy, 64 coordinates of eight tokens a warp at once: stores of eight threads fall on 32 different banks.
-        const bool values = warp >= 12;
         constexpr int HALVES = DP / 64, N = 4 * HALVES;  // copies of a thread: tokens tok0 + 32 i, coordinates 16 ch and 64 + 16 ch
-        const int p = tid - (values ? 384 : 256), ch = p % 4, tok0 = p / 4;
+        const int p = tid - 256, ch = p % 4, tok0 = p / 4;
         const int32_t* const table = a.c.page_table + (int64_t)max(0, min(tile.slot, a.c.n_slots - 1)) * a.c.max_pages;
         auto page_of = [&](int kv) {  // lanes 0 to 7: the tile's pages
             const int index = (b_begin + kv) * AT_PAGES + (lane & 7);
             const int page = kv < n_kv && index < a.c.max_pages && index * KV_PAGE < k_end ? table[index] : -1;
             return page < a.c.n_pages ? max(page, -1) : -1;
         };
-        const int64_t page_rows = (int64_t)2 * a.c.n_kv * KV_PAGE;
-        const uint8_t* const from = a.c.values + (a.c.row(0, values ? 1 : 0, head) + tok0 % KV_PAGE) * dim + 16 * ch;
-        const float* const v_scales = a.c.scales + a.c.row(0, 1, head);
-        uint4 raw[N];
-        float own[4];       // scales of the thread's tokens (values)
-        float4 four;        // of tokens 4 lane .. 4 lane + 3 (values); of token p: key's, value's (keys)
+        const int page_rows = 2 * a.c.n_kv * KV_PAGE, page_bytes = page_rows * dim, to_values = a.c.n_kv * KV_PAGE;
+        const uint8_t* const k_from = a.c.values + ((int64_t)head * KV_PAGE + tok0 % KV_PAGE) * dim + 16 * ch;
+        const uint8_t* const v_from = k_from + (int64_t)to_values * dim;
+        const float* const s_from = a.c.scales + head * KV_PAGE;
+        uint4 raw_k[N], raw_v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) raw_k[i] = raw_v[i] = make_uint4(0, 0, 0, 0);
+        float own[4] = {};                           // scales of the thread's tokens' values
+        float4 four = make_float4(0.f, 0.f, 0.f, 0.f);  // of tokens 4 lane .. 4 lane + 3
+        float sk = 0.f, sv = 0.f;                       // of token p
         // A value's scale as it counts: none of what no row of the block sees, nor of what is NaN or infinite
         auto counts = [&](float s, int token) { return s > 0.f && s < INFINITY && token >= k_begin && token < k_end; };
-        auto load = [&](int kv, int pages) {
+        // (of a page that is not there the first one's rows are taken: nobody sees them)
+        auto load = [&](uint4 (&raw)[N], const uint8_t* from, int pages) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int page = __shfl_sync(0xFFFFFFFFu, pages, tok0 / KV_PAGE + 2 * i);
-                const int64_t rows = (int64_t)max(page, 0) * page_rows;
-                const uint8_t* const row = from + rows * dim;
+                const uint8_t* const row = from + (int64_t)max(__shfl_sync(0xFFFFFFFFu, pages, tok0 / KV_PAGE + 2 * i), 0) * page_bytes;
 #pragma unroll
-                for (int h = 0; h < HALVES; ++h) {
-                    raw[HALVES * i + h] = make_uint4(0, 0, 0, 0);
-                    if (page >= 0 && 64 * h + 16 * ch < dim) raw[HALVES * i + h] = __ldg(reinterpret_cast<const uint4*>(row + 64 * h));
-                }
-                if (!F32 && values) own[i] = page >= 0 ? __ldg(v_scales + rows + tok0 % KV_PAGE) : 0.f;
+                for (int h = 0; h < HALVES; ++h)
+                    if (64 * h + 16 * ch < dim) raw[HALVES * i + h] = __ldg(reinterpret_cast<const uint4*>(row + 64 * h));
             }
-            four = make_float4(0.f, 0.f, 0.f, 0.f);
-            const int page = __shfl_sync(0xFFFFFFFFu, pages, values ? lane / 4 : p / KV_PAGE);
-            if (page >= 0) {
-                const float* const at = v_scales + (int64_t)page * page_rows;
-                if (!values) {
-                    four.x = __ldg(at + p % KV_PAGE - (int64_t)a.c.n_kv * KV_PAGE);
-                    four.y = __ldg(at + p % KV_PAGE);
-                } else if (!F32) {
-                    four = __ldg(reinterpret_cast<const float4*>(at + 4 * lane % KV_PAGE));
+        };
+        auto load_scales = [&](int pages) {
+            const int mine = __shfl_sync(0xFFFFFFFFu, pages, p / KV_PAGE);
+            const float* const at = s_from + (int64_t)max(mine, 0) * page_rows + p % KV_PAGE;
+            sk = __ldg(at);
+            sv = mine >= 0 ? __ldg(at + to_values) : 0.f;
+            if constexpr (!F32) {
+                const int page = __shfl_sync(0xFFFFFFFFu, pages, lane / 4);
+                four = page >= 0 ? __ldg(reinterpret_cast<const float4*>(s_from + (int64_t)page * page_rows + to_values + 4 * lane % KV_PAGE)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int of = __shfl_sync(0xFFFFFFFFu, pages, tok0 / KV_PAGE + 2 * i);
+                    own[i] = of >= 0 ? __ldg(s_from + (int64_t)of * page_rows + to_values + tok0 % KV_PAGE) : 0.f;
                 }
             }
         };
-        uint8_t* const to0 = (values ? vs_ : ks_) + tok0 * 128;
         const int u0 = ((2 * ch) ^ (tok0 & 7)) * 16, u1 = ((2 * ch + 1) ^ (tok0 & 7)) * 16;
-        uint64_t *const full = values ? v_full : k_full, *const empty = values ? v_empty : k_empty;
-        int pages = page_of(0);
-        load(0, pages);
-        for (int kv = 0; kv < n_kv; ++kv) {
-            const int st = kv % STAGES, use = kv / STAGES, slot = kv % AT_RING, key0 = (b_begin + kv) * AT_KEYS;
-            const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
-            const int next = page_of(kv + 1);
-            uint32_t by[4] = {};  // what values are multiplied by, as pairs of fp16
-            float sk = 0.f, sv = 0.f;
-            uint32_t big;
-            if (values) {
-                if constexpr (!F32) {
-                    const int k = key0 + 4 * lane;
-                    big = max(max(counts(four.x, k) ? __float_as_uint(four.x) : 0u, counts(four.y, k + 1) ? __float_as_uint(four.y) : 0u),
-                              max(counts(four.z, k + 2) ? __float_as_uint(four.z) : 0u, counts(four.w, k + 3) ? __float_as_uint(four.w) : 0u));
-                    const float lift = __uint_as_float((uint32_t)(127 + AT_UP - at_power(__reduce_max_sync(0xFFFFFFFFu, big))) << 23);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float f = counts(own[i], key0 + tok0 + 32 * i) ? own[i] * lift : 0.f;
-                        by[i] = af_pack(f, f);
-                    }
-                }
-            } else {
-                sv = counts(four.y, key0 + p) ? four.y : 0.f;
-                sk = four.y < INFINITY && four.y > -INFINITY ? four.x : __uint_as_float(0x7FC00000u);
-                big = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(sv));
-            }
-            if (use > 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&empty[st], (uint32_t)((use - 1) & 1)));
-            if (!ok) break;
-            uint8_t* const to = to0 + st * Sh::TILE;
+        auto store = [&](const uint4 (&raw)[N], uint8_t* to, const uint32_t (&by)[4], bool values) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 uint32_t h[8];
@@ -377,35 +374,71 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                         if constexpr (!F32) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(by[i / HALVES]));
                     }
                 }
-                uint8_t* const row = to + i / HALVES * (32 * 128) + i % HALVES * (128 * 128);
+                uint8_t* const row = to + tok0 * 128 + i / HALVES * (32 * 128) + i % HALVES * (128 * 128);
                 *reinterpret_cast<uint4*>(row + u0) = make_uint4(h[0], h[1], h[2], h[3]);
                 *reinterpret_cast<uint4*>(row + u1) = make_uint4(h[4], h[5], h[6], h[7]);
             }
-            if (!values) {
-                k_scale[slot][p] = sk;
-                if constexpr (F32) v_scale[slot][p] = sv;
+        };
+        auto hand_over = [&](uint64_t* bar) {
+            at_fence_smem();
+            __syncwarp();
+            if (lane == 0) tc5_arrive(bar);
+        };
+        int pages = page_of(0);
+        load(raw_k, k_from, pages);
+        load_scales(pages);
+        load(raw_v, v_from, pages);
+        for (int kv = 0; kv < n_kv; ++kv) {
+            const int st = kv % STAGES, use = kv / STAGES, slot = kv % AT_RING, key0 = (b_begin + kv) * AT_KEYS;
+            const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
+            pages = page_of(kv + 1);
+            uint32_t by[4] = {};  // what values are multiplied by, as pairs of fp16
+            if constexpr (!F32) {
+                const int k = key0 + 4 * lane;
+                const uint32_t big = max(max(counts(four.x, k) ? __float_as_uint(four.x) : 0u, counts(four.y, k + 1) ? __float_as_uint(four.y) : 0u),
+                                         max(counts(four.z, k + 2) ? __float_as_uint(four.z) : 0u, counts(four.w, k + 3) ? __float_as_uint(four.w) : 0u));
+                const float lift = __uint_as_float((uint32_t)(127 + AT_UP - at_power(__reduce_max_sync(0xFFFFFFFFu, big))) << 23);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float f = counts(own[i], key0 + tok0 + 32 * i) ? own[i] * lift : 0.f;
+                    by[i] = af_pack(f, f);
+                }
+            }
+            if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&k_empty[st], (uint32_t)((use - 1) & 1)));
+            if (!ok) break;
+            store(raw_k, ks_ + st * Sh::TILE, by, false);
+            {
+                const float v = counts(sv, key0 + p) ? sv : 0.f;
+                k_scale[slot][p] = sv < INFINITY && sv > -INFINITY ? sk : __uint_as_float(0x7FC00000u);
+                if constexpr (F32) v_scale[slot][p] = v;
+                const uint32_t big = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v));
                 if (lane == 0) largest_s[slot][warp - 8] = big;
                 if (p == 0) gone_s[slot] = gone;
             }
-            at_fence_smem();
-            __syncwarp();
-            if (lane == 0) tc5_arrive(&full[st]);
-            pages = next;
-            if (kv + 1 < n_kv) load(kv + 1, pages);
+            hand_over(&k_full[st]);
+            if (kv + 1 < n_kv) {
+                load(raw_k, k_from, pages);
+                load_scales(pages);
+            }
+            if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&v_empty[st], (uint32_t)((use - 1) & 1)));
+            if (!ok) break;
+            store(raw_v, vs_ + st * Sh::TILE, by, true);
+            hand_over(&v_full[st]);
+            if (kv + 1 < n_kv) load(raw_v, v_from, pages);
         }
         if (parts > 1) {
             cluster_sync();
             cluster_sync();
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;\n");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");
         const int t = warp >> 2, r = 32 * (warp & 3) + lane, row = (KEYS ? 0 : 128 * t) + r;  // of the block's rows
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), S = lanes + 128u * t, O = lanes + 256u + (uint32_t)(DP * t);
-        const int at = tile.row0 + row, pos = tile.len - tile.rows + at / group;
+        const int pos = pos_first + token_of(row);
         const int limit = row < tile.n ? min(pos, held - 1) : -1, low = a.window > 0 ? pos - a.window + 1 : 0;
         // keys that all rows of the group see
         const int row_a = KEYS ? 0 : 128 * t, row_b = min(row_a + 127, tile.n - 1);
-        const int whole_to = min(tile.len - tile.rows + (tile.row0 + row_a) / group, held - 1), whole_from = a.window > 0 ? tile.len - tile.rows + (tile.row0 + row_b) / group - a.window + 1 : 0;
+        const int whole_to = min(pos_first + token_of(row_a), held - 1), whole_from = a.window > 0 ? pos_first + token_of(row_b) - a.window + 1 : 0;
         const int mine = t >= groups ? 0 : (jobs - t + groups - 1) / groups;  // jobs of the group
         // ── queries: fp16 operands, eight values a thread and row ──
         float c;  // scale log2(e) / what the row is multiplied by; never 0, since scores of -inf are multiplied by it
@@ -417,12 +450,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             uint4 raw[COUNT][F32 ? 2 : 1];
 #pragma unroll
             for (int i = 0; i < COUNT; ++i) {
-                const int q = first + i * AT_ONCE, where = tile.row0 + q;
+                const int q = first + i * AT_ONCE;
 #pragma unroll
                 for (int e = 0; e < (F32 ? 2 : 1); ++e) {
                     raw[i][e] = make_uint4(0, 0, 0, 0);
                     if (q < tile.n && 8 * u < dim)
-                        raw[i][e] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(tile.first + where / group) * a.ldq + (int64_t)(head * group + where % group) * dim + 8 * u)[e];
+                        raw[i][e] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + offset_of(q, a.ldq) + 8 * u)[e];
                 }
             }
 #pragma unroll
@@ -470,68 +503,51 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             ok = __all_sync(0xFFFFFFFFu, tc5_wait(&s_full[t], (uint32_t)(i & 1)));
             if (!ok) break;
             at_after();
-            uint64_t s0[16], s1[16];  // 32 scores each, two a register pair
-            at_ld32(S, s0);
+            uint64_t s[4][16];  // 32 scores each, two a register pair
+#pragma unroll
+            for (int q = 0; q < 4; ++q) at_ld32(S + 32 * q, s[q]);
             const uint4 big = *reinterpret_cast<const uint4*>(largest_s[slot]);
             const int power = at_power(max(max(big.x, big.y), max(big.z, big.w))) - (F32 ? 0 : AT_UP);
             const uint32_t gone = gone_s[slot];
-            // scores times their scale go back to tensor memory; the largest
+            const bool masked = gone != 0 || key0 < whole_from || key0 + AT_KEYS - 1 > whole_to;
             float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
-            auto scaled = [&](uint64_t (&s)[16], int k0) {
-                const ulonglong2* const f = reinterpret_cast<const ulonglong2*>(&k_scale[slot][k0]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                at_wait_for(s[q]);
+                const ulonglong2* const f = reinterpret_cast<const ulonglong2*>(&k_scale[slot][32 * q]);
 #pragma unroll
                 for (int k = 0; k < 16; k += 2) {
                     const ulonglong2 w = f[k / 2];
-                    s[k] = at_mul2(s[k], w.x);
-                    s[k + 1] = at_mul2(s[k + 1], w.y);
-                }
-            };
-            auto largest = [&](const uint64_t (&s)[16]) {
-#pragma unroll
-                for (int k = 0; k < 16; k += 4) {
-                    b0 = at_max3(b0, s[k]);
-                    b1 = at_max3(b1, s[k + 1]);
-                    b2 = at_max3(b2, s[k + 2]);
-                    b3 = at_max3(b3, s[k + 3]);
-                }
-            };
-            if (gone == 0 && key0 >= whole_from && key0 + AT_KEYS - 1 <= whole_to) {
-#pragma unroll 1
-                for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {  // the next 32 are on their way while these are looked at
-                    at_wait_for(s0);
-                    at_ld32(S + k0 + 32, s1);
-                    scaled(s0, k0);
-                    largest(s0);
-                    at_st32(S + k0, s0);
-                    at_wait_for(s1);
-                    if (k0 + 64 < AT_KEYS) at_ld32(S + k0 + 64, s0);
-                    scaled(s1, k0 + 32);
-                    largest(s1);
-                    at_st32(S + k0 + 32, s1);
-                }
-            } else {
-                const int hi = limit - key0, lo = low - key0;
-#pragma unroll 1
-                for (int k0 = 0; k0 < AT_KEYS; k0 += 32) {
-                    if (k0 > 0) at_ld32(S + k0, s0);
-                    const int from = lo - k0, to = hi - k0;
-                    uint32_t bits = to >= 31 ? 0xFFFFFFFFu : to < 0 ? 0u : (2u << to) - 1u;  // of the keys that the row sees
-                    bits = from <= 0 ? bits : from > 31 ? 0u : bits & (0xFFFFFFFFu << from);
-                    const uint32_t no = gone >> (k0 / KV_PAGE);
-                    bits &= ~((no & 1 ? 0xFFFFu : 0u) | (no & 2 ? 0xFFFF0000u : 0u));
-                    at_wait_for(s0);
-                    scaled(s0, k0);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 f = at_two(s0[k]);
-                        s0[k] = at_pair(bits >> (2 * k) & 1 ? f.x : -INFINITY, bits >> (2 * k + 1) & 1 ? f.y : -INFINITY);
-                    }
-                    largest(s0);
-                    at_st32(S + k0, s0);
+                    s[q][k] = at_mul2(s[q][k], w.x);
+                    s[q][k + 1] = at_mul2(s[q][k + 1], w.y);
                 }
             }
-            at_wait_st();
-            at_ld32(S, s0);
+            if (masked) {  // (a branch around it: selected at each value it would be three instructions more for every tile)
+                const int hi = limit - key0, lo = low - key0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int from = lo - 32 * q, to = hi - 32 * q;
+                    uint32_t bits = to >= 31 ? 0xFFFFFFFFu : to < 0 ? 0u : (2u << to) - 1u;  // of the keys that the row sees
+                    bits = from <= 0 ? bits : from > 31 ? 0u : bits & (0xFFFFFFFFu << from);
+                    const uint32_t no = gone >> (2 * q);
+                    bits &= ~((no & 1 ? 0xFFFFu : 0u) | (no & 2 ? 0xFFFF0000u : 0u));
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 f = at_two(s[q][k]);
+                        s[q][k] = at_pair(bits >> (2 * k) & 1 ? f.x : -INFINITY, bits >> (2 * k + 1) & 1 ? f.y : -INFINITY);
+                    }
+                    asm volatile("" ::: "memory");
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    b0 = at_max3(b0, s[q][k]);
+                    b1 = at_max3(b1, s[q][k + 1]);
+                    b2 = at_max3(b2, s[q][k + 2]);
+                    b3 = at_max3(b3, s[q][k + 3]);
+                }
             const float x = fmaf(fmaxf(fmaxf(b0, b1), fmaxf(b2, b3)), c, (float)power);
             const bool moves = x > m + AT_MOST;
             if (__any_sync(0xFFFFFFFFu, moves)) {
@@ -553,44 +569,38 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             const float base = (m == -INFINITY ? 0.f : -m) + (F32 ? 0.f : (float)power);
             const uint64_t c2 = at_pair(c, c), base2 = at_pair(base, base);
             uint64_t sum0 = 0, sum1 = 0;
-            auto weights = [&](const uint64_t (&s)[16], int k0) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
                 uint32_t w_hi[16];
                 [[maybe_unused]] uint32_t w_lo[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    float2 p = at_two(at_fma2(s[k], c2, base2));
+                    float2 p = at_two(at_fma2(s[q][k], c2, base2));
                     p.x = af_ex2(p.x);
                     p.y = af_ex2(p.y);
                     const uint64_t pair = at_pair(p.x, p.y);
                     if (k % 2) sum1 = at_add2(sum1, pair);
                     else sum0 = at_add2(sum0, pair);
                     if constexpr (F32) {
-                        const float2 w = at_two(at_mul2(pair, *reinterpret_cast<const uint64_t*>(&v_scale[slot][k0 + 2 * k])));
+                        const float2 w = at_two(at_mul2(pair, *reinterpret_cast<const uint64_t*>(&v_scale[slot][32 * q + 2 * k])));
                         af_split(w.x, w.y, w_hi[k], w_lo[k]);
                     } else {
                         w_hi[k] = af_pack(p.x, p.y);
                     }
                 }
-                if constexpr (F32) {  // over the scores that they come from
-                    at_st16(S + k0, w_hi);
-                    at_st16(S + k0 + 16, w_lo);
+                if constexpr (F32) {
+                    at_st16(S + 32 * q, w_hi);
+                    at_st16(S + 32 * q + 16, w_lo);
                 } else {
-                    at_st16(S + k0 / 2, w_hi);
+                    at_st16(S + 16 * q, w_hi);
                 }
-            };
-#pragma unroll 1
-            for (int k0 = 0; k0 < AT_KEYS; k0 += 64) {
-                at_wait_for(s0);
-                at_ld32(S + k0 + 32, s1);
-                weights(s0, k0);
-                at_wait_for(s1);
-                if (k0 + 64 < AT_KEYS) at_ld32(S + k0 + 64, s0);
-                weights(s1, k0 + 32);
+                if (q % 2) {
+                    at_wait_st();
+                    at_before();
+                    __syncwarp();
+                    if (lane == 0) tc5_arrive(&p_full[t][q / 2]);
+                }
             }
-            at_wait_st();
-            at_before();
-            __syncwarp();
-            if (lane == 0) tc5_arrive(&p_full[t]);
             const float2 sum = at_two(at_add2(sum0, sum1));
             l = fmaf(sum.x + sum.y, F32 ? 1.f : __uint_as_float((uint32_t)(127 - power) << 23), l);
         }
@@ -598,7 +608,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         if (jobs > 0) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&o_full, 0));
         else asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
         at_after();
-        T* const out = static_cast<T*>(a.out) + (int64_t)head * group * dim;
+        T* const out = static_cast<T*>(a.out);
         if (!KEYS && parts == 1) {
             const float by = l == 0.f || mine == 0 ? 0.f : 1.f / l;
             // A warp's 32 rows through its part of shared memory (the operands have been read), so that stores write whole lines
@@ -634,10 +644,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             const int row_w = (KEYS ? 0 : 128 * t) + 32 * (warp & 3), unit = lane % UNITS;
 #pragma unroll 1
             for (int q0 = 0; ok && q0 < 32; q0 += AT_ONCE) {
-                const int q = q0 + lane / UNITS, where = tile.row0 + row_w + q;
+                const int q = q0 + lane / UNITS;
                 const uint4 w = *reinterpret_cast<const uint4*>(mem + q * (16 * UNITS) + ((unit & ~7) | ((unit ^ q) & 7)) * 16);
                 if (row_w + q < tile.n && unit * 16 < dim * (int)sizeof(T))
-                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + (int64_t)(tile.first + where / group) * a.ldo + (int64_t)(where % group) * dim) + unit * 16) = w;
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + offset_of(row_w + q, a.ldo)) + unit * 16) = w;
             }
         } else {
             float* const sums = reinterpret_cast<float*>(smem);  // [group][row][LDO], over the operands, which have been read
@@ -701,8 +711,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                         y.w = fmaf(v[x].w, w, y.w);
                     }
                 }
-                const int where = tile.row0 + of;
-                T* const to = out + (int64_t)(tile.first + where / group) * a.ldo + (int64_t)(where % group) * dim + d;
+                T* const to = out + offset_of(of, a.ldo) + d;
                 if (!ok) continue;
                 if constexpr (F32) *reinterpret_cast<float4*>(to) = y;
                 else *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
@@ -713,7 +722,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     if (!ok) report_wait(a.waits, WAIT_ATTENTION);
     at_before();
     __syncthreads();
-    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
 }
 
 template <typename T, int DP, bool KEYS>
