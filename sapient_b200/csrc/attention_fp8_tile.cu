@@ -384,15 +384,19 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             __syncwarp();
             if (lane == 0) tc5_arrive(bar);
         };
-        int pages = page_of(0);
+        int pages = page_of(0), next = page_of(1);  // (looked up a tile ahead of the rows, which are requested a tile ahead of their use)
         load(raw_k, k_from, pages);
         load_scales(pages);
         load(raw_v, v_from, pages);
         for (int kv = 0; kv < n_kv; ++kv) {
             const int st = kv % STAGES, use = kv / STAGES, slot = kv % AT_RING, key0 = (b_begin + kv) * AT_KEYS;
             const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
-            pages = page_of(kv + 1);
+            pages = next;
+            next = page_of(kv + 2);
             uint32_t by[4] = {};  // what values are multiplied by, as pairs of fp16
+            if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&k_empty[st], (uint32_t)((use - 1) & 1)));
+            if (!ok) break;
+            store(raw_k, ks_ + st * Sh::TILE, by, false);
             if constexpr (!F32) {
                 const int k = key0 + 4 * lane;
                 const uint32_t big = max(max(counts(four.x, k) ? __float_as_uint(four.x) : 0u, counts(four.y, k + 1) ? __float_as_uint(four.y) : 0u),
@@ -404,9 +408,6 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                     by[i] = af_pack(f, f);
                 }
             }
-            if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&k_empty[st], (uint32_t)((use - 1) & 1)));
-            if (!ok) break;
-            store(raw_k, ks_ + st * Sh::TILE, by, false);
             {
                 const float v = counts(sv, key0 + p) ? sv : 0.f;
                 k_scale[slot][p] = sv < INFINITY && sv > -INFINITY ? sk : __uint_as_float(0x7FC00000u);
