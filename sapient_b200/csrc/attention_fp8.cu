@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(AR_THREADS) attention_rows_kernel(const Attent
             }
             most = warp_max(most);
             float by, back;
-            af_row_scale(most, by, back);
+            af_row_scale(most, 12, by, back);
             if (lane == 0) row_factor[r] = back * a.scale * AF_LOG2E;
             // element e: chunk c = e / 16 is thread t = c % 4's, h = c / 4; step 4 h + (e % 16) / 4; of its four bytes the first two in
             // the registers of columns 2 t, the others in those of columns 2 t + 8
@@ -428,7 +428,8 @@ static cudaError_t launch_rows(const AttentionFp8Args& a, cudaStream_t st) {
 template <typename T>
 static cudaError_t attention_as(const AttentionFp8Args& a, cudaStream_t st) {
     const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv);
-    if (rows > 32) return launch_attention_fp8_tiles(a, sizeof(T) == 2, st);
+    const bool tiles = (int64_t)a.c.n_pages * 2 * a.c.n_kv * KV_PAGE <= INT32_MAX;  // (a copy's row is counted in 32 bits)
+    if (rows > 32 && tiles) return launch_attention_fp8_tiles(a, sizeof(T) == 2, st);
     const bool few = rows <= 16;
     if (a.c.dim <= 64) return few ? launch_rows<T, 64, 1>(a, st) : launch_rows<T, 64, 2>(a, st);
     return few ? launch_rows<T, 128, 1>(a, st) : launch_rows<T, 128, 2>(a, st);

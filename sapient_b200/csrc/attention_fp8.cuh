@@ -50,11 +50,11 @@ __device__ __forceinline__ void af_copy16(uint32_t dst, const void* src, bool th
 __device__ __forceinline__ void af_copy8(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
 }
-// A power of two by which a row is multiplied so that its largest value lies in [2^12, 2^13), and its reciprocal. Rows of zeros and
+// A power of two by which a row is multiplied so that its largest value lies in [2^to, 2^(to + 1)), and its reciprocal. Rows of zeros and
 // those with infinities or NaN: 1.
-__device__ __forceinline__ void af_row_scale(float most, float& by, float& back) {
+__device__ __forceinline__ void af_row_scale(float most, int to, float& by, float& back) {
     const int e = (int)(__float_as_uint(most) >> 23);  // (most >= 0)
-    const int up = e == 0 || e == 255 ? 0 : min(max(139 - e, -126), 126);
+    const int up = e == 0 || e == 255 ? 0 : min(max(127 + to - e, -126), 126);
     by = __uint_as_float((uint32_t)(127 + up) << 23);
     back = __uint_as_float((uint32_t)(127 - up) << 23);
 }

@@ -4,8 +4,13 @@
 // tensor memory, a row a lane. While one group turns scores into weights, the tensor cores work for the other:
 //   warps 0-3, 4-7   weights: a thread has a row of S in registers; its maximum, exponentials, which go back over S as fp16, half a tile at a time,
 //                    and are the first operand of the second product from there. O is rescaled only when a row's reference moves.
-//   warps 8-11       keys and values: e4m3 rows to fp16 in shared memory (128-byte swizzle; keys K-major, values as they lie: MN-major)
+//   warps 8-11       values: e4m3 rows to fp16 in shared memory, as they lie (MN-major, 128-byte swizzle); f32: keys as well (K-major)
 //   warp 12          issues the products
+//   warp 13          keys of bf16 rows, as they are, a page a TMA copy, and the scales
+// bf16 rows are multiplied with the keys' own bytes: q is two e4m3 digits, whose products run at twice fp16's rate. A row scaled so that its largest
+// value lies in [128, 256) is its digits' sum exactly, but for values below 2^-9 of the largest, which are off by up to 2^-17 of that. What
+// bounds the tiles is the shared memory's bandwidth (operands, their conversion, scales), so that keys that need no conversion count for more
+// than the instructions: 8192 x 8192, 8B shape, XXX.
 // ROWS: the groups have 128 rows each of 256, and keys in common. KEYS (up to 128 rows): the same rows, key tiles by turns; their sums
 // are added up at the end. Keys may be shared out to the blocks of a cluster as well, which add up through shared memory.
 //
@@ -13,8 +18,9 @@
 // fp16 (off by 2^-11 of themselves), so that a weight is one exponential, 2^(z - M + u - 7); for f32 rows values stay exact and weights
 // are 2^(z - M) s', as fp16 plus the fp16 of the remainder. Either way they must stay below 2^16: the row's reference M is moved when
 // z + u - 7 (f32: z + u) passes M + 15, to 9 below it, and the sums move along. A scale that is NaN or infinite counts as 0 and makes the token's scores NaN.
+#include <cuda_fp8.h>
+
 #include <algorithm>
-#include <type_traits>
 
 #include "attention_fp8.cuh"
 #include "kernels.h"
@@ -25,24 +31,30 @@ namespace sp {
 
 cudaError_t count_launch_and_check();  // kernels.cu
 
-constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 512, AT_RING = 4, AT_MAX_PARTS = 8;
+constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 512, AT_RING = 8, AT_MAX_PARTS = 8;
 constexpr float AT_MOST = 15.f, AT_SET = 9.f;  // log2 of the largest weight, and of it when M is set
 constexpr int AT_UP = 7, AT_LEAST = -80;       // values times 2^7 are below 2^16; smaller u would let a sum of 2^(z - M) pass 2^127
 
 template <typename T, int DP, bool KEYS>
 struct AtShape {
     static constexpr bool F32 = sizeof(T) == 4;
-    static constexpr int PLANES = F32 ? 2 : 1, TILES = KEYS ? 1 : 2;      // of Q
-    static constexpr int STAGES = F32 && !KEYS && DP == 128 ? 1 : 2;      // of keys and of values
-    static constexpr int TILE = 128 * DP * 2;                             // bytes of 128 rows in fp16
-    static constexpr int Q = PLANES * TILES * TILE, SMEM = Q + 2 * STAGES * TILE + 1024;
-    static constexpr int LDO = DP + 4, SUMS = 2 * 128 * LDO * 4;          // takes the operands' place
-    static constexpr int WEIGHTS = KEYS ? 128 * 2 * 4 : 256 * 4;           // of the sums of a block's share of rows, behind them (parts x rows of a share is at most that)
+    static constexpr int PLANES = 2, TILES = KEYS ? 1 : 2;                      // of Q: digits, or fp16 and remainders
+    static constexpr int K_STAGES = !F32 ? 3 : !KEYS && DP == 128 ? 1 : 2, V_STAGES = F32 && !KEYS && DP == 128 ? 1 : 2;
+    static constexpr int TILE = 128 * DP * 2, K_TILE = F32 ? TILE : 128 * 128;  // bytes of 128 rows in fp16; of keys and of a plane of Q
+    static constexpr int Q = PLANES * TILES * K_TILE, SMEM = Q + K_STAGES * K_TILE + V_STAGES * TILE + 1024;
+    static constexpr int LDO = DP + 4, SUMS = 2 * 128 * LDO * 4;                // takes the operands' place
+    static constexpr int WEIGHTS = KEYS ? 128 * 2 * 4 : 256 * 4;                // of the sums of a block's share of rows, behind them (parts x rows of a share is at most that)
     static_assert(SUMS + WEIGHTS <= SMEM - 1024, "sums of both groups");
 };
 
 // log2 of the power of two not below a scale, given by its bits (positive and finite, or 0).
 __device__ __forceinline__ int at_power(uint32_t bits) { return max((int)((bits + 0x7FFFFFu) >> 23) - 127, AT_LEAST); }
+
+// Four values as e4m3, to nearest even.
+__device__ __forceinline__ uint32_t at_digits(const float* x) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
 
 // tc5_wait for warps that are ahead of the others: it looks now and then, so that the others have the issue slots.
 __device__ __forceinline__ bool at_wait_idle(uint64_t* bar, uint32_t parity) {
@@ -60,6 +72,15 @@ __device__ __forceinline__ uint32_t at_idesc(int n, bool b_mn) { return (1u << 4
 // Values as they lie: rows of 64 coordinates (128 bytes, swizzled) a token, 8 tokens 1024 bytes apart; the next 64 coordinates 128 tokens on.
 __device__ __forceinline__ uint64_t at_desc_values(uint32_t saddr) {
     return (tc5_desc(saddr) & ~((uint64_t)0x3FFF << 16)) | (uint64_t)(128 * 128 >> 4) << 16;
+}
+__device__ __forceinline__ void at_mma_digits(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {  // e4m3 x e4m3, 32 columns
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 __device__ __forceinline__ void at_mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -177,15 +198,15 @@ __device__ __forceinline__ float at_max3(float a, uint64_t two) {
 }
 
 template <typename T, int DP, bool KEYS>
-__global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const AttentionFp8Args a, int parts, int tiles) {
+__global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const AttentionFp8Args a, int parts, int tiles, const __grid_constant__ CUtensorMap map) {
     using Sh = AtShape<T, DP, KEYS>;
     constexpr bool F32 = Sh::F32;
-    constexpr int STAGES = Sh::STAGES, ROWS = 128 * Sh::TILES;
+    constexpr int K_STAGES = Sh::K_STAGES, V_STAGES = Sh::V_STAGES, ROWS = 128 * Sh::TILES;
     extern __shared__ uint8_t at_smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2][2], o_full, q_full;
+    __shared__ __align__(8) uint64_t k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES], s_full[2], p_full[2][2], o_full, q_full;
     __shared__ __align__(16) float k_scale[AT_RING][AT_KEYS], v_scale[AT_RING][F32 ? AT_KEYS : 4];
-    __shared__ uint32_t gone_s[AT_RING];  // pages of the tile that are not there
-    __shared__ __align__(16) uint32_t largest_s[AT_RING][4];  // scales of values, of 32 tokens each
+    __shared__ uint32_t gone_s[AT_RING];     // pages of the tile that are not there
+    __shared__ __align__(16) uint32_t largest_s[AT_RING][4];  // scales of values that count, of 32 tokens each
     __shared__ float row_factor[ROWS];
     __shared__ float part_m[2][128], part_l[2][128];
     __shared__ uint32_t tmem_slot;
@@ -197,7 +218,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     const AfTile tile = af_tile(a, blockIdx.y, tiles - 1 - blockIdx.x / a.c.n_kv, ROWS);
     if (tile.n <= 0) return;  // (the whole cluster)
     uint8_t* const smem = at_smem_raw + ((1024u - (tc5_smem_u32(at_smem_raw) & 1023u)) & 1023u);
-    uint8_t *const ks_ = smem + Sh::Q, *const vs_ = ks_ + STAGES * Sh::TILE;
+    uint8_t *const ks_ = smem + Sh::Q, *const vs_ = ks_ + K_STAGES * Sh::K_TILE;
     // ── the block's keys ──
     const int last_row = tile.row0 + tile.n - 1;
     // Token and head of the block's row q: with rem = row0 % group, (rem + q) / group by a reciprocal is exact, since (rem + q + 1/2) / group is at
@@ -223,10 +244,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     if (tid == 32) {
-        for (int i = 0; i < STAGES; ++i) {
-            at_init(&k_full[i], 4);
-            at_init(&v_full[i], 4);
+        for (int i = 0; i < K_STAGES; ++i) {
+            at_init(&k_full[i], F32 ? 4 : 1);
             at_init(&k_empty[i], 1);
+        }
+        for (int i = 0; i < V_STAGES; ++i) {
+            at_init(&v_full[i], 4);
             at_init(&v_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -243,27 +266,85 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     at_after();
     const uint32_t tmem = tmem_slot;  // S of the groups at columns 0 and 128, O at 256 and 256 + DP
     bool ok = true;
+    // ── where the keys and values are ──
+    const int32_t* const table = a.c.page_table + (int64_t)max(0, min(tile.slot, a.c.n_slots - 1)) * a.c.max_pages;
+    auto page_of = [&](int kv) {  // lanes 0 to 7 (and so on): the tile's pages; -1: none
+        const int index = (b_begin + kv) * AT_PAGES + (lane & 7);
+        const int page = kv < n_kv && index < a.c.max_pages && index * KV_PAGE < k_end ? table[index] : -1;
+        return page < a.c.n_pages ? max(page, -1) : -1;
+    };
+    const int page_rows = 2 * a.c.n_kv * KV_PAGE, page_bytes = page_rows * dim, to_values = a.c.n_kv * KV_PAGE;
+    const float* const s_from = a.c.scales + head * KV_PAGE;
+    // A value's scale as it counts: none of what no row of the block sees, nor of what is NaN or infinite
+    auto counts = [&](float s, int token) { return s > 0.f && s < INFINITY && token >= k_begin && token < k_end; };
     if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");  // 128 x 56 + 128 x 104 + 256 x 176 = 512 x 128
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");  // 128 x 56 + 128 x 88 + 256 x 184 = 512 x 128 (f32: 56, 104, 176)
+        if (!F32 && warp == 13) {
+            // a lane looks after tokens 4 lane .. 4 lane + 3 of a tile, lanes 0 to 7 after a page
+            int pages = page_of(0), next = page_of(1);
+            float4 sk, sv;
+            auto load = [&]() {
+                const int page = __shfl_sync(0xFFFFFFFFu, pages, lane / 4);
+                const float4* const at = reinterpret_cast<const float4*>(s_from + (int64_t)max(page, 0) * page_rows + 4 * lane % KV_PAGE);
+                sk = __ldg(at);
+                sv = page >= 0 ? __ldg(at + to_values / 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            };
+            if (n_kv > 0) load();
+            int issued = 0;
+            for (int kv = 0; kv < n_kv; ++kv) {
+                const int st = kv % K_STAGES, use = kv / K_STAGES, slot = kv % AT_RING, token = (b_begin + kv) * AT_KEYS + 4 * lane;
+                if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&k_empty[st], (uint32_t)((use - 1) & 1)));
+                if (!ok) break;
+                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
+                const float v[4] = {sv.x, sv.y, sv.z, sv.w}, k[4] = {sk.x, sk.y, sk.z, sk.w};
+                float4 to;
+                float* const f = &to.x;
+                uint32_t big = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f[j] = v[j] < INFINITY && v[j] > -INFINITY ? k[j] : __uint_as_float(0x7FC00000u);
+                    if (counts(v[j], token + j)) big = max(big, __float_as_uint(v[j]));
+                }
+                *reinterpret_cast<float4*>(&k_scale[slot][4 * lane]) = to;
+                big = __reduce_max_sync(0xFFFFFFFFu, big);
+                if (lane == 0) {
+                    *reinterpret_cast<uint4*>(largest_s[slot]) = make_uint4(big, big, big, big);
+                    gone_s[slot] = gone;
+                }
+                __syncwarp();
+                const uint32_t bar = tc5_smem_u32(&k_full[st]);
+                if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((uint32_t)(AT_PAGES - __popc(gone)) * KV_PAGE * 128u) : "memory");
+                __syncwarp();
+                if (lane < AT_PAGES && pages >= 0) tc5_tma_2d(tc5_smem_u32(ks_ + st * Sh::K_TILE) + lane * (KV_PAGE * 128), &map, 0, (pages * 2 * a.c.n_kv + head) * KV_PAGE, bar);
+                issued = kv + 1;
+                pages = next;
+                next = page_of(kv + 2);
+                if (kv + 1 < n_kv) load();
+            }
+            // no copy is on its way to this block when it goes on to the end
+            for (int kv = max(0, issued - K_STAGES); kv < issued; ++kv) ok = tc5_wait(&k_full[kv % K_STAGES], (uint32_t)((kv / K_STAGES) & 1)) && ok;
+        }
         if (warp == 12) {
         const bool leader = tc5_elect();
         const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
         const uint32_t id_s = at_idesc(AT_KEYS, false), id_o = at_idesc(dim, true);
         const uint64_t qd = tc5_desc(tc5_smem_u32(smem)), kd = tc5_desc(tc5_smem_u32(ks_)), vd = at_desc_values(tc5_smem_u32(vs_));
-        const int steps = dim / 16;
+        const int steps = F32 ? dim / 16 : (dim + 31) / 32;  // of 32 bytes
         if (jobs > 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&q_full, 0));
         auto scores = [&](int j) {
-            const int t = groups == 2 ? j & 1 : 0, kv = KEYS || groups == 1 ? j : j >> 1, st = kv % STAGES;
-            if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&k_full[st], (uint32_t)((kv / STAGES) & 1)));
+            const int t = groups == 2 ? j & 1 : 0, kv = KEYS || groups == 1 ? j : j >> 1, st = kv % K_STAGES;
+            if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&k_full[st], (uint32_t)((kv / K_STAGES) & 1)));
             if (!ok) return;
             at_after();
             if (leader) {
-                const uint64_t q = qd + (uint64_t)((KEYS ? 0 : t) * (Sh::TILE >> 4)), k = kd + (uint64_t)(st * (Sh::TILE >> 4));
+                const uint64_t q = qd + (uint64_t)((KEYS ? 0 : t) * (Sh::K_TILE >> 4)), k = kd + (uint64_t)(st * (Sh::K_TILE >> 4));
 #pragma unroll
                 for (int p = Sh::PLANES - 1; p >= 0; --p)
                     for (int s = 0; s < steps; ++s) {
-                        const uint64_t at = (uint64_t)((s >> 2) * (128 * 128 >> 4) + (s & 3) * 2);
-                        tc5_mma(tm + 128u * t, q + at + (uint64_t)(p * Sh::TILES * (Sh::TILE >> 4)), k + at, id_s, p != Sh::PLANES - 1 || s > 0);
+                        const uint64_t at = (uint64_t)((s >> 2) * (128 * 128 >> 4) + (s & 3) * 2), from = q + at + (uint64_t)(p * Sh::TILES * (Sh::K_TILE >> 4));
+                        const uint32_t more = p != Sh::PLANES - 1 || s > 0;
+                        if constexpr (F32) tc5_mma(tm + 128u * t, from, k + at, id_s, more);
+                        else at_mma_digits(tm + 128u * t, from, k + at, id_s, more);
                     }
                 tc5_commit(&s_full[t]);
                 if (KEYS || t == groups - 1) tc5_commit(&k_empty[st]);
@@ -272,8 +353,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         };
         for (int j = 0; j < groups && j < jobs && ok; ++j) scores(j);
         for (int j = 0; j < jobs && ok; ++j) {
-            const int t = groups == 2 ? j & 1 : 0, i = groups == 2 ? j >> 1 : j, kv = KEYS ? j : i, st = kv % STAGES;
-            if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&v_full[st], (uint32_t)((kv / STAGES) & 1)));
+            const int t = groups == 2 ? j & 1 : 0, i = groups == 2 ? j >> 1 : j, kv = KEYS ? j : i, st = kv % V_STAGES;
+            if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&v_full[st], (uint32_t)((kv / V_STAGES) & 1)));
 #pragma unroll 1
             for (int half = 0; half < 2 && ok; ++half) {
                 ok = __all_sync(0xFFFFFFFFu, tc5_wait(&p_full[t][half], (uint32_t)(i & 1)));
@@ -285,9 +366,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
 #pragma unroll
-                        for (int p = Sh::PLANES - 1; p >= 0; --p)
+                        for (int p = F32 ? 1 : 0; p >= 0; --p)
                             at_mma_tmem(tm + 256u + (uint32_t)(DP * t), w + (uint32_t)(F32 ? 32 * (s / 2) + 16 * p + 8 * (s % 2) : 8 * s), v + (uint64_t)(s * (2048 >> 4)), id_o,
-                                        i > 0 || half > 0 || s > 0 || p != Sh::PLANES - 1);
+                                        i > 0 || half > 0 || s > 0 || (F32 && p == 0));
                     if (half == 1 && (KEYS || t == groups - 1)) tc5_commit(&v_empty[st]);
                 }
                 __syncwarp();
@@ -299,10 +380,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             if (ok && leader) tc5_commit(&o_full);
             __syncwarp();
             // no arrival is on its way to this block when it goes on to the end
-            for (int kv = max(0, n_kv - STAGES); kv < n_kv; ++kv) {
-                const uint32_t parity = (uint32_t)((kv / STAGES) & 1);
-                ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&k_empty[kv % STAGES], parity) && tc5_wait(&v_empty[kv % STAGES], parity));
-            }
+            for (int kv = max(0, n_kv - K_STAGES); kv < n_kv; ++kv) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&k_empty[kv % K_STAGES], (uint32_t)((kv / K_STAGES) & 1)));
+            for (int kv = max(0, n_kv - V_STAGES); kv < n_kv; ++kv) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&v_empty[kv % V_STAGES], (uint32_t)((kv / V_STAGES) & 1)));
             ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&o_full, 0));
         }
         }
@@ -311,70 +390,39 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             cluster_sync();
         }
     } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
-        // Sixteen bytes of a row a copy, 64 coordinates of eight tokens a warp at once: stores of eight threads fall on 32 different banks.
-        constexpr int HALVES = DP / 64, N = 4 * HALVES;  // copies of a thread: tokens tok0 + 32 i, coordinates 16 ch and 64 + 16 ch
-        const int p = tid - 256, ch = p % 4, tok0 = p / 4;
-        const int32_t* const table = a.c.page_table + (int64_t)max(0, min(tile.slot, a.c.n_slots - 1)) * a.c.max_pages;
-        auto page_of = [&](int kv) {  // lanes 0 to 7: the tile's pages
-            const int index = (b_begin + kv) * AT_PAGES + (lane & 7);
-            const int page = kv < n_kv && index < a.c.max_pages && index * KV_PAGE < k_end ? table[index] : -1;
-            return page < a.c.n_pages ? max(page, -1) : -1;
-        };
-        const int page_rows = 2 * a.c.n_kv * KV_PAGE, page_bytes = page_rows * dim, to_values = a.c.n_kv * KV_PAGE;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(F32 ? 104 : 88));
+        // of a tile: 16 bytes of tokens tok0 + PER i a copy; a warp's threads have whole rows, so that a request is few lines
+        constexpr int CH = DP / 16, N = CH, PER = 128 / CH;
+        const int p = tid - 256, ch = p % CH, tok0 = p / CH;
         const uint8_t* const k_from = a.c.values + ((int64_t)head * KV_PAGE + tok0 % KV_PAGE) * dim + 16 * ch;
         const uint8_t* const v_from = k_from + (int64_t)to_values * dim;
-        const float* const s_from = a.c.scales + head * KV_PAGE;
-        uint4 raw_k[N], raw_v[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) raw_k[i] = raw_v[i] = make_uint4(0, 0, 0, 0);
-        float own[4] = {};                           // scales of the thread's tokens' values
-        float4 four = make_float4(0.f, 0.f, 0.f, 0.f);  // of tokens 4 lane .. 4 lane + 3
-        float sk = 0.f, sv = 0.f;                       // of token p
-        // A value's scale as it counts: none of what no row of the block sees, nor of what is NaN or infinite
-        auto counts = [&](float s, int token) { return s > 0.f && s < INFINITY && token >= k_begin && token < k_end; };
         // (of a page that is not there the first one's rows are taken: nobody sees them)
         auto load = [&](uint4 (&raw)[N], const uint8_t* from, int pages) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint8_t* const row = from + (int64_t)max(__shfl_sync(0xFFFFFFFFu, pages, tok0 / KV_PAGE + 2 * i), 0) * page_bytes;
-#pragma unroll
-                for (int h = 0; h < HALVES; ++h)
-                    if (64 * h + 16 * ch < dim) raw[HALVES * i + h] = __ldg(reinterpret_cast<const uint4*>(row + 64 * h));
+            for (int i = 0; i < N; ++i) {
+                const int page = __shfl_sync(0xFFFFFFFFu, pages, (tok0 + PER * i) / KV_PAGE);
+                if (16 * ch < dim) raw[i] = __ldg(reinterpret_cast<const uint4*>(from + (int64_t)max(page, 0) * page_bytes));
             }
         };
-        auto load_scales = [&](int pages) {
-            const int mine = __shfl_sync(0xFFFFFFFFu, pages, p / KV_PAGE);
-            const float* const at = s_from + (int64_t)max(mine, 0) * page_rows + p % KV_PAGE;
-            sk = __ldg(at);
-            sv = mine >= 0 ? __ldg(at + to_values) : 0.f;
-            if constexpr (!F32) {
-                const int page = __shfl_sync(0xFFFFFFFFu, pages, lane / 4);
-                four = page >= 0 ? __ldg(reinterpret_cast<const float4*>(s_from + (int64_t)page * page_rows + to_values + 4 * lane % KV_PAGE)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int of = __shfl_sync(0xFFFFFFFFu, pages, tok0 / KV_PAGE + 2 * i);
-                    own[i] = of >= 0 ? __ldg(s_from + (int64_t)of * page_rows + to_values + tok0 % KV_PAGE) : 0.f;
-                }
-            }
-        };
-        const int u0 = ((2 * ch) ^ (tok0 & 7)) * 16, u1 = ((2 * ch + 1) ^ (tok0 & 7)) * 16;
-        auto store = [&](const uint4 (&raw)[N], uint8_t* to, const uint32_t (&by)[4], bool values) {
+        // The second half of a row's threads swap the halves of their 16 bytes: eight threads' stores fall on 32 different banks.
+        const bool odd = ch / 4;
+        const int x = tok0 & 7, u0 = ((2 * (ch % 4) + odd) ^ x) * 16, u1 = ((2 * (ch % 4) + 1 - odd) ^ x) * 16;
+        auto store = [&](const uint4 (&raw)[N], uint8_t* tile_at, const uint32_t (&by)[N], bool values) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 uint32_t h[8];
-                af_halves(raw[i].x, h[0], h[1]);
-                af_halves(raw[i].y, h[2], h[3]);
-                af_halves(raw[i].z, h[4], h[5]);
-                af_halves(raw[i].w, h[6], h[7]);
+                af_halves(odd ? raw[i].z : raw[i].x, h[0], h[1]);
+                af_halves(odd ? raw[i].w : raw[i].y, h[2], h[3]);
+                af_halves(odd ? raw[i].x : raw[i].z, h[4], h[5]);
+                af_halves(odd ? raw[i].y : raw[i].w, h[6], h[7]);
                 if (values) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         h[j] = af_finite(h[j]);
-                        if constexpr (!F32) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(by[i / HALVES]));
+                        if constexpr (!F32) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(by[i]));
                     }
                 }
-                uint8_t* const row = to + tok0 * 128 + i / HALVES * (32 * 128) + i % HALVES * (128 * 128);
+                uint8_t* const row = tile_at + ch / 4 * (128 * 128) + (tok0 + PER * i) * 128;
                 *reinterpret_cast<uint4*>(row + u0) = make_uint4(h[0], h[1], h[2], h[3]);
                 *reinterpret_cast<uint4*>(row + u1) = make_uint4(h[4], h[5], h[6], h[7]);
             }
@@ -384,47 +432,71 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             __syncwarp();
             if (lane == 0) tc5_arrive(bar);
         };
-        int pages = page_of(0), next = page_of(1);  // (looked up a tile ahead of the rows, which are requested a tile ahead of their use)
-        load(raw_k, k_from, pages);
-        load_scales(pages);
-        load(raw_v, v_from, pages);
-        for (int kv = 0; kv < n_kv; ++kv) {
-            const int st = kv % STAGES, use = kv / STAGES, slot = kv % AT_RING, key0 = (b_begin + kv) * AT_KEYS;
-            const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
-            pages = next;
-            next = page_of(kv + 2);
-            uint32_t by[4] = {};  // what values are multiplied by, as pairs of fp16
-            if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&k_empty[st], (uint32_t)((use - 1) & 1)));
-            if (!ok) break;
-            store(raw_k, ks_ + st * Sh::TILE, by, false);
-            if constexpr (!F32) {
-                const int k = key0 + 4 * lane;
-                const uint32_t big = max(max(counts(four.x, k) ? __float_as_uint(four.x) : 0u, counts(four.y, k + 1) ? __float_as_uint(four.y) : 0u),
-                                         max(counts(four.z, k + 2) ? __float_as_uint(four.z) : 0u, counts(four.w, k + 3) ? __float_as_uint(four.w) : 0u));
-                const float lift = __uint_as_float((uint32_t)(127 + AT_UP - at_power(__reduce_max_sync(0xFFFFFFFFu, big))) << 23);
+        [[maybe_unused]] uint4 raw_k[N];
+        uint4 raw_v[N];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f = counts(own[i], key0 + tok0 + 32 * i) ? own[i] * lift : 0.f;
-                    by[i] = af_pack(f, f);
-                }
+        for (int i = 0; i < N; ++i) raw_k[i] = raw_v[i] = make_uint4(0, 0, 0, 0);
+        [[maybe_unused]] float sk = 0.f, sv = 0.f;  // f32: of token p
+        float four[4] = {};                         // bf16: of the values of tokens 4 lane .. 4 lane + 3
+        auto load_scales = [&](int pages) {
+            const int page = __shfl_sync(0xFFFFFFFFu, pages, F32 ? p / KV_PAGE : lane / 4);
+            const float* const at = s_from + (int64_t)max(page, 0) * page_rows;
+            if constexpr (F32) {
+                sk = __ldg(at + p % KV_PAGE);
+                sv = page >= 0 ? __ldg(at + to_values + p % KV_PAGE) : 0.f;
+            } else {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(at + to_values + 4 * lane % KV_PAGE));
+                four[0] = f.x; four[1] = f.y; four[2] = f.z; four[3] = f.w;
             }
-            {
+        };
+        int pages = page_of(0), next = page_of(1);  // (looked up a tile ahead of the rows, which are requested a tile ahead of their use)
+        if (n_kv > 0) {
+            if constexpr (F32) load(raw_k, k_from, pages);
+            load_scales(pages);
+            load(raw_v, v_from, pages);
+        }
+        for (int kv = 0; kv < n_kv; ++kv) {
+            const int key0 = (b_begin + kv) * AT_KEYS;
+            uint32_t by[N] = {};  // what values are multiplied by, as pairs of fp16
+            if constexpr (F32) {
+                const int st = kv % K_STAGES, use = kv / K_STAGES, slot = kv % AT_RING;
+                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
+                if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&k_empty[st], (uint32_t)((use - 1) & 1)));
+                if (!ok) break;
+                store(raw_k, ks_ + st * Sh::K_TILE, by, false);
                 const float v = counts(sv, key0 + p) ? sv : 0.f;
                 k_scale[slot][p] = sv < INFINITY && sv > -INFINITY ? sk : __uint_as_float(0x7FC00000u);
-                if constexpr (F32) v_scale[slot][p] = v;
+                v_scale[slot][p] = v;
                 const uint32_t big = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v));
                 if (lane == 0) largest_s[slot][warp - 8] = big;
                 if (p == 0) gone_s[slot] = gone;
+                hand_over(&k_full[st]);
+                if (kv + 1 < n_kv) load(raw_k, k_from, next);
+            } else {
+                const int mine = __shfl_sync(0xFFFFFFFFu, pages, lane / 4), token = key0 + 4 * lane;
+                uint32_t big = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (mine < 0 || !counts(four[j], token + j)) four[j] = 0.f;
+                    big = max(big, __float_as_uint(four[j]));
+                }
+                const float lift = __uint_as_float((uint32_t)(127 + AT_UP - at_power(__reduce_max_sync(0xFFFFFFFFu, big))) << 23);
+                const uint32_t two0 = af_pack(four[0] * lift, four[1] * lift), two1 = af_pack(four[2] * lift, four[3] * lift);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int tok = tok0 + PER * i;
+                    const uint32_t a0 = __shfl_sync(0xFFFFFFFFu, two0, tok / 4), a1 = __shfl_sync(0xFFFFFFFFu, two1, tok / 4);
+                    by[i] = __byte_perm(tok & 2 ? a1 : a0, 0, tok & 1 ? 0x3232 : 0x1010);
+                }
             }
-            hand_over(&k_full[st]);
-            if (kv + 1 < n_kv) {
-                load(raw_k, k_from, pages);
-                load_scales(pages);
-            }
+            if (kv + 1 < n_kv) load_scales(next);
+            const int st = kv % V_STAGES, use = kv / V_STAGES;
             if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&v_empty[st], (uint32_t)((use - 1) & 1)));
             if (!ok) break;
             store(raw_v, vs_ + st * Sh::TILE, by, true);
             hand_over(&v_full[st]);
+            pages = next;
+            next = page_of(kv + 2);
             if (kv + 1 < n_kv) load(raw_v, v_from, pages);
         }
         if (parts > 1) {
@@ -432,7 +504,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             cluster_sync();
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(F32 ? 176 : 184));
         const int t = warp >> 2, r = 32 * (warp & 3) + lane, row = (KEYS ? 0 : 128 * t) + r;  // of the block's rows
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), S = lanes + 128u * t, O = lanes + 256u + (uint32_t)(DP * t);
         const int pos = pos_first + token_of(row);
@@ -481,16 +553,34 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
 #pragma unroll
                 for (int o = PER / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
                 float by, back;
-                af_row_scale(most, by, back);
+                af_row_scale(most, F32 ? 12 : 7, by, back);
                 if (a.scale < 0.f) by = -by;
                 if (u == 0) row_factor[q] = fmaxf(back * fabsf(a.scale) * AF_LOG2E, 0x1p-149f);
-                uint4 hi, lo;
-                uint32_t *const h = &hi.x, *const l = &lo.x;
+                if constexpr (F32) {
+                    uint4 hi, lo;
+                    uint32_t *const h = &hi.x, *const l = &lo.x;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) af_split(x[2 * j] * by, x[2 * j + 1] * by, h[j], l[j]);
-                uint8_t* const to = smem + q / 128 * Sh::TILE + u / 8 * (128 * 128) + q % 128 * 128 + ((u % 8) ^ (q & 7)) * 16;
-                *reinterpret_cast<uint4*>(to) = hi;
-                if constexpr (F32) *reinterpret_cast<uint4*>(to + Sh::TILES * Sh::TILE) = lo;
+                    for (int j = 0; j < 4; ++j) af_split(x[2 * j] * by, x[2 * j + 1] * by, h[j], l[j]);
+                    uint8_t* const to = smem + q / 128 * Sh::K_TILE + u / 8 * (128 * 128) + q % 128 * 128 + ((u % 8) ^ (q & 7)) * 16;
+                    *reinterpret_cast<uint4*>(to) = hi;
+                    *reinterpret_cast<uint4*>(to + Sh::TILES * Sh::K_TILE) = lo;
+                } else {
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[4 * j + e] *= by;
+                        hi[j] = at_digits(x + 4 * j);
+                        uint32_t h0, h1;
+                        af_halves(hi[j], h0, h1);
+                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                        const float r[4] = {x[4 * j] - f0.x, x[4 * j + 1] - f0.y, x[4 * j + 2] - f1.x, x[4 * j + 3] - f1.y};
+                        lo[j] = at_digits(r);
+                    }
+                    uint8_t* const to = smem + q / 128 * Sh::K_TILE + q % 128 * 128 + ((u / 2) ^ (q & 7)) * 16 + u % 2 * 8;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(to + Sh::TILES * Sh::K_TILE) = make_uint2(lo[0], lo[1]);
+                }
             }
             at_fence_smem();
             if constexpr (KEYS) asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");  // (the factors of rows that other warps have done)
@@ -733,11 +823,21 @@ static cudaError_t launch_tiles(const AttentionFp8Args& a, cudaStream_t st) {
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(attention_tile_kernel<T, DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM); });
     if (e != cudaSuccess) return e;
     const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv), height = 128 * Sh::TILES, tiles = (rows + height - 1) / height, clusters = tiles * a.c.n_kv * a.n_seqs;
+    CUtensorMap map{};
+    if (!Sh::F32) {  // rows of the pool, 16 of them (a page's keys of a head) a copy, filled up to 128 bytes with zeros
+        const PFN_encodeTiled encode = tensor_map_encoder();
+        if (!encode) return cudaErrorNotSupported;
+        const cuuint64_t dims[2] = {(cuuint64_t)a.c.dim, (cuuint64_t)a.c.n_pages * 2 * a.c.n_kv * KV_PAGE}, strides[1] = {(cuuint64_t)a.c.dim};
+        const cuuint32_t box[2] = {128, KV_PAGE}, each[2] = {1, 1};
+        if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a.c.values, dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    }
     // an SM a block, each with four tiles of keys at least
     int parts = 1;
     while (parts < AT_MAX_PARTS && clusters * parts * 2 <= device_sm_count() && (int64_t)a.max_len >= 4 * AT_KEYS * 2 * parts) parts *= 2;
     e = launch_pdl_cluster(attention_tile_kernel<T, DP, KEYS>, dim3((unsigned)(tiles * a.c.n_kv), (unsigned)a.n_seqs, (unsigned)parts), dim3(AT_THREADS), Sh::SMEM, st, parts, a,
-                           parts, (int)tiles);
+                           parts, (int)tiles, map);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
