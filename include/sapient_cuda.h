@@ -202,7 +202,7 @@ int32_t sp_cuda_upload_weight_fp8(int32_t device, int64_t n, int64_t k, const vo
  * values[page][keys | values][n_kv_heads][16 tokens][head_dim] in e4m3, scales[page][keys | values][n_kv_heads][16] in f32: a token's head is
  * an fp8 row as above with one scale. page_table[slot][i] is the page of tokens 16 i .. 16 i + 15 of a slot; an entry that is not a page's
  * number is not followed. All of it is the caller's device memory, of one layer; values, scales and page_table start on 16, 16 and 4
- * bytes. head_dim is a multiple of 16, at most 128. `cache` of a call is an SpCacheFp8's address, which is read during the call only; device, n_pages, n_slots, max_pages and
+ * bytes. head_dim is a multiple of 16, at most 128; n_pages x 2 x n_kv_heads x 16 is below 2^31. `cache` of a call is an SpCacheFp8's address, which is read during the call only; device, n_pages, n_slots, max_pages and
  * n_kv_heads are positive but for device.
  * The calls take device pointers, launch one kernel on `stream` and do not wait; they keep nothing between calls, so that they may run at
  * the same time on several streams and be captured into graphs. dtype (SP_F32 or SP_BF16) is the type of q, k, v, q_out and out; rows of

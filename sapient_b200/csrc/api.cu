@@ -185,6 +185,7 @@ int check_cache(const void* cache, int dtype, CacheFp8* out) {
         set_error("cache_fp8: bad shape");
         return SP_ERR_SHAPE;
     }
+    if ((int64_t)c->n_pages * c->n_kv_heads > INT32_MAX / (2 * KV_PAGE)) { set_error("cache_fp8: n_pages x 2 x n_kv_heads x 16 must be below 2^31"); return SP_ERR_SHAPE; }
     if (unaligned(c->values, 16) || unaligned(c->scales, 16) || unaligned(c->page_table, 4)) { set_error("cache_fp8: values and scales must be 16-byte aligned"); return SP_ERR_ARG; }
     *out = CacheFp8{static_cast<uint8_t*>(c->values), c->scales, c->page_table, c->n_pages, c->n_slots, c->max_pages, c->n_kv_heads, c->head_dim};
     return SP_OK;

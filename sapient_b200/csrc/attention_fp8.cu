@@ -11,43 +11,65 @@
 // plus the fp16 of the remainder. The weights e^(z - m) s' enter the second product as fp16 (11 bits, where the result has bf16's 8) or,
 // for f32, as fp16 plus remainder, multiplied by a power of two that keeps them out of fp16's subnormals: with the largest scale so far, R,
 // rounded up to a power of two and e^(z - m) <= 2^LAZY, the weights are e^(z - m) s' 2^(15 - LAZY) / R <= 2^15. Sums, maxima and the output are f32.
+#include <cuda_fp8.h>
+
 #include <algorithm>
+#include <cmath>
+#include <cstdlib>
+#include <type_traits>
 
 #include "attention_fp8.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
+#include "tc5_ptx.cuh"
 
 namespace sp {
 
 cudaError_t count_launch_and_check();  // kernels.cu
 
 // ── Few rows: mma.sync, a warp takes 32 keys at a time ──
-// The cache is read once, which is what bounds it: every warp keeps a ring of asynchronous copies in flight. A thread copies just the
-// bytes that it multiplies itself: keys as the second operand of q K^T, four consecutive bytes of a row being one thread's part of a
-// product of 16 columns (the order of columns does not matter where q has the same), values of four tokens as the second operand
-// of P V, 16 neighbouring columns each, so that a column of the product is a coordinate of each sixteen. So nothing is rearranged but pairs of
-// tokens' bytes, and the accumulators of the first product are the first operand of the second.
+// The cache is read once, which is what bounds it: every warp keeps asynchronous copies in flight. Keys and values are the first operands of
+// K q^T and V^T P^T, 16 keys or coordinates high, so that eight rows are a product's width. A thread's part of a product of 16 columns is four
+// neighbouring bytes of a key's row (the order of columns does not matter where q has the same), and of values it has four tokens'
+// 16 neighbouring coordinates, two a product. So nothing is rearranged but pairs of tokens' bytes, and the weights, which two 8 x 8
+// transpositions make the second product's operand. (e4m3 operands of mma.sync are converted to fp16 at every use on this GPU: two digits
+// of q against the keys' own bytes took 982 instructions for 32 keys.) A page's keys or values of a head are one TMA copy, whose 128-byte
+// swizzle lets eight threads' reads fall on 32 different banks; copied by threads, 16 bytes each, every one was a request of its own to L2:
+// 131072 keys of the 8B shape 106 us, now XXX.
 // Keys are shared out to the warps of a block and the blocks of a cluster, which add up their parts through shared memory: no workspace.
-constexpr int AR_WARPS = 4, AR_THREADS = 32 * AR_WARPS, AR_KEYS = 32, AR_PAGES = AR_KEYS / KV_PAGE, AR_STAGES = 3, AR_MAX_PARTS = 16;
+constexpr int AR_KEYS = 32, AR_PAGES = AR_KEYS / KV_PAGE, AR_MAX_PARTS = 16;
+static int env(const char*n,int d){const char*e=getenv(n);return e?atoi(e):d;}
+#define AR_FIXED env("AR_FIXED",2)
+#define AR_WIDE(c) ((c) <= env("AR_WIDE",64))
 
-template <typename T, int DP, int R>
+
+template <typename T, int DP, int NT, int W>
 struct ArShape {
     static constexpr bool F32 = sizeof(T) == 4;
-    static constexpr int PLANES = F32 ? 2 : 1, STEPS = DP / 16, CHUNKS = DP / 64;
-    static constexpr int KBYTES = AR_KEYS * DP, STAGE = 2 * KBYTES + 2 * AR_KEYS * 4;  // keys, values, their scales
-    static constexpr int Q = R * PLANES * STEPS * 512, RING = AR_WARPS * AR_STAGES * STAGE;
-    static constexpr int ROWS = 16 * R, LDO = DP + 4;
-    static constexpr int SUMS = AR_WARPS * ROWS * LDO * 4;  // takes the ring's place
-    static constexpr int SMEM = Q + (RING > SUMS ? RING : SUMS);
+    static constexpr int PLANES = F32 ? 2 : 1, STEPS = DP / 16, CHUNKS = DP / 64;       // of q: products of 16 columns
+    static constexpr int STAGES = W == 4 ? 2 : 3;
+    static constexpr int PAGE = KV_PAGE * 128, STAGE = 2 * AR_PAGES * PAGE, SCALES = 2 * AR_KEYS * 4;  // [page][keys, values], their scales
+    static constexpr int Q = NT * PLANES * STEPS * 256, RING = W * STAGES * (STAGE + SCALES);
+    static constexpr int ROWS = 8 * NT, LDO = DP + 4;
+    static constexpr int SUMS = W * ROWS * LDO * 4;  // takes the ring's place
+    static constexpr int SMEM = Q + (RING > SUMS ? RING : SUMS) + 1024;
 };
 
-template <typename T, int DP, int R>
-__global__ void __launch_bounds__(AR_THREADS) attention_rows_kernel(const AttentionFp8Args a, int parts) {
-    using Sh = ArShape<T, DP, R>;
-    constexpr bool F32 = Sh::F32;
-    extern __shared__ __align__(16) uint8_t ar_smem[];
-    __shared__ float row_factor[Sh::ROWS];              // scale log2(e) / what the row was multiplied by
-    __shared__ float warp_m[AR_WARPS][Sh::ROWS], warp_l[AR_WARPS][Sh::ROWS];
+__device__ __forceinline__ uint32_t af_transpose(uint32_t v) {  // of an 8 x 8 matrix of 16-bit values, a row of pairs four threads
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(v));
+    return d;
+}
+
+template <typename T, int DP, int NT, int W>
+__global__ void __launch_bounds__(32 * W, NT > 2 ? 1 : W == 4 ? 3 : 1) attention_rows_kernel(const AttentionFp8Args a, int parts, const __grid_constant__ CUtensorMap map) {
+    using Sh = ArShape<T, DP, NT, W>;
+    constexpr bool F32 = Sh::F32, HELD = NT == 1;  // q stays in registers
+    constexpr int STAGES = Sh::STAGES;
+    extern __shared__ uint8_t ar_smem_raw[];
+    __shared__ __align__(8) uint64_t full[W][STAGES];
+    __shared__ float row_factor[Sh::ROWS];  // scale log2(e) / what the row was multiplied by
+    __shared__ float warp_m[W][Sh::ROWS], warp_l[W][Sh::ROWS];
     __shared__ float part_m[Sh::ROWS], part_l[Sh::ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int head = blockIdx.x % a.c.n_kv, part = blockIdx.z, group = a.n_heads / a.c.n_kv, dim = a.c.dim;
@@ -55,253 +77,229 @@ __global__ void __launch_bounds__(AR_THREADS) attention_rows_kernel(const Attent
     pdl_trigger();
     const AfTile tile = af_tile(a, blockIdx.y, blockIdx.x / a.c.n_kv, Sh::ROWS);
     if (tile.n <= 0) return;  // (the whole cluster)
-    // ── queries: fp16 operands in the order in which they are used ──
-    uint8_t* const qs = ar_smem;
-    {
-        for (int r = warp; r < Sh::ROWS; r += AR_WARPS) {
-            const int row = tile.row0 + min(r, tile.n - 1);
-            const T* const src = static_cast<const T*>(a.q) + (int64_t)(tile.first + row / group) * a.ldq + (int64_t)(head * group + row % group) * dim;
-            float x[DP / 32];
-            float most = 0.f;
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const int e = 32 * i + lane;
-                x[i] = r < tile.n && e < dim ? to_f32(src[e]) : 0.f;
-                most = fmaxf(most, fabsf(x[i]));
-            }
-            most = warp_max(most);
-            float by, back;
-            af_row_scale(most, 12, by, back);
-            if (lane == 0) row_factor[r] = back * a.scale * AF_LOG2E;
-            // element e: chunk c = e / 16 is thread t = c % 4's, h = c / 4; step 4 h + (e % 16) / 4; of its four bytes the first two in
-            // the registers of columns 2 t, the others in those of columns 2 t + 8
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const int e = 32 * i + lane, c = e / 16, step = 4 * (c / 4) + e % 16 / 4, of = 4 * (r % 8) + c % 4, reg = (e & 2) + (r % 16 >= 8);
-                const float v = x[i] * by;
-                const __half hi = __float2half_rn(v);
-                uint8_t* const to = qs + (size_t)(r / 16 * Sh::PLANES * Sh::STEPS + step) * 512 + of * 16 + reg * 4 + (e & 1) * 2;
-                *reinterpret_cast<__half*>(to) = hi;
-                if constexpr (F32) *reinterpret_cast<__half*>(to + Sh::STEPS * 512) = __float2half_rn(v - __half2float(hi));
-            }
-        }
-    }
-    __syncthreads();
     // ── this warp's keys ──
-    const int last_row = tile.row0 + tile.n - 1;
-    const int pos_first = tile.len - tile.rows + tile.row0 / group, pos_last = tile.len - tile.rows + last_row / group;  // of the tile's rows
+    const int pos_base = tile.len - tile.rows;
+    const int pos_first = pos_base + tile.row0 / group, pos_last = pos_base + (tile.row0 + tile.n - 1) / group;  // of the tile's rows
     const int held = (int)min((int64_t)tile.len, (int64_t)a.c.max_pages * KV_PAGE);
     const int k_end = min(pos_last + 1, held), k_begin = a.window > 0 ? max(0, pos_first - a.window + 1) : 0;
     const int s_begin = k_begin / AR_KEYS, s_end = k_end > k_begin ? (k_end + AR_KEYS - 1) / AR_KEYS : s_begin;
     const int per = (s_end - s_begin + parts - 1) / parts;
     const int b_begin = min(s_end, s_begin + part * per), b_end = min(s_end, b_begin + per);
-    const int steps = max(0, (b_end - b_begin - warp + AR_WARPS - 1) / AR_WARPS);  // of this warp: b_begin + warp + i AR_WARPS
+    const int steps = max(0, (b_end - b_begin - warp + W - 1) / W);  // of this warp: b_begin + warp + i W
     const int32_t* const table = a.c.page_table + (int64_t)max(0, min(tile.slot, a.c.n_slots - 1)) * a.c.max_pages;
-    uint8_t* const ring = ar_smem + Sh::Q + warp * AR_STAGES * Sh::STAGE;
-    const uint32_t ring_at = smem_addr(ring);
+    uint8_t* const ar_smem = ar_smem_raw + ((1024u - (smem_addr(ar_smem_raw) & 1023u)) & 1023u);
+    uint8_t *const ring = ar_smem + warp * STAGES * Sh::STAGE, *const scale_ring = ar_smem + W * STAGES * Sh::STAGE + warp * STAGES * Sh::SCALES;
+    uint8_t* const qs = ar_smem + (Sh::SMEM - 1024 - Sh::Q);
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(tc5_smem_u32(&full[warp][i])) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    __syncwarp();
     // pages of the warp's steps: a group of 16 steps in the lanes, the next one on its way
     constexpr int GROUP = 32 / AR_PAGES;
     auto look_up = [&](int i0) {
-        const int i = i0 + lane / AR_PAGES, index = (b_begin + warp + i * AR_WARPS) * AR_PAGES + lane % AR_PAGES;
+        const int i = i0 + lane / AR_PAGES, index = (b_begin + warp + i * W) * AR_PAGES + lane % AR_PAGES;
         const int page = i < steps && index < a.c.max_pages && index * KV_PAGE < k_end ? table[index] : -1;
         return page < a.c.n_pages ? page : -1;
     };
     int pages = look_up(0), pages_next = -1;
     uint32_t present = 0;  // a bit for each page of the ring's steps: it is one
-    auto copy_step = [&](int i) {
-        const int stage = i % AR_STAGES;
-        const uint32_t at = ring_at + (uint32_t)(stage * Sh::STAGE);
-#pragma unroll
-        for (int pg = 0; pg < AR_PAGES; ++pg) {
-            const int page = __shfl_sync(0xFFFFFFFFu, pages, i % GROUP * AR_PAGES + pg);
-            const bool there = page >= 0;
-            const uint32_t bit = 1u << (stage * AR_PAGES + pg);
-            present = there ? present | bit : present & ~bit;
-            const int64_t krow = a.c.row(max(page, 0), 0, head), vrow = krow + (int64_t)a.c.n_kv * KV_PAGE;
-            const uint8_t *const k = a.c.values + krow * dim, *const v = a.c.values + vrow * dim;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int h = 0; h < Sh::CHUNKS; ++h) {
-                    const int c = 16 * (t + 4 * h);
-                    const bool in = there && c < dim;
-                    af_copy16(at + (uint32_t)((((pg * 2 + j) * Sh::CHUNKS + h) * 32 + lane) * 16), in ? k + (8 * j + g) * dim + c : k, in);
-                }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int key = 2 * t + (j & 1) + 8 * (j >> 1), c = DP / 8 * g;
-                const bool in = there && c < dim;
-                const uint8_t* const src = in ? v + key * dim + c : v;
-                if constexpr (DP == 128) af_copy16(at + (uint32_t)(Sh::KBYTES + ((pg * 4 + j) * 32 + lane) * 16), src, in);
-                else af_copy8(at + (uint32_t)(Sh::KBYTES + ((pg * 4 + j) * 32 + lane) * 8), src, in);
-            }
-            if (lane / 8 == pg) {  // scales: 64 bytes of the keys, then of the values
-                const int q = lane % 8;
-                af_copy16(at + (uint32_t)(2 * Sh::KBYTES + (q / 4 * AR_KEYS + pg * KV_PAGE + q % 4 * 4) * 4), a.c.scales + (q < 4 ? krow : vrow) + q % 4 * 4, there);
-            }
+    // lanes 0 to 3 copy a page's keys or values each, lanes 4 to 7 their scales
+    const int pg_of = lane / 2 % AR_PAGES, row_of = (lane % 2 * a.c.n_kv + head) * KV_PAGE, page_rows = 2 * a.c.n_kv * KV_PAGE;
+    auto copy_step = [&](int i, int stage) {
+        const int page = __shfl_sync(0xFFFFFFFFu, pages, i % GROUP * AR_PAGES + pg_of);
+        const uint32_t here = __ballot_sync(0xFFFFFFFFu, page >= 0), bits = (here & 1) | (here >> 1 & 2);  // of lanes 0 and 2: the step's pages
+        present = (present & ~(3u << (2 * stage))) | bits << (2 * stage);
+        const uint32_t bar = tc5_smem_u32(&full[warp][stage]);
+        if (lane == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((uint32_t)__popc(bits) * (2u * Sh::PAGE + 2u * KV_PAGE * 4u)) : "memory");
+        __syncwarp();
+        if (page >= 0) {
+            const int row = page * page_rows + row_of;
+            if (lane < 4) tc5_tma_2d(tc5_smem_u32(ring + stage * Sh::STAGE) + lane * Sh::PAGE, &map, 0, row, bar);
+            else if (lane < 8)
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                                 tc5_smem_u32(scale_ring + stage * Sh::SCALES) + (uint32_t)((lane % 2 * AR_KEYS + pg_of * KV_PAGE) * 4)),
+                             "l"(a.c.scales + row), "r"(KV_PAGE * 4), "r"(bar)
+                             : "memory");
         }
     };
-    // ── scores, weights, sums ──
-    float o[R][DP / 8][4], m[R][2], l[R][2], factor[R][2];
-    float ref = 0x1p-100f;     // R of the header: o is the sum times AF_LIFT / ref
-    int limit[R][2], low[R][2];  // a row sees keys low .. limit
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
+    for (int i = 0; i < STAGES - 1; ++i)
+        if (i < steps) copy_step(i, i);
+    // ── queries: operands in the order in which they are used ──
+    for (int r = warp; r < Sh::ROWS; r += W) {
+        const int row = tile.row0 + min(r, tile.n - 1);
+        const T* const src = static_cast<const T*>(a.q) + (int64_t)(tile.first + row / group) * a.ldq + (int64_t)(head * group + row % group) * dim;
+        float x[DP / 32];
+        float most = 0.f;
 #pragma unroll
-        for (int j = 0; j < DP / 8; ++j) o[r][j][0] = o[r][j][1] = o[r][j][2] = o[r][j][3] = 0.f;
+        for (int i = 0; i < DP / 32; ++i) {
+            const int e = 32 * i + lane;
+            x[i] = r < tile.n && e < dim ? to_f32(src[e]) : 0.f;
+            most = fmaxf(most, fabsf(x[i]));
+        }
+        most = warp_max(most);
+        float by, back;
+        af_row_scale(most, 12, by, back);
+        if (lane == 0) row_factor[r] = back * a.scale * AF_LOG2E;
+        // element e: 16 of them (c = e / 16) are thread t's, its chunk h; four make a product's part, the first two in the first register
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+            const int e = 32 * i + lane, c = e / 16, step = 4 * (c % Sh::CHUNKS) + e % 16 / 4, of = 4 * (r % 8) + c / Sh::CHUNKS;
+            const float v = x[i] * by;
+            const __half hi = __float2half_rn(v);
+            uint8_t* const to = qs + (size_t)(r / 8 * Sh::PLANES * Sh::STEPS + step) * 256 + of * 8 + e % 4 * 2;
+            *reinterpret_cast<__half*>(to) = hi;
+            if constexpr (F32) *reinterpret_cast<__half*>(to + Sh::STEPS * 256) = __float2half_rn(v - __half2float(hi));
+        }
+    }
+    __syncthreads();
+    auto query = [&](int n, int p, int step) { return *reinterpret_cast<const uint2*>(qs + ((n * Sh::PLANES + p) * Sh::STEPS + step) * 256 + lane * 8); };
+    uint2 q_held[HELD ? Sh::PLANES : 1][HELD ? Sh::STEPS : 1];
+    if constexpr (HELD) {
+#pragma unroll
+        for (int p = 0; p < Sh::PLANES; ++p)
+#pragma unroll
+            for (int i = 0; i < Sh::STEPS; ++i) q_held[p][i] = query(0, p, i);
+    }
+    // ── scores, weights, sums: of rows 8 n + 2 t and + 1 ──
+    float o[NT][DP / 16][4], m[NT][2], l[NT][2], factor[NT][2];
+    float ref = 0x1p-100f;         // R of the header: o is the sum times AF_LIFT / ref
+    int limit[NT][2], low[NT][2];  // a row sees keys low .. limit
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int row = 16 * r + g + 8 * e, pos = tile.len - tile.rows + (tile.row0 + row) / group;
-            m[r][e] = -INFINITY;
-            l[r][e] = 0.f;
-            limit[r][e] = row < tile.n ? min(pos, held - 1) : -1;
-            low[r][e] = a.window > 0 ? pos - a.window + 1 : 0;
-            factor[r][e] = row_factor[row];
+            const int row = 8 * n + 2 * t + e, pos = pos_base + (tile.row0 + row) / group;
+            m[n][e] = -INFINITY;
+            l[n][e] = 0.f;
+            limit[n][e] = row < tile.n ? min(pos, held - 1) : -1;
+            low[n][e] = a.window > 0 ? pos - a.window + 1 : 0;
+            factor[n][e] = row_factor[row];
         }
     }
     const int whole_from = a.window > 0 ? pos_last - a.window + 1 : 0, whole_to = min(pos_first, held - 1);  // keys that all rows see
+    // MASK: some row does not see some key. Only then can a byte that is NaN belong to a key that a row does not see.
+    auto work = [&](auto with_mask, const uint8_t* at, const float* scales, int key0, uint32_t gone) {
+        constexpr bool MASK = decltype(with_mask)::value;
+        float s[NT][2][4];  // keys 16 pg + g and + 8
 #pragma unroll
-    for (int i = 0; i < AR_STAGES - 1; ++i) {
-        if (i < steps) copy_step(i);
-        cp_async_commit();
-    }
-    for (int i = 0; i < steps; ++i) {
-        const int ahead = i + AR_STAGES - 1, stage = i % AR_STAGES;
-        if (ahead % GROUP == 0) pages = pages_next;
-        if (ahead % GROUP == GROUP / 2) pages_next = look_up(ahead / GROUP * GROUP + GROUP);
-        cp_async_wait<AR_STAGES - 2>();
-        __syncwarp();  // every lane's copies of this step have come, and the stage that the next copies go to has been read
-        const uint32_t gone = ~present >> (stage * AR_PAGES) & ((1u << AR_PAGES) - 1);
-        if (ahead < steps) copy_step(ahead);
-        cp_async_commit();
-        const uint8_t* const at = ring + stage * Sh::STAGE;
-        const int key0 = (b_begin + warp + i * AR_WARPS) * AR_KEYS;
-        float s[R][4][4];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[r][j][0] = s[r][j][1] = s[r][j][2] = s[r][j][3] = 0.f;
+            for (int pg = 0; pg < 2; ++pg) s[n][pg][0] = s[n][pg][1] = s[n][pg][2] = s[n][pg][3] = 0.f;
 #pragma unroll
         for (int h = 0; h < Sh::CHUNKS; ++h)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint4 qv[R][Sh::PLANES];
+            for (int pg = 0; pg < 2; ++pg) {
+                const uint8_t* const from = at + 2 * pg * Sh::PAGE + g * 128 + ((Sh::CHUNKS * t + h) ^ g) * 16;
+                const uint4 k0 = *reinterpret_cast<const uint4*>(from), k1 = *reinterpret_cast<const uint4*>(from + 8 * 128);
+                const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-                for (int r = 0; r < R; ++r)
+                for (int w = 0; w < 4; ++w) {
+                    uint4 k;
+                    af_halves(w0[w], k.x, k.z);
+                    af_halves(w1[w], k.y, k.w);
 #pragma unroll
-                    for (int p = 0; p < Sh::PLANES; ++p)
-                        qv[r][p] = *reinterpret_cast<const uint4*>(qs + ((r * Sh::PLANES + p) * Sh::STEPS + 4 * h + w) * 512 + lane * 16);
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t k = *reinterpret_cast<const uint32_t*>(at + ((j * Sh::CHUNKS + h) * 32 + lane) * 16 + 4 * w);
-                    uint32_t b0, b1;
-                    af_halves(k, b0, b1);
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int p = Sh::PLANES - 1; p >= 0; --p) af_mma(s[r][j], qv[r][p], b0, b1);
+                        for (int p = Sh::PLANES - 1; p >= 0; --p) {
+                            uint2 q;
+                            if constexpr (HELD) q = q_held[p][4 * h + w];
+                            else q = query(n, p, 4 * h + w);
+                            af_mma(s[n][pg], k, q.x, q.y);
+                        }
                 }
             }
-        const float* const scales = reinterpret_cast<const float*>(at + 2 * Sh::KBYTES);
-        float2 ks[4], vs[4];
+        float ks[4], vs[4];  // of keys g + 8 j
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            ks[j] = *reinterpret_cast<const float2*>(scales + 8 * j + 2 * t);
-            vs[j] = *reinterpret_cast<const float2*>(scales + AR_KEYS + 8 * j + 2 * t);
+            ks[j] = scales[8 * j];
+            vs[j] = scales[AR_KEYS + 8 * j];
         }
-        const bool masked = gone != 0 || key0 < whole_from || key0 + AR_KEYS - 1 > whole_to;
         float big = 0.f;  // the largest finite scale of values that a row of the tile may see
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int k = key0 + 8 * j + 2 * t;
-            if (vs[j].x < INFINITY && (!masked || (k >= k_begin && k < k_end))) big = fmaxf(big, vs[j].x);
-            if (vs[j].y < INFINITY && (!masked || (k + 1 >= k_begin && k + 1 < k_end))) big = fmaxf(big, vs[j].y);
-        }
-        float best[R][2];
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                best[r][e] = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float& z = s[r][j][2 * e + c];
-                        z = z * (c ? ks[j].y : ks[j].x) * factor[r][e];
-                        if (masked) {
-                            const int k = key0 + 8 * j + 2 * t + c;
-                            if (k > limit[r][e] || k < low[r][e] || (gone >> (j / 2) & 1)) z = -INFINITY;
-                        }
-                        best[r][e] = fmaxf(best[r][e], z);
-                    }
-            }
-#pragma unroll
-        for (int x = 1; x <= 2; x <<= 1) {
-            big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) best[r][e] = fmaxf(best[r][e], __shfl_xor_sync(0xFFFFFFFFu, best[r][e], x));
+            const int k = key0 + 8 * j + g;
+            if (vs[j] < INFINITY && (!MASK || (k >= k_begin && k < k_end && !(gone >> (j / 2) & 1)))) big = fmaxf(big, vs[j]);
         }
         bool move = big > ref;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) move |= best[r][e] > m[r][e] + AF_LAZY;  // (of -inf: as soon as there is a score)
-        if (__any_sync(0xFFFFFFFFu, move)) {
+            for (int e = 0; e < 2; ++e) {
+                float best = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float& z = s[n][j / 2][2 * (j % 2) + e];
+                    z = z * ks[j] * factor[n][e];
+                    if (MASK) {
+                        const int k = key0 + 8 * j + g;
+                        if (k > limit[n][e] || k < low[n][e] || (gone >> (j / 2) & 1)) z = -INFINITY;
+                    }
+                    best = fmaxf(best, z);
+                }
+                move |= best > m[n][e] + AF_LAZY;  // (of -inf: as soon as there is a score)
+            }
+        if (__any_sync(0xFFFFFFFFu, move)) {  // the rows' largest scores and the largest scale, over the threads that share them
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
             const float up = fmaxf(ref, af_power(big)), shrink = ref / up;  // (powers of two)
             ref = up;
 #pragma unroll
-            for (int r = 0; r < R; ++r)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float to = fmaxf(m[r][e], best[r][e]), by = m[r][e] == to ? 1.f : af_ex2(m[r][e] - to);
-                    m[r][e] = to;
-                    l[r][e] *= by;
+                    float best = fmaxf(fmaxf(s[n][0][e], s[n][0][2 + e]), fmaxf(s[n][1][e], s[n][1][2 + e]));
 #pragma unroll
-                    for (int j = 0; j < DP / 8; ++j) {
-                        o[r][j][2 * e] *= by * shrink;
-                        o[r][j][2 * e + 1] *= by * shrink;
+                    for (int x = 4; x <= 16; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xFFFFFFFFu, best, x));
+                    const float to = fmaxf(m[n][e], best), by = m[n][e] == to ? 1.f : af_ex2(m[n][e] - to);
+                    m[n][e] = to;
+                    l[n][e] *= by;
+#pragma unroll
+                    for (int j = 0; j < DP / 16; ++j) {
+                        o[n][j][e] *= by * shrink;
+                        o[n][j][2 + e] *= by * shrink;
                     }
                 }
         }
         const float lift = AF_LIFT / ref;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int j = 0; j < 4; ++j) vs[j] *= lift;
+        uint2 pb[NT][F32 ? 2 : 1][2];  // weights as the second product's operand, of 16 keys each
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float from = m[r][e] == -INFINITY ? 0.f : m[r][e];
+        for (int n = 0; n < NT; ++n) {
+            const float from0 = m[n][0] == -INFINITY ? 0.f : m[n][0], from1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+            uint32_t hi[4];
+            [[maybe_unused]] uint32_t lo[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float& z = s[r][j][2 * e + c];
-                        const float w = af_ex2(z - from);
-                        l[r][e] += w;
-                        z = masked && z == -INFINITY ? 0.f : w * ((c ? vs[j].y : vs[j].x) * lift);  // (what is masked may have any scale)
-                    }
+            for (int j = 0; j < 4; ++j) {
+                const float z0 = s[n][j / 2][2 * (j % 2)], z1 = s[n][j / 2][2 * (j % 2) + 1];
+                float w0 = af_ex2(z0 - from0), w1 = af_ex2(z1 - from1);
+                l[n][0] += w0;
+                l[n][1] += w1;
+                w0 = MASK && z0 == -INFINITY ? 0.f : w0 * vs[j];  // (what is masked may have any scale)
+                w1 = MASK && z1 == -INFINITY ? 0.f : w1 * vs[j];
+                if constexpr (F32) af_split(w0, w1, hi[j], lo[j]);
+                else hi[j] = af_pack(w0, w1);
             }
 #pragma unroll
-        for (int pg = 0; pg < AR_PAGES; ++pg) {
-            uint4 pa[R][Sh::PLANES];
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const float (&u)[4] = s[r][2 * pg], (&v)[4] = s[r][2 * pg + 1];
-                if constexpr (F32) {
-                    af_split(u[0], u[1], pa[r][0].x, pa[r][1].x);
-                    af_split(u[2], u[3], pa[r][0].y, pa[r][1].y);
-                    af_split(v[0], v[1], pa[r][0].z, pa[r][1].z);
-                    af_split(v[2], v[3], pa[r][0].w, pa[r][1].w);
-                } else {
-                    pa[r][0] = make_uint4(af_pack(u[0], u[1]), af_pack(u[2], u[3]), af_pack(v[0], v[1]), af_pack(v[2], v[3]));
-                }
+            for (int pg = 0; pg < 2; ++pg) {
+                pb[n][0][pg] = make_uint2(af_transpose(hi[2 * pg]), af_transpose(hi[2 * pg + 1]));
+                if constexpr (F32) pb[n][1][pg] = make_uint2(af_transpose(lo[2 * pg]), af_transpose(lo[2 * pg + 1]));
             }
+        }
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) {
             constexpr int WORDS = DP / 32;  // of a thread's part of a token's values
             uint32_t vw[4][WORDS];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint8_t* const from = at + Sh::KBYTES + ((pg * 4 + j) * 32 + lane) * (DP / 8);
+                const int key = 2 * t + (j & 1) + 8 * (j >> 1);
+                const uint8_t* const from = at + (2 * pg + 1) * Sh::PAGE + key * 128 + ((DP / 8 * g / 16) ^ (key & 7)) * 16 + DP / 8 * g % 16;
                 if constexpr (DP == 128) {
                     const uint4 v = *reinterpret_cast<const uint4*>(from);
                     vw[j][0] = v.x; vw[j][1] = v.y; vw[j][2] = v.z; vw[j][3] = v.w;
@@ -312,57 +310,81 @@ __global__ void __launch_bounds__(AR_THREADS) attention_rows_kernel(const Attent
             }
 #pragma unroll
             for (int w = 0; w < WORDS; ++w) {
-                uint32_t b0[4], b1[4];  // of four coordinates: tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
-                af_halves(__byte_perm(vw[0][w], vw[1][w], 0x5140), b0[0], b0[1]);
-                af_halves(__byte_perm(vw[0][w], vw[1][w], 0x7362), b0[2], b0[3]);
-                af_halves(__byte_perm(vw[2][w], vw[3][w], 0x5140), b1[0], b1[1]);
-                af_halves(__byte_perm(vw[2][w], vw[3][w], 0x7362), b1[2], b1[3]);
+                uint4 v[2];  // of two coordinates each: tokens 2 t, 2 t + 1 of the one and the other, tokens 2 t + 8, 2 t + 9
+                af_halves(__byte_perm(vw[0][w], vw[1][w], 0x5140), v[0].x, v[0].y);
+                af_halves(__byte_perm(vw[2][w], vw[3][w], 0x5140), v[0].z, v[0].w);
+                af_halves(__byte_perm(vw[0][w], vw[1][w], 0x7362), v[1].x, v[1].y);
+                af_halves(__byte_perm(vw[2][w], vw[3][w], 0x7362), v[1].z, v[1].w);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    b0[q] = af_finite(b0[q]);
-                    b1[q] = af_finite(b1[q]);
+                for (int q = 0; q < 2; ++q) {
+                    if (MASK) v[q] = make_uint4(af_finite(v[q].x), af_finite(v[q].y), af_finite(v[q].z), af_finite(v[q].w));
 #pragma unroll
-                    for (int r = 0; r < R; ++r)
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int p = Sh::PLANES - 1; p >= 0; --p) af_mma(o[r][4 * w + q], pa[r][p], b0[q], b1[q]);
+                        for (int p = F32 ? 1 : 0; p >= 0; --p) af_mma(o[n][2 * w + q], v[q], pb[n][p][pg].x, pb[n][p][pg].y);
                 }
             }
         }
+    };
+    bool ok = true;
+    uint32_t parity = 0;
+    for (int i = 0, stage = 0; i < steps; ++i) {
+        const int ahead = i + STAGES - 1;
+        if (ahead % GROUP == 0) pages = pages_next;
+        if (ahead % GROUP == GROUP / 2) pages_next = look_up(ahead / GROUP * GROUP + GROUP);
+        __syncwarp();  // the stage that the next copies go to has been read
+        if (ahead < steps) copy_step(ahead, stage == 0 ? STAGES - 1 : stage - 1);
+        ok = __all_sync(0xFFFFFFFFu, tc5_wait(&full[warp][stage], parity));
+        if (!ok) break;
+        const uint32_t gone = ~present >> (stage * AR_PAGES) & ((1u << AR_PAGES) - 1);
+        const uint8_t* const at = ring + stage * Sh::STAGE;
+        const float* const scales = reinterpret_cast<const float*>(scale_ring + stage * Sh::SCALES) + g;
+        const int key0 = (b_begin + warp + i * W) * AR_KEYS;
+        if (gone != 0 || key0 < whole_from || key0 + AR_KEYS - 1 > whole_to) work(std::true_type{}, at, scales, key0, gone);
+        else work(std::false_type{}, at, scales, key0, 0u);
+        if (++stage == STAGES) {
+            stage = 0;
+            parity ^= 1;
+        }
     }
-    cp_async_wait<0>();
+    if (!ok && lane == 0) {  // copies on their way to this block are waited for, for as long again
+        report_wait(a.waits, WAIT_ATTENTION);
+        for (int i = 0; i < STAGES; ++i) tc5_wait(&full[warp][i], parity);
+    }
+    __syncwarp();
     // ── the warps' sums into one, then the blocks' ──
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            l[r][e] += __shfl_xor_sync(0xFFFFFFFFu, l[r][e], 1);
-            l[r][e] += __shfl_xor_sync(0xFFFFFFFFu, l[r][e], 2);
-            if (t == 0) {
-                warp_m[warp][16 * r + g + 8 * e] = m[r][e];
-                warp_l[warp][16 * r + g + 8 * e] = l[r][e];
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) l[n][e] += __shfl_xor_sync(0xFFFFFFFFu, l[n][e], x);
+            if (g == 0) {
+                warp_m[warp][8 * n + 2 * t + e] = m[n][e];
+                warp_l[warp][8 * n + 2 * t + e] = l[n][e];
             }
         }
     __syncthreads();  // the rings have been read
-    float* const sums = reinterpret_cast<float*>(ar_smem + Sh::Q);  // [warp][row][LDO]
+    float* const sums = reinterpret_cast<float*>(ar_smem);  // [warp][row][LDO]
     const float back = ref * (1.f / AF_LIFT);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < DP / 8; ++j)
+        for (int j = 0; j < DP / 16; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)  // column c of product j is coordinate DP / 8 c + j
-                sums[(warp * Sh::ROWS + 16 * r + g + 8 * (q / 2)) * Sh::LDO + DP / 8 * (2 * t + q % 2) + j] = o[r][j][q] * back;
+            for (int e = 0; e < 2; ++e)  // coordinates DP / 8 g + 2 j and + 1
+                *reinterpret_cast<float2*>(&sums[(warp * Sh::ROWS + 8 * n + 2 * t + e) * Sh::LDO + DP / 8 * g + 2 * j]) = make_float2(o[n][j][e] * back, o[n][j][2 + e] * back);
     __syncthreads();
     auto store = [&](int row, int col, float y) {
         const int at = tile.row0 + row;
         static_cast<T*>(a.out)[(int64_t)(tile.first + at / group) * a.ldo + (int64_t)(head * group + at % group) * dim + col] = from_f32<T>(y);
     };
-    for (int row = warp; row < tile.n; row += AR_WARPS) {
-        float top = -INFINITY, total = 0.f, w[AR_WARPS], y[DP / 32];
+    for (int row = warp; row < tile.n; row += W) {
+        float top = -INFINITY, total = 0.f, w[W], y[DP / 32];
 #pragma unroll
-        for (int i = 0; i < AR_WARPS; ++i) top = fmaxf(top, warp_m[i][row]);
+        for (int i = 0; i < W; ++i) top = fmaxf(top, warp_m[i][row]);
 #pragma unroll
-        for (int i = 0; i < AR_WARPS; ++i) {
+        for (int i = 0; i < W; ++i) {
             w[i] = warp_m[i][row] == -INFINITY ? 0.f : af_ex2(warp_m[i][row] - top);
             total += warp_l[i][row] * w[i];
         }
@@ -370,7 +392,7 @@ __global__ void __launch_bounds__(AR_THREADS) attention_rows_kernel(const Attent
         for (int c = 0; c < DP / 32; ++c) {
             y[c] = 0.f;
 #pragma unroll
-            for (int i = 0; i < AR_WARPS; ++i) y[c] = fmaf(sums[(i * Sh::ROWS + row) * Sh::LDO + 32 * c + lane], w[i], y[c]);
+            for (int i = 0; i < W; ++i) y[c] = fmaf(sums[(i * Sh::ROWS + row) * Sh::LDO + 32 * c + lane], w[i], y[c]);
         }
         if (parts == 1) {
             const float by = total == 0.f ? 0.f : 1.f / total;
@@ -388,7 +410,7 @@ __global__ void __launch_bounds__(AR_THREADS) attention_rows_kernel(const Attent
     }
     if (parts == 1) return;
     cluster_sync();
-    for (int row = part + parts * warp; row < tile.n; row += parts * AR_WARPS) {  // the cluster's warps share the rows out
+    for (int row = part + parts * warp; row < tile.n; row += parts * W) {  // the cluster's warps share the rows out
         // lane i looks at part i
         const float pm = lane < parts ? ld_peer(peer_smem(smem_addr(&part_m[row]), lane)) : -INFINITY;
         const float pl = lane < parts ? ld_peer(peer_smem(smem_addr(&part_l[row]), lane)) : 0.f;
@@ -408,31 +430,91 @@ __global__ void __launch_bounds__(AR_THREADS) attention_rows_kernel(const Attent
     cluster_sync();  // nobody leaves while its parts are being read
 }
 
-template <typename T, int DP, int R>
+// The pool's rows, 16 of them (a page's keys or values of a head) a copy, filled up to 128 bytes with zeros, 128-byte swizzle.
+cudaError_t af_page_map(const CacheFp8& c, CUtensorMap* map) {
+    const PFN_encodeTiled encode = tensor_map_encoder();
+    if (!encode) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)c.dim, (cuuint64_t)c.n_pages * 2 * c.n_kv * KV_PAGE}, strides[1] = {(cuuint64_t)c.dim};
+    const cuuint32_t box[2] = {128, KV_PAGE}, each[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.values, dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+// Blocks of a cluster for `clusters` of them, each with `steps` equal pieces of work: as many as shorten the longest wave. What fits on
+// the GPU at once depends on where its SMs are: of 148, clusters of 16 blocks that fill an SM hold 112, of 10 or of 8 110 and 120.
+struct ClusterSizes {
+    int fit[AR_MAX_PARTS + 1];  // clusters of that many blocks at once
+};
+int af_parts(const ClusterSizes& c, int most, int64_t clusters, double steps, double fixed) {
+    int best = 1;
+    double least = 1e30;
+    for (int p = 1; p <= most; ++p) {
+        if (c.fit[p] < 1) continue;
+        const double waves = (double)((clusters + c.fit[p] - 1) / c.fit[p]), time = waves * (std::ceil(steps / p) + fixed) + (p > 1 ? fixed : 0.);
+        if (time < least * 0.999) {
+            least = time;
+            best = p;
+        }
+    }
+    return best;
+}
+cudaError_t af_sizes(const void* kernel, int threads, int smem, int most, ClusterSizes* out) {
+    for (int p = 0; p <= AR_MAX_PARTS; ++p) out->fit[p] = 0;
+    for (int p = 1; p <= most; ++p) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(1, 1, (unsigned)(64 * p));
+        cfg.blockDim = dim3((unsigned)threads);
+        cfg.dynamicSmemBytes = (size_t)smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = (unsigned)p;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&out->fit[p], kernel, &cfg);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+template <typename T, int DP, int NT, int W>
 static cudaError_t launch_rows(const AttentionFp8Args& a, cudaStream_t st) {
-    using Sh = ArShape<T, DP, R>;
+    using Sh = ArShape<T, DP, NT, W>;
     static PerDeviceOnce once;
-    cudaError_t e = once.run([] {
-        const cudaError_t f = cudaFuncSetAttribute(attention_rows_kernel<T, DP, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
-        return f != cudaSuccess ? f : cudaFuncSetAttribute(attention_rows_kernel<T, DP, R>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);  // (more than eight blocks)
+    static ClusterSizes sizes[SP_MAX_DEVICES];
+    const auto kernel = attention_rows_kernel<T, DP, NT, W>;
+    ClusterSizes& fits = sizes[current_device_index()];
+    cudaError_t e = once.run([&] {
+        cudaError_t f = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
+        if (f == cudaSuccess) f = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);  // (more than eight blocks)
+        ClusterSizes found;
+        if (f == cudaSuccess) f = af_sizes(reinterpret_cast<const void*>(kernel), 32 * W, Sh::SMEM, AR_MAX_PARTS, &found);
+        if (f == cudaSuccess) fits = found;
+        return f;
     });
     if (e != cudaSuccess) return e;
+    CUtensorMap map{};
+    if ((e = af_page_map(a.c, &map)) != cudaSuccess) return e;
     const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv), tiles = (rows + Sh::ROWS - 1) / Sh::ROWS, clusters = tiles * a.c.n_kv * a.n_seqs;
-    // two blocks an SM, each with 256 keys at least
-    int parts = 1;
-    while (parts < AR_MAX_PARTS && clusters * parts * 2 <= 2 * device_sm_count() && (int64_t)a.max_len >= 256 * 2 * parts) parts *= 2;
-    e = launch_pdl_cluster(attention_rows_kernel<T, DP, R>, dim3((unsigned)(tiles * a.c.n_kv), (unsigned)a.n_seqs, (unsigned)parts), dim3(AR_THREADS), Sh::SMEM, st, parts, a, parts);
+    const int len = a.window > 0 ? (int)std::min<int64_t>(a.max_len, (int64_t)a.window + a.max_rows) : a.max_len;
+    int parts = af_parts(fits, AR_MAX_PARTS, clusters, (double)len / (AR_KEYS * W), AR_FIXED);
+    if (getenv("AR_PARTS")) parts = env("AR_PARTS", 1);
+    e = launch_pdl_cluster(kernel, dim3((unsigned)(tiles * a.c.n_kv), (unsigned)a.n_seqs, (unsigned)parts), dim3(32 * W), Sh::SMEM, st, parts, a, parts, map);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
+template <typename T, int W>
+static cudaError_t rows_as(const AttentionFp8Args& a, int64_t rows, cudaStream_t st) {
+    if (a.c.dim <= 64) return rows <= 8 ? launch_rows<T, 64, 1, W>(a, st) : rows <= 16 ? launch_rows<T, 64, 2, W>(a, st) : launch_rows<T, 64, 4, 4>(a, st);
+    return rows <= 8 ? launch_rows<T, 128, 1, W>(a, st) : rows <= 16 ? launch_rows<T, 128, 2, W>(a, st) : launch_rows<T, 128, 4, 4>(a, st);
+}
 template <typename T>
 static cudaError_t attention_as(const AttentionFp8Args& a, cudaStream_t st) {
     const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv);
-    const bool tiles = (int64_t)a.c.n_pages * 2 * a.c.n_kv * KV_PAGE <= INT32_MAX;  // (a copy's row is counted in 32 bits)
-    if (rows > 32 && tiles) return launch_attention_fp8_tiles(a, sizeof(T) == 2, st);
-    const bool few = rows <= 16;
-    if (a.c.dim <= 64) return few ? launch_rows<T, 64, 1>(a, st) : launch_rows<T, 64, 2>(a, st);
-    return few ? launch_rows<T, 128, 1>(a, st) : launch_rows<T, 128, 2>(a, st);
+    if (rows > env("AR_ROWS", 32)) return launch_attention_fp8_tiles(a, sizeof(T) == 2, st);
+    return AR_WIDE(a.c.n_kv * (int64_t)a.n_seqs) ? rows_as<T, 8>(a, rows, st) : rows_as<T, 4>(a, rows, st);
 }
 cudaError_t launch_attention_fp8(const AttentionFp8Args& a, bool bf, cudaStream_t st) { return bf ? attention_as<bf16>(a, st) : attention_as<float>(a, st); }
 

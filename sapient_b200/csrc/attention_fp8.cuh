@@ -1,5 +1,6 @@
 // What the kernels of attention over a cache of 8-bit rows share (attention_fp8.cu, attention_fp8_tile.cu).
 #pragma once
+#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include "cache_fp8.h"
@@ -44,12 +45,6 @@ __device__ __forceinline__ void af_mma(float (&c)[4], const uint4& a, uint32_t b
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void af_copy16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void af_copy8(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
-}
 // A power of two by which a row is multiplied so that its largest value lies in [2^to, 2^(to + 1)), and its reciprocal. Rows of zeros and
 // those with infinities or NaN: 1.
 __device__ __forceinline__ void af_row_scale(float most, int to, float& by, float& back) {
@@ -63,6 +58,8 @@ __device__ __forceinline__ float af_power(float s) {
     const uint32_t u = (__float_as_uint(s) + 0x7FFFFFu) & 0x7F800000u;
     return __uint_as_float(min(max(u, 1u << 23), 253u << 23));
 }
+
+cudaError_t af_page_map(const CacheFp8& c, CUtensorMap* map);  // attention_fp8.cu
 
 // What a block works on: rows of one key head of one sequence.
 struct AfTile {

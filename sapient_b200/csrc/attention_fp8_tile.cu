@@ -824,15 +824,7 @@ static cudaError_t launch_tiles(const AttentionFp8Args& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv), height = 128 * Sh::TILES, tiles = (rows + height - 1) / height, clusters = tiles * a.c.n_kv * a.n_seqs;
     CUtensorMap map{};
-    if (!Sh::F32) {  // rows of the pool, 16 of them (a page's keys of a head) a copy, filled up to 128 bytes with zeros
-        const PFN_encodeTiled encode = tensor_map_encoder();
-        if (!encode) return cudaErrorNotSupported;
-        const cuuint64_t dims[2] = {(cuuint64_t)a.c.dim, (cuuint64_t)a.c.n_pages * 2 * a.c.n_kv * KV_PAGE}, strides[1] = {(cuuint64_t)a.c.dim};
-        const cuuint32_t box[2] = {128, KV_PAGE}, each[2] = {1, 1};
-        if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a.c.values, dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return cudaErrorInvalidValue;
-    }
+    if (!Sh::F32 && (e = af_page_map(a.c, &map)) != cudaSuccess) return e;
     // an SM a block, each with four tiles of keys at least
     int parts = 1;
     while (parts < AT_MAX_PARTS && clusters * parts * 2 <= device_sm_count() && (int64_t)a.max_len >= 4 * AT_KEYS * 2 * parts) parts *= 2;
