@@ -15,7 +15,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <type_traits>
 
 #include "attention_fp8.cuh"
@@ -37,17 +36,14 @@ cudaError_t count_launch_and_check();  // kernels.cu
 // swizzle lets eight threads' reads fall on 32 different banks; copied by threads, 16 bytes each, every one was a request of its own to L2:
 // 131072 keys of the 8B shape 106 us, now XXX.
 // Keys are shared out to the warps of a block and the blocks of a cluster, which add up their parts through shared memory: no workspace.
-constexpr int AR_KEYS = 32, AR_PAGES = AR_KEYS / KV_PAGE, AR_MAX_PARTS = 16;
-static int env(const char*n,int d){const char*e=getenv(n);return e?atoi(e):d;}
-#define AR_FIXED env("AR_FIXED",2)
-#define AR_WIDE(c) ((c) <= env("AR_WIDE",64))
+constexpr int AR_KEYS = 32, AR_PAGES = AR_KEYS / KV_PAGE;
 
 
 template <typename T, int DP, int NT, int W>
 struct ArShape {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int PLANES = F32 ? 2 : 1, STEPS = DP / 16, CHUNKS = DP / 64;       // of q: products of 16 columns
-    static constexpr int STAGES = W == 4 ? 2 : 3;
+    static constexpr int STAGES = 2;
     static constexpr int PAGE = KV_PAGE * 128, STAGE = 2 * AR_PAGES * PAGE, SCALES = 2 * AR_KEYS * 4;  // [page][keys, values], their scales
     static constexpr int Q = NT * PLANES * STEPS * 256, RING = W * STAGES * (STAGE + SCALES);
     static constexpr int ROWS = 8 * NT, LDO = DP + 4;
@@ -62,7 +58,7 @@ __device__ __forceinline__ uint32_t af_transpose(uint32_t v) {  // of an 8 x 8 m
 }
 
 template <typename T, int DP, int NT, int W>
-__global__ void __launch_bounds__(32 * W, NT > 2 ? 1 : W == 4 ? 3 : 1) attention_rows_kernel(const AttentionFp8Args a, int parts, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(const AttentionFp8Args a, int parts, const __grid_constant__ CUtensorMap map) {
     using Sh = ArShape<T, DP, NT, W>;
     constexpr bool F32 = Sh::F32, HELD = NT == 1;  // q stays in registers
     constexpr int STAGES = Sh::STAGES;
@@ -442,27 +438,11 @@ cudaError_t af_page_map(const CacheFp8& c, CUtensorMap* map) {
                : cudaErrorInvalidValue;
 }
 
-// Blocks of a cluster for `clusters` of them, each with `steps` equal pieces of work: as many as shorten the longest wave. What fits on
-// the GPU at once depends on where its SMs are: of 148, clusters of 16 blocks that fill an SM hold 112, of 10 or of 8 110 and 120.
-struct ClusterSizes {
-    int fit[AR_MAX_PARTS + 1];  // clusters of that many blocks at once
-};
-int af_parts(const ClusterSizes& c, int most, int64_t clusters, double steps, double fixed) {
-    int best = 1;
-    double least = 1e30;
-    for (int p = 1; p <= most; ++p) {
-        if (c.fit[p] < 1) continue;
-        const double waves = (double)((clusters + c.fit[p] - 1) / c.fit[p]), time = waves * (std::ceil(steps / p) + fixed) + (p > 1 ? fixed : 0.);
-        if (time < least * 0.999) {
-            least = time;
-            best = p;
-        }
-    }
-    return best;
-}
-cudaError_t af_sizes(const void* kernel, int threads, int smem, int most, ClusterSizes* out) {
-    for (int p = 0; p <= AR_MAX_PARTS; ++p) out->fit[p] = 0;
-    for (int p = 1; p <= most; ++p) {
+cudaError_t af_fits(const void* kernel, int threads, int smem, ClusterFits* out) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);  // (more than eight blocks)
+    ClusterFits found{};
+    for (int p = 1; p <= AF_MAX_PARTS && e == cudaSuccess; ++p) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(1, 1, (unsigned)(64 * p));
         cfg.blockDim = dim3((unsigned)threads);
@@ -473,48 +453,64 @@ cudaError_t af_sizes(const void* kernel, int threads, int smem, int most, Cluste
         at[0].val.clusterDim.z = (unsigned)p;
         cfg.attrs = at;
         cfg.numAttrs = 1;
-        const cudaError_t e = cudaOccupancyMaxActiveClusters(&out->fit[p], kernel, &cfg);
-        if (e != cudaSuccess) return e;
+        e = cudaOccupancyMaxActiveClusters(&found.at_once[p], kernel, &cfg);
     }
-    return cudaSuccess;
+    if (e == cudaSuccess) *out = found;
+    return e;
 }
 
+AfShare af_share(const ClusterFits& fits, int64_t clusters, int64_t pieces, double piece, double fixed, double joined) {
+    AfShare best{1, 1e30};
+    for (int p = 1; p <= AF_MAX_PARTS; ++p) {
+        if (fits.at_once[p] < 1) continue;
+        const double rounds = (double)clusters / fits.at_once[p], waves = rounds <= 1. ? 1. : (rounds + std::ceil(rounds)) / 2;
+        const double time = waves * ((double)((pieces + p - 1) / p) * piece + fixed + (p > 1 ? joined : 0.));
+        if (time < best.time) best = AfShare{p, time};
+    }
+    return best;
+}
+
+// Microseconds of a warp's step with twelve warps on an SM, and of a block's start and end (measured: 131072 keys of the 8B shape in one to
+// 16 parts, 518 keys); with cluster_sync.
+constexpr double AR_STEP = 1.4, AR_FIXED = 4., AR_JOINED = 0.5;
+
 template <typename T, int DP, int NT, int W>
-static cudaError_t launch_rows(const AttentionFp8Args& a, cudaStream_t st) {
+struct RowsLaunch {
     using Sh = ArShape<T, DP, NT, W>;
-    static PerDeviceOnce once;
-    static ClusterSizes sizes[SP_MAX_DEVICES];
-    const auto kernel = attention_rows_kernel<T, DP, NT, W>;
-    ClusterSizes& fits = sizes[current_device_index()];
-    cudaError_t e = once.run([&] {
-        cudaError_t f = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
-        if (f == cudaSuccess) f = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);  // (more than eight blocks)
-        ClusterSizes found;
-        if (f == cudaSuccess) f = af_sizes(reinterpret_cast<const void*>(kernel), 32 * W, Sh::SMEM, AR_MAX_PARTS, &found);
-        if (f == cudaSuccess) fits = found;
-        return f;
-    });
-    if (e != cudaSuccess) return e;
+    static constexpr auto kernel = attention_rows_kernel<T, DP, NT, W>;
+    static cudaError_t share(const AttentionFp8Args& a, int64_t clusters, int64_t len, AfShare* out) {
+        static PerDeviceOnce once;
+        static ClusterFits fits[SP_MAX_DEVICES];
+        ClusterFits& mine = fits[current_device_index()];
+        const cudaError_t e = once.run([&] { return af_fits(reinterpret_cast<const void*>(kernel), 32 * W, Sh::SMEM, &mine); });
+        if (e == cudaSuccess) *out = af_share(mine, clusters, (len + AR_KEYS * W - 1) / (AR_KEYS * W), AR_STEP, AR_FIXED, AR_JOINED);
+        return e;
+    }
+    static cudaError_t go(const AttentionFp8Args& a, const CUtensorMap& map, int parts, cudaStream_t st) {
+        return launch_pdl_cluster(kernel, dim3((unsigned)a.c.n_kv, (unsigned)a.n_seqs, (unsigned)parts), dim3(32 * W), Sh::SMEM, st, parts, a, parts, map);
+    }
+};
+
+// Blocks of 12 warps fill an SM; of four, three share one: many short sequences (1000 of up to 90 keys: XXX).
+template <typename T, int DP, int NT>
+static cudaError_t launch_rows(const AttentionFp8Args& a, cudaStream_t st) {
+    const int64_t clusters = (int64_t)a.c.n_kv * a.n_seqs, len = af_keys(a);
+    AfShare wide, narrow;
     CUtensorMap map{};
-    if ((e = af_page_map(a.c, &map)) != cudaSuccess) return e;
-    const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv), tiles = (rows + Sh::ROWS - 1) / Sh::ROWS, clusters = tiles * a.c.n_kv * a.n_seqs;
-    const int len = a.window > 0 ? (int)std::min<int64_t>(a.max_len, (int64_t)a.window + a.max_rows) : a.max_len;
-    int parts = af_parts(fits, AR_MAX_PARTS, clusters, (double)len / (AR_KEYS * W), AR_FIXED);
-    if (getenv("AR_PARTS")) parts = env("AR_PARTS", 1);
-    e = launch_pdl_cluster(kernel, dim3((unsigned)(tiles * a.c.n_kv), (unsigned)a.n_seqs, (unsigned)parts), dim3(32 * W), Sh::SMEM, st, parts, a, parts, map);
+    cudaError_t e = RowsLaunch<T, DP, NT, 12>::share(a, clusters, len, &wide);
+    if (e == cudaSuccess) e = RowsLaunch<T, DP, NT, 4>::share(a, clusters, len, &narrow);
+    if (e == cudaSuccess) e = af_page_map(a.c, &map);
+    if (e == cudaSuccess)
+        e = wide.time <= narrow.time ? RowsLaunch<T, DP, NT, 12>::go(a, map, wide.parts, st) : RowsLaunch<T, DP, NT, 4>::go(a, map, narrow.parts, st);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
-template <typename T, int W>
-static cudaError_t rows_as(const AttentionFp8Args& a, int64_t rows, cudaStream_t st) {
-    if (a.c.dim <= 64) return rows <= 8 ? launch_rows<T, 64, 1, W>(a, st) : rows <= 16 ? launch_rows<T, 64, 2, W>(a, st) : launch_rows<T, 64, 4, 4>(a, st);
-    return rows <= 8 ? launch_rows<T, 128, 1, W>(a, st) : rows <= 16 ? launch_rows<T, 128, 2, W>(a, st) : launch_rows<T, 128, 4, 4>(a, st);
-}
 template <typename T>
 static cudaError_t attention_as(const AttentionFp8Args& a, cudaStream_t st) {
     const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv);
-    if (rows > env("AR_ROWS", 32)) return launch_attention_fp8_tiles(a, sizeof(T) == 2, st);
-    return AR_WIDE(a.c.n_kv * (int64_t)a.n_seqs) ? rows_as<T, 8>(a, rows, st) : rows_as<T, 4>(a, rows, st);
+    if (rows > 16) return launch_attention_fp8_tiles(a, sizeof(T) == 2, st);
+    if (a.c.dim <= 64) return rows <= 8 ? launch_rows<T, 64, 1>(a, st) : launch_rows<T, 64, 2>(a, st);
+    return rows <= 8 ? launch_rows<T, 128, 1>(a, st) : launch_rows<T, 128, 2>(a, st);
 }
 cudaError_t launch_attention_fp8(const AttentionFp8Args& a, bool bf, cudaStream_t st) { return bf ? attention_as<bf16>(a, st) : attention_as<float>(a, st); }
 

@@ -3,6 +3,8 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "cache_fp8.h"
 #include "plan_common.cuh"
 
@@ -59,7 +61,24 @@ __device__ __forceinline__ float af_power(float s) {
     return __uint_as_float(min(max(u, 1u << 23), 253u << 23));
 }
 
-cudaError_t af_page_map(const CacheFp8& c, CUtensorMap* map);  // attention_fp8.cu
+// ── attention_fp8.cu ──
+cudaError_t af_page_map(const CacheFp8& c, CUtensorMap* map);
+// How keys are shared out to the blocks of a cluster. What fits on the GPU at once depends on where its SMs are: of 148, clusters of 16 blocks that
+// fill an SM each hold 112, of 10 or 8 110 and 120, of 6 132; eight clusters of 16 are two rounds.
+constexpr int AF_MAX_PARTS = 16;
+struct ClusterFits {
+    int at_once[AF_MAX_PARTS + 1];  // clusters of that many blocks
+};
+cudaError_t af_fits(const void* kernel, int threads, int smem, ClusterFits* out);  // and the kernel's attributes for it
+struct AfShare {
+    int parts;
+    double time;  // us
+};
+// The number of parts for which `clusters` of them take least, a block for `piece` of each of its share of `pieces`, and `fixed` and `joined` (where
+// there are parts to add up) besides. Rounds that do not fill the GPU count half: blocks are of unequal length.
+AfShare af_share(const ClusterFits& fits, int64_t clusters, int64_t pieces, double piece, double fixed, double joined);
+// Keys that a row can see, of the longest sequence.
+inline int64_t af_keys(const AttentionFp8Args& a) { return a.window > 0 ? std::min<int64_t>(a.max_len, (int64_t)a.window + a.max_rows) : a.max_len; }
 
 // What a block works on: rows of one key head of one sequence.
 struct AfTile {

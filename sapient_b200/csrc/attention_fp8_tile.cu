@@ -31,7 +31,7 @@ namespace sp {
 
 cudaError_t count_launch_and_check();  // kernels.cu
 
-constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 512, AT_RING = 8, AT_MAX_PARTS = 8;
+constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 512, AT_RING = 8;
 constexpr float AT_MOST = 15.f, AT_SET = 9.f;  // log2 of the largest weight, and of it when M is set
 constexpr int AT_UP = 7, AT_LEAST = -80;       // values times 2^7 are below 2^16; smaller u would let a sum of 2^(z - M) pass 2^127
 
@@ -43,7 +43,7 @@ struct AtShape {
     static constexpr int TILE = 128 * DP * 2, K_TILE = F32 ? TILE : 128 * 128;  // bytes of 128 rows in fp16; of keys and of a plane of Q
     static constexpr int Q = PLANES * TILES * K_TILE, SMEM = Q + K_STAGES * K_TILE + V_STAGES * TILE + 1024;
     static constexpr int LDO = DP + 4, SUMS = 2 * 128 * LDO * 4;                // takes the operands' place
-    static constexpr int WEIGHTS = KEYS ? 128 * 2 * 4 : 256 * 4;                // of the sums of a block's share of rows, behind them (parts x rows of a share is at most that)
+    static constexpr int WEIGHTS = (128 * TILES + AF_MAX_PARTS) * (KEYS ? 2 : 1) * 4;  // of the sums of a block's share of rows, behind them
     static_assert(SUMS + WEIGHTS <= SMEM - 1024, "sums of both groups");
 };
 
@@ -816,20 +816,23 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
 }
 
+// Microseconds of a tile of keys (of two groups' rows, or one), of a block's start and end, of adding parts up: 8B shape, 512 rows at 8704, 128 at 32768.
+constexpr double AT_PIECE = 2.2, AT_PIECE_KEYS = 1.3, AT_FIXED = 9., AT_JOINED = 5.;
+
 template <typename T, int DP, bool KEYS>
 static cudaError_t launch_tiles(const AttentionFp8Args& a, cudaStream_t st) {
     using Sh = AtShape<T, DP, KEYS>;
     static PerDeviceOnce once;
-    cudaError_t e = once.run([] { return cudaFuncSetAttribute(attention_tile_kernel<T, DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM); });
+    static ClusterFits fits[SP_MAX_DEVICES];
+    const auto kernel = attention_tile_kernel<T, DP, KEYS>;
+    ClusterFits& mine = fits[current_device_index()];
+    cudaError_t e = once.run([&] { return af_fits(reinterpret_cast<const void*>(kernel), AT_THREADS, Sh::SMEM, &mine); });
     if (e != cudaSuccess) return e;
-    const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv), height = 128 * Sh::TILES, tiles = (rows + height - 1) / height, clusters = tiles * a.c.n_kv * a.n_seqs;
     CUtensorMap map{};
     if (!Sh::F32 && (e = af_page_map(a.c, &map)) != cudaSuccess) return e;
-    // an SM a block, each with four tiles of keys at least
-    int parts = 1;
-    while (parts < AT_MAX_PARTS && clusters * parts * 2 <= device_sm_count() && (int64_t)a.max_len >= 4 * AT_KEYS * 2 * parts) parts *= 2;
-    e = launch_pdl_cluster(attention_tile_kernel<T, DP, KEYS>, dim3((unsigned)(tiles * a.c.n_kv), (unsigned)a.n_seqs, (unsigned)parts), dim3(AT_THREADS), Sh::SMEM, st, parts, a,
-                           parts, (int)tiles, map);
+    const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv), height = 128 * Sh::TILES, tiles = (rows + height - 1) / height, clusters = tiles * a.c.n_kv * a.n_seqs;
+    const int parts = af_share(mine, clusters, (af_keys(a) + AT_KEYS - 1) / AT_KEYS, KEYS ? AT_PIECE_KEYS : AT_PIECE, AT_FIXED, AT_JOINED).parts;
+    e = launch_pdl_cluster(kernel, dim3((unsigned)(tiles * a.c.n_kv), (unsigned)a.n_seqs, (unsigned)parts), dim3(AT_THREADS), Sh::SMEM, st, parts, a, parts, (int)tiles, map);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
