@@ -36,7 +36,7 @@ cudaError_t count_launch_and_check();  // kernels.cu
 // swizzle lets eight threads' reads fall on 32 different banks; copied by threads, 16 bytes each, every one was a request of its own to L2:
 // 131072 keys of the 8B shape 106 us, now XXX.
 // Keys are shared out to the warps of a block and the blocks of a cluster, which add up their parts through shared memory: no workspace.
-constexpr int AR_KEYS = 32, AR_PAGES = AR_KEYS / KV_PAGE;
+constexpr int AR_KEYS = 32, AR_PAGES = AR_KEYS / KV_PAGE, AR_FLUSH = 8;
 
 
 template <typename T, int DP, int NT, int W>
@@ -60,7 +60,7 @@ __device__ __forceinline__ uint32_t af_transpose(uint32_t v) {  // of an 8 x 8 m
 template <typename T, int DP, int NT, int W>
 __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(const AttentionFp8Args a, int parts, const __grid_constant__ CUtensorMap map) {
     using Sh = ArShape<T, DP, NT, W>;
-    constexpr bool F32 = Sh::F32, HELD = NT == 1;  // q stays in registers
+    constexpr bool F32 = Sh::F32, HELD = NT == 1 && !F32;  // q stays in registers
     constexpr int STAGES = Sh::STAGES;
     extern __shared__ uint8_t ar_smem_raw[];
     __shared__ __align__(8) uint64_t full[W][STAGES];
@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
     }
     // ── scores, weights, sums: of rows 8 n + 2 t and + 1 ──
     float o[NT][DP / 16][4], m[NT][2], l[NT][2], factor[NT][2];
+    float o_sum[F32 ? NT : 1][F32 ? DP / 16 : 1][4] = {};  // f32: what o has been added to
     float ref = 0x1p-100f;         // R of the header: o is the sum times AF_LIFT / ref
     int limit[NT][2], low[NT][2];  // a row sees keys low .. limit
 #pragma unroll
@@ -183,10 +184,16 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
     auto work = [&](auto with_mask, const uint8_t* at, const float* scales, int key0, uint32_t gone) {
         constexpr bool MASK = decltype(with_mask)::value;
         float s[NT][2][4];  // keys 16 pg + g and + 8
+        // The tensor cores cut off what falls below an accumulator's last bits, always towards zero. f32 rows therefore have three short sums, of the
+        // remainders and of each 64 columns, instead of one (518 keys: 1.3e-6 off in all, 3.8e-7 so), and o is added up apart every AR_FLUSH steps.
+        constexpr int SUMS = F32 ? 1 + Sh::CHUNKS : 1;
+        float sums[SUMS][NT][2][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int c = 0; c < SUMS; ++c)
 #pragma unroll
-            for (int pg = 0; pg < 2; ++pg) s[n][pg][0] = s[n][pg][1] = s[n][pg][2] = s[n][pg][3] = 0.f;
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int pg = 0; pg < 2; ++pg) sums[c][n][pg][0] = sums[c][n][pg][1] = sums[c][n][pg][2] = sums[c][n][pg][3] = 0.f;
 #pragma unroll
         for (int h = 0; h < Sh::CHUNKS; ++h)
 #pragma unroll
@@ -206,10 +213,20 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
                             uint2 q;
                             if constexpr (HELD) q = q_held[p][4 * h + w];
                             else q = query(n, p, 4 * h + w);
-                            af_mma(s[n][pg], k, q.x, q.y);
+                            af_mma(sums[!F32 || p == 1 ? 0 : 1 + h][n][pg], k, q.x, q.y);
                         }
                 }
             }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if constexpr (!F32) s[n][pg][c] = sums[0][n][pg][c];
+                    else if constexpr (Sh::CHUNKS == 1) s[n][pg][c] = sums[1][n][pg][c] + sums[0][n][pg][c];
+                    else s[n][pg][c] = sums[1][n][pg][c] + sums[2][n][pg][c] + sums[0][n][pg][c];
+                }
         float ks[4], vs[4];  // of keys g + 8 j
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -259,6 +276,10 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
                     for (int j = 0; j < DP / 16; ++j) {
                         o[n][j][e] *= by * shrink;
                         o[n][j][2 + e] *= by * shrink;
+                        if constexpr (F32) {
+                            o_sum[n][j][e] *= by * shrink;
+                            o_sum[n][j][2 + e] *= by * shrink;
+                        }
                     }
                 }
         }
@@ -338,6 +359,15 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
         const int key0 = (b_begin + warp + i * W) * AR_KEYS;
         if (gone != 0 || key0 < whole_from || key0 + AR_KEYS - 1 > whole_to) work(std::true_type{}, at, scales, key0, gone);
         else work(std::false_type{}, at, scales, key0, 0u);
+        if constexpr (F32) {
+            if (i % AR_FLUSH == AR_FLUSH - 1) {
+#pragma unroll
+                for (int j = 0; j < NT * DP / 16 * 4; ++j) {
+                    (&o_sum[0][0][0])[j] += (&o[0][0][0])[j];
+                    (&o[0][0][0])[j] = 0.f;
+                }
+            }
+        }
         if (++stage == STAGES) {
             stage = 0;
             parity ^= 1;
@@ -363,6 +393,10 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
     __syncthreads();  // the rings have been read
     float* const sums = reinterpret_cast<float*>(ar_smem);  // [warp][row][LDO]
     const float back = ref * (1.f / AF_LIFT);
+    if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < NT * DP / 16 * 4; ++j) (&o[0][0][0])[j] += (&o_sum[0][0][0])[j];
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -507,10 +541,13 @@ static cudaError_t launch_rows(const AttentionFp8Args& a, cudaStream_t st) {
 
 template <typename T>
 static cudaError_t attention_as(const AttentionFp8Args& a, cudaStream_t st) {
+    // f32: eight, since two sets of sums of 16 rows do not fit the registers
     const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv);
-    if (rows > 16) return launch_attention_fp8_tiles(a, sizeof(T) == 2, st);
-    if (a.c.dim <= 64) return rows <= 8 ? launch_rows<T, 64, 1>(a, st) : launch_rows<T, 64, 2>(a, st);
-    return rows <= 8 ? launch_rows<T, 128, 1>(a, st) : launch_rows<T, 128, 2>(a, st);
+    constexpr bool F32 = sizeof(T) == 4;
+    if (rows > (F32 ? 8 : 16)) return launch_attention_fp8_tiles(a, !F32, st);
+    if constexpr (!F32)
+        if (rows > 8) return a.c.dim <= 64 ? launch_rows<T, 64, 2>(a, st) : launch_rows<T, 128, 2>(a, st);
+    return a.c.dim <= 64 ? launch_rows<T, 64, 1>(a, st) : launch_rows<T, 128, 1>(a, st);
 }
 cudaError_t launch_attention_fp8(const AttentionFp8Args& a, bool bf, cudaStream_t st) { return bf ? attention_as<bf16>(a, st) : attention_as<float>(a, st); }
 

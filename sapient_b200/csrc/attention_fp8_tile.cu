@@ -12,7 +12,8 @@
 // bounds the tiles is the shared memory's bandwidth (operands, their conversion, scales), so that keys that need no conversion count for more
 // than the instructions: 8192 x 8192, 8B shape, XXX.
 // ROWS: the groups have 128 rows each of 256, and keys in common. KEYS (up to 128 rows): the same rows, key tiles by turns; their sums
-// are added up at the end. Keys may be shared out to the blocks of a cluster as well, which add up through shared memory.
+// are added up at the end. f32: one group with two tiles of scores; the tensor cores cut off what falls below a sum's last bits, always towards
+// zero (2^-26 of it an addition: 1.8e-5 after 8192 keys), so that O is added to a sum of its own by the vector units every AT_FLUSH tiles. Keys may be shared out to the blocks of a cluster as well, which add up through shared memory.
 //
 // A tile's values have a power of two 2^u, not below the largest of their scales. For bf16 rows they are multiplied by s' 2^(7 - u) as they become
 // fp16 (off by 2^-11 of themselves), so that a weight is one exponential, 2^(z - M + u - 7); for f32 rows values stay exact and weights
@@ -32,6 +33,7 @@ namespace sp {
 cudaError_t count_launch_and_check();  // kernels.cu
 
 constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 512, AT_RING = 8;
+constexpr int AT_FLUSH = 4;
 constexpr float AT_MOST = 15.f, AT_SET = 9.f;  // log2 of the largest weight, and of it when M is set
 constexpr int AT_UP = 7, AT_LEAST = -80;       // values times 2^7 are below 2^16; smaller u would let a sum of 2^(z - M) pass 2^127
 
@@ -39,11 +41,12 @@ template <typename T, int DP, bool KEYS>
 struct AtShape {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int PLANES = 2, TILES = KEYS ? 1 : 2;                      // of Q: digits, or fp16 and remainders
-    static constexpr int K_STAGES = !F32 ? 3 : !KEYS && DP == 128 ? 1 : 2, V_STAGES = F32 && !KEYS && DP == 128 ? 1 : 2;
+    static constexpr int K_STAGES = F32 ? 2 : 3, V_STAGES = 2, SETS = KEYS && !F32 ? 2 : 1;  // SETS: sums of a row
+    static_assert(KEYS || !F32, "f32: tiles of 128 rows");
     static constexpr int TILE = 128 * DP * 2, K_TILE = F32 ? TILE : 128 * 128;  // bytes of 128 rows in fp16; of keys and of a plane of Q
     static constexpr int Q = PLANES * TILES * K_TILE, SMEM = Q + K_STAGES * K_TILE + V_STAGES * TILE + 1024;
     static constexpr int LDO = DP + 4, SUMS = 2 * 128 * LDO * 4;                // takes the operands' place
-    static constexpr int WEIGHTS = (128 * TILES + AF_MAX_PARTS) * (KEYS ? 2 : 1) * 4;  // of the sums of a block's share of rows, behind them
+    static constexpr int WEIGHTS = (128 * TILES + AF_MAX_PARTS) * SETS * 4;              // of the sums of a block's share of rows, behind them
     static_assert(SUMS + WEIGHTS <= SMEM - 1024, "sums of both groups");
 };
 
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     constexpr bool F32 = Sh::F32;
     constexpr int K_STAGES = Sh::K_STAGES, V_STAGES = Sh::V_STAGES, ROWS = 128 * Sh::TILES;
     extern __shared__ uint8_t at_smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES], s_full[2], p_full[2][2], o_full, q_full;
+    __shared__ __align__(8) uint64_t k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES], s_full[2], p_full[2][2], o_done, o_full, q_full;
     __shared__ __align__(16) float k_scale[AT_RING][AT_KEYS], v_scale[AT_RING][F32 ? AT_KEYS : 4];
     __shared__ uint32_t gone_s[AT_RING];     // pages of the tile that are not there
     __shared__ __align__(16) uint32_t largest_s[AT_RING][4];  // scales of values that count, of 32 tokens each
@@ -258,6 +261,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             at_init(&p_full[i][1], 4);
         }
         at_init(&o_full, 1);
+        at_init(&o_done, 1);
         at_init(&q_full, 8);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -351,8 +355,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             }
             __syncwarp();
         };
-        for (int j = 0; j < groups && j < jobs && ok; ++j) scores(j);
+        for (int j = 0; j < (F32 ? 1 : groups) && j < jobs && ok; ++j) scores(j);
         for (int j = 0; j < jobs && ok; ++j) {
+            if (F32 && j + 1 < jobs) scores(j + 1);  // into the other tile of scores
+            if (!ok) break;
             const int t = groups == 2 ? j & 1 : 0, i = groups == 2 ? j >> 1 : j, kv = KEYS ? j : i, st = kv % V_STAGES;
             if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&v_full[st], (uint32_t)((kv / V_STAGES) & 1)));
 #pragma unroll 1
@@ -367,14 +373,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                     for (int s = 0; s < 4; ++s)
 #pragma unroll
                         for (int p = F32 ? 1 : 0; p >= 0; --p)
-                            at_mma_tmem(tm + 256u + (uint32_t)(DP * t), w + (uint32_t)(F32 ? 32 * (s / 2) + 16 * p + 8 * (s % 2) : 8 * s), v + (uint64_t)(s * (2048 >> 4)), id_o,
-                                        i > 0 || half > 0 || s > 0 || (F32 && p == 0));
+                            at_mma_tmem(tm + 256u + (uint32_t)(F32 ? 0 : DP * t), w + (uint32_t)(F32 ? 32 * (s / 2) + 16 * p + 8 * (s % 2) : 8 * s), v + (uint64_t)(s * (2048 >> 4)), id_o,
+                                        (F32 ? j % AT_FLUSH > 0 : i > 0) || half > 0 || s > 0 || (F32 && p == 0));
                     if (half == 1 && (KEYS || t == groups - 1)) tc5_commit(&v_empty[st]);
+                    if (F32 && half == 1) tc5_commit(&o_done);
                 }
                 __syncwarp();
             }
             if (!ok) break;
-            if (j + groups < jobs) scores(j + groups);
+            if (!F32 && j + groups < jobs) scores(j + groups);
         }
         if (jobs > 0) {
             if (ok && leader) tc5_commit(&o_full);
@@ -506,13 +513,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(F32 ? 176 : 184));
         const int t = warp >> 2, r = 32 * (warp & 3) + lane, row = (KEYS ? 0 : 128 * t) + r;  // of the block's rows
-        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), S = lanes + 128u * t, O = lanes + 256u + (uint32_t)(DP * t);
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), O = lanes + 256u + (uint32_t)(F32 ? 0 : DP * t);
+        [[maybe_unused]] const uint32_t O_sum = O + DP;  // f32: what O has been added to
         const int pos = pos_first + token_of(row);
         const int limit = row < tile.n ? min(pos, held - 1) : -1, low = a.window > 0 ? pos - a.window + 1 : 0;
         // keys that all rows of the group see
         const int row_a = KEYS ? 0 : 128 * t, row_b = min(row_a + 127, tile.n - 1);
         const int whole_to = min(pos_first + token_of(row_a), held - 1), whole_from = a.window > 0 ? pos_first + token_of(row_b) - a.window + 1 : 0;
-        const int mine = t >= groups ? 0 : (jobs - t + groups - 1) / groups;  // jobs of the group
+        const int mine = F32 ? (t == 0 ? jobs : 0) : t >= groups ? 0 : (jobs - t + groups - 1) / groups;  // jobs of the group
         // ── queries: fp16 operands, eight values a thread and row ──
         float c;  // scale log2(e) / what the row is multiplied by; never 0, since scores of -inf are multiplied by it
         {
@@ -589,11 +597,30 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             c = row_factor[row];
         }
         float m = -INFINITY, l = 0.f;
-        for (int i = 0; i < mine; ++i) {
-            const int kv = KEYS ? 2 * i + t : i, key0 = (b_begin + kv) * AT_KEYS, slot = kv % AT_RING;
-            ok = __all_sync(0xFFFFFFFFu, tc5_wait(&s_full[t], (uint32_t)(i & 1)));
+        for (int job = 0; job < mine; ++job) {
+            const int of = F32 ? job & 1 : t, i = F32 ? job >> 1 : job;  // the tile of scores, its how manieth use
+            const int kv = KEYS && !F32 ? 2 * i + t : job, key0 = (b_begin + kv) * AT_KEYS, slot = kv % AT_RING;
+            const uint32_t S = lanes + 128u * of;
+            ok = __all_sync(0xFFFFFFFFu, tc5_wait(&s_full[of], (uint32_t)(i & 1)));
             if (!ok) break;
             at_after();
+            const bool flush = F32 && job > 0 && job % AT_FLUSH == 0;
+            if (flush) {
+                ok = __all_sync(0xFFFFFFFFu, tc5_wait(&o_done, (uint32_t)((job - 1) & 1)));
+                if (!ok) break;
+                at_after();
+#pragma unroll 1
+                for (int d = 0; d < dim; d += 16) {
+                    uint32_t o[16], sum[16];
+                    tc5_ld16(O + d, o);
+                    if (job > AT_FLUSH) tc5_ld16(O_sum + d, sum);
+                    at_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + (job > AT_FLUSH ? __uint_as_float(sum[j]) : 0.f));
+                    at_st16(O_sum + d, o);
+                }
+                at_wait_st();
+            }
             uint64_t s[4][16];  // 32 scores each, two a register pair
 #pragma unroll
             for (int q = 0; q < 4; ++q) at_ld32(S + 32 * q, s[q]);
@@ -645,16 +672,27 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 const float to = moves ? x - AT_SET : m, by = moves ? af_ex2(m - to) : 1.f;  // (m = -inf: 0)
                 m = to;
                 l *= by;
-                if (i > 0) {
+                auto scale = [&](uint32_t at) {
 #pragma unroll 1
                     for (int d = 0; d < dim; d += 16) {
                         uint32_t o[16];
-                        tc5_ld16(O + d, o);
+                        tc5_ld16(at + d, o);
                         at_wait_ld();
 #pragma unroll
                         for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
-                        at_st16(O + d, o);
+                        at_st16(at + d, o);
                     }
+                };
+                if constexpr (F32) {
+                    if (job % AT_FLUSH > 0) {
+                        ok = __all_sync(0xFFFFFFFFu, tc5_wait(&o_done, (uint32_t)((job - 1) & 1)));
+                        if (!ok) break;
+                        at_after();
+                        scale(O);
+                    }
+                    if (job >= AT_FLUSH) scale(O_sum);
+                } else if (i > 0) {
+                    scale(O);
                 }
             }
             const float base = (m == -INFINITY ? 0.f : -m) + (F32 ? 0.f : (float)power);
@@ -689,7 +727,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                     at_wait_st();
                     at_before();
                     __syncwarp();
-                    if (lane == 0) tc5_arrive(&p_full[t][q / 2]);
+                    if (lane == 0) tc5_arrive(&p_full[of][q / 2]);
                 }
             }
             const float2 sum = at_two(at_add2(sum0, sum1));
@@ -749,10 +787,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 if (mine > 0 && ok) {
                     at_ld32(O + d, o);
                     at_wait_for(o);
+                    if (F32 && mine > AT_FLUSH) {
+                        uint64_t sum[16];
+                        at_ld32(O_sum + d, sum);
+                        at_wait_for(sum);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = at_add2(o[j], sum[j]);
+                    }
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) o[j] = 0;
                 }
+                if (t >= Sh::SETS && KEYS) break;  // (f32: the second group has no sum)
 #pragma unroll
                 for (int j = 0; j < 16; j += 2)
                     if (d + 2 * j < dim) *reinterpret_cast<ulonglong2*>(&sums[(128 * t + r) * Sh::LDO + d + 2 * j]) = make_ulonglong2(o[j], o[j + 1]);
@@ -763,7 +809,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             if (parts > 1) cluster_sync();
             // The blocks share the rows out: row q of the block's is part + parts q of the tile. Sum s of a row is part s / SETS's, group s % SETS's
             // (KEYS) or its own group's.
-            constexpr int SETS = KEYS ? 2 : 1;
+            constexpr int SETS = Sh::SETS;
             const int sets = parts * SETS, rows_here = (tile.n - part + parts - 1) / parts;
             for (int e = tid; e < rows_here * sets; e += 256) {
                 const int q = e / sets, s = e - q * sets, of = part + parts * q;
@@ -838,7 +884,8 @@ static cudaError_t launch_tiles(const AttentionFp8Args& a, cudaStream_t st) {
 
 template <typename T, int DP>
 static cudaError_t tiles_as(const AttentionFp8Args& a, cudaStream_t st) {
-    return (int64_t)a.max_rows * (a.n_heads / a.c.n_kv) <= 128 ? launch_tiles<T, DP, true>(a, st) : launch_tiles<T, DP, false>(a, st);
+    if constexpr (sizeof(T) == 4) return launch_tiles<T, DP, true>(a, st);
+    else return (int64_t)a.max_rows * (a.n_heads / a.c.n_kv) <= 128 ? launch_tiles<T, DP, true>(a, st) : launch_tiles<T, DP, false>(a, st);
 }
 cudaError_t launch_attention_fp8_tiles(const AttentionFp8Args& a, bool bf, cudaStream_t st) {
     if (a.c.dim <= 64) return bf ? tiles_as<bf16, 64>(a, st) : tiles_as<float, 64>(a, st);
