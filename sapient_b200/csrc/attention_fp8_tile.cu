@@ -2,7 +2,7 @@
 //
 // A block has two groups of four warps, each with 128 rows whose scores S = Q K^T [128 x 128 keys] and sums O [128 x head_dim] lie in
 // tensor memory, a row a lane. While one group turns scores into weights, the tensor cores work for the other:
-//   warps 0-3, 4-7   weights: a thread has a row of S in registers; its maximum, exponentials, which go back over S as fp16, half a tile at a time,
+//   warps 0-3, 4-7   weights: a thread has a row of S in registers; its maximum, exponentials, which go back over S as fp16 (handed over in two parts),
 //                    and are the first operand of the second product from there. O is rescaled only when a row's reference moves.
 //   warps 8-11       values: e4m3 rows to fp16 in shared memory, as they lie (MN-major, 128-byte swizzle); f32: keys as well (K-major)
 //   warp 12          issues the products
@@ -362,15 +362,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             const int t = groups == 2 ? j & 1 : 0, i = groups == 2 ? j >> 1 : j, kv = KEYS ? j : i, st = kv % V_STAGES;
             if (KEYS || t == 0) ok = __all_sync(0xFFFFFFFFu, tc5_wait(&v_full[st], (uint32_t)((kv / V_STAGES) & 1)));
 #pragma unroll 1
-            for (int half = 0; half < 2 && ok; ++half) {
+            for (int half = 0; half < 2 && ok; ++half) {  // three quarters of the tile's keys, the last
                 ok = __all_sync(0xFFFFFFFFu, tc5_wait(&p_full[t][half], (uint32_t)(i & 1)));
                 if (!ok) break;
                 at_after();
                 if (leader) {
-                    const uint64_t v = vd + (uint64_t)(st * (Sh::TILE >> 4) + half * (4 * 2048 >> 4));
-                    const uint32_t w = tm + 128u * t + (F32 ? 64u : 32u) * half;
-#pragma unroll
-                    for (int s = 0; s < 4; ++s)
+                    const uint64_t v = vd + (uint64_t)(st * (Sh::TILE >> 4) + half * (6 * 2048 >> 4));
+                    const uint32_t w = tm + 128u * t + (F32 ? 96u : 48u) * half;
+#pragma unroll 2
+                    for (int s = 0; s < (half ? 2 : 6); ++s)
 #pragma unroll
                         for (int p = F32 ? 1 : 0; p >= 0; --p)
                             at_mma_tmem(tm + 256u + (uint32_t)(F32 ? 0 : DP * t), w + (uint32_t)(F32 ? 32 * (s / 2) + 16 * p + 8 * (s % 2) : 8 * s), v + (uint64_t)(s * (2048 >> 4)), id_o,
@@ -524,70 +524,80 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         // ── queries: fp16 operands, eight values a thread and row ──
         float c;  // scale log2(e) / what the row is multiplied by; never 0, since scores of -inf are multiplied by it
         {
-            constexpr int PER = DP / 8, AT_ONCE = 32 / PER, N = 32 / AT_ONCE;  // threads of a row, rows at once, rows of a thread
-            // KEYS: the groups share the rows out, 16 a warp
-            constexpr int COUNT = KEYS ? N / 2 : N;
-            const int u = lane % PER, first = KEYS ? 16 * warp + lane / PER : 128 * t + 32 * (warp & 3) + lane / PER;
-            uint4 raw[COUNT][F32 ? 2 : 1];
+            constexpr int PER = DP / 8, AT_ONCE = 32 / PER, ROWS_OF = KEYS ? 16 : 32;  // threads of a row, rows at once, rows of a warp (KEYS: the groups share them out)
+            constexpr int COUNT = ROWS_OF / AT_ONCE, BATCH = COUNT < 8 ? COUNT : 8;    // rows of a thread, and at a time, so that one's latencies hide the others'
+            const int u = lane % PER, first = KEYS ? 16 * warp : 128 * t + 32 * (warp & 3);
+            const int64_t mine_at = offset_of(first + lane % ROWS_OF, a.ldq);
+#pragma unroll 1
+            for (int i0 = 0; i0 < COUNT; i0 += BATCH) {
+                uint4 raw[BATCH][F32 ? 2 : 1];
+                uint32_t most[BATCH];  // absolute values as whole numbers: NaN is the largest
 #pragma unroll
-            for (int i = 0; i < COUNT; ++i) {
-                const int q = first + i * AT_ONCE;
+                for (int i = 0; i < BATCH; ++i) {
+                    const int r = (i0 + i) * AT_ONCE + lane / PER;
+                    const int64_t from = __shfl_sync(0xFFFFFFFFu, mine_at, r);
 #pragma unroll
-                for (int e = 0; e < (F32 ? 2 : 1); ++e) {
-                    raw[i][e] = make_uint4(0, 0, 0, 0);
-                    if (q < tile.n && 8 * u < dim)
-                        raw[i][e] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + offset_of(q, a.ldq) + 8 * u)[e];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < COUNT; ++i) {
-                const int q = first + i * AT_ONCE;
-                float x[8];
-                if constexpr (F32) {
-                    const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w, raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
-                } else {
-                    const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        x[2 * j] = __uint_as_float(w[j] << 16);
-                        x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+                    for (int e = 0; e < (F32 ? 2 : 1); ++e) {
+                        raw[i][e] = make_uint4(0, 0, 0, 0);
+                        if (first + r < tile.n && 8 * u < dim) raw[i][e] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + from + 8 * u)[e];
                     }
                 }
-                float most = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
-#pragma unroll
-                for (int o = PER / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-                float by, back;
-                af_row_scale(most, F32 ? 12 : 7, by, back);
-                if (a.scale < 0.f) by = -by;
-                if (u == 0) row_factor[q] = fmaxf(back * fabsf(a.scale) * AF_LOG2E, 0x1p-149f);
-                if constexpr (F32) {
-                    uint4 hi, lo;
-                    uint32_t *const h = &hi.x, *const l = &lo.x;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) af_split(x[2 * j] * by, x[2 * j + 1] * by, h[j], l[j]);
-                    uint8_t* const to = smem + q / 128 * Sh::K_TILE + u / 8 * (128 * 128) + q % 128 * 128 + ((u % 8) ^ (q & 7)) * 16;
-                    *reinterpret_cast<uint4*>(to) = hi;
-                    *reinterpret_cast<uint4*>(to + Sh::TILES * Sh::K_TILE) = lo;
-                } else {
-                    uint32_t hi[2], lo[2];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[4 * j + e] *= by;
-                        hi[j] = at_digits(x + 4 * j);
-                        uint32_t h0, h1;
-                        af_halves(hi[j], h0, h1);
-                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                        const float r[4] = {x[4 * j] - f0.x, x[4 * j + 1] - f0.y, x[4 * j + 2] - f1.x, x[4 * j + 3] - f1.y};
-                        lo[j] = at_digits(r);
+                for (int i = 0; i < BATCH; ++i) {
+                    if constexpr (F32) {
+                        const uint4 v = raw[i][0], w = raw[i][1];
+                        most[i] = max(max(max(v.x & 0x7FFFFFFFu, v.y & 0x7FFFFFFFu), max(v.z & 0x7FFFFFFFu, v.w & 0x7FFFFFFFu)),
+                                      max(max(w.x & 0x7FFFFFFFu, w.y & 0x7FFFFFFFu), max(w.z & 0x7FFFFFFFu, w.w & 0x7FFFFFFFu)));
+                    } else {
+                        const uint4 v = raw[i][0];
+                        most[i] = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+                        most[i] = max(most[i] & 0xFFFF0000u, most[i] << 16);  // as f32
                     }
-                    uint8_t* const to = smem + q / 128 * Sh::K_TILE + q % 128 * 128 + ((u / 2) ^ (q & 7)) * 16 + u % 2 * 8;
-                    *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
-                    *reinterpret_cast<uint2*>(to + Sh::TILES * Sh::K_TILE) = make_uint2(lo[0], lo[1]);
+                }
+#pragma unroll
+                for (int o = PER / 2; o > 0; o >>= 1)
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) most[i] = max(most[i], __shfl_xor_sync(0xFFFFFFFFu, most[i], o));
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const int q = first + (i0 + i) * AT_ONCE + lane / PER;
+                    float by, back;
+                    af_row_scale(__uint_as_float(most[i]), F32 ? 12 : 7, by, back);
+                    if (a.scale < 0.f) by = -by;
+                    if (u == 0) row_factor[q] = fmaxf(back * fabsf(a.scale) * AF_LOG2E, 0x1p-149f);
+                    float x[8];
+                    if constexpr (F32) {
+                        const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w, raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]) * by;
+                        uint4 hi, lo;
+                        uint32_t *const h = &hi.x, *const l = &lo.x;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) af_split(x[2 * j], x[2 * j + 1], h[j], l[j]);
+                        uint8_t* const to = smem + q / 128 * Sh::K_TILE + u / 8 * (128 * 128) + q % 128 * 128 + ((u % 8) ^ (q & 7)) * 16;
+                        *reinterpret_cast<uint4*>(to) = hi;
+                        *reinterpret_cast<uint4*>(to + Sh::TILES * Sh::K_TILE) = lo;
+                    } else {
+                        const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            x[2 * j] = __uint_as_float(w[j] << 16) * by;
+                            x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u) * by;
+                        }
+                        uint32_t hi[2], lo[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            hi[j] = at_digits(x + 4 * j);
+                            uint32_t h0, h1;
+                            af_halves(hi[j], h0, h1);
+                            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                            const float d[4] = {x[4 * j] - f0.x, x[4 * j + 1] - f0.y, x[4 * j + 2] - f1.x, x[4 * j + 3] - f1.y};
+                            lo[j] = at_digits(d);
+                        }
+                        uint8_t* const to = smem + q / 128 * Sh::K_TILE + q % 128 * 128 + ((u / 2) ^ (q & 7)) * 16 + u % 2 * 8;
+                        *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2*>(to + Sh::TILES * Sh::K_TILE) = make_uint2(lo[0], lo[1]);
+                    }
                 }
             }
             at_fence_smem();
@@ -723,11 +733,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 } else {
                     at_st16(S + 16 * q, w_hi);
                 }
-                if (q % 2) {
+                if (q >= 2) {
                     at_wait_st();
                     at_before();
                     __syncwarp();
-                    if (lane == 0) tc5_arrive(&p_full[of][q / 2]);
+                    if (lane == 0) tc5_arrive(&p_full[of][q - 2]);
                 }
             }
             const float2 sum = at_two(at_add2(sum0, sum1));
@@ -771,12 +781,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             }
             __syncwarp();
             const int row_w = (KEYS ? 0 : 128 * t) + 32 * (warp & 3), unit = lane % UNITS;
-#pragma unroll 1
+            const int64_t mine_to = offset_of(row_w + lane, a.ldo);
+#pragma unroll 4
             for (int q0 = 0; ok && q0 < 32; q0 += AT_ONCE) {
                 const int q = q0 + lane / UNITS;
+                const int64_t to = __shfl_sync(0xFFFFFFFFu, mine_to, q);
                 const uint4 w = *reinterpret_cast<const uint4*>(mem + q * (16 * UNITS) + ((unit & ~7) | ((unit ^ q) & 7)) * 16);
                 if (row_w + q < tile.n && unit * 16 < dim * (int)sizeof(T))
-                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + offset_of(row_w + q, a.ldo)) + unit * 16) = w;
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + to) + unit * 16) = w;
             }
         } else {
             float* const sums = reinterpret_cast<float*>(smem);  // [group][row][LDO], over the operands, which have been read
@@ -811,41 +823,49 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             // (KEYS) or its own group's.
             constexpr int SETS = Sh::SETS;
             const int sets = parts * SETS, rows_here = (tile.n - part + parts - 1) / parts;
-            for (int e = tid; e < rows_here * sets; e += 256) {
-                const int q = e / sets, s = e - q * sets, of = part + parts * q;
-                float pm = 0.f, top = -INFINITY, total = 0.f;
-                for (int x = 0; x < sets; ++x) {
-                    const int g = KEYS ? x % SETS : of / 128;
+            const int width = sets > 1 ? 1 << (32 - __clz(sets - 1)) : 1, x = lane & (width - 1);  // lanes of a row
+#pragma unroll 1
+            for (int q0 = tid / 32 * (32 / width); q0 < rows_here; q0 += 256 / width) {
+                const int q = q0 + lane / width;
+                float m = -INFINITY, l = 0.f;
+                if (q < rows_here && x < sets) {
+                    const int of = part + parts * q, g = KEYS ? x % SETS : of / 128;
                     const uint32_t at_m = smem_addr(&part_m[g][of % 128]), at_l = smem_addr(&part_l[g][of % 128]);
-                    const float xm = parts > 1 ? ld_peer(peer_smem(at_m, x / SETS)) : part_m[g][of % 128], xl = parts > 1 ? ld_peer(peer_smem(at_l, x / SETS)) : part_l[g][of % 128];
-                    const float to = fmaxf(top, xm);
-                    total = total * (top == to ? 1.f : af_ex2(top - to)) + (xm == to ? xl : xl * af_ex2(xm - to));
-                    top = to;
-                    if (x == s) pm = xm;
+                    m = parts > 1 ? ld_peer(peer_smem(at_m, x / SETS)) : part_m[g][of % 128];
+                    l = parts > 1 ? ld_peer(peer_smem(at_l, x / SETS)) : part_l[g][of % 128];
                 }
-                weights[e] = total == 0.f || pm == -INFINITY ? 0.f : af_ex2(pm - top) / total;
+                float top = m;
+                for (int o = width / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                const float w = m == -INFINITY ? 0.f : af_ex2(m - top);
+                float total = l * w;
+                for (int o = width / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+                if (q < rows_here && x < sets) weights[q * sets + x] = w == 0.f || total == 0.f ? 0.f : w / total;
             }
             asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
             const int quads = dim / 4;
+            constexpr int SUMS = 8;  // on their way at a time: a load from another block takes half a microsecond
+#pragma unroll 1
             for (int e = tid; e < rows_here * quads; e += 256) {
                 const int q = e / quads, d = 4 * (e - q * quads), of = part + parts * q;
                 float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int x0 = 0; x0 < sets; x0 += 4) {
-                    float4 v[4];
+#pragma unroll 1
+                for (int x0 = 0; x0 < sets; x0 += SUMS) {
+                    float4 v[SUMS];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        if (x0 + x >= sets) break;
-                        const float* const src = sums + ((KEYS ? (x0 + x) % SETS : of / 128) * 128 + of % 128) * Sh::LDO + d;
-                        v[x] = parts > 1 ? at_peer4(peer_smem(smem_addr(src), (x0 + x) / SETS)) : *reinterpret_cast<const float4*>(src);
+                    for (int i = 0; i < SUMS; ++i) {
+                        if (x0 + i >= sets) break;
+                        const int x = x0 + i;
+                        const float* const src = sums + ((KEYS ? x % SETS : of / 128) * 128 + of % 128) * Sh::LDO + d;
+                        v[i] = parts > 1 ? at_peer4(peer_smem(smem_addr(src), x / SETS)) : *reinterpret_cast<const float4*>(src);
                     }
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        if (x0 + x >= sets) break;
-                        const float w = weights[q * sets + x0 + x];
-                        y.x = fmaf(v[x].x, w, y.x);
-                        y.y = fmaf(v[x].y, w, y.y);
-                        y.z = fmaf(v[x].z, w, y.z);
-                        y.w = fmaf(v[x].w, w, y.w);
+                    for (int i = 0; i < SUMS; ++i) {
+                        if (x0 + i >= sets) break;
+                        const float w = weights[q * sets + x0 + i];
+                        y.x = fmaf(v[i].x, w, y.x);
+                        y.y = fmaf(v[i].y, w, y.y);
+                        y.z = fmaf(v[i].z, w, y.z);
+                        y.w = fmaf(v[i].w, w, y.w);
                     }
                 }
                 T* const to = out + offset_of(of, a.ldo) + d;
