@@ -6,11 +6,12 @@
 // gives zeros. The queries of a key head are rows of one product (row = token x heads per key head + head), so that its keys are read
 // once for all of them.
 //
-// Precision. e4m3 values are exact in fp16, the scales are applied in f32. A row of q is multiplied by a power of two so that its
-// largest value lies in [2^12, 2^13): bf16 values are then exact in fp16 (down to 2^-30 of the largest), f32 values are taken as fp16
-// plus the fp16 of the remainder. The weights e^(z - m) s' enter the second product as fp16 (11 bits, where the result has bf16's 8) or,
-// for f32, as fp16 plus remainder, multiplied by a power of two that keeps them out of fp16's subnormals: with the largest scale so far, R,
-// rounded up to a power of two and e^(z - m) <= 2^LAZY, the weights are e^(z - m) s' 2^(15 - LAZY) / R <= 2^15. Sums, maxima and the output are f32.
+// Precision. e4m3 values are exact in fp16, the scales are applied in f32. Here (few rows; attention_fp8_tile.cu has its own) a row of q is
+// multiplied by a power of two so that its largest value lies in [2^12, 2^13): bf16 values are then exact in fp16 (down to 2^-30 of the largest),
+// f32 values are taken as fp16 plus the fp16 of the remainder. The weights e^(z - m) s' enter the second product as fp16 (11 bits, where the result
+// has bf16's 8) or, for f32, as fp16 plus remainder, multiplied by a power of two that keeps them out of fp16's subnormals: with the largest scale
+// so far, R, rounded up to a power of two and e^(z - m) <= 2^LAZY, the weights are e^(z - m) s' 2^(15 - LAZY) / R <= 2^15. Sums, maxima and the
+// output are f32.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -37,7 +38,6 @@ cudaError_t count_launch_and_check();  // kernels.cu
 // 131072 keys of the 8B shape 106 us, now XXX.
 // Keys are shared out to the warps of a block and the blocks of a cluster, which add up their parts through shared memory: no workspace.
 constexpr int AR_KEYS = 32, AR_PAGES = AR_KEYS / KV_PAGE, AR_FLUSH = 8;
-
 
 template <typename T, int DP, int NT, int W>
 struct ArShape {
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
     const int pos_base = tile.len - tile.rows;
     const int pos_first = pos_base + tile.row0 / group, pos_last = pos_base + (tile.row0 + tile.n - 1) / group;  // of the tile's rows
     const int held = (int)min((int64_t)tile.len, (int64_t)a.c.max_pages * KV_PAGE);
-    const int k_end = min(pos_last + 1, held), k_begin = a.window > 0 ? max(0, pos_first - a.window + 1) : 0;
+    const int k_end = min(pos_last + 1, held), k_begin = a.window > 0 ? max(0, max(pos_first, 0) - a.window + 1) : 0;
     const int s_begin = k_begin / AR_KEYS, s_end = k_end > k_begin ? (k_end + AR_KEYS - 1) / AR_KEYS : s_begin;
     const int per = (s_end - s_begin + parts - 1) / parts;
     const int b_begin = min(s_end, s_begin + part * per), b_end = min(s_end, b_begin + per);
@@ -175,11 +175,11 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
             m[n][e] = -INFINITY;
             l[n][e] = 0.f;
             limit[n][e] = row < tile.n ? min(pos, held - 1) : -1;
-            low[n][e] = a.window > 0 ? pos - a.window + 1 : 0;
+            low[n][e] = a.window > 0 ? max(pos, 0) - a.window + 1 : 0;
             factor[n][e] = row_factor[row];
         }
     }
-    const int whole_from = a.window > 0 ? pos_last - a.window + 1 : 0, whole_to = min(pos_first, held - 1);  // keys that all rows see
+    const int whole_from = a.window > 0 ? max(pos_last, 0) - a.window + 1 : 0, whole_to = min(pos_first, held - 1);  // keys that all rows see
     // MASK: some row does not see some key. Only then can a byte that is NaN belong to a key that a row does not see.
     auto work = [&](auto with_mask, const uint8_t* at, const float* scales, int key0, uint32_t gone) {
         constexpr bool MASK = decltype(with_mask)::value;
@@ -475,7 +475,6 @@ cudaError_t af_page_map(const CacheFp8& c, CUtensorMap* map) {
 cudaError_t af_fits(const void* kernel, int threads, int smem, ClusterFits* out) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);  // (more than eight blocks)
-    ClusterFits found{};
     for (int p = 1; p <= AF_MAX_PARTS && e == cudaSuccess; ++p) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(1, 1, (unsigned)(64 * p));
@@ -487,17 +486,19 @@ cudaError_t af_fits(const void* kernel, int threads, int smem, ClusterFits* out)
         at[0].val.clusterDim.z = (unsigned)p;
         cfg.attrs = at;
         cfg.numAttrs = 1;
-        e = cudaOccupancyMaxActiveClusters(&found.at_once[p], kernel, &cfg);
+        int found = 0;
+        e = cudaOccupancyMaxActiveClusters(&found, kernel, &cfg);
+        out->at_once[p].store(found, std::memory_order_relaxed);
     }
-    if (e == cudaSuccess) *out = found;
     return e;
 }
 
 AfShare af_share(const ClusterFits& fits, int64_t clusters, int64_t pieces, double piece, double fixed, double joined) {
     AfShare best{1, 1e30};
     for (int p = 1; p <= AF_MAX_PARTS; ++p) {
-        if (fits.at_once[p] < 1) continue;
-        const double rounds = (double)clusters / fits.at_once[p], waves = rounds <= 1. ? 1. : (rounds + std::ceil(rounds)) / 2;
+        const int at_once = fits.at_once[p].load(std::memory_order_relaxed);
+        if (at_once < 1) continue;
+        const double rounds = (double)clusters / at_once, waves = rounds <= 1. ? 1. : (rounds + std::ceil(rounds)) / 2;
         const double time = waves * ((double)((pieces + p - 1) / p) * piece + fixed + (p > 1 ? joined : 0.));
         if (time < best.time) best = AfShare{p, time};
     }

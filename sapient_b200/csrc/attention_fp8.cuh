@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "cache_fp8.h"
 #include "plan_common.cuh"
@@ -67,7 +68,7 @@ cudaError_t af_page_map(const CacheFp8& c, CUtensorMap* map);
 // fill an SM each hold 112, of 10 or 8 110 and 120, of 6 132; eight clusters of 16 are two rounds.
 constexpr int AF_MAX_PARTS = 16;
 struct ClusterFits {
-    int at_once[AF_MAX_PARTS + 1];  // clusters of that many blocks
+    std::atomic<int> at_once[AF_MAX_PARTS + 1];  // clusters of that many blocks (threads whose first calls coincide all write them)
 };
 cudaError_t af_fits(const void* kernel, int threads, int smem, ClusterFits* out);  // and the kernel's attributes for it
 struct AfShare {
@@ -87,10 +88,11 @@ struct AfTile {
 };
 __device__ __forceinline__ AfTile af_tile(const AttentionFp8Args& a, int seq, int tile, int height) {
     AfTile t;
+    const int len = a.seq_len[seq], end = a.row_start[seq + 1];  // (all on their way at once)
     t.first = a.row_start[seq];
-    t.rows = a.row_start[seq + 1] - t.first;
     t.slot = a.seq_slot ? a.seq_slot[seq] : seq;
-    t.len = t.slot >= 0 && t.slot < a.c.n_slots ? max(a.seq_len[seq], 0) : 0;  // (a slot that is not there holds nothing)
+    t.rows = end - t.first;
+    t.len = t.slot >= 0 && t.slot < a.c.n_slots ? max(len, 0) : 0;  // (a slot that is not there holds nothing)
     t.row0 = tile * height;
     t.n = min(height, min(t.rows, a.max_rows) * (a.n_heads / a.c.n_kv) - t.row0);
     return t;

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     };
     const int pos_first = tile.len - tile.rows + tok_base, pos_last = tile.len - tile.rows + last_row / group;
     const int held = (int)min((int64_t)tile.len, (int64_t)a.c.max_pages * KV_PAGE);
-    const int k_end = min(pos_last + 1, held), k_begin = a.window > 0 ? max(0, pos_first - a.window + 1) : 0;
+    const int k_end = min(pos_last + 1, held), k_begin = a.window > 0 ? max(0, max(pos_first, 0) - a.window + 1) : 0;
     const int t_begin = k_begin / AT_KEYS, t_end = k_end > k_begin ? (k_end + AT_KEYS - 1) / AT_KEYS : t_begin;
     const int per = (t_end - t_begin + parts - 1) / parts;
     const int b_begin = min(t_end, t_begin + part * per), n_kv = min(t_end, b_begin + per) - b_begin;  // key tiles of the block
@@ -516,10 +516,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), O = lanes + 256u + (uint32_t)(F32 ? 0 : DP * t);
         [[maybe_unused]] const uint32_t O_sum = O + DP;  // f32: what O has been added to
         const int pos = pos_first + token_of(row);
-        const int limit = row < tile.n ? min(pos, held - 1) : -1, low = a.window > 0 ? pos - a.window + 1 : 0;
+        const int limit = row < tile.n ? min(pos, held - 1) : -1, low = a.window > 0 ? max(pos, 0) - a.window + 1 : 0;
         // keys that all rows of the group see
         const int row_a = KEYS ? 0 : 128 * t, row_b = min(row_a + 127, tile.n - 1);
-        const int whole_to = min(pos_first + token_of(row_a), held - 1), whole_from = a.window > 0 ? pos_first + token_of(row_b) - a.window + 1 : 0;
+        const int whole_to = min(pos_first + token_of(row_a), held - 1), whole_from = a.window > 0 ? max(pos_first + token_of(row_b), 0) - a.window + 1 : 0;
         const int mine = F32 ? (t == 0 ? jobs : 0) : t >= groups ? 0 : (jobs - t + groups - 1) / groups;  // jobs of the group
         // ── queries: fp16 operands, eight values a thread and row ──
         float c;  // scale log2(e) / what the row is multiplied by; never 0, since scores of -inf are multiplied by it

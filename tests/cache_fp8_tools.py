@@ -46,8 +46,9 @@ class Cache:
         return y
 
 
-def attention64(c, q, seqs, scale, window=0):
-    """seqs: (slot, rows, length) of each sequence; q [rows, heads, dim]. Outputs in 64 bits and how far a call's may be off."""
+def attention64(c, q, seqs, scale, window=0, digits=False):
+    """seqs: (slot, rows, length) of each sequence; q [rows, heads, dim]. Outputs in 64 bits and how far a call's may be off. digits: with what
+    bf16 queries as two e4m3 digits add, which counts where a few coordinates are much larger than the others."""
     heads, dim = q.shape[1:]
     group = heads // c.kv
     out, far = torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape, dtype=torch.float64, device=q.device)
@@ -83,6 +84,8 @@ def attention64(c, q, seqs, scale, window=0):
                 planes = 2 if f32 else 1
                 size = (x.abs() @ k[:, h // group].nan_to_num().abs().T * scale).masked_fill(~seen, 0).amax(-1, keepdim=True)
                 dz = size * (2.0**-22 * f32 + planes * dim / 16 * 2.0**-23 + 6 * 2.0**-23) + 2.0**-21
+                if digits:  # the lowest digit's step is 2^-9 where the row's largest value is 2^7 or more: each coordinate is off by 2^-17 of that
+                    dz = dz + 1.45 * scale * 2.0**-17 * x.abs().amax(-1, keepdim=True) * (k[:, h // group].nan_to_num().abs().sum(-1) * seen).amax(-1, keepdim=True)
                 w = 2 * (dz + planes * (held / 16 + 2) * 2.0**-23 + 64 * 2.0**-22) + (2.0**-22 if f32 else (1 + 2.0**-11) ** 3 - 1)
                 far[at: at + r, h] = w * (p @ u.abs()) + (2 * STEP[ops.F32] if f32 else 1.01 * STEP[ops.BF16]) * y.abs() + 2.0**-100
         at += r
@@ -112,10 +115,10 @@ class Step:
                               self.c.dim**-0.5 if scale is None else scale, window=window, seq_slot=self.slot.data_ptr(), dtype=self.ty, ldq=self.ld, ldo=self.ld, stream=st)
         return self.out
 
-    def check(self, scale=None, window=0):
+    def check(self, scale=None, window=0, digits=False):
         wide = self.heads * self.c.dim
         q = self.q[: self.n, :wide].reshape(self.n, self.heads, self.c.dim)
-        want, far = attention64(self.c, q, self.seqs, self.c.dim**-0.5 if scale is None else scale, window)
+        want, far = attention64(self.c, q, self.seqs, self.c.dim**-0.5 if scale is None else scale, window, digits)
         got = self.out[: self.n, :wide].reshape(want.shape).double()
         assert torch.equal(got.isnan(), want.isnan())
         off = (got - want).abs().nan_to_num()

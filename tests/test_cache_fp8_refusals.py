@@ -42,6 +42,8 @@ def test_caches(call):
     for kw in (dict(head_dim=0), dict(head_dim=40), dict(head_dim=144), dict(head_dim=-16), dict(n_pages=0), dict(n_slots=0), dict(max_pages=0), dict(n_kv_heads=0),
                dict(max_pages=2**31 - 1), dict(n_kv_heads=70000)):
         refused(SP_ERR_SHAPE, call, cache(**kw))
+    for kw in (dict(n_pages=2**26, n_kv_heads=1), dict(n_pages=1025, n_kv_heads=65535)):  # n_pages x 2 x n_kv_heads x 16 >= 2^31
+        refused(SP_ERR_SHAPE, call, cache(**kw))
     for ty in (ops.F16, 99, -1):
         refused(SP_ERR_DTYPE, call, dtype=ty)
     assert _lib.lib().sp_cuda_cache_fp8_read_dev(None, 0, 1, A, A, A, 128, A, 128, None) == SP_ERR_ARG
