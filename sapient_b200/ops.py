@@ -369,7 +369,6 @@ def attention_fp8_dev(cache: CacheFp8, q: int, n_heads: int, out: int, n_seqs: i
         check(status)
 
 
-
 def set_gemv_path(path: int) -> None:
     """0: tensor-core GEMV on tile-repacked weights (default); 1: CUDA-core GEMV on raw blocks; 3: per-warp streaming
     variant; 4: bulk-copy ring GEMV for calls of 1-5 rows."""
