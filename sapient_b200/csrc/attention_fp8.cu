@@ -35,7 +35,7 @@ cudaError_t count_launch_and_check();  // kernels.cu
 // transpositions make the second product's operand. (e4m3 operands of mma.sync are converted to fp16 at every use on this GPU: two digits
 // of q against the keys' own bytes took 982 instructions for 32 keys.) A page's keys or values of a head are one TMA copy, whose 128-byte
 // swizzle lets eight threads' reads fall on 32 different banks; copied by threads, 16 bytes each, every one was a request of its own to L2:
-// 131072 keys of the 8B shape 106 us, now XXX.
+// 131072 keys of the 8B shape 106 us, 74 so (61 with blocks of 12 warps).
 // Keys are shared out to the warps of a block and the blocks of a cluster, which add up their parts through shared memory: no workspace.
 constexpr int AR_KEYS = 32, AR_PAGES = AR_KEYS / KV_PAGE, AR_FLUSH = 8;
 
@@ -505,51 +505,67 @@ AfShare af_share(const ClusterFits& fits, int64_t clusters, int64_t pieces, doub
     return best;
 }
 
-// Microseconds of a warp's step with twelve warps on an SM, and of a block's start and end (measured: 131072 keys of the 8B shape in one to
-// 16 parts, 518 keys); with cluster_sync.
-constexpr double AR_STEP = 1.4, AR_FIXED = 4., AR_JOINED = 0.5;
+// Microseconds of a warp's step with twelve warps on an SM, of a block's start and end, and of adding parts up. Few bf16 rows: measured, 131072 keys of
+// the 8B shape in one to 16 parts, 518 keys; the others are fitted to 64 calls (3 to 35 rows a head, 240 to 32768 keys, 1 to 32 sequences, 8B, 1.5B and
+// 0.5B shapes), from which they are 3 to 8 % off.
+template <typename T, int DP, int NT>
+struct ArTimes {
+    static constexpr bool F32 = sizeof(T) == 4, FEW = NT == 1 && !F32;
+    static constexpr double STEP = FEW ? 1.4 : F32 ? (DP == 128 ? 2.2 : 1.8) : DP == 128 ? 2.4 : 2.1;
+    static constexpr double FIXED = FEW ? 4. : F32 ? (DP == 128 ? 5. : 4.) : DP == 128 ? 6.5 : 5., JOINED = FEW ? 0.5 : F32 && DP == 128 ? 1.5 : 2.;
+};
 
 template <typename T, int DP, int NT, int W>
 struct RowsLaunch {
     using Sh = ArShape<T, DP, NT, W>;
+    using At = ArTimes<T, DP, NT>;
     static constexpr auto kernel = attention_rows_kernel<T, DP, NT, W>;
     static cudaError_t share(const AttentionFp8Args& a, int64_t clusters, int64_t len, AfShare* out) {
         static PerDeviceOnce once;
         static ClusterFits fits[SP_MAX_DEVICES];
         ClusterFits& mine = fits[current_device_index()];
         const cudaError_t e = once.run([&] { return af_fits(reinterpret_cast<const void*>(kernel), 32 * W, Sh::SMEM, &mine); });
-        if (e == cudaSuccess) *out = af_share(mine, clusters, (len + AR_KEYS * W - 1) / (AR_KEYS * W), AR_STEP, AR_FIXED, AR_JOINED);
+        if (e == cudaSuccess) *out = af_share(mine, clusters, (len + AR_KEYS * W - 1) / (AR_KEYS * W), At::STEP, At::FIXED, At::JOINED);
         return e;
     }
-    static cudaError_t go(const AttentionFp8Args& a, const CUtensorMap& map, int parts, cudaStream_t st) {
-        return launch_pdl_cluster(kernel, dim3((unsigned)a.c.n_kv, (unsigned)a.n_seqs, (unsigned)parts), dim3(32 * W), Sh::SMEM, st, parts, a, parts, map);
+    static cudaError_t go(const AttentionFp8Args& a, const CUtensorMap& map, int tiles, int parts, cudaStream_t st) {
+        return launch_pdl_cluster(kernel, dim3((unsigned)(a.c.n_kv * tiles), (unsigned)a.n_seqs, (unsigned)parts), dim3(32 * W), Sh::SMEM, st, parts, a, parts, map);
     }
 };
 
-// Blocks of 12 warps fill an SM; of four, three share one: many short sequences (1000 of up to 90 keys: XXX).
+// Blocks of 12 warps fill an SM, and the longest sequences are fastest with them (64 x 1024 keys of the 1.5B shape 10.8 us, 10.9 if four were taken); of
+// four, three share one, which many short sequences want (1000 x 90 keys 36.3 us, with 12 warps 72.2; 300 x 200 17.8, 26.9). More rows than one
+// block has are shared out to several, which read the same keys, or go to the tiles, whichever takes less by the times above (f32, 24 rows at 4096
+// keys of the 8B shape 12 us, tiles 20.5; 8 x 32 rows 56, 65; 32 x 56 rows at 1024 of the 0.5B shape 28, 18; bf16, 4 x 30 at 32768 of
+// the 1.5B shape 42, 56; 8 x 64 at 4096 of the 8B shape 65, 38; 16 rows, one block's: 8 x 4096 keys 24, 36).
 template <typename T, int DP, int NT>
 static cudaError_t launch_rows(const AttentionFp8Args& a, cudaStream_t st) {
-    const int64_t clusters = (int64_t)a.c.n_kv * a.n_seqs, len = af_keys(a);
+    const int tiles = (int)(((int64_t)a.max_rows * (a.n_heads / a.c.n_kv) + 8 * NT - 1) / (8 * NT));
+    const int64_t clusters = (int64_t)a.c.n_kv * tiles * a.n_seqs, len = af_keys(a);
     AfShare wide, narrow;
     CUtensorMap map{};
     cudaError_t e = RowsLaunch<T, DP, NT, 12>::share(a, clusters, len, &wide);
     if (e == cudaSuccess) e = RowsLaunch<T, DP, NT, 4>::share(a, clusters, len, &narrow);
+    if (e == cudaSuccess && tiles > 1) {
+        AfShare other;
+        e = launch_attention_fp8_tiles(a, sizeof(T) == 2, st, &other);
+        if (e == cudaSuccess && other.time < std::min(wide.time, narrow.time)) return launch_attention_fp8_tiles(a, sizeof(T) == 2, st, nullptr);
+    }
     if (e == cudaSuccess) e = af_page_map(a.c, &map);
     if (e == cudaSuccess)
-        e = wide.time <= narrow.time ? RowsLaunch<T, DP, NT, 12>::go(a, map, wide.parts, st) : RowsLaunch<T, DP, NT, 4>::go(a, map, narrow.parts, st);
+        e = wide.time <= narrow.time ? RowsLaunch<T, DP, NT, 12>::go(a, map, tiles, wide.parts, st) : RowsLaunch<T, DP, NT, 4>::go(a, map, tiles, narrow.parts, st);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
-template <typename T>
+template <typename T, int DP>
 static cudaError_t attention_as(const AttentionFp8Args& a, cudaStream_t st) {
-    // f32: eight, since two sets of sums of 16 rows do not fit the registers
-    const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv);
-    constexpr bool F32 = sizeof(T) == 4;
-    if (rows > (F32 ? 8 : 16)) return launch_attention_fp8_tiles(a, !F32, st);
-    if constexpr (!F32)
-        if (rows > 8) return a.c.dim <= 64 ? launch_rows<T, 64, 2>(a, st) : launch_rows<T, 128, 2>(a, st);
-    return a.c.dim <= 64 ? launch_rows<T, 64, 1>(a, st) : launch_rows<T, 128, 1>(a, st);
+    if constexpr (sizeof(T) == 2)  // (f32: two sets of sums of 16 rows do not fit the registers)
+        if ((int64_t)a.max_rows * (a.n_heads / a.c.n_kv) > 8) return launch_rows<T, DP, 2>(a, st);
+    return launch_rows<T, DP, 1>(a, st);
 }
-cudaError_t launch_attention_fp8(const AttentionFp8Args& a, bool bf, cudaStream_t st) { return bf ? attention_as<bf16>(a, st) : attention_as<float>(a, st); }
+cudaError_t launch_attention_fp8(const AttentionFp8Args& a, bool bf, cudaStream_t st) {
+    if (a.c.dim <= 64) return bf ? attention_as<bf16, 64>(a, st) : attention_as<float, 64>(a, st);
+    return bf ? attention_as<bf16, 128>(a, st) : attention_as<float, 128>(a, st);
+}
 
 }  // namespace sp

@@ -10,7 +10,8 @@
 // bf16 rows are multiplied with the keys' own bytes: q is two e4m3 digits, whose products run at twice fp16's rate. A row scaled so that its largest
 // value lies in [128, 256) is its digits' sum exactly, but for values below 2^-9 of the largest, which are off by up to 2^-17 of that. What
 // bounds the tiles is the shared memory's bandwidth (operands, their conversion, scales), so that keys that need no conversion count for more
-// than the instructions: 8192 x 8192, 8B shape, XXX.
+// than the instructions: 8192 x 8192, 8B shape, 690 us with keys converted to fp16, 605 to 640 (0.9 PFLOP/s; power limit) so; 2.1 us a tile of 256 rows by
+// 128 keys. Short prompts are bound by a block's start (5 us until its queries are operands) and end (2 us): 9 x 1500 rows, 2.7B shape, 247 us.
 // ROWS: the groups have 128 rows each of 256, and keys in common. KEYS (up to 128 rows): the same rows, key tiles by turns; their sums
 // are added up at the end. f32: one group with two tiles of scores; the tensor cores cut off what falls below a sum's last bits, always towards
 // zero (2^-26 of it an addition: 1.8e-5 after 8192 keys), so that O is added to a sum of its own by the vector units every AT_FLUSH tiles. Keys may be shared out to the blocks of a cluster as well, which add up through shared memory.
@@ -235,6 +236,26 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         const int tok = token_of(q);
         return (q_first + tok) * ld + (int64_t)(head * group + rem + q - tok * group) * dim;
     };
+    // ── queries: the first are on their way while the block sets itself up (8 prompts of 512 rows, 8B shape, 65.1 us, 62.1 so) ──
+    constexpr int PER = DP / 8, AT_ONCE = 32 / PER, ROWS_OF = KEYS ? 16 : 32;  // threads of a row, rows at once, rows of a warp (KEYS: the groups share them out)
+    constexpr int COUNT = ROWS_OF / AT_ONCE, BATCH = COUNT < 8 ? COUNT : 8;    // rows of a thread, and at a time, so that one's latencies hide the others'
+    static_assert(!F32 || COUNT == BATCH, "f32: one batch");
+    const int q_part = lane % PER, q_row = ROWS_OF * (warp & 7);
+    const int64_t q_at = offset_of(q_row + lane % ROWS_OF, a.ldq);
+    uint4 q_raw[BATCH][F32 ? 2 : 1], q_next[COUNT > BATCH ? BATCH : 1][F32 ? 2 : 1];
+    auto load_q = [&](auto& to, int i0) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int r = (i0 + i) * AT_ONCE + lane / PER;
+            const int64_t from = __shfl_sync(0xFFFFFFFFu, q_at, r);
+#pragma unroll
+            for (int e = 0; e < (F32 ? 2 : 1); ++e) {
+                to[i][e] = make_uint4(0, 0, 0, 0);
+                if (q_row + r < tile.n && 8 * q_part < dim) to[i][e] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + from + 8 * q_part)[e];
+            }
+        }
+    };
+    if (warp < 8) load_q(q_raw, 0);
     const int pos_first = tile.len - tile.rows + tok_base, pos_last = tile.len - tile.rows + last_row / group;
     const int held = (int)min((int64_t)tile.len, (int64_t)a.c.max_pages * KV_PAGE);
     const int k_end = min(pos_last + 1, held), k_begin = a.window > 0 ? max(0, max(pos_first, 0) - a.window + 1) : 0;
@@ -521,35 +542,22 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         const int row_a = KEYS ? 0 : 128 * t, row_b = min(row_a + 127, tile.n - 1);
         const int whole_to = min(pos_first + token_of(row_a), held - 1), whole_from = a.window > 0 ? max(pos_first + token_of(row_b), 0) - a.window + 1 : 0;
         const int mine = F32 ? (t == 0 ? jobs : 0) : t >= groups ? 0 : (jobs - t + groups - 1) / groups;  // jobs of the group
-        // ── queries: fp16 operands, eight values a thread and row ──
+        // ── queries as operands, eight values a thread and row ──
         float c;  // scale log2(e) / what the row is multiplied by; never 0, since scores of -inf are multiplied by it
         {
-            constexpr int PER = DP / 8, AT_ONCE = 32 / PER, ROWS_OF = KEYS ? 16 : 32;  // threads of a row, rows at once, rows of a warp (KEYS: the groups share them out)
-            constexpr int COUNT = ROWS_OF / AT_ONCE, BATCH = COUNT < 8 ? COUNT : 8;    // rows of a thread, and at a time, so that one's latencies hide the others'
-            const int u = lane % PER, first = KEYS ? 16 * warp : 128 * t + 32 * (warp & 3);
-            const int64_t mine_at = offset_of(first + lane % ROWS_OF, a.ldq);
 #pragma unroll 1
             for (int i0 = 0; i0 < COUNT; i0 += BATCH) {
-                uint4 raw[BATCH][F32 ? 2 : 1];
+                if constexpr (COUNT > BATCH)
+                    if (i0 + BATCH < COUNT) load_q(q_next, i0 + BATCH);
                 uint32_t most[BATCH];  // absolute values as whole numbers: NaN is the largest
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
-                    const int r = (i0 + i) * AT_ONCE + lane / PER;
-                    const int64_t from = __shfl_sync(0xFFFFFFFFu, mine_at, r);
-#pragma unroll
-                    for (int e = 0; e < (F32 ? 2 : 1); ++e) {
-                        raw[i][e] = make_uint4(0, 0, 0, 0);
-                        if (first + r < tile.n && 8 * u < dim) raw[i][e] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + from + 8 * u)[e];
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < BATCH; ++i) {
                     if constexpr (F32) {
-                        const uint4 v = raw[i][0], w = raw[i][1];
+                        const uint4 v = q_raw[i][0], w = q_raw[i][1];
                         most[i] = max(max(max(v.x & 0x7FFFFFFFu, v.y & 0x7FFFFFFFu), max(v.z & 0x7FFFFFFFu, v.w & 0x7FFFFFFFu)),
                                       max(max(w.x & 0x7FFFFFFFu, w.y & 0x7FFFFFFFu), max(w.z & 0x7FFFFFFFu, w.w & 0x7FFFFFFFu)));
                     } else {
-                        const uint4 v = raw[i][0];
+                        const uint4 v = q_raw[i][0];
                         most[i] = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
                         most[i] = max(most[i] & 0xFFFF0000u, most[i] << 16);  // as f32
                     }
@@ -560,25 +568,25 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                     for (int i = 0; i < BATCH; ++i) most[i] = max(most[i], __shfl_xor_sync(0xFFFFFFFFu, most[i], o));
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
-                    const int q = first + (i0 + i) * AT_ONCE + lane / PER;
+                    const int q = q_row + (i0 + i) * AT_ONCE + lane / PER;
                     float by, back;
                     af_row_scale(__uint_as_float(most[i]), F32 ? 12 : 7, by, back);
                     if (a.scale < 0.f) by = -by;
-                    if (u == 0) row_factor[q] = fmaxf(back * fabsf(a.scale) * AF_LOG2E, 0x1p-149f);
+                    if (q_part == 0) row_factor[q] = fmaxf(back * fabsf(a.scale) * AF_LOG2E, 0x1p-149f);
                     float x[8];
                     if constexpr (F32) {
-                        const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w, raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
+                        const uint32_t w[8] = {q_raw[i][0].x, q_raw[i][0].y, q_raw[i][0].z, q_raw[i][0].w, q_raw[i][1].x, q_raw[i][1].y, q_raw[i][1].z, q_raw[i][1].w};
 #pragma unroll
                         for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]) * by;
                         uint4 hi, lo;
                         uint32_t *const h = &hi.x, *const l = &lo.x;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) af_split(x[2 * j], x[2 * j + 1], h[j], l[j]);
-                        uint8_t* const to = smem + q / 128 * Sh::K_TILE + u / 8 * (128 * 128) + q % 128 * 128 + ((u % 8) ^ (q & 7)) * 16;
+                        uint8_t* const to = smem + q / 128 * Sh::K_TILE + q_part / 8 * (128 * 128) + q % 128 * 128 + ((q_part % 8) ^ (q & 7)) * 16;
                         *reinterpret_cast<uint4*>(to) = hi;
                         *reinterpret_cast<uint4*>(to + Sh::TILES * Sh::K_TILE) = lo;
                     } else {
-                        const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+                        const uint32_t w[4] = {q_raw[i][0].x, q_raw[i][0].y, q_raw[i][0].z, q_raw[i][0].w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             x[2 * j] = __uint_as_float(w[j] << 16) * by;
@@ -594,10 +602,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                             const float d[4] = {x[4 * j] - f0.x, x[4 * j + 1] - f0.y, x[4 * j + 2] - f1.x, x[4 * j + 3] - f1.y};
                             lo[j] = at_digits(d);
                         }
-                        uint8_t* const to = smem + q / 128 * Sh::K_TILE + q % 128 * 128 + ((u / 2) ^ (q & 7)) * 16 + u % 2 * 8;
+                        uint8_t* const to = smem + q / 128 * Sh::K_TILE + q % 128 * 128 + ((q_part / 2) ^ (q & 7)) * 16 + q_part % 2 * 8;
                         *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
                         *reinterpret_cast<uint2*>(to + Sh::TILES * Sh::K_TILE) = make_uint2(lo[0], lo[1]);
                     }
+                }
+                if constexpr (COUNT > BATCH) {
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) q_raw[i][0] = q_next[i][0];
                 }
             }
             at_fence_smem();
@@ -882,11 +894,17 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
 }
 
-// Microseconds of a tile of keys (of two groups' rows, or one), of a block's start and end, of adding parts up: 8B shape, 512 rows at 8704, 128 at 32768.
-constexpr double AT_PIECE = 2.2, AT_PIECE_KEYS = 1.3, AT_FIXED = 9., AT_JOINED = 5.;
+// Microseconds of a tile of keys, of a block's start and end, and of adding parts up. KEYS: fitted to 64 calls (3 to 35 rows a head, 240 to 32768 keys,
+// 1 to 32 sequences, 8B, 1.5B and 0.5B shapes), from which they are 3 to 8 % off; ROWS: 512 rows at 8704.
+template <typename T, int DP, bool KEYS>
+struct AtTimes {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr double PIECE = !KEYS ? 2.2 : F32 ? (DP == 128 ? 3.4 : 2.5) : DP == 128 ? 1.7 : 1.2;
+    static constexpr double FIXED = !KEYS ? 9. : F32 ? (DP == 128 ? 6.5 : 5.5) : DP == 128 ? 7. : 6.5, JOINED = !KEYS ? 5. : F32 ? 2.5 : DP == 128 ? 3.5 : 3.;
+};
 
 template <typename T, int DP, bool KEYS>
-static cudaError_t launch_tiles(const AttentionFp8Args& a, cudaStream_t st) {
+static cudaError_t launch_tiles(const AttentionFp8Args& a, cudaStream_t st, AfShare* plan) {
     using Sh = AtShape<T, DP, KEYS>;
     static PerDeviceOnce once;
     static ClusterFits fits[SP_MAX_DEVICES];
@@ -894,22 +912,28 @@ static cudaError_t launch_tiles(const AttentionFp8Args& a, cudaStream_t st) {
     ClusterFits& mine = fits[current_device_index()];
     cudaError_t e = once.run([&] { return af_fits(reinterpret_cast<const void*>(kernel), AT_THREADS, Sh::SMEM, &mine); });
     if (e != cudaSuccess) return e;
+    const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv), height = 128 * Sh::TILES, tiles = (rows + height - 1) / height, clusters = tiles * a.c.n_kv * a.n_seqs;
+    using At = AtTimes<T, DP, KEYS>;
+    const AfShare share = af_share(mine, clusters, (af_keys(a) + AT_KEYS - 1) / AT_KEYS, At::PIECE, At::FIXED, At::JOINED);
+    const int parts = share.parts;
+    if (plan) {
+        *plan = share;
+        return cudaSuccess;
+    }
     CUtensorMap map{};
     if (!Sh::F32 && (e = af_page_map(a.c, &map)) != cudaSuccess) return e;
-    const int64_t rows = (int64_t)a.max_rows * (a.n_heads / a.c.n_kv), height = 128 * Sh::TILES, tiles = (rows + height - 1) / height, clusters = tiles * a.c.n_kv * a.n_seqs;
-    const int parts = af_share(mine, clusters, (af_keys(a) + AT_KEYS - 1) / AT_KEYS, KEYS ? AT_PIECE_KEYS : AT_PIECE, AT_FIXED, AT_JOINED).parts;
     e = launch_pdl_cluster(kernel, dim3((unsigned)(tiles * a.c.n_kv), (unsigned)a.n_seqs, (unsigned)parts), dim3(AT_THREADS), Sh::SMEM, st, parts, a, parts, (int)tiles, map);
     return e != cudaSuccess ? e : count_launch_and_check();
 }
 
 template <typename T, int DP>
-static cudaError_t tiles_as(const AttentionFp8Args& a, cudaStream_t st) {
-    if constexpr (sizeof(T) == 4) return launch_tiles<T, DP, true>(a, st);
-    else return (int64_t)a.max_rows * (a.n_heads / a.c.n_kv) <= 128 ? launch_tiles<T, DP, true>(a, st) : launch_tiles<T, DP, false>(a, st);
+static cudaError_t tiles_as(const AttentionFp8Args& a, cudaStream_t st, AfShare* plan) {
+    if constexpr (sizeof(T) == 4) return launch_tiles<T, DP, true>(a, st, plan);
+    else return (int64_t)a.max_rows * (a.n_heads / a.c.n_kv) <= 128 ? launch_tiles<T, DP, true>(a, st, plan) : launch_tiles<T, DP, false>(a, st, plan);
 }
-cudaError_t launch_attention_fp8_tiles(const AttentionFp8Args& a, bool bf, cudaStream_t st) {
-    if (a.c.dim <= 64) return bf ? tiles_as<bf16, 64>(a, st) : tiles_as<float, 64>(a, st);
-    return bf ? tiles_as<bf16, 128>(a, st) : tiles_as<float, 128>(a, st);
+cudaError_t launch_attention_fp8_tiles(const AttentionFp8Args& a, bool bf, cudaStream_t st, AfShare* plan) {
+    if (a.c.dim <= 64) return bf ? tiles_as<bf16, 64>(a, st, plan) : tiles_as<float, 64>(a, st, plan);
+    return bf ? tiles_as<bf16, 128>(a, st, plan) : tiles_as<float, 128>(a, st, plan);
 }
 
 }  // namespace sp

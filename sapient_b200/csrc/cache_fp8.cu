@@ -20,7 +20,8 @@ cudaError_t count_launch_and_check();  // kernels.cu
 // A head is 4 or 8 threads of 16 coordinates each: eight pairs that are rotated together, so that nothing is exchanged but a sum and a
 // maximum. The teams of a token take its heads in turn, the next one on its way; place and angles are loaded once. Few tokens are spread over
 // as many threads as they have heads for (1 token of the 8B shape 2.2 us, with two warps 3.3), of many a token is two warps' (8192 tokens 39.2
-// us, with a team for each head 57.6; two or three heads at a time 46 and 49: registers). What is left above the bytes' 28.4 us is XXX.
+// us, with a team for each head 57.6; two or three heads at a time 46 and 49: registers). What is left above the bytes' 28.4 us
+// is a start in which SMs wait for their first rows, and writes beside reads.
 constexpr int CA_THREADS = 256;
 
 template <typename T, int TEAM>

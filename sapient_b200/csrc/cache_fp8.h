@@ -70,6 +70,5 @@ struct AttentionFp8Args {
     int* waits;             // WaitFlags of the launch's owner
 };
 cudaError_t launch_attention_fp8(const AttentionFp8Args& a, bool bf, cudaStream_t st);
-cudaError_t launch_attention_fp8_tiles(const AttentionFp8Args& a, bool bf, cudaStream_t st);  // attention_fp8_tile.cu
 
 }  // namespace sp
