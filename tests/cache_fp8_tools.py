@@ -108,22 +108,33 @@ class Step:
         self.n, self.start, self.len, self.slot = n, ints(start), ints([x for _, _, x in seqs]), ints([s for s, _, _ in seqs])
         self.max_rows, self.max_len = max(r for _, r, _ in seqs), max(0, max(x for _, _, x in seqs))
 
-    def run(self, scale=None, window=0, max_rows=None, max_len=None, stream=None):
+    def run(self, scale=None, window=0, max_rows=None, max_len=None, stream=None, empty=0, out=None):
+        """empty: sequences without rows or tokens behind the others."""
         st = torch.cuda.current_stream().cuda_stream if stream is None else stream
-        ops.attention_fp8_dev(self.c.own, self.q.data_ptr(), self.heads, self.out.data_ptr(), len(self.seqs), self.start.data_ptr(), self.len.data_ptr(),
+        start, length, slot = self.start, self.len, self.slot
+        if empty:
+            start, length, slot = (torch.cat([x, last.expand(empty)]) for x, last in ((start, start[-1:]), (length, ints([0])), (slot, ints([0]))))
+        out = self.out if out is None else out
+        ops.attention_fp8_dev(self.c.own, self.q.data_ptr(), self.heads, out.data_ptr(), len(self.seqs) + empty, start.data_ptr(), length.data_ptr(),
                               self.max_rows if max_rows is None else max_rows, self.max_len if max_len is None else max_len,
-                              self.c.dim**-0.5 if scale is None else scale, window=window, seq_slot=self.slot.data_ptr(), dtype=self.ty, ldq=self.ld, ldo=self.ld, stream=st)
-        return self.out
+                              self.c.dim**-0.5 if scale is None else scale, window=window, seq_slot=slot.data_ptr(), dtype=self.ty, ldq=self.ld, ldo=self.ld, stream=st)
+        return out
 
     def check(self, scale=None, window=0, digits=False):
+        """What is in out, and what the call leaves where large bounds, or sequences with nothing to do, make it share the work out otherwise."""
         wide = self.heads * self.c.dim
         q = self.q[: self.n, :wide].reshape(self.n, self.heads, self.c.dim)
         want, far = attention64(self.c, q, self.seqs, self.c.dim**-0.5 if scale is None else scale, window, digits)
-        got = self.out[: self.n, :wide].reshape(want.shape).double()
-        assert torch.equal(got.isnan(), want.isnan())
-        off = (got - want).abs().nan_to_num()
-        assert (off <= far.nan_to_num(nan=1.0)).all(), f"off by {float((off / far.nan_to_num(nan=1.0)).max())} of what it may be"
-        assert (self.out[self.n:] == 7).all() and (self.out[:, wide:] == 7).all()  # what is behind the last row and beside the heads
+        outs = {"as asked": self.out}
+        some = 128 * self.c.kv // self.heads  # tokens with which a key head has 128 rows
+        for name, most, empty in (("many rows", 4096, 0), ("many sequences", 1, 64), ("some rows of many", some, 70), ("some rows of some", some, 18)):
+            outs[name] = self.run(scale, window, max(most, self.max_rows), empty=empty, out=torch.full_like(self.out, 7.0))
+        for name, out in outs.items():
+            got = out[: self.n, :wide].reshape(want.shape).double()
+            assert torch.equal(got.isnan(), want.isnan()), name
+            off = (got - want).abs().nan_to_num()
+            assert (off <= far.nan_to_num(nan=1.0)).all(), f"{name}: off by {float((off / far.nan_to_num(nan=1.0)).max())} of what it may be"
+            assert (out[self.n:] == 7).all() and (out[:, wide:] == 7).all(), name  # what is behind the last row and beside the heads
 
 
 def rotated64(x, angles, rotary, pairs):

@@ -135,14 +135,14 @@ def test_values_of_very_different_size(rows, ty):
 
 @BOTH
 def test_rows_with_nan_or_infinities_keep_to_themselves(ty):
-    for rows in (3, 140):
+    for rows, most in ((3, None), (140, None), (140, 4096), (3, 4096)):
         c = Cache([400], 2, 128, 11)
         s = Step(c, [(0, rows, 400)], 4, ty, 12)
-        s.run()
+        s.run(max_rows=most)
         want = s.out.clone()
         s.q[1, :128] = math.nan
         s.q[2, 130] = math.inf
-        s.run()
+        s.run(max_rows=most)
         got = s.out.clone()
         assert got[1, :128].isnan().all() and not got[0].isnan().any()
         want[1, :128] = want[2, 128:256] = got[1, :128] = got[2, 128:256] = 0
@@ -156,9 +156,13 @@ def test_strides_and_in_place(rows, ty):
     s = Step(c, [(0, rows, 250)], 4, ty, 14, ld=4 * 80 + 24)
     s.run()
     s.check()
-    want = s.out[: s.n, : 4 * 80].clone()
-    ops.attention_fp8_dev(c.own, s.q.data_ptr(), 4, s.q.data_ptr(), 1, s.start.data_ptr(), s.len.data_ptr(), rows, 250, 80**-0.5, dtype=ty, ldq=s.ld, ldo=s.ld)
-    assert torch.equal(s.q[:, : 4 * 80], want)
+    q = s.q.clone()
+    for most in (rows, 128, 4096):
+        s.q.copy_(q)
+        s.run(max_rows=max(rows, most))
+        want = s.out[: s.n, : 4 * 80].clone()
+        ops.attention_fp8_dev(c.own, s.q.data_ptr(), 4, s.q.data_ptr(), 1, s.start.data_ptr(), s.len.data_ptr(), max(rows, most), 250, 80**-0.5, dtype=ty, ldq=s.ld, ldo=s.ld)
+        assert torch.equal(s.q[:, : 4 * 80], want)
 
 
 @BOTH
