@@ -14,7 +14,9 @@
 // 128 keys. Short prompts are bound by a block's start (5 us until its queries are operands) and end (2 us): 9 x 1500 rows, 2.7B shape, 247 us.
 // ROWS: the groups have 128 rows each of 256, and keys in common. KEYS (up to 128 rows): the same rows, key tiles by turns; their sums
 // are added up at the end. f32: one group with two tiles of scores; the tensor cores cut off what falls below a sum's last bits, always towards
-// zero (2^-26 of it an addition: 1.8e-5 after 8192 keys), so that O is added to a sum of its own by the vector units every AT_FLUSH tiles. Keys may be shared out to the blocks of a cluster as well, which add up through shared memory.
+// zero (2^-26 of it an addition: 1.8e-5 after 8192 keys), so that O is added to a sum of its own by the vector units every AT_FLUSH tiles (64 rows at
+// 131072 keys: 1.7e-6 off with four, 1.2e-6 with two, which take 2 % longer). Keys may be shared out to the blocks of a cluster as well, which add
+// up through shared memory.
 //
 // A tile's values have a power of two 2^u, not below the largest of their scales. For bf16 rows they are multiplied by s' 2^(7 - u) as they become
 // fp16 (off by 2^-11 of themselves), so that a weight is one exponential, 2^(z - M + u - 7); for f32 rows values stay exact and weights
@@ -34,7 +36,7 @@ namespace sp {
 cudaError_t count_launch_and_check();  // kernels.cu
 
 constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 512, AT_RING = 8;
-constexpr int AT_FLUSH = 4;
+constexpr int AT_FLUSH = 2;
 constexpr float AT_MOST = 15.f, AT_SET = 9.f;  // log2 of the largest weight, and of it when M is set
 constexpr int AT_UP = 7, AT_LEAST = -80;       // values times 2^7 are below 2^16; smaller u would let a sum of 2^(z - M) pass 2^127
 
