@@ -233,3 +233,37 @@ def test_append_attention_and_read_one_after_the_other(rows, ty):
     for (_, s), w in zip(steps, outs):
         assert torch.equal(s.out[: s.n], w[: s.n])
     check(lib().sp_cuda_check_kernels(0))
+
+
+@BOTH
+@pytest.mark.parametrize("heads,kv,dim", [(32, 8, 128), (14, 2, 64)])
+def test_append_long_prompt(heads, kv, dim, ty):
+    """So many tokens that one is only two warps' work."""
+    go([(0, 3 + i) for i in range(5000)], [5003], heads, kv, dim, ty, dim)
+
+
+@BOTH
+@pytest.mark.parametrize("n", [9999, 10000, 12347])
+def test_read_many(n, ty):
+    """Enough tokens that a warp takes four, some of which are not there; keys and values, and either alone."""
+    kv, dim = 3, 48
+    c = Cache([900, 0, 333], kv, dim, 12)
+    c.table[0, 5], c.table[2, 3], c.table[2, 4] = -1, c.n_pages, 2**31 - 1
+    g = torch.Generator(device="cuda").manual_seed(n)
+    slot = torch.randint(-1, 4, (n,), generator=g, device="cuda").int()
+    pos = torch.randint(-3, 16 * c.max_pages + 3, (n,), generator=g, device="cuda").int()
+    s, p = slot.long().clamp(0, 2), pos.long().clamp(0, 16 * c.max_pages - 1)
+    page = c.table[s, p // PAGE].long()
+    there = (slot >= 0) & (slot < 3) & (pos >= 0) & (pos < 16 * c.max_pages) & (page >= 0) & (page < c.n_pages)
+    assert there.any() and not there.all()
+    page = torch.where(there, page, 0)
+    for both in (3, 1, 2):
+        out = [torch.full((n + 1, kv * dim), 7.0, device="cuda", dtype=TYPES[ty]) for _ in range(2)]
+        ops.cache_fp8_read_dev(c.own, n, slot.data_ptr(), pos.data_ptr(), *(y.data_ptr() if both >> i & 1 else 0 for i, y in enumerate(out)), dtype=ty)
+        for which, y in enumerate(out):
+            want = c.values[page, which, :, p % PAGE].view(torch.float8_e4m3fn).double() * c.scales[page, which, :, p % PAGE].double().unsqueeze(-1)
+            off = (y[:n].double() - want.reshape(n, -1)).abs()
+            if both >> which & 1:
+                assert (off <= want.reshape(n, -1).abs() * STEP[ty])[there].all() and (y[:n][~there] == 7).all() and (y[n] == 7).all()
+            else:
+                assert (y == 7).all()
