@@ -132,8 +132,10 @@ __global__ void __launch_bounds__(CA_THREADS) cache_append_kernel(const CacheApp
 template <typename T>
 static cudaError_t append_as(const CacheAppendArgs& a, cudaStream_t st) {
     const int team = a.c.dim <= 64 ? 4 : 8, heads = (a.q ? a.n_heads : 0) + 2 * a.c.n_kv;
+    // fewer threads a token as soon as eleven warps an SM are left (8B shape, bf16, 256 and 64 threads: 128 tokens 2.8 and 4.3 us, 512 6.0 and 5.2, 1024 9.6
+    // and 8.8, 4096 31.3 and 22.8; 0.5B shape, 96 and 64: 1024 2.8 and 3.5, 4096 8.2 and 7.8)
     int per_token = std::min(CA_THREADS, (heads * team + 31) / 32 * 32);
-    while (per_token > 64 && a.n_tok * (per_token / 2) >= (int64_t)device_sm_count() * 1024) per_token = (per_token / 2 + 31) / 32 * 32;
+    while (per_token > 64 && a.n_tok * (per_token / 2) >= (int64_t)device_sm_count() * 352) per_token = (per_token / 2 + 31) / 32 * 32;
     const int tokens = std::max(1, 64 / per_token), threads = tokens * per_token;
     const cudaError_t e = launch_pdl(team == 4 ? cache_append_kernel<T, 4> : cache_append_kernel<T, 8>, dim3((unsigned)((a.n_tok + tokens - 1) / tokens)), dim3(threads), 0, st, a, per_token);
     return e != cudaSuccess ? e : count_launch_and_check();

@@ -236,10 +236,11 @@ def test_append_attention_and_read_one_after_the_other(rows, ty):
 
 
 @BOTH
+@pytest.mark.parametrize("n", [500, 5000])
 @pytest.mark.parametrize("heads,kv,dim", [(32, 8, 128), (14, 2, 64)])
-def test_append_long_prompt(heads, kv, dim, ty):
-    """So many tokens that one is only two warps' work."""
-    go([(0, 3 + i) for i in range(5000)], [5003], heads, kv, dim, ty, dim)
+def test_append_long_prompt(heads, kv, dim, n, ty):
+    """So many tokens that one is only four or two warps' work."""
+    go([(0, 3 + i) for i in range(n)], [n + 3], heads, kv, dim, ty, dim)
 
 
 @BOTH
