@@ -230,8 +230,8 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
         float ks[4], vs[4];  // of keys g + 8 j
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            ks[j] = scales[8 * j];
-            vs[j] = scales[AR_KEYS + 8 * j];
+            ks[j] = af_number(scales[8 * j]);
+            vs[j] = af_number(scales[AR_KEYS + 8 * j]);
         }
         float big = 0.f;  // the largest finite scale of values that a row of the tile may see
 #pragma unroll

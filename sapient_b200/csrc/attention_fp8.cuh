@@ -32,6 +32,8 @@ __device__ __forceinline__ uint32_t af_finite(uint32_t two) {
     asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(two), "r"(0x5F005F00u));
     return d;
 }
+// A scale; NaN for one that is infinite, with which a score of the wrong sign would be the weight 0.
+__device__ __forceinline__ float af_number(float s) { return fmaf(s, 0.f, s); }
 __device__ __forceinline__ uint32_t af_pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);

@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 uint32_t big = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    f[j] = v[j] < INFINITY && v[j] > -INFINITY ? k[j] : __uint_as_float(0x7FC00000u);
+                    f[j] = v[j] < INFINITY && v[j] > -INFINITY ? af_number(k[j]) : __uint_as_float(0x7FC00000u);
                     if (counts(v[j], token + j)) big = max(big, __float_as_uint(v[j]));
                 }
                 *reinterpret_cast<float4*>(&k_scale[slot][4 * lane]) = to;
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 if (!ok) break;
                 store(raw_k, ks_ + st * Sh::K_TILE, by, false);
                 const float v = counts(sv, key0 + p) ? sv : 0.f;
-                k_scale[slot][p] = sv < INFINITY && sv > -INFINITY ? sk : __uint_as_float(0x7FC00000u);
+                k_scale[slot][p] = sv < INFINITY && sv > -INFINITY ? af_number(sk) : __uint_as_float(0x7FC00000u);
                 v_scale[slot][p] = v;
                 const uint32_t big = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v));
                 if (lane == 0) largest_s[slot][warp - 8] = big;

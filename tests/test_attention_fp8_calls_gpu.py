@@ -111,3 +111,28 @@ def test_a_wait_that_ran_out():
     with pytest.raises(SapientCudaError, match="attention"):
         check(lib().sp_cuda_check_kernels(0))
     check(lib().sp_cuda_check_kernels(0))
+
+
+@pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
+@pytest.mark.parametrize("rows", [1, 5, 140])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("scale", [float("inf"), float("nan")])
+def test_scales_that_are_no_numbers(scale, which, rows, ty):
+    """Rows that see a key or value with such a scale are NaN, whatever the sign of its score; earlier ones are not."""
+    c = Cache([300], 2, 64, 70)
+    s = Step(c, [(0, rows, 300)], 4, ty, 71)
+    for back in (0, min(rows - 1, 3)):  # tokens behind the one
+        old = c.scales.clone()
+        at = 299 - back
+        page = int(c.table[0, at // 16])
+        c.values.view(torch.float8_e4m3fn)[page, which, :, at % 16] = 2.0
+        c.scales[page, which, :, at % 16] = scale
+        for most, empty in ((rows, 0), (32, 70), (4096, 0)):
+            for sign in (1, -1):
+                q = s.q.clone()
+                s.q.copy_(sign * s.q.abs())
+                s.run(max_rows=max(most, rows), empty=empty)
+                s.q.copy_(q)
+                sees = torch.arange(rows, device="cuda") >= rows - 1 - back
+                assert s.out[: s.n].isnan().all(-1)[sees].all() and not s.out[: s.n].isnan().any(-1)[~sees].any()
+        c.scales.copy_(old)
