@@ -50,12 +50,13 @@ __device__ __forceinline__ void af_mma(float (&c)[4], const uint4& a, uint32_t b
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-// A power of two by which a row is multiplied so that its largest value lies in [2^to, 2^(to + 1)), and its reciprocal. Rows of zeros and
-// those with infinities or NaN: 1.
+// A power of two by which a row is multiplied so that its largest value lies in [2^to, 2^(to + 1)), and its reciprocal. Rows of zeros: 1. Rows with
+// infinities or NaN are multiplied by NaN: their scores are infinite or NaN, and so softmax has no value, but an infinity that is converted to e4m3
+// would be a large number there.
 __device__ __forceinline__ void af_row_scale(float most, int to, float& by, float& back) {
     const int e = (int)(__float_as_uint(most) >> 23);  // (most >= 0)
     const int up = e == 0 || e == 255 ? 0 : min(max(127 + to - e, -126), 126);
-    by = __uint_as_float((uint32_t)(127 + up) << 23);
+    by = __uint_as_float(e == 255 ? 0x7FC00000u : (uint32_t)(127 + up) << 23);
     back = __uint_as_float((uint32_t)(127 - up) << 23);
 }
 // The smallest power of two that is not below a scale (positive and finite), within what has a reciprocal.
