@@ -236,8 +236,9 @@ int32_t sp_cuda_cache_fp8_read_dev(const void* cache, int32_t dtype, int64_t n_t
  * tokens on pages that are not there are not seen. out may be q with the same stride. max_rows: of any sequence, not less than they
  * have (rows past it stay as they are); max_len: of any sequence (a wrong one costs time only). By both the kernel is chosen and the work
  * shared out, so that bounds far above what the sequences have cost time. Rows in front of row_start[0] and behind row_start[n_seqs] stay as
- * they are. Scales are not negative; a key or value row whose scale is NaN or infinite makes the rows that see it NaN, and no others. A row's
- * head whose query has a NaN or an infinity is NaN if it sees a key, and no other is. n_seqs is at most 65535.
+ * they are. Scales are not negative; a key or value row whose scale is NaN or infinite makes the rows that see it NaN, and no others; so
+ * do bytes that are NaN beside a finite scale (_append leaves none), those of values in their coordinate at least. A row's head whose query has
+ * a NaN or an infinity is NaN if it sees a key, and no other is. n_seqs is at most 65535.
  * Precision: weights have 11 bits for bf16 rows, 22 for f32 rows (a value whose scale is below 2^-20 of the largest beside it fewer); f32
  * queries have 22 bits; bf16 ones are exact where up to 16 rows share a key head (tokens x heads), with more they may be off by up to 2^-17
  * of a head's largest coordinate, and values times their scale have 11 bits. Sums are f32, in an order that depends on the sizes,

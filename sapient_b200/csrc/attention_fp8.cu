@@ -180,7 +180,9 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
         }
     }
     const int whole_from = a.window > 0 ? max(pos_last, 0) - a.window + 1 : 0, whole_to = min(pos_first, held - 1);  // keys that all rows see
-    // MASK: some row does not see some key. Only then can a byte that is NaN belong to a key that a row does not see.
+    uint32_t dropped = 0;  // values' bytes that are NaN, where MASK
+    // MASK: some row does not see some key. Only then can a byte that is NaN belong to a key that a row does not see; else the product makes its
+    // coordinate NaN.
     auto work = [&](auto with_mask, const uint8_t* at, const float* scales, int key0, uint32_t gone) {
         constexpr bool MASK = decltype(with_mask)::value;
         float s[NT][2][4];  // keys 16 pg + g and + 8
@@ -313,6 +315,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
         for (int pg = 0; pg < 2; ++pg) {
             constexpr int WORDS = DP / 32;  // of a thread's part of a token's values
             uint32_t vw[4][WORDS];
+            [[maybe_unused]] uint32_t near = 0, far = 0;  // tokens 2 t, 2 t + 1 and tokens 2 t + 8, 2 t + 9 with such bytes
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int key = 2 * t + (j & 1) + 8 * (j >> 1);
@@ -334,12 +337,18 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
                 af_halves(__byte_perm(vw[2][w], vw[3][w], 0x7362), v[1].z, v[1].w);
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    if (MASK) v[q] = make_uint4(af_finite(v[q].x), af_finite(v[q].y), af_finite(v[q].z), af_finite(v[q].w));
+                    if (MASK) v[q] = make_uint4(af_finite(v[q].x, near), af_finite(v[q].y, near), af_finite(v[q].z, far), af_finite(v[q].w, far));
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int p = F32 ? 1 : 0; p >= 0; --p) af_mma(o[n][2 * w + q], v[q], pb[n][p][pg].x, pb[n][p][pg].y);
                 }
+            }
+            if (MASK && !(gone >> pg & 1)) {  // (bytes that nobody sees may be anything)
+                auto counts = [&](int token) { return key0 + token >= k_begin && key0 + token < k_end; };
+                const int k = KV_PAGE * pg + 2 * t;
+                dropped |= near & ((counts(k) ? 0xFFFFu : 0u) | (counts(k + 1) ? 0xFFFF0000u : 0u));
+                dropped |= far & ((counts(k + 8) ? 0xFFFFu : 0u) | (counts(k + 9) ? 0xFFFF0000u : 0u));
             }
         }
     };
@@ -378,6 +387,18 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
         for (int i = 0; i < STAGES; ++i) tc5_wait(&full[warp][i], parity);
     }
     __syncwarp();
+    if (__any_sync(0xFFFFFFFFu, dropped != 0)) {
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {
+            const int key0 = (b_begin + warp + i * W) * AR_KEYS;
+            const uint32_t tokens = af_nan_tokens(a.c, table, head, key0, k_end);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (af_sees(tokens, key0, low[n][e], limit[n][e])) l[n][e] = __uint_as_float(0x7FC00000u);
+        }
+    }
     // ── the warps' sums into one, then the blocks' ──
 #pragma unroll
     for (int n = 0; n < NT; ++n)

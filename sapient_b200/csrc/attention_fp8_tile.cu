@@ -203,6 +203,32 @@ __device__ __forceinline__ float at_max3(float a, uint64_t two) {
     return d;
 }
 
+// 16 bytes of N tokens, PER apart, as fp16 to `to` (of the first) and u0, u1. Keys as they are; values without NaN and times `by` (f32 rows: as they
+// are). The second half of a row's threads (odd) swap the halves of their 16 bytes: eight threads' stores fall on 32 different banks. Back: whether
+// values had NaN.
+template <bool F32, bool VALUES, int PER, int N>
+__device__ __forceinline__ uint32_t at_convert(const uint4 (&raw)[N], const uint32_t (&by)[N], uint8_t* to, int u0, int u1, bool odd) {
+    uint32_t dropped = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        uint32_t h[8];
+        af_halves(odd ? raw[i].z : raw[i].x, h[0], h[1]);
+        af_halves(odd ? raw[i].w : raw[i].y, h[2], h[3]);
+        af_halves(odd ? raw[i].x : raw[i].z, h[4], h[5]);
+        af_halves(odd ? raw[i].y : raw[i].w, h[6], h[7]);
+        if constexpr (VALUES) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[j] = af_finite(h[j], dropped);
+                if constexpr (!F32) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(by[i]));
+            }
+        }
+        *reinterpret_cast<uint4*>(to + PER * i * 128 + u0) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(to + PER * i * 128 + u1) = make_uint4(h[4], h[5], h[6], h[7]);
+    }
+    return dropped;
+}
+
 template <typename T, int DP, bool KEYS>
 __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const AttentionFp8Args a, int parts, int tiles, const __grid_constant__ CUtensorMap map) {
     using Sh = AtShape<T, DP, KEYS>;
@@ -212,6 +238,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     __shared__ __align__(8) uint64_t k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES], s_full[2], p_full[2][2], o_done, o_full, q_full;
     __shared__ __align__(16) float k_scale[AT_RING][AT_KEYS], v_scale[AT_RING][F32 ? AT_KEYS : 4];
     __shared__ uint32_t gone_s[AT_RING];     // pages of the tile that are not there
+    __shared__ uint32_t nan_dropped;         // some value bytes were NaN
     __shared__ __align__(16) uint32_t largest_s[AT_RING][4];  // scales of values that count, of 32 tokens each
     __shared__ float row_factor[ROWS];
     __shared__ float part_m[2][128], part_l[2][128];
@@ -270,6 +297,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     if (tid == 32) {
+        nan_dropped = 0;
         for (int i = 0; i < K_STAGES; ++i) {
             at_init(&k_full[i], F32 ? 4 : 1);
             at_init(&k_empty[i], 1);
@@ -434,29 +462,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 if (16 * ch < dim) raw[i] = __ldg(reinterpret_cast<const uint4*>(from + (int64_t)max(page, 0) * page_bytes));
             }
         };
-        // The second half of a row's threads swap the halves of their 16 bytes: eight threads' stores fall on 32 different banks.
         const bool odd = ch / 4;
-        const int x = tok0 & 7, u0 = ((2 * (ch % 4) + odd) ^ x) * 16, u1 = ((2 * (ch % 4) + 1 - odd) ^ x) * 16;
-        auto store = [&](const uint4 (&raw)[N], uint8_t* tile_at, const uint32_t (&by)[N], bool values) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                uint32_t h[8];
-                af_halves(odd ? raw[i].z : raw[i].x, h[0], h[1]);
-                af_halves(odd ? raw[i].w : raw[i].y, h[2], h[3]);
-                af_halves(odd ? raw[i].x : raw[i].z, h[4], h[5]);
-                af_halves(odd ? raw[i].y : raw[i].w, h[6], h[7]);
-                if (values) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        h[j] = af_finite(h[j]);
-                        if constexpr (!F32) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(by[i]));
-                    }
-                }
-                uint8_t* const row = tile_at + ch / 4 * (128 * 128) + (tok0 + PER * i) * 128;
-                *reinterpret_cast<uint4*>(row + u0) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4*>(row + u1) = make_uint4(h[4], h[5], h[6], h[7]);
-            }
-        };
+        const int x = tok0 & 7, u0 = ((2 * (ch % 4) + odd) ^ x) * 16, u1 = ((2 * (ch % 4) + 1 - odd) ^ x) * 16, row0 = ch / 4 * (128 * 128) + tok0 * 128;
         auto hand_over = [&](uint64_t* bar) {
             at_fence_smem();
             __syncwarp();
@@ -487,13 +494,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         }
         for (int kv = 0; kv < n_kv; ++kv) {
             const int key0 = (b_begin + kv) * AT_KEYS;
+            const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
             uint32_t by[N] = {};  // what values are multiplied by, as pairs of fp16
             if constexpr (F32) {
                 const int st = kv % K_STAGES, use = kv / K_STAGES, slot = kv % AT_RING;
-                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
                 if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&k_empty[st], (uint32_t)((use - 1) & 1)));
                 if (!ok) break;
-                store(raw_k, ks_ + st * Sh::K_TILE, by, false);
+                at_convert<F32, false, PER>(raw_k, by, ks_ + st * Sh::K_TILE + row0, u0, u1, odd);
                 const float v = counts(sv, key0 + p) ? sv : 0.f;
                 k_scale[slot][p] = sv < INFINITY && sv > -INFINITY ? af_number(sk) : __uint_as_float(0x7FC00000u);
                 v_scale[slot][p] = v;
@@ -523,7 +530,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             const int st = kv % V_STAGES, use = kv / V_STAGES;
             if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&v_empty[st], (uint32_t)((use - 1) & 1)));
             if (!ok) break;
-            store(raw_v, vs_ + st * Sh::TILE, by, true);
+            if (gone != 0 || key0 < k_begin || key0 + (AT_KEYS - 1) >= k_end) {  // bytes that nobody sees may be anything
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int token = tok0 + PER * i;
+                    if (gone >> (token / KV_PAGE) & 1 || key0 + token < k_begin || key0 + token >= k_end) raw_v[i] = make_uint4(0, 0, 0, 0);
+                }
+            }
+            if (at_convert<F32, true, PER>(raw_v, by, vs_ + st * Sh::TILE + row0, u0, u1, odd) != 0) nan_dropped = 1;
             hand_over(&v_full[st]);
             pages = next;
             next = page_of(kv + 2);
@@ -761,6 +775,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         if (jobs > 0) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&o_full, 0));
         else asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
         at_after();
+        if (jobs > 0 && ok && nan_dropped != 0) {  // (set before the products whose end has been waited for)
+#pragma unroll 1
+            for (int i = 0; i < n_kv * (AT_KEYS / 32); ++i) {
+                const int key0 = b_begin * AT_KEYS + 32 * i;
+                if (af_sees(af_nan_tokens(a.c, table, head, key0, k_end), key0, low, limit)) l = __uint_as_float(0x7FC00000u);
+            }
+        }
         T* const out = static_cast<T*>(a.out);
         if (!KEYS && parts == 1) {
             const float by = l == 0.f || mine == 0 ? 0.f : 1.f / l;
