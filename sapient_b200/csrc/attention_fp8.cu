@@ -21,6 +21,7 @@
 #include "attention_fp8.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
+#include "ring.h"
 #include "tc5_ptx.cuh"
 
 namespace sp {
@@ -354,7 +355,8 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
     };
     bool ok = true;
     uint32_t parity = 0;
-    for (int i = 0, stage = 0; i < steps; ++i) {
+    int i = 0;
+    for (int stage = 0; i < steps; ++i) {
         const int ahead = i + STAGES - 1;
         if (ahead % GROUP == 0) pages = pages_next;
         if (ahead % GROUP == GROUP / 2) pages_next = look_up(ahead / GROUP * GROUP + GROUP);
@@ -382,9 +384,9 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
             parity ^= 1;
         }
     }
-    if (!ok && lane == 0) {  // copies on their way to this block are waited for, for as long again
+    if (!ok && lane == 0) {  // copies on their way to this block are waited for, for as long again each
         report_wait(a.waits, WAIT_ATTENTION);
-        for (int i = 0; i < STAGES; ++i) tc5_wait(&full[warp][i], parity);
+        for (int k = i; k < ring_requested(i, STAGES, steps); ++k) tc5_wait(&full[warp][ring_at(k, STAGES).stage], ring_at(k, STAGES).parity);
     }
     __syncwarp();
     if (__any_sync(0xFFFFFFFFu, dropped != 0)) {

@@ -435,12 +435,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             if (!F32 && j + groups < jobs) scores(j + groups);
         }
         if (jobs > 0) {
-            if (ok && leader) tc5_commit(&o_full);
+            if (leader) tc5_commit(&o_full);  // (after a wait that ran out too: no product is under way when its tensor memory is given back)
             __syncwarp();
             // no arrival is on its way to this block when it goes on to the end
             for (int kv = max(0, n_kv - K_STAGES); kv < n_kv; ++kv) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&k_empty[kv % K_STAGES], (uint32_t)((kv / K_STAGES) & 1)));
             for (int kv = max(0, n_kv - V_STAGES); kv < n_kv; ++kv) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&v_empty[kv % V_STAGES], (uint32_t)((kv / V_STAGES) & 1)));
-            ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&o_full, 0));
+            ok = __all_sync(0xFFFFFFFFu, tc5_wait(&o_full, 0) && ok);
         }
         }
         if (parts > 1) {
