@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
     const int pos_first = pos_base + tile.row0 / group, pos_last = pos_base + (tile.row0 + tile.n - 1) / group;  // of the tile's rows
     const int held = (int)min((int64_t)tile.len, (int64_t)a.c.max_pages * KV_PAGE);
     const int k_end = min(pos_last + 1, held), k_begin = a.window > 0 ? max(0, max(pos_first, 0) - a.window + 1) : 0;
-    const int s_begin = k_begin / AR_KEYS, s_end = k_end > k_begin ? (k_end + AR_KEYS - 1) / AR_KEYS : s_begin;
+    const int s_begin = k_begin / AR_KEYS, s_end = k_end > k_begin ? (k_end - 1) / AR_KEYS + 1 : s_begin;  // (k_end may be near 2^31)
     const int per = (s_end - s_begin + parts - 1) / parts;
     const int b_begin = min(s_end, s_begin + part * per), b_end = min(s_end, b_begin + per);
     const int steps = max(0, (b_end - b_begin - warp + W - 1) / W);  // of this warp: b_begin + warp + i W

@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     const int pos_first = tile.len - tile.rows + tok_base, pos_last = tile.len - tile.rows + last_row / group;
     const int held = (int)min((int64_t)tile.len, (int64_t)a.c.max_pages * KV_PAGE);
     const int k_end = min(pos_last + 1, held), k_begin = a.window > 0 ? max(0, max(pos_first, 0) - a.window + 1) : 0;
-    const int t_begin = k_begin / AT_KEYS, t_end = k_end > k_begin ? (k_end + AT_KEYS - 1) / AT_KEYS : t_begin;
+    const int t_begin = k_begin / AT_KEYS, t_end = k_end > k_begin ? (k_end - 1) / AT_KEYS + 1 : t_begin;  // (k_end may be near 2^31)
     const int per = (t_end - t_begin + parts - 1) / parts;
     const int b_begin = min(t_end, t_begin + part * per), n_kv = min(t_end, b_begin + per) - b_begin;  // key tiles of the block
     const int groups = KEYS || tile.n > 128 ? 2 : 1, jobs = KEYS ? n_kv : groups * n_kv;  // job j is group j % groups'
