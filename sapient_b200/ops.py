@@ -6,6 +6,7 @@ and the resident-weight kernel API of its GPU context
 from __future__ import annotations
 
 import ctypes as C
+import warnings
 
 import numpy as np
 
@@ -325,14 +326,19 @@ def cache_fp8_bytes(n_pages: int, n_kv_heads: int, head_dim: int) -> tuple[int, 
     return rows * head_dim, rows * 4
 
 
-def rope_table(n_positions: int, rotary_dim: int, base: float, factor: float = 1.0, original: int = 0, low: float = 0.25, high: float = 1.0) -> np.ndarray:
+def rope_table(n_positions: int, rotary_dim: int, base: float, factor: float = 1.0, original: int = 0, low: float | None = None, high: float | None = None) -> np.ndarray:
     """Angles for cache_fp8_append_dev: [n_positions, rotary_dim / 2, 2] f32 cosines and sines of position x base^(-2 i / rotary_dim), made in
     64 bits. For contexts longer than a model was trained on: factor alone divides every frequency; with `original` (the length of
-    training) only those that make at most `low` turns within it are divided, those of `high` turns and more stay, and between the two it goes over."""
+    training) only those that make at most `low` turns within it are divided, those of `high` turns and more stay, and between the two it goes over.
+    low and high are a model's low_freq_factor and high_freq_factor (1 and 4 where its configuration has rope_type llama3): give them. Without
+    them a ramp of 0.25 to 1 turns is taken, which is no published rule, and a warning says so."""
+    if original and (low is None or high is None):
+        warnings.warn("rope_table: original without low and high: 0.25 and 1 turns are taken where a model has its low_freq_factor and high_freq_factor (usually 1 and 4)", stacklevel=2)
+    low, high = 0.25 if low is None else low, 1.0 if high is None else high
     if n_positions < 0 or rotary_dim < 0 or rotary_dim % 2:
         raise SapientCudaError(_lib.SP_ERR_SHAPE, "rope_table: rotary_dim must be even")
-    if not (factor > 0 and base > 0) or (original and not 0 <= low < high):
-        raise SapientCudaError(_lib.SP_ERR_ARG, "rope_table: factor and base must be positive, low below high")
+    if not (factor > 0 and base > 0) or original < 0 or (original and not 0 <= low < high):
+        raise SapientCudaError(_lib.SP_ERR_ARG, "rope_table: factor and base must be positive, original not negative, low below high")
     f = float(base) ** (-np.arange(0, rotary_dim, 2, dtype=np.float64) / max(rotary_dim, 1))
     keep = np.clip((original * f / (2 * np.pi) - low) / (high - low), 0, 1) if original else np.zeros_like(f)
     angle = np.arange(n_positions, dtype=np.float64)[:, None] * (f * keep + f / factor * (1 - keep))
