@@ -315,8 +315,13 @@ class CacheFp8:
     [n_pages, 2, n_kv_heads, 16] (f32) and page_table [n_slots, max_pages] (int32), which stay the caller's."""
 
     def __init__(self, values: int, scales: int, page_table: int, n_pages: int, n_slots: int, max_pages: int, n_kv_heads: int, head_dim: int, device: int = 0):
+        sizes = device, n_pages, n_slots, max_pages, n_kv_heads, head_dim
+        if any(not -(2**31) <= n < 2**31 for n in sizes):  # (a field of 32 bits would keep its last ones)
+            raise SapientCudaError(_lib.SP_ERR_SHAPE, "CacheFp8: a size does not fit 32 bits")
+        if any(not 0 <= at < 2**64 for at in (values, scales, page_table)):
+            raise SapientCudaError(_lib.SP_ERR_ARG, "CacheFp8: an address does not fit 64 bits")
         self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
-        self.desc = _lib.SpCacheFp8(values, scales, page_table, device, n_pages, n_slots, max_pages, n_kv_heads, head_dim)
+        self.desc = _lib.SpCacheFp8(values, scales, page_table, *sizes)
         self.at = C.addressof(self.desc)
 
 
