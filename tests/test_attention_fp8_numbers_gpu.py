@@ -1,11 +1,13 @@
-"""Attention over a cache of 8-bit rows where numbers end: infinite queries and bytes that are NaN."""
+"""Attention over a cache of 8-bit rows where numbers end: infinite queries, bytes that are NaN, factors of the scores that are zero, negative or
+large, and long sums of f32 rows."""
 import math
 
 import pytest
 import torch
 
-from cache_fp8_tools import PAGE, Cache, Step
+from cache_fp8_tools import PAGE, Cache, Step, attention64
 from sapient_b200 import ops
+from sapient_b200._lib import check, lib
 
 pytestmark = pytest.mark.gpu
 BOTH = pytest.mark.parametrize("ty", [ops.F32, ops.BF16])
@@ -92,3 +94,46 @@ def test_nan_on_pages_of_others(rows, ty):
     s.run()
     s.check()
     assert not s.out.isnan().any()
+
+
+@BOTH
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.09, 2.0, -30.0, 1e-30])
+@pytest.mark.parametrize("rows,dim", [(1, 128), (20, 64), (140, 128), (300, 64)])
+def test_factors_of_the_scores(rows, dim, scale, ty):
+    """-scale and q are scale and -q: the bounds on errors are those of the latter. 0: the mean of what a row sees."""
+    c = Cache([700, 300, 300], 2, dim, 7)
+    s = Step(c, [(0, rows, 700), (1, rows, rows // 2), (2, rows, 0)], 4, ty, 8)
+    c.table[0, 5] = -1
+    q = s.q[: s.n].reshape(s.n, 4, dim)
+    for window in (0, 33):
+        want, far = attention64(c, -q if scale < 0 else q, s.seqs, abs(scale), window, True)
+        for most, empty in ways(s):
+            got = s.run(scale=scale, window=window, max_rows=most, empty=empty, out=torch.full_like(s.out, 7.0))
+            off = (got[: s.n].view(want.shape).double() - want).abs()
+            assert (off <= far).all(), (most, empty, float((off / far).max()))
+            assert (got[s.n:] == 7).all()
+    check(lib().sp_cuda_check_kernels(0))
+
+
+@pytest.mark.parametrize("rows,n,steps,keys", [(1, 300000, 12 * 32, 4), (64, 60000, 128, 128)])
+def test_long_sums_of_f32_rows(rows, n, steps, keys):
+    """A block for each key head of 148 sequences, whose sums run over all of the keys: what the tensor cores cut off does not grow with their number."""
+    dim, seqs = 64, 148
+    c = Cache([n], 1, dim, 9)
+    c.values[:, 1] &= 0x7F  # of one sign, so that errors are relative to the sum itself
+    s = Step(c, [(0, rows, n)] * seqs, 1, ops.F32, 10, size=0.05)
+    s.q[:] = s.q[:rows].repeat(seqs, 1)
+    want, _ = attention64(c, s.q[:rows].view(rows, 1, dim), [(0, rows, n)], dim**-0.5)
+    got = s.run(max_rows=128 if rows > 1 else 1)[: s.n].view(seqs, rows, 1, dim)
+    assert (got == got[0]).all()
+    # Between two additions apart 256 keys in two planes, 16 at a time, are added up: 32 additions, each of which cuts off up to 2^-23 of the sum. The sums
+    # apart and those of the weights round to nearest, n times off by 2^-24 / 3 sqrt(n) of the result (a standard deviation, the sum growing evenly), six of
+    # which are allowed; rows: of the 12 warps, or 96 threads, that share a row, whose errors are added up as squares. Weights: q is small, z below 1 in size,
+    # its error (formula in cache_fp8_tools.py) below 2^-21, ex2's 2^-22, in numerator and denominator; fp16 plus remainder 2^-22; last roundings 2^-23.
+    flushes, adds = n / steps / (8 if rows == 1 else 2), n / steps * (keys if rows == 1 else 1) + 32
+    shared = 12 if rows == 1 else 1
+    six = 6 * 2.0**-24 / 3 * (math.sqrt(flushes / shared) + math.sqrt(adds / (8 * shared if rows == 1 else 1)))
+    far = 32 * 2.0**-23 + six + 2 * (2.0**-21 + 2.0**-22) + 2.0**-22 + 2.0**-23
+    assert far < 1.3e-5
+    off = ((got[0].double() - want).abs() / want).max()
+    assert off <= far, (float(off), far)
