@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
                     float best = fmaxf(fmaxf(s[n][0][e], s[n][0][2 + e]), fmaxf(s[n][1][e], s[n][1][2 + e]));
 #pragma unroll
                     for (int x = 4; x <= 16; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xFFFFFFFFu, best, x));
-                    const float to = fmaxf(m[n][e], best), by = m[n][e] == to ? 1.f : af_ex2(m[n][e] - to);
+                    const float to = fmaxf(m[n][e], best), by = m[n][e] == to ? 1.f : ex2_approx(m[n][e] - to);
                     m[n][e] = to;
                     l[n][e] *= by;
 #pragma unroll
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float z0 = s[n][j / 2][2 * (j % 2)], z1 = s[n][j / 2][2 * (j % 2) + 1];
-                float w0 = af_ex2(z0 - from0), w1 = af_ex2(z1 - from1);
+                float w0 = ex2_approx(z0 - from0), w1 = ex2_approx(z1 - from1);
                 l[n][0] += w0;
                 l[n][1] += w1;
                 w0 = MASK && z0 == -INFINITY ? 0.f : w0 * vs[j];  // (what is masked may have any scale)
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
         for (int i = 0; i < W; ++i) top = fmaxf(top, warp_m[i][row]);
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            w[i] = warp_m[i][row] == -INFINITY ? 0.f : af_ex2(warp_m[i][row] - top);
+            w[i] = warp_m[i][row] == -INFINITY ? 0.f : ex2_approx(warp_m[i][row] - top);
             total += warp_l[i][row] * w[i];
         }
 #pragma unroll
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
         // lane i looks at part i
         const float pm = lane < parts ? ld_peer(peer_smem(smem_addr(&part_m[row]), lane)) : -INFINITY;
         const float pl = lane < parts ? ld_peer(peer_smem(smem_addr(&part_l[row]), lane)) : 0.f;
-        const float top = warp_max(pm), w = pm == -INFINITY ? 0.f : af_ex2(pm - top), total = warp_sum(pl * w);
+        const float top = warp_max(pm), w = pm == -INFINITY ? 0.f : ex2_approx(pm - top), total = warp_sum(pl * w);
         float y[DP / 32] = {};
         for (int i = 0; i < parts; ++i) {
             const float wi = __shfl_sync(0xFFFFFFFFu, w, i);
@@ -543,7 +543,7 @@ struct RowsLaunch {
     using Sh = ArShape<T, DP, NT, W>;
     using At = ArTimes<T, DP, NT>;
     static constexpr auto kernel = attention_rows_kernel<T, DP, NT, W>;
-    static cudaError_t share(const AttentionFp8Args& a, int64_t clusters, int64_t len, AfShare* out) {
+    static cudaError_t share(int64_t clusters, int64_t len, AfShare* out) {
         static PerDeviceOnce once;
         static ClusterFits fits[SP_MAX_DEVICES];
         ClusterFits& mine = fits[current_device_index()];
@@ -567,8 +567,8 @@ static cudaError_t launch_rows(const AttentionFp8Args& a, cudaStream_t st) {
     const int64_t clusters = (int64_t)a.c.n_kv * tiles * a.n_seqs, len = af_keys(a);
     AfShare wide, narrow;
     CUtensorMap map{};
-    cudaError_t e = RowsLaunch<T, DP, NT, 12>::share(a, clusters, len, &wide);
-    if (e == cudaSuccess) e = RowsLaunch<T, DP, NT, 4>::share(a, clusters, len, &narrow);
+    cudaError_t e = RowsLaunch<T, DP, NT, 12>::share(clusters, len, &wide);
+    if (e == cudaSuccess) e = RowsLaunch<T, DP, NT, 4>::share(clusters, len, &narrow);
     if (e == cudaSuccess && tiles > 1) {
         AfShare other;
         e = launch_attention_fp8_tiles(a, sizeof(T) == 2, st, &other);

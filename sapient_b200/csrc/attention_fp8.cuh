@@ -7,6 +7,7 @@
 #include <atomic>
 
 #include "cache_fp8.h"
+#include "fp8_rows.cuh"
 #include "plan_common.cuh"
 
 namespace sp {
@@ -16,11 +17,6 @@ constexpr float AF_LOG2E = 1.4426950408889634f;
 constexpr float AF_LAZY = 6.f;
 constexpr float AF_LIFT = 512.f;  // 2^(15 - LAZY)
 
-__device__ __forceinline__ float af_ex2(float v) {
-    float d;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v));
-    return d;
-}
 // Four e4m3 values of a word as two pairs of fp16.
 __device__ __forceinline__ void af_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
     asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}\n" : "=r"(lo), "=r"(hi) : "r"(w));

@@ -123,29 +123,6 @@ __device__ __forceinline__ void at_ld32(uint32_t taddr, uint64_t (&v)[16]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void at_st32(uint32_t taddr, const uint64_t (&v)[16]) {
-    asm volatile(
-        "{\n.reg .b32 r<32>;\n"
-        "mov.b64 {r0, r1}, %0;\n"
-        "mov.b64 {r2, r3}, %1;\n"
-        "mov.b64 {r4, r5}, %2;\n"
-        "mov.b64 {r6, r7}, %3;\n"
-        "mov.b64 {r8, r9}, %4;\n"
-        "mov.b64 {r10, r11}, %5;\n"
-        "mov.b64 {r12, r13}, %6;\n"
-        "mov.b64 {r14, r15}, %7;\n"
-        "mov.b64 {r16, r17}, %8;\n"
-        "mov.b64 {r18, r19}, %9;\n"
-        "mov.b64 {r20, r21}, %10;\n"
-        "mov.b64 {r22, r23}, %11;\n"
-        "mov.b64 {r24, r25}, %12;\n"
-        "mov.b64 {r26, r27}, %13;\n"
-        "mov.b64 {r28, r29}, %14;\n"
-        "mov.b64 {r30, r31}, %15;\n"
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%16], {r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15, r16, r17, r18, r19, r20, r21, r22, r23, r24, r25, r26, r27, r28, r29, r30, r31};\n"
-        "}\n" ::"l"(v[0]), "l"(v[1]), "l"(v[2]), "l"(v[3]), "l"(v[4]), "l"(v[5]), "l"(v[6]), "l"(v[7]), "l"(v[8]), "l"(v[9]), "l"(v[10]), "l"(v[11]), "l"(v[12]), "l"(v[13]), "l"(v[14]), "l"(v[15]), "r"(taddr)
-        : "memory");
-}
 __device__ __forceinline__ void at_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
@@ -166,11 +143,6 @@ __device__ __forceinline__ void at_before() { asm volatile("tcgen05.fence::befor
 __device__ __forceinline__ void at_fence_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
 // Two values an instruction, kept in register pairs.
-__device__ __forceinline__ uint64_t at_pair(float a, float b) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-    return d;
-}
 __device__ __forceinline__ float2 at_two(uint64_t v) {
     float2 f;
     asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
@@ -690,7 +662,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         const float2 f = at_two(s[q][k]);
-                        s[q][k] = at_pair(bits >> (2 * k) & 1 ? f.x : -INFINITY, bits >> (2 * k + 1) & 1 ? f.y : -INFINITY);
+                        s[q][k] = pack2(bits >> (2 * k) & 1 ? f.x : -INFINITY, bits >> (2 * k + 1) & 1 ? f.y : -INFINITY);
                     }
                     asm volatile("" ::: "memory");
                 }
@@ -707,7 +679,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             const float x = fmaf(fmaxf(fmaxf(b0, b1), fmaxf(b2, b3)), c, (float)power);
             const bool moves = x > m + AT_MOST;
             if (__any_sync(0xFFFFFFFFu, moves)) {
-                const float to = moves ? x - AT_SET : m, by = moves ? af_ex2(m - to) : 1.f;  // (m = -inf: 0)
+                const float to = moves ? x - AT_SET : m, by = moves ? ex2_approx(m - to) : 1.f;  // (m = -inf: 0)
                 m = to;
                 l *= by;
                 auto scale = [&](uint32_t at) {
@@ -734,7 +706,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 }
             }
             const float base = (m == -INFINITY ? 0.f : -m) + (F32 ? 0.f : (float)power);
-            const uint64_t c2 = at_pair(c, c), base2 = at_pair(base, base);
+            const uint64_t c2 = pack2(c, c), base2 = pack2(base, base);
             uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -743,9 +715,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     float2 p = at_two(at_fma2(s[q][k], c2, base2));
-                    p.x = af_ex2(p.x);
-                    p.y = af_ex2(p.y);
-                    const uint64_t pair = at_pair(p.x, p.y);
+                    p.x = ex2_approx(p.x);
+                    p.y = ex2_approx(p.y);
+                    const uint64_t pair = pack2(p.x, p.y);
                     if (k % 2) sum1 = at_add2(sum1, pair);
                     else sum0 = at_add2(sum0, pair);
                     if constexpr (F32) {
@@ -783,11 +755,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             }
         }
         T* const out = static_cast<T*>(a.out);
-        if (!KEYS && parts == 1) {
+        if (!KEYS && parts == 1) {  // (bf16 rows, 256 of them)
             const float by = l == 0.f || mine == 0 ? 0.f : 1.f / l;
             // A warp's 32 rows through its part of shared memory (the operands have been read), so that stores write whole lines
-            constexpr int UNITS = DP * (int)sizeof(T) / 16, AT_ONCE = 32 / UNITS;  // pieces of a row, rows a store
-            uint8_t* const mem = smem + warp * (32 * DP * (int)sizeof(T));
+            constexpr int UNITS = DP / 8, AT_ONCE = 32 / UNITS;  // pieces of a row, rows a store
+            uint8_t* const mem = smem + warp * (32 * DP * 2);
 #pragma unroll 1
             for (int d = 0; d < DP; d += 32) {
                 uint64_t o[16];
@@ -795,35 +767,29 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                     at_ld32(O + d, o);
                     at_wait_for(o);
                 }
-                const uint64_t by2 = at_pair(by, by);
+                const uint64_t by2 = pack2(by, by);
 #pragma unroll
-                for (int j = 0; j < 16; j += 8 / (int)sizeof(T)) {
+                for (int j = 0; j < 16; j += 4) {
                     uint4 w;
                     uint32_t* const u = &w.x;
 #pragma unroll
-                    for (int q = 0; q < 4; q += F32 ? 2 : 1) {
-                        const float2 f = at_two(mine > 0 ? at_mul2(o[j + (F32 ? q / 2 : q)], by2) : 0);
-                        if constexpr (F32) {
-                            u[q] = __float_as_uint(f.x);
-                            u[q + 1] = __float_as_uint(f.y);
-                        } else {
-                            u[q] = pack_bf16(f.x, f.y);
-                        }
+                    for (int q = 0; q < 4; ++q) {
+                        const float2 f = at_two(mine > 0 ? at_mul2(o[j + q], by2) : 0);
+                        u[q] = pack_bf16(f.x, f.y);
                     }
-                    const int unit = (d + 2 * j) * (int)sizeof(T) / 16;
+                    const int unit = (d + 2 * j) / 8;
                     *reinterpret_cast<uint4*>(mem + lane * (16 * UNITS) + ((unit & ~7) | ((unit ^ lane) & 7)) * 16) = w;
                 }
             }
             __syncwarp();
-            const int row_w = (KEYS ? 0 : 128 * t) + 32 * (warp & 3), unit = lane % UNITS;
+            const int row_w = 128 * t + 32 * (warp & 3), unit = lane % UNITS;
             const int64_t mine_to = offset_of(row_w + lane, a.ldo);
 #pragma unroll 4
             for (int q0 = 0; ok && q0 < 32; q0 += AT_ONCE) {
                 const int q = q0 + lane / UNITS;
                 const int64_t to = __shfl_sync(0xFFFFFFFFu, mine_to, q);
                 const uint4 w = *reinterpret_cast<const uint4*>(mem + q * (16 * UNITS) + ((unit & ~7) | ((unit ^ q) & 7)) * 16);
-                if (row_w + q < tile.n && unit * 16 < dim * (int)sizeof(T))
-                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + to) + unit * 16) = w;
+                if (row_w + q < tile.n && unit * 8 < dim) *reinterpret_cast<uint4*>(out + to + unit * 8) = w;
             }
         } else {
             float* const sums = reinterpret_cast<float*>(smem);  // [group][row][LDO], over the operands, which have been read
@@ -871,7 +837,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 }
                 float top = m;
                 for (int o = width / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-                const float w = m == -INFINITY ? 0.f : af_ex2(m - top);
+                const float w = m == -INFINITY ? 0.f : ex2_approx(m - top);
                 float total = l * w;
                 for (int o = width / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
                 if (q < rows_here && x < sets) weights[q * sets + x] = w == 0.f || total == 0.f ? 0.f : w / total;
