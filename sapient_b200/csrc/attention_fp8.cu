@@ -68,6 +68,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
     __shared__ float row_factor[Sh::ROWS];  // scale log2(e) / what the row was multiplied by
     __shared__ float warp_m[W][Sh::ROWS], warp_l[W][Sh::ROWS];
     __shared__ float part_m[Sh::ROWS], part_l[Sh::ROWS];
+    __shared__ uint32_t nan_dropped[W];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int head = blockIdx.x % a.c.n_kv, part = blockIdx.z, group = a.n_heads / a.c.n_kv, dim = a.c.dim;
     pdl_wait();
@@ -88,6 +89,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
     uint8_t *const ring = ar_smem + warp * STAGES * Sh::STAGE, *const scale_ring = ar_smem + W * STAGES * Sh::STAGE + warp * STAGES * Sh::SCALES;
     uint8_t* const qs = ar_smem + (Sh::SMEM - 1024 - Sh::Q);
     if (lane == 0) {
+        if (F32) nan_dropped[warp] = 0;
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(tc5_smem_u32(&full[warp][i])) : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -181,7 +183,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
         }
     }
     const int whole_from = a.window > 0 ? max(pos_last, 0) - a.window + 1 : 0, whole_to = min(pos_first, held - 1);  // keys that all rows see
-    uint32_t dropped = 0;  // values' bytes that are NaN, where MASK
+    [[maybe_unused]] uint32_t dropped = 0;  // values' bytes that are NaN, where MASK (f32: nan_dropped, one register less: 8 x 8 rows at 4096 57.3 us, 56.1 so)
     // MASK: some row does not see some key. Only then can a byte that is NaN belong to a key that a row does not see; else the product makes its
     // coordinate NaN.
     auto work = [&](auto with_mask, const uint8_t* at, const float* scales, int key0, uint32_t gone) {
@@ -348,8 +350,10 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
             if (MASK && !(gone >> pg & 1)) {  // (bytes that nobody sees may be anything)
                 auto counts = [&](int token) { return key0 + token >= k_begin && key0 + token < k_end; };
                 const int k = KV_PAGE * pg + 2 * t;
-                dropped |= near & ((counts(k) ? 0xFFFFu : 0u) | (counts(k + 1) ? 0xFFFF0000u : 0u));
-                dropped |= far & ((counts(k + 8) ? 0xFFFFu : 0u) | (counts(k + 9) ? 0xFFFF0000u : 0u));
+                const uint32_t here = (near & ((counts(k) ? 0xFFFFu : 0u) | (counts(k + 1) ? 0xFFFF0000u : 0u))) |
+                                      (far & ((counts(k + 8) ? 0xFFFFu : 0u) | (counts(k + 9) ? 0xFFFF0000u : 0u)));
+                if constexpr (!F32) dropped |= here;
+                else if (here != 0) nan_dropped[warp] = 1;
             }
         }
     };
@@ -389,7 +393,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
         for (int k = i; k < ring_requested(i, STAGES, steps); ++k) tc5_wait(&full[warp][ring_at(k, STAGES).stage], ring_at(k, STAGES).parity);
     }
     __syncwarp();
-    if (__any_sync(0xFFFFFFFFu, dropped != 0)) {
+    if (F32 ? nan_dropped[warp] != 0 : __any_sync(0xFFFFFFFFu, dropped != 0)) {
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
             const int key0 = (b_begin + warp + i * W) * AR_KEYS;

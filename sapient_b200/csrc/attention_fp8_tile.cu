@@ -36,7 +36,7 @@ namespace sp {
 cudaError_t count_launch_and_check();  // kernels.cu
 
 constexpr int AT_KEYS = 128, AT_PAGES = AT_KEYS / KV_PAGE, AT_THREADS = 512, AT_RING = 8;
-constexpr int AT_FLUSH = 2;
+constexpr int AT_FLUSH = 2, AT_NONE = INT32_MAX;
 constexpr float AT_MOST = 15.f, AT_SET = 9.f;  // log2 of the largest weight, and of it when M is set
 constexpr int AT_UP = 7, AT_LEAST = -80;       // values times 2^7 are below 2^16; smaller u would let a sum of 2^(z - M) pass 2^127
 
@@ -175,9 +175,8 @@ __device__ __forceinline__ float at_max3(float a, uint64_t two) {
     return d;
 }
 
-// 16 bytes of N tokens, PER apart, as fp16 to `to` (of the first) and u0, u1. Keys as they are; values without NaN and times `by` (f32 rows: as they
-// are). The second half of a row's threads (odd) swap the halves of their 16 bytes: eight threads' stores fall on 32 different banks. Back: whether
-// values had NaN.
+// 16 bytes of N tokens, PER apart, as fp16 to `to` (of the first) and u0, u1. Keys as they are; values without NaN and, for bf16 rows, times `by`. The second
+// half of a row's threads (odd) swap the halves of their 16 bytes: eight threads' stores fall on 32 different banks. Back: whether values had NaN.
 template <bool F32, bool VALUES, int PER, int N>
 __device__ __forceinline__ uint32_t at_convert(const uint4 (&raw)[N], const uint32_t (&by)[N], uint8_t* to, int u0, int u1, bool odd) {
     uint32_t dropped = 0;
@@ -210,7 +209,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
     __shared__ __align__(8) uint64_t k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES], s_full[2], p_full[2][2], o_done, o_full, q_full;
     __shared__ __align__(16) float k_scale[AT_RING][AT_KEYS], v_scale[AT_RING][F32 ? AT_KEYS : 4];
     __shared__ uint32_t gone_s[AT_RING];     // pages of the tile that are not there
-    __shared__ uint32_t nan_dropped;         // some value bytes were NaN
+    __shared__ int nan_from;                 // the first tile with value bytes that are NaN (AT_NONE: none)
     __shared__ __align__(16) uint32_t largest_s[AT_RING][4];  // scales of values that count, of 32 tokens each
     __shared__ float row_factor[ROWS];
     __shared__ float part_m[2][128], part_l[2][128];
@@ -269,7 +268,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     if (tid == 32) {
-        nan_dropped = 0;
+        nan_from = AT_NONE;
         for (int i = 0; i < K_STAGES; ++i) {
             at_init(&k_full[i], F32 ? 4 : 1);
             at_init(&k_empty[i], 1);
@@ -466,10 +465,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         }
         for (int kv = 0; kv < n_kv; ++kv) {
             const int key0 = (b_begin + kv) * AT_KEYS;
-            const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
             uint32_t by[N] = {};  // what values are multiplied by, as pairs of fp16
             if constexpr (F32) {
                 const int st = kv % K_STAGES, use = kv / K_STAGES, slot = kv % AT_RING;
+                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
                 if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&k_empty[st], (uint32_t)((use - 1) & 1)));
                 if (!ok) break;
                 at_convert<F32, false, PER>(raw_k, by, ks_ + st * Sh::K_TILE + row0, u0, u1, odd);
@@ -502,14 +501,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             const int st = kv % V_STAGES, use = kv / V_STAGES;
             if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&v_empty[st], (uint32_t)((use - 1) & 1)));
             if (!ok) break;
-            if (gone != 0 || key0 < k_begin || key0 + (AT_KEYS - 1) >= k_end) {  // bytes that nobody sees may be anything
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int token = tok0 + PER * i;
-                    if (gone >> (token / KV_PAGE) & 1 || key0 + token < k_begin || key0 + token >= k_end) raw_v[i] = make_uint4(0, 0, 0, 0);
-                }
-            }
-            if (at_convert<F32, true, PER>(raw_v, by, vs_ + st * Sh::TILE + row0, u0, u1, odd) != 0) nan_dropped = 1;
+            if (at_convert<F32, true, PER>(raw_v, by, vs_ + st * Sh::TILE + row0, u0, u1, odd) != 0) atomicMin(&nan_from, kv);
             hand_over(&v_full[st]);
             pages = next;
             next = page_of(kv + 2);
@@ -747,9 +739,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         if (jobs > 0) ok = __all_sync(0xFFFFFFFFu, ok && tc5_wait(&o_full, 0));
         else asm volatile("barrier.cta.sync 1, 256;\n" ::: "memory");
         at_after();
-        if (jobs > 0 && ok && nan_dropped != 0) {  // (set before the products whose end has been waited for)
+        if (jobs > 0 && ok && nan_from != AT_NONE) {  // (written before the products whose end has been waited for; bytes that nobody sees may be among them)
 #pragma unroll 1
-            for (int i = 0; i < n_kv * (AT_KEYS / 32); ++i) {
+            for (int i = nan_from * (AT_KEYS / 32); i < n_kv * (AT_KEYS / 32); ++i) {
                 const int key0 = b_begin * AT_KEYS + 32 * i;
                 if (af_sees(af_nan_tokens(a.c, table, head, key0, k_end), key0, low, limit)) l = __uint_as_float(0x7FC00000u);
             }
