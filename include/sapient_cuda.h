@@ -220,7 +220,8 @@ typedef struct SpCacheFp8 {
  * pairs 0: coordinates c and c + rotary_dim / 2 are a pair, 1: coordinates 2 c and 2 c + 1. Queries go to q_out, which may be q with the
  * same stride; keys and values (those as they are) go to the cache as fp8 rows, at positions[i] of slot slots[i]. A token whose slot is not
  * one of the cache's, or whose position lies past its page table or past the angles, is skipped with all that belongs to it; where its page is
- * not one, only its keys and values are. A place of the cache may occur once in a call. h^2 is added up in f32: |x| up to 2^63 / sqrt(head_dim). */
+ * not one, only its keys and values are. A place of the cache may occur once in a call. h^2 is added up in f32: |x| up to 2^63 / sqrt(head_dim),
+ * mean(x^2) + eps from 2^-126 on; a normed head of zeros at eps = 0 is 0 / 0, NaN. */
 int32_t sp_cuda_cache_fp8_append_dev(const void* cache, int32_t dtype, int64_t n_tok, const int32_t* slots, const int32_t* positions,
                                      const void* q, int64_t ldq, int32_t n_heads, void* q_out, int64_t ldqo, const void* k, int64_t ldk,
                                      const void* v, int64_t ldv, const float* q_w, const float* k_w, float eps, const float* angles,
@@ -236,7 +237,7 @@ int32_t sp_cuda_cache_fp8_read_dev(const void* cache, int32_t dtype, int64_t n_t
  * tokens on pages that are not there are not seen. out may be q with the same stride. max_rows: of any sequence, not less than they
  * have (rows past it stay as they are); max_len: of any sequence (a wrong one costs time only). By both the kernel is chosen and the work
  * shared out, so that bounds far above what the sequences have cost time. Rows in front of row_start[0] and behind row_start[n_seqs] stay as
- * they are. Scales are not negative; a key or value row whose scale is NaN or infinite makes the rows that see it NaN, and no others; so
+ * they are. Scales are not negative, those of keys at most 2^99 (|k| up to 2^107; scores are formed in f32); a key or value row whose scale is NaN or infinite makes the rows that see it NaN, and no others; so
  * do bytes that are NaN beside a finite scale (_append leaves none), those of values in their coordinate at least. A row's head whose query has
  * a NaN or an infinity is NaN if it sees a key, and no other is. n_seqs is at most 65535.
  * Precision: weights have 11 bits for bf16 rows, 22 for f32 rows (a value whose scale is below 2^-20 of the largest beside it fewer); f32

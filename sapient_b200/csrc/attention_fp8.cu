@@ -534,7 +534,7 @@ AfShare af_share(const ClusterFits& fits, int64_t clusters, int64_t pieces, doub
 
 // Microseconds of a warp's step with twelve warps on an SM, of a block's start and end, and of adding parts up. Few bf16 rows: measured, 131072 keys of
 // the 8B shape in one to 16 parts, 518 keys; the others are fitted to 64 calls (3 to 35 rows a head, 240 to 32768 keys, 1 to 32 sequences, 8B, 1.5B and
-// 0.5B shapes), from which they are 3 to 8 % off.
+// 0.5B shapes), from which they are 3 to 8 % off. Other calls are not checked against them; head sizes between 64 and 128 take 128's.
 template <typename T, int DP, int NT>
 struct ArTimes {
     static constexpr bool F32 = sizeof(T) == 4, FEW = NT == 1 && !F32;

@@ -97,7 +97,8 @@ struct AfShare {
     double time;  // us
 };
 // The number of parts for which `clusters` of them take least, a block for `piece` of each of its share of `pieces`, and `fixed` and `joined` (where
-// there are parts to add up) besides. Rounds that do not fill the GPU count half: blocks are of unequal length.
+// there are parts to add up) besides. Rounds that do not fill the GPU count half: blocks are of unequal length. `pieces` are the longest sequence's for every
+// block: prompts and ragged batches have about half of that, so that their times come out too long.
 AfShare af_share(const ClusterFits& fits, int64_t clusters, int64_t pieces, double piece, double fixed, double joined);
 // attention_fp8_tile.cu; plan: nothing is launched, only how it would be, and how long it would take, is said
 cudaError_t launch_attention_fp8_tiles(const AttentionFp8Args& a, bool bf, cudaStream_t st, AfShare* plan);

@@ -10,8 +10,9 @@
 // bf16 rows are multiplied with the keys' own bytes: q is two e4m3 digits, whose products run at twice fp16's rate. A row scaled so that its largest
 // value lies in [128, 256) is its digits' sum exactly, but for values below 2^-9 of the largest, which are off by up to 2^-17 of that. What
 // bounds the tiles is the shared memory's bandwidth (operands, their conversion, scales), so that keys that need no conversion count for more
-// than the instructions: 8192 x 8192, 8B shape, 690 us with keys converted to fp16, 605 to 640 (0.9 PFLOP/s; power limit) so; 2.1 us a tile of 256 rows by
-// 128 keys. Short prompts are bound by a block's start (5 us until its queries are operands) and end (2 us): 9 x 1500 rows, 2.7B shape, 247 us.
+// than the instructions: 8192 x 8192, 8B shape, 690 us with keys converted to fp16, 620 so on the same day (640 to 680 from call to call since:
+// the power limit, 0.81 to 0.86 PFLOP/s); 2.1 us a tile of 256 rows by 128 keys. Short prompts are bound by a block's start (5 us until its queries are
+// operands) and end (2 us): 9 x 1500 rows, 2.7B shape, 244 to 249 us. Values' bytes that are NaN are looked for as they are converted (af_finite).
 // ROWS: the groups have 128 rows each of 256, and keys in common. KEYS (up to 128 rows): the same rows, key tiles by turns; their sums
 // are added up at the end. f32: one group with two tiles of scores; the tensor cores cut off what falls below a sum's last bits, always towards
 // zero (2^-26 of it an addition: 1.8e-5 after 8192 keys), so that O is added to a sum of its own by the vector units every AT_FLUSH tiles (64 rows at
@@ -876,7 +877,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
 }
 
 // Microseconds of a tile of keys, of a block's start and end, and of adding parts up. KEYS: fitted to 64 calls (3 to 35 rows a head, 240 to 32768 keys,
-// 1 to 32 sequences, 8B, 1.5B and 0.5B shapes), from which they are 3 to 8 % off; ROWS: 512 rows at 8704.
+// 1 to 32 sequences, 8B, 1.5B and 0.5B shapes), from which they are 3 to 8 % off; ROWS: 512 rows at 8704 of the 8B shape, taken for all head sizes. Other
+// calls are not checked against them; head sizes between 64 and 128 take 128's.
 template <typename T, int DP, bool KEYS>
 struct AtTimes {
     static constexpr bool F32 = sizeof(T) == 4;

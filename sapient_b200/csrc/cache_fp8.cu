@@ -20,8 +20,8 @@ cudaError_t count_launch_and_check();  // kernels.cu
 // A head is 4 or 8 threads of 16 coordinates each: eight pairs that are rotated together, so that nothing is exchanged but a sum and a
 // maximum. The teams of a token take its heads in turn, the next one on its way; place and angles are loaded once. Few tokens are spread over
 // as many threads as they have heads for (1 token of the 8B shape 2.2 us, with two warps 3.3), of many a token is two warps' (8192 tokens 39.2
-// us, with a team for each head 57.6; two or three heads at a time 46 and 49: registers). What is left above the bytes' 28.4 us
-// is a start in which SMs wait for their first rows, and writes beside reads.
+// us, with a team for each head 57.6; two or three heads at a time 46 and 49: registers). What is left above the bytes' 28.4 us (1024 tokens 8.9 of 3.6,
+// 4096 23.2 of 14.5) is a start in which SMs wait for their first rows, and too few of them on their way: 80 registers leave a third of an SM's warps.
 constexpr int CA_THREADS = 256;
 
 template <typename T, int TEAM>
@@ -144,8 +144,9 @@ cudaError_t launch_cache_append(const CacheAppendArgs& a, bool bf, cudaStream_t 
 
 // ── read ──
 // A thread takes eight coordinates at a time. Few tokens: a block has one. Many: a warp has four, whose pages are looked up at once, and eight
-// requests on their way (8B shape: 65536 tokens 71 us, a block a token 99; 20000 18.7 and 19.0; 8192 11.5 and 8.9; 2048 7.2 and 3.8; 0.5B shape:
-// 20000 9.2 and 13.4, 8192 5.5 and 6.0, 4096 5.2 and 3.4).
+// requests on their way where a token's pieces are that many (from memory, bf16, four tokens a warp and a token a block; 8B shape, 256 pieces: 65536 tokens
+// 76.9 us and 90.7, 20000 28.1 and 29.4, 8192 13.9 and 13.8, 2048 7.3 and 4.1; 0.5B shape, 32 pieces: 65536 31.8 and 68.6, 20000 11.8 and 21.4,
+// 8192 6.3 and 9.3, 2048 5.0 and 3.8). The border is set for wide tokens: narrow ones would cross over near 4000.
 constexpr int CR_THREADS = 128, CR_TOKENS = 4, CR_MANY = 10000;
 
 template <typename T, int TOKENS>
