@@ -397,12 +397,13 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 3 : 1) attention_rows_kernel(
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
             const int key0 = (b_begin + warp + i * W) * AR_KEYS;
-            const uint32_t tokens = af_nan_tokens(a.c, table, head, key0, k_end);
+            uint32_t tokens[1];
+            af_nan_tokens(a.c, table, head, key0, k_end, tokens);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    if (af_sees(tokens, key0, low[n][e], limit[n][e])) l[n][e] = __uint_as_float(0x7FC00000u);
+                    if (af_sees(tokens[0], key0, low[n][e], limit[n][e])) l[n][e] = __uint_as_float(0x7FC00000u);
         }
     }
     // ── the warps' sums into one, then the blocks' ──

@@ -34,16 +34,23 @@ __device__ __forceinline__ bool af_has_nan(const uint4& v) {
     auto of = [](uint32_t four) { return (four & 0x7F7F7F7Fu) + 0x01010101u; };  // a byte of 0x7F or 0xFF carries into its sign
     return ((of(v.x) | of(v.y) | of(v.z) | of(v.w)) & 0x80808080u) != 0;
 }
-// Of the 32 tokens from key0 (a multiple of 32) to k_end, a bit for each that has a NaN among its values' bytes.
-__device__ __forceinline__ uint32_t af_nan_tokens(const CacheFp8& c, const int32_t* table, int head, int key0, int k_end) {
-    const int key = key0 + (int)(threadIdx.x & 31), page = key < k_end ? table[key / KV_PAGE] : -1;
-    bool nan = false;
-    if (page >= 0 && page < c.n_pages) {
-        const uint4* const row = reinterpret_cast<const uint4*>(c.values + (c.row(page, 1, head) + key % KV_PAGE) * c.dim);
-#pragma unroll 4
-        for (int i = 0; i < c.dim / 16; ++i) nan |= af_has_nan(row[i]);
+// Of the 32 N tokens from key0 (a multiple of 32) to k_end, a bit for each that has a NaN among its values' bytes.
+template <int N>
+__device__ __forceinline__ void af_nan_tokens(const CacheFp8& c, const int32_t* table, int head, int key0, int k_end, uint32_t (&tokens)[N]) {
+    const uint4* row[N];
+    bool nan[N] = {};
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int key = key0 + 32 * n + (int)(threadIdx.x & 31), page = key < k_end ? table[key / KV_PAGE] : -1;
+        row[n] = page >= 0 && page < c.n_pages ? reinterpret_cast<const uint4*>(c.values + (c.row(page, 1, head) + key % KV_PAGE) * c.dim) : nullptr;
     }
-    return __ballot_sync(0xFFFFFFFFu, nan);
+#pragma unroll 4
+    for (int i = 0; i < c.dim / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (row[n]) nan[n] |= af_has_nan(row[n][i]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) tokens[n] = __ballot_sync(0xFFFFFFFFu, nan[n]);
 }
 // Whether a row that sees keys low .. limit sees one of those tokens.
 __device__ __forceinline__ bool af_sees(uint32_t tokens, int key0, int low, int limit) {

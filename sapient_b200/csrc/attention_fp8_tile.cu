@@ -742,9 +742,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
         at_after();
         if (jobs > 0 && ok && nan_from != AT_NONE) {  // (written before the products whose end has been waited for; bytes that nobody sees may be among them)
 #pragma unroll 1
-            for (int i = nan_from * (AT_KEYS / 32); i < n_kv * (AT_KEYS / 32); ++i) {
-                const int key0 = b_begin * AT_KEYS + 32 * i;
-                if (af_sees(af_nan_tokens(a.c, table, head, key0, k_end), key0, low, limit)) l = __uint_as_float(0x7FC00000u);
+            for (int kv = nan_from; kv < n_kv; ++kv) {
+                const int key0 = (b_begin + kv) * AT_KEYS;
+                uint32_t tokens[AT_KEYS / 32];
+                af_nan_tokens(a.c, table, head, key0, k_end, tokens);
+#pragma unroll
+                for (int q = 0; q < AT_KEYS / 32; ++q)
+                    if (af_sees(tokens[q], key0 + 32 * q, low, limit)) l = __uint_as_float(0x7FC00000u);
             }
         }
         T* const out = static_cast<T*>(a.out);
