@@ -24,10 +24,10 @@ __device__ __forceinline__ void af_halves(uint32_t w, uint32_t& lo, uint32_t& hi
 // NaN bytes of values become 448: they must not reach rows that do not see them through 0 x NaN. `dropped`, else 0, is NaN from the first on
 // (a sum of zeros, on the pipe that has the least to do here; collected by the vector units' logic it took 3 to 5 % of the f32 tiles); then the rows that do
 // see one are looked for at the end (af_nan_tokens, af_sees) and get NaN as their sum of weights.
-__device__ __forceinline__ uint32_t af_finite(uint32_t two, uint32_t& dropped) {
+__device__ __forceinline__ uint32_t af_finite(uint32_t two, uint32_t& dropped, bool live = true) {
     uint32_t d;
     asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(two), "r"(0x5F005F00u));
-    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(dropped) : "r"(two), "r"(0u));
+    if (live) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(dropped) : "r"(two), "r"(0u));
     return d;
 }
 __device__ __forceinline__ bool af_has_nan(const uint4& v) {

@@ -177,9 +177,10 @@ __device__ __forceinline__ float at_max3(float a, uint64_t two) {
 }
 
 // 16 bytes of N tokens, PER apart, as fp16 to `to` (of the first) and u0, u1. Keys as they are; values without NaN and, for bf16 rows, times `by`. The second
-// half of a row's threads (odd) swap the halves of their 16 bytes: eight threads' stores fall on 32 different banks. Back: whether values had NaN.
+// half of a row's threads (odd) swap the halves of their 16 bytes: eight threads' stores fall on 32 different banks. Back: whether values had NaN,
+// of tokens less than `live` behind the first: past a sequence's end bytes may be anything, and to look for rows that see them would take 5 us.
 template <bool F32, bool VALUES, int PER, int N>
-__device__ __forceinline__ uint32_t at_convert(const uint4 (&raw)[N], const uint32_t (&by)[N], uint8_t* to, int u0, int u1, bool odd) {
+__device__ __forceinline__ uint32_t at_convert(const uint4 (&raw)[N], const uint32_t (&by)[N], uint8_t* to, int u0, int u1, bool odd, int live) {
     uint32_t dropped = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -191,7 +192,7 @@ __device__ __forceinline__ uint32_t at_convert(const uint4 (&raw)[N], const uint
         if constexpr (VALUES) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                h[j] = af_finite(h[j], dropped);
+                h[j] = af_finite(h[j], dropped, PER * i < live);
                 if constexpr (!F32) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[j]) : "r"(by[i]));
             }
         }
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
                 const uint32_t gone = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
                 if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&k_empty[st], (uint32_t)((use - 1) & 1)));
                 if (!ok) break;
-                at_convert<F32, false, PER>(raw_k, by, ks_ + st * Sh::K_TILE + row0, u0, u1, odd);
+                at_convert<F32, false, PER>(raw_k, by, ks_ + st * Sh::K_TILE + row0, u0, u1, odd, 0);
                 const float v = counts(sv, key0 + p) ? sv : 0.f;
                 k_scale[slot][p] = sv < INFINITY && sv > -INFINITY ? af_number(sk) : __uint_as_float(0x7FC00000u);
                 v_scale[slot][p] = v;
@@ -502,7 +503,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_tile_kernel(const Att
             const int st = kv % V_STAGES, use = kv / V_STAGES;
             if (use > 0) ok = __all_sync(0xFFFFFFFFu, at_wait_idle(&v_empty[st], (uint32_t)((use - 1) & 1)));
             if (!ok) break;
-            if (at_convert<F32, true, PER>(raw_v, by, vs_ + st * Sh::TILE + row0, u0, u1, odd) != 0) atomicMin(&nan_from, kv);
+            if (at_convert<F32, true, PER>(raw_v, by, vs_ + st * Sh::TILE + row0, u0, u1, odd, k_end - key0 - tok0) != 0) atomicMin(&nan_from, kv);
             hand_over(&v_full[st]);
             pages = next;
             next = page_of(kv + 2);
