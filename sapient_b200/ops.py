@@ -337,7 +337,7 @@ def rope_table(n_positions: int, rotary_dim: int, base: float, factor: float = 1
     training) only those that make at most `low` turns within it are divided, those of `high` turns and more stay, and between the two it goes over.
     low and high are a model's low_freq_factor and high_freq_factor (1 and 4 where its configuration has rope_type llama3): give them. Without
     them a ramp of 0.25 to 1 turns is taken, which is no published rule, and a warning says so."""
-    if original and (low is None or high is None):
+    if original and factor != 1 and (low is None or high is None):
         warnings.warn("rope_table: original without low and high: 0.25 and 1 turns are taken where a model has its low_freq_factor and high_freq_factor (usually 1 and 4)", stacklevel=2)
     low, high = 0.25 if low is None else low, 1.0 if high is None else high
     if n_positions < 0 or rotary_dim < 0 or rotary_dim % 2:

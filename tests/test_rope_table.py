@@ -42,6 +42,7 @@ def test_without_a_models_factors_it_warns():
         warnings.simplefilter("error")
         ops.rope_table(2, 64, 10000.0)
         ops.rope_table(2, 64, 10000.0, factor=4.0)
+        assert np.array_equal(ops.rope_table(2, 64, 10000.0, original=4096), ops.rope_table(2, 64, 10000.0))  # nothing is divided by 1
 
 
 def test_refusals():
