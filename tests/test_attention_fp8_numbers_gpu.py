@@ -1,5 +1,5 @@
 """Attention over a cache of 8-bit rows where numbers end: infinite queries, bytes that are NaN, factors of the scores that are zero, negative or
-large, and long sums of f32 rows."""
+large, the largest key scales, and long sums of f32 rows."""
 import math
 
 import pytest
@@ -137,3 +137,18 @@ def test_long_sums_of_f32_rows(rows, n, steps, keys):
     assert far < 1.3e-5
     off = ((got[0].double() - want).abs() / want).max()
     assert off <= far, (float(off), far)
+
+
+@BOTH
+@pytest.mark.parametrize("rows,dim", [(1, 128), (20, 64), (140, 128), (300, 64)])
+def test_the_largest_key_scales(rows, dim, ty):
+    """Key scales up to 2^99 against queries that are as small as they are large: no score passes f32's range on its way."""
+    c = Cache([700], 2, dim, 11)
+    c.scales[:, 0] = 2.0**99 * (0.5 + 0.5 * torch.rand_like(c.scales[:, 0]))
+    c.scales[int(c.table[0, 1]), 0] = 2.0**99
+    s = Step(c, [(0, rows, 700)], 4, ty, 12, size=2.0**-107)
+    want, far = attention64(c, s.q[: s.n].view(s.n, 4, dim), s.seqs, dim**-0.5, 0, True)
+    for most, empty in ways(s):
+        got = s.run(max_rows=most, empty=empty, out=torch.full_like(s.out, 7.0))
+        off = (got[: s.n].view(want.shape).double() - want).abs()
+        assert (off <= far).all(), (most, empty, float((off / far).max()))
